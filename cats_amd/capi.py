@@ -24,7 +24,8 @@ SYMBOLS = (
     "cats_gate_compact", "cats_read_count", "cats_up_flag", "cats_down_flag", "cats_gate_up", "cats_mlp",
     "cats_mlp_rowmajor_down", "cats_mlp_norm_residual", "cats_up_down", "cats_set_tuning", "cats_mlp_stage", "cats_mlp_noalloc", "cats_up_index", "cats_down_index",
     "cats_probe_read", "cats_mlp_norm_residual_norm", "cats_linear", "cats_attention_step", "cats_mlp_gate_cols", "cats_silu_mask_mul",
-    "cats_prompt_scratch_bytes", "cats_prompt_mlp", "cats_prompt_plan",
+    "cats_prompt_scratch_bytes", "cats_prompt_mlp", "cats_prompt_plan", "cats_kv8_append", "cats_kv8_attention_scratch_bytes",
+    "cats_kv8_attention", "cats_beam_scratch_bytes", "cats_beam_select", "cats_cache_reorder",
 )
 
 
@@ -75,6 +76,16 @@ def lib() -> ctypes.CDLL:
         L.cats_down_index.argtypes = [vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, sz, vp]; L.cats_down_index.restype = i32
         if hasattr(L, "cats_mlp_gate_cols"):
             L.cats_mlp_gate_cols.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, f32, vp, sz, vp]; L.cats_mlp_gate_cols.restype = i32
+        if hasattr(L, "cats_kv8_append"):
+            i64 = ctypes.c_int64
+            L.cats_kv8_append.argtypes = [vp, vp, vp, vp, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]
+            L.cats_kv8_append.restype = i32
+            L.cats_kv8_attention_scratch_bytes.argtypes = [i32] * 7; L.cats_kv8_attention_scratch_bytes.restype = sz
+            L.cats_kv8_attention.argtypes = [vp, vp, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, f32, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, sz, vp]
+            L.cats_kv8_attention.restype = i32
+            L.cats_beam_scratch_bytes.argtypes = [i32] * 4; L.cats_beam_scratch_bytes.restype = sz
+            L.cats_beam_select.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, sz, vp]; L.cats_beam_select.restype = i32
+            L.cats_cache_reorder.argtypes = [vp, i32, vp, vp, i32, i32, i32, vp]; L.cats_cache_reorder.restype = i32
         L.cats_set_tuning.argtypes = [i32, i32, i32, i32]; L.cats_set_tuning.restype = i32
         _lib = L
     return _lib

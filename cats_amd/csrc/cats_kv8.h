@@ -1,0 +1,525 @@
+// A cache of keys and values in 8 bits, and attention over it (16-bit models).
+//
+// Format.  A row (sequence) of the cache has `blocks` blocks of 64 tokens.  A block that is complete is held as e4m3 numbers with one
+// power of two as scale for a head's keys and one for its values: the smallest that brings the block's largest finite magnitude within 448.
+// e4m3 is a floating format, so a power of two costs no precision against a free scale, and scaling is exact: a value is rounded once
+// (by at most 2^-4 of itself) and what the products use is what is stored.  Values that are not finite are stored as NaN.
+//   k8 (B, kv_heads, blocks, 64, D)   v8 (B, kv_heads, blocks, D, 64)   scales (B, kv_heads, blocks) float
+// The block that holds a row's last token, complete or not, is always read as it was given, from
+//   k_tail (B, kv_heads, 64, D)       v_tail (B, kv_heads, D, 64)        slot = position % 64
+// so every token is rounded once, from what was given, whatever pieces the tokens come in.
+// Values lie with the tokens of one element side by side: that is the order in which the matrix cores want them, both as operand of
+// v_mfma_f32_16x16x32 and of 32x32x16, where 64 tokens of one element are 16 bytes of each of four lanes.
+#pragma once
+#include <float.h>
+
+#include "cats_down_mma.h"
+#include "cats_rows_mma.h"
+
+namespace cats {
+
+constexpr int kKvBlock = 64;
+
+struct KvCache {
+  uint8_t* k8;
+  uint8_t* v8;
+  float* ks;
+  float* vs;
+  uint16_t* kt;
+  uint16_t* vt;
+  int heads;   // of the cache
+  int blocks;  // of a row; at most 2^24, so that positions are ints
+};
+
+// Where a row's new tokens lie: positions start .. start + n - 1, as many of the call's T tokens as its count says.
+struct KvSpan {
+  const int64_t* start;
+  const int64_t* count;  // nullptr: all T
+  int start_step;        // 0: one start for all rows
+  int count_step;
+};
+__device__ __forceinline__ bool kv_span(const KvSpan& s, int b, int T, int blocks, int& start, int& n) {
+  const long long a = s.start[(size_t)b * s.start_step], c = s.count ? s.count[(size_t)b * s.count_step] : T;
+  n = (int)(c < 0 ? 0 : c > T ? T : c);
+  const bool ok = a >= 0 && a <= (long long)blocks * kKvBlock - n;
+  start = ok ? (int)a : 0;
+  return ok;
+}
+
+// What differs between the two types.  HEAD: attention's weights are held as 2^HEAD times themselves, so that in fp16 the normal numbers
+// reach down to 2^-29 of the largest weight.
+template <class DT> struct Kv;
+template <> struct Kv<F16> {
+  static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
+  static constexpr float HEAD = 15.f;
+  template <bool HI>
+  static __device__ __forceinline__ uint32_t cvt(uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI)); }
+};
+template <> struct Kv<BF16> {
+  static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u;
+  static constexpr float HEAD = 0.f;
+  template <bool HI>
+  static __device__ __forceinline__ uint32_t cvt(uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI)); }
+};
+// Eight e4m3 numbers as an operand of sixteen bits, exactly.
+template <class DT>
+__device__ __forceinline__ u32x4 kv_wide(uint32_t a, uint32_t b) {
+  return u32x4{Kv<DT>::template cvt<false>(a), Kv<DT>::template cvt<true>(a), Kv<DT>::template cvt<false>(b), Kv<DT>::template cvt<true>(b)};
+}
+
+// ---- storing ----------------------------------------------------------------------------------------------------------------------
+
+// The smallest power of two with amax <= 448 * scale, between 2^-60 and 2^120 (values below 2^-70 become 0); 1 for a block of zeros.
+__device__ __forceinline__ float kv_scale_of(float amax) {
+  if (!(amax > 0.f)) return 1.f;
+  const uint32_t bits = __float_as_uint(amax);
+  int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);  // 448 = 1.75 * 2^8
+  e = e < -60 ? -60 : e;
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+__device__ __forceinline__ float kv_code_of(float x, float inv) { return fmaf(x, 0.f, x * inv); }  // NaN where x is not finite
+
+struct KvAppendArgs {
+  const uint16_t* k;  // (B, T, heads, D) in elements: strides of a row, a token and a head
+  const uint16_t* v;
+  long long k_row, k_tok, k_head, v_row, v_tok, v_head;
+  KvSpan span;
+  KvCache c;
+  int T;
+};
+
+// Workgroup (i, head, row) quantises block start / 64 + i if these tokens complete it; the first one also stores the tail.  It is the only one that
+// reads the tail (the tokens of the first block that were there before) and the only one that writes it, behind a barrier.
+// Bound by memory: 2 bytes of a value read and one written.
+template <class DT, int D>
+__global__ __launch_bounds__(256) void kv8_append_kernel(KvAppendArgs p) {
+  constexpr int E = D / 4, NV = E / 8;  // elements and vectors of a token that one of its four threads holds
+  const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+  int start, n;
+  if (!kv_span(p.span, b, p.T, p.c.blocks, start, n) || n == 0) return;
+  const int end = start + n, last = (end - 1) / kKvBlock, blk = start / kKvBlock + blockIdx.x;
+  if (blk > last) return;
+  const size_t pair = (size_t)b * p.c.heads + h;
+  uint16_t* kt = p.c.kt + pair * kKvBlock * D;
+  uint16_t* vt = p.c.vt + pair * kKvBlock * D;
+  const uint16_t* k = p.k + b * p.k_row + h * p.k_head;
+  const uint16_t* v = p.v + b * p.v_row + h * p.v_head;
+
+  __shared__ uint32_t s_max[2][4];
+  __shared__ uint8_t s_v[D][kKvBlock + 4];
+  if ((blk + 1) * kKvBlock <= end) {
+    const int tok = tid / 4, d0 = tid % 4 * E, at = blk * kKvBlock + tok - start;
+    u32x4 kx[NV], vx[NV];
+    if (at >= 0) {
+#pragma unroll
+      for (int i = 0; i < NV; i++) kx[i] = load_stream((const u32x4*)(k + at * p.k_tok + d0) + i);
+#pragma unroll
+      for (int i = 0; i < NV; i++) vx[i] = load_stream((const u32x4*)(v + at * p.v_tok + d0) + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; i++) kx[i] = ((const u32x4*)(kt + tok * D + d0))[i];
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          vx[i][e] = vt[(d0 + 8 * i + 2 * e) * kKvBlock + tok] | (uint32_t)vt[(d0 + 8 * i + 2 * e + 1) * kKvBlock + tok] << 16;
+    }
+    // magnitudes of 16-bit floats are ordered as integers
+    auto most = [](const u32x4 (&x)[NV]) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint32_t w = x[i][e], lo = w & 0x7fffu, hi = w >> 16 & 0x7fffu;
+          m = max(m, max(lo < Kv<DT>::kExp ? lo : 0u, hi < Kv<DT>::kExp ? hi : 0u));
+        }
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, kWave));
+      return m;
+    };
+    const uint32_t mk = most(kx), mv = most(vx);
+    if (tid % kWave == 0) {
+      s_max[0][tid / kWave] = mk;
+      s_max[1][tid / kWave] = mv;
+    }
+    __syncthreads();
+    auto scale_of = [&](int i) {
+      return kv_scale_of(DT::tof((uint16_t)max(max(s_max[i][0], s_max[i][1]), max(s_max[i][2], s_max[i][3]))));
+    };
+    const float ks = scale_of(0), vs = scale_of(1);
+    const size_t block = pair * p.c.blocks + blk;
+    if (tid == 0) {
+      p.c.ks[block] = ks;
+      p.c.vs[block] = vs;
+    }
+    auto codes = [](u32x4 x, float inv) {  // of eight values
+      uint32_t out[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const uint32_t a = x[2 * i], c = x[2 * i + 1];
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(kv_code_of(DT::tof((uint16_t)a), inv), kv_code_of(DT::tof((uint16_t)(a >> 16)), inv), 0, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(kv_code_of(DT::tof((uint16_t)c), inv), kv_code_of(DT::tof((uint16_t)(c >> 16)), inv), w, true);
+        out[i] = (uint32_t)w;
+      }
+      return u32x2{out[0], out[1]};
+    };
+    const float ki = 1.f / ks, vi = 1.f / vs;  // powers of two
+    u32x2* k8 = (u32x2*)(p.c.k8 + block * kKvBlock * D + tok * D + d0);
+#pragma unroll
+    for (int i = 0; i < NV; i++) k8[i] = codes(kx[i], ki);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const u32x2 w = codes(vx[i], vi);
+#pragma unroll
+      for (int e = 0; e < 8; e++) s_v[d0 + 8 * i + e][tok] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
+    }
+    __syncthreads();
+    u32x4* v8 = (u32x4*)(p.c.v8 + block * kKvBlock * D);
+    for (int i = tid; i < D * 4; i += 256) {
+      const uint32_t* s = (const uint32_t*)&s_v[i / 4][i % 4 * 16];
+      v8[i] = u32x4{s[0], s[1], s[2], s[3]};
+    }
+  }
+  if (blockIdx.x != 0) return;
+  __syncthreads();  // what the tail held has been read
+  const int from = max(start, last * kKvBlock), live = end - from;  // new tokens of the last block
+  for (int i = tid; i < live * (D / 8); i += 256) {
+    const int t = i / (D / 8), d = i % (D / 8) * 8;
+    *(u32x4*)(kt + (from + t) % kKvBlock * D + d) = *(const u32x4*)(k + (from + t - start) * p.k_tok + d);
+  }
+  const int t = tid % kWave;
+  if (t < live)
+    for (int d = tid / kWave * 8; d < D; d += 32) {
+      const u32x4 x = *(const u32x4*)(v + (from + t - start) * p.v_tok + d);
+#pragma unroll
+      for (int e = 0; e < 8; e++) vt[(d + e) * kKvBlock + (from + t) % kKvBlock] = (uint16_t)(x[e / 2] >> (16 * (e & 1)));
+    }
+}
+
+// ---- attention ---------------------------------------------------------------------------------------------------------------------
+
+struct KvAttnArgs {
+  const uint16_t* q;  // (B, T, heads, D) in elements: strides of a row, a token and a head
+  long long q_row, q_tok, q_head;
+  uint16_t* out;      // (B, T, heads, D)
+  KvSpan span;
+  KvCache c;
+  float* part;        // [pair][split][row][D] sums and, behind them, [pair][split][row][2] largest exponent and sum of weights
+  float scale;        // log2(e) * the softmax's scale
+  int T, group;       // group: query heads of a cached head
+  int window;         // keys that a query sees, at most; 0: all
+  int pairs, splits;  // pairs: rows x cached heads
+};
+
+// Row r of a (row, cached head) pair is head r % group of token r / group: the queries of a step that share a cached head are one
+// operand of the matrix cores.  ROWS of them are a workgroup's; UNIT tiles of 64 tokens at a time are shared out over the splits.
+struct KvTiles {
+  int pos_lo, pos_hi;    // positions of the first and the last query
+  int tile_lo, tile_hi;  // first and last tile of 64 keys
+  int last;              // tile that is read from the tail
+  int active;            // splits that have tiles
+};
+template <int ROWS, int UNIT>
+__device__ __forceinline__ bool kv_tiles(const KvAttnArgs& p, int r0, int start, int n, KvTiles& t) {
+  const int lo = r0 / p.group, hi = min((r0 + ROWS - 1) / p.group, n - 1);
+  if (lo >= n) return false;
+  t.pos_lo = start + lo;
+  t.pos_hi = start + hi;
+  t.tile_lo = p.window ? max(0, t.pos_lo - p.window + 1) / kKvBlock : 0;
+  t.tile_hi = t.pos_hi / kKvBlock;
+  t.last = (start + n - 1) / kKvBlock;
+  t.active = min(p.splits, (t.tile_hi - t.tile_lo + UNIT) / UNIT);
+  return true;
+}
+
+__device__ __forceinline__ uint16_t* kv_out_row(const KvAttnArgs& p, int pair, int r, int D) {
+  const int b = pair / p.c.heads, h = pair - b * p.c.heads, t = r / p.group, g = r - t * p.group;
+  return p.out + (((size_t)b * p.T + t) * p.c.heads * p.group + h * p.group + g) * D;
+}
+
+// Rows behind the last query are zeros, and all rows NaN where the row's tokens do not lie in the cache.
+template <class DT>
+__device__ __forceinline__ void kv_fill_rows(const KvAttnArgs& p, int pair, int r0, int rows, int n, bool ok, int D, int tid, int threads) {
+  for (int i = tid; i < rows * (D / 8); i += threads) {
+    const int r = r0 + i / (D / 8);
+    if (r >= p.T * p.group) return;
+    const uint32_t w = ok || r / p.group >= n ? 0u : DT::fromf(NAN) * 0x10001u;
+    ((u32x4*)kv_out_row(p, pair, r, D))[i % (D / 8)] = u32x4{w, w, w, w};
+  }
+}
+
+// Sets numbers that are not finite to 0 and says where they were: `ones` has 1 (e4m3 or the type itself) there and 0 elsewhere.
+__device__ __forceinline__ uint32_t kv_fix8(uint32_t& w) {
+  const uint32_t m = (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+  w &= ~(m * 0xffu);
+  return m * 0x38u;
+}
+template <class DT>
+__device__ __forceinline__ uint32_t kv_fix16(uint32_t& w) {
+  const uint32_t lo = (w & Kv<DT>::kExp) == Kv<DT>::kExp ? 1u : 0u, hi = (w >> 16 & Kv<DT>::kExp) == Kv<DT>::kExp ? 0x10000u : 0u;
+  const uint32_t m = lo | hi;
+  w &= ~(m * 0xffffu);
+  return m * Kv<DT>::kOne;
+}
+
+// One new token, or a few: ROWS = 16 rows of queries, the cache split over workgroups and over the four waves of each, the waves' results
+// joined in LDS and the workgroups' by kv8_join_kernel.  Each wave takes 64 tokens at a time:
+//   S^T = K . Q^T   tile t, row 4 g + i of the 16x16 result: token 16 g + 4 t + i, in lanes of group g = lane / 16; columns are queries
+//   O^T += V^T . P  the weights of lane group g are those of tokens 16 g .. + 15 in order: what the lane has to supply as operand
+// so weights go from one product into the other without leaving their lane, and every load of the cache is 16 bytes a lane of 1 KiB in a
+// row (V) or of whole lines (K).  The numbers become 16-bit operands (two an instruction), the blocks' scales go into the
+// exponent: with w = s * ks * scale + log2(vs), weights are 2^(w - max w) <= 1, O sums them times the codes, and the sum of
+// weights adds them divided by vs.
+// A masked weight is 0, but 0 times a NaN is not: where a tile is seen in part, numbers of V that are not finite are taken out and the
+// rows that see one are set to NaN.
+template <class DT, int D>
+__global__ __launch_bounds__(256) void kv8_attn_step_kernel(KvAttnArgs p) {
+  constexpr int W = 4, ROWS = 16, C = D / 64, NU = D / 16, NK = D >= 64 ? C : 1;
+  typedef Kv<DT> F;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+  const int pair = blockIdx.x, split = blockIdx.y, r0 = blockIdx.z * ROWS, rows = p.T * p.group;
+  const int b = pair / p.c.heads;
+  int start, n;
+  KvTiles t;
+  const bool ok = kv_span(p.span, b, p.T, p.c.blocks, start, n);
+  if (!kv_tiles<ROWS, W>(p, r0, start, n, t) || !ok) {
+    if (split == 0) kv_fill_rows<DT>(p, pair, r0, ROWS, n, ok, D, threadIdx.x, 256);
+    return;
+  }
+  if (split >= t.active) return;
+
+  // queries: operand of step (c, v) is elements 64 c + 16 g + 8 v .. + 7 (of 32 elements: 8 g .. + 7)
+  const int row = min(r0 + m, rows - 1), tok = min(row / p.group, n - 1), pos = start + tok;
+  const uint16_t* q = p.q + b * p.q_row + (row / p.group) * p.q_tok + ((pair - b * p.c.heads) * p.group + row % p.group) * p.q_head;
+  u32x4 qf[NK][2];
+#pragma unroll
+  for (int c = 0; c < NK; c++)
+#pragma unroll
+    for (int v = 0; v < (D >= 64 ? 2 : 1); v++) qf[c][v] = *(const u32x4*)(q + (D >= 64 ? 64 * c + 16 * g + 8 * v : 8 * g));
+
+  const size_t kv = (size_t)pair;
+  const uint8_t* k8 = p.c.k8 + kv * p.c.blocks * kKvBlock * D;
+  const uint8_t* v8 = p.c.v8 + kv * p.c.blocks * kKvBlock * D;
+  const int ktok = 16 * (m >> 2) + (m & 3);  // token of this lane's row of K in tile 0; 4 more in each of the next
+
+  float top = -FLT_MAX, sum = 0.f;
+  f32x4 o[NU];
+#pragma unroll
+  for (int u = 0; u < NU; u++) o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (int tile = t.tile_lo + split * W + wave; tile <= t.tile_hi; tile += t.active * W) {
+    const bool tail = tile == t.last;
+    const int key0 = tile * kKvBlock + 16 * g;  // of this lane's weights
+    const bool part = tail || tile * kKvBlock + kKvBlock - 1 > t.pos_lo || (p.window && tile * kKvBlock <= t.pos_hi - p.window);
+    f32x4 s[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    u32x4 vv[NU];
+    float ks = 1.f, vs = 1.f;
+    if (!tail) {
+      const uint8_t* kb = k8 + (size_t)tile * kKvBlock * D;
+      const uint8_t* vb = v8 + (size_t)tile * kKvBlock * D;
+      ks = p.c.ks[kv * p.c.blocks + tile];
+      vs = p.c.vs[kv * p.c.blocks + tile];
+      if constexpr (D >= 64) {
+        u32x4 kk[4][NK];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int c = 0; c < NK; c++) kk[i][c] = load_stream((const u32x4*)(kb + (ktok + 4 * i) * D + 64 * c + 16 * g));
+#pragma unroll
+        for (int u = 0; u < NU; u++) vv[u] = load_stream((const u32x4*)(vb + (16 * u + m) * kKvBlock + 16 * g));
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int c = 0; c < NK; c++) {
+            s[i] = Mma<DT>::run(kv_wide<DT>(kk[i][c][0], kk[i][c][1]), qf[c][0], s[i]);
+            s[i] = Mma<DT>::run(kv_wide<DT>(kk[i][c][2], kk[i][c][3]), qf[c][1], s[i]);
+          }
+      } else {
+        u32x2 kk[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) kk[i] = *(const u32x2*)(kb + (ktok + 4 * i) * D + 8 * g);
+#pragma unroll
+        for (int u = 0; u < NU; u++) vv[u] = load_stream((const u32x4*)(vb + (16 * u + m) * kKvBlock + 16 * g));
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] = Mma<DT>::run(kv_wide<DT>(kk[i][0], kk[i][1]), qf[0][0], s[i]);
+      }
+    } else {
+      const uint16_t* kb = p.c.kt + kv * kKvBlock * D;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int c = 0; c < NK; c++)
+#pragma unroll
+          for (int v = 0; v < (D >= 64 ? 2 : 1); v++)
+            s[i] = Mma<DT>::run(*(const u32x4*)(kb + (ktok + 4 * i) * D + (D >= 64 ? 64 * c + 16 * g + 8 * v : 8 * g)), qf[c][v], s[i]);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[i][e] = fmaf(s[i][e], 0.f, s[i][e]);  // a key that is not finite makes the score NaN, as in e4m3
+    }
+    if (part) {
+      const int first = p.window ? pos - p.window : -1;  // the query sees first + 1 .. pos
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int key = key0 + 4 * i + e;
+          s[i][e] = key <= pos && key > first ? s[i][e] : -INFINITY;
+        }
+    }
+    const float sc = p.scale * ks, lv = __builtin_amdgcn_logf(vs);
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[i][e]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+    const float now = fmaxf(top, fmaf(mx, sc, lv)), keep = __builtin_amdgcn_exp2f(top - now), off = lv + F::HEAD - now;
+    top = now;
+    float add = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], sc, off));
+        add += s[i][e];
+      }
+    sum = fmaf(sum, keep, add * __builtin_amdgcn_rcpf(vs));
+    u32x4 pf[2];  // the weights, rounded to the type the products take: half a step each, independent of one another
+#pragma unroll
+    for (int v = 0; v < 2; v++)
+      pf[v] = u32x4{DT::pack(s[2 * v][0], s[2 * v][1]), DT::pack(s[2 * v][2], s[2 * v][3]), DT::pack(s[2 * v + 1][0], s[2 * v + 1][1]),
+                    DT::pack(s[2 * v + 1][2], s[2 * v + 1][3])};
+#pragma unroll
+    for (int u = 0; u < NU; u++) o[u] *= keep;
+    if (!part) {
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
+        o[u] = Mma<DT>::run(kv_wide<DT>(vv[u][0], vv[u][1]), pf[0], o[u]);
+        o[u] = Mma<DT>::run(kv_wide<DT>(vv[u][2], vv[u][3]), pf[1], o[u]);
+      }
+    } else {
+      u32x4 seen[2];  // 1 where the query sees the key
+      const int first = p.window ? pos - p.window : -1;
+      auto one = [&](int j) { return key0 + j <= pos && key0 + j > first ? Kv<DT>::kOne : 0u; };
+#pragma unroll
+      for (int v = 0; v < 2; v++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) seen[v][e] = one(8 * v + 2 * e) | one(8 * v + 2 * e + 1) << 16;
+      const uint16_t* vb = p.c.vt + kv * kKvBlock * D;
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
+        u32x4 a[2], bad[2];
+        if (tail) {
+#pragma unroll
+          for (int v = 0; v < 2; v++) {
+            a[v] = *(const u32x4*)(vb + (16 * u + m) * kKvBlock + 16 * g + 8 * v);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              uint32_t w = a[v][e];
+              bad[v][e] = kv_fix16<DT>(w);
+              a[v][e] = w;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int v = 0; v < 2; v++) {
+            uint32_t w0 = vv[u][2 * v], w1 = vv[u][2 * v + 1];
+            const uint32_t b0 = kv_fix8(w0), b1 = kv_fix8(w1);
+            a[v] = kv_wide<DT>(w0, w1);
+            bad[v] = kv_wide<DT>(b0, b1);
+          }
+        }
+        f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < 2; v++) {
+          o[u] = Mma<DT>::run(a[v], pf[v], o[u]);
+          z = Mma<DT>::run(bad[v], seen[v], z);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[u][e] = z[e] > 0.f ? NAN : o[u][e];
+      }
+    }
+  }
+  sum += __shfl_xor(sum, 16, kWave);
+  sum += __shfl_xor(sum, 32, kWave);
+
+  // the four waves' results
+  __shared__ __align__(16) float s_o[W][ROWS][D + 4];
+  __shared__ float s_top[W][ROWS], s_sum[W][ROWS];
+#pragma unroll
+  for (int u = 0; u < NU; u++) *(f32x4*)&s_o[wave][m][16 * u + 4 * g] = o[u];
+  if (g == 0) {
+    s_top[wave][m] = top;
+    s_sum[wave][m] = sum;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < ROWS * (D / 4); i += 256) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    if (r0 + r >= rows) break;
+    float most = s_top[0][r];
+#pragma unroll
+    for (int w = 1; w < W; w++) most = fmaxf(most, s_top[w][r]);
+    f32x4 num = f32x4{0.f, 0.f, 0.f, 0.f};
+    float den = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+      const float f = __builtin_amdgcn_exp2f(s_top[w][r] - most);
+      const f32x4 x = *(const f32x4*)&s_o[w][r][d];
+#pragma unroll
+      for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e]);
+      den = fmaf(f, s_sum[w][r], den);
+    }
+    if (t.active == 1) {
+      const bool dead = (r0 + r) / p.group >= n;
+#pragma unroll
+      for (int e = 0; e < 4; e++) num[e] = dead ? 0.f : num[e] / den;
+      *(u32x2*)(kv_out_row(p, pair, r0 + r, D) + d) = u32x2{DT::pack(num[0], num[1]), DT::pack(num[2], num[3])};
+    } else {
+      const size_t at = ((size_t)pair * p.splits + split) * rows + r0 + r;
+      *(f32x4*)(p.part + at * D + d) = num;
+      if (d == 0) {
+        float* ml = p.part + (size_t)p.pairs * p.splits * rows * D + 2 * at;
+        ml[0] = most;
+        ml[1] = den;
+      }
+    }
+  }
+}
+
+// The splits' results, in a fixed order.  A workgroup per (pair, 16 rows); rows whose cache was one split's are done already.
+template <class DT, int D, int ROWS, int UNIT>
+__global__ __launch_bounds__(256) void kv8_join_kernel(KvAttnArgs p) {
+  const int pair = blockIdx.x, rows = p.T * p.group, j0 = blockIdx.y * 16;
+  int start, n;
+  KvTiles t;
+  if (!kv_span(p.span, pair / p.c.heads, p.T, p.c.blocks, start, n) || !kv_tiles<ROWS, UNIT>(p, j0 / ROWS * ROWS, start, n, t) || t.active == 1) return;
+  const float* ml = p.part + (size_t)p.pairs * p.splits * rows * D;
+  for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
+    const int r = j0 + i / (D / 4), d = i % (D / 4) * 4;
+    if (r >= rows) return;
+    const size_t at = (size_t)pair * p.splits * rows + r;
+    float most = -FLT_MAX;
+    for (int s = 0; s < t.active; s++) most = fmaxf(most, ml[2 * (at + (size_t)s * rows)]);
+    f32x4 num = f32x4{0.f, 0.f, 0.f, 0.f};
+    float den = 0.f;
+    for (int s = 0; s < t.active; s++) {
+      const size_t a = at + (size_t)s * rows;
+      const float f = __builtin_amdgcn_exp2f(ml[2 * a] - most);
+      const f32x4 x = *(const f32x4*)(p.part + a * D + d);
+#pragma unroll
+      for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e]);
+      den = fmaf(f, ml[2 * a + 1], den);
+    }
+    const bool dead = r / p.group >= n;
+#pragma unroll
+    for (int e = 0; e < 4; e++) num[e] = dead ? 0.f : num[e] / den;
+    *(u32x2*)(kv_out_row(p, pair, r, D) + d) = u32x2{DT::pack(num[0], num[1]), DT::pack(num[2], num[3])};
+  }
+}
+
+}  // namespace cats

@@ -570,6 +570,168 @@ at::Tensor cats_prompt_mlp_op(const at::Tensor& x, const at::Tensor& w_gate, con
   return y;
 }
 
+// ---- the cache in 8 bits and beam search ------------------------------------------------------------------
+
+// k, v or q (B, T, heads, D) with elements of a head side by side and every head on a 16-byte boundary; anything else is copied.
+at::Tensor tokens_of(const at::Tensor& t) {
+  bool fits = t.stride(3) == 1 && ((uintptr_t)t.data_ptr() & 15u) == 0;
+  for (int i = 0; i < 3; i++) fits = fits && (t.size(i) == 1 || (t.stride(i) >= 0 && t.stride(i) % 8 == 0));
+  return fits ? t : t.contiguous();
+}
+struct Strides {
+  int64_t s[3];
+  explicit Strides(const at::Tensor& t) {
+    for (int i = 0; i < 3; i++) s[i] = t.size(i) == 1 ? 0 : t.stride(i);
+  }
+};
+
+// start or count: one int64 for all rows or one for each.
+const int64_t* words_of(const at::Tensor& t, const at::Tensor& like, int64_t rows, const char* name, const char* op, int& step) {
+  check_dev(t, name);
+  TORCH_CHECK(t.scalar_type() == at::kLong && t.device() == like.device() && (t.numel() == 1 || (t.dim() == 1 && t.numel() == rows)), "flash_gemv.",
+              op, ": ", name, " must be one int64 or one for each of the ", rows, " rows, on the caches' device");
+  step = t.numel() == 1 ? 0 : 1;
+  return t.data_ptr<int64_t>();
+}
+
+struct Kv8 {
+  int64_t B, heads, blocks, D;
+};
+// `like` is k or q: (B, T, ., D) in the model's type
+Kv8 check_kv8(const at::Tensor& like, const at::Tensor& k8, const at::Tensor& v8, const at::Tensor& k_scale, const at::Tensor& v_scale,
+              const at::Tensor& k_tail, const at::Tensor& v_tail, const char* op) {
+  TORCH_CHECK(like.is_cuda(), "flash_gemv.", op, ": the tensors must be on the GPU");
+  TORCH_CHECK(like.dim() == 4, "flash_gemv.", op, ": new tokens must be (B, T, heads, D), got ", like.sizes());
+  TORCH_CHECK(like.scalar_type() == at::kHalf || like.scalar_type() == at::kBFloat16, "flash_gemv.", op, ": half or bfloat16, got ", like.scalar_type());
+  TORCH_CHECK(k8.dim() == 5, "flash_gemv.", op, ": k8 must be (B, kv_heads, blocks, 64, D), got ", k8.sizes());
+  const Kv8 c = {like.size(0), k8.size(1), k8.size(2), like.size(3)};
+  TORCH_CHECK(c.D == 32 || c.D == 64 || c.D == 128 || c.D == 256, "flash_gemv.", op, ": heads of 32, 64, 128 or 256 elements, got ", c.D);
+  auto is = [&](const at::Tensor& t, at::IntArrayRef shape, at::ScalarType type, const char* name) {
+    check_dev(t, name);
+    TORCH_CHECK(t.sizes() == shape && t.scalar_type() == type && t.device() == like.device(), "flash_gemv.", op, ": ", name, " must be ", shape, " of ", type,
+                " on the device of the new tokens, got ", t.sizes(), " of ", t.scalar_type());
+  };
+  is(k8, {c.B, c.heads, c.blocks, 64, c.D}, at::kFloat8_e4m3fn, "k8");
+  is(v8, {c.B, c.heads, c.blocks, c.D, 64}, at::kFloat8_e4m3fn, "v8");
+  is(k_scale, {c.B, c.heads, c.blocks}, at::kFloat, "k_scale");
+  is(v_scale, {c.B, c.heads, c.blocks}, at::kFloat, "v_scale");
+  is(k_tail, {c.B, c.heads, 64, c.D}, like.scalar_type(), "k_tail");
+  is(v_tail, {c.B, c.heads, c.D, 64}, like.scalar_type(), "v_tail");
+  TORCH_CHECK(c.B <= INT_MAX && c.heads <= INT_MAX && c.blocks <= INT_MAX && like.size(1) <= INT_MAX, "flash_gemv.", op, ": too large");
+  return c;
+}
+
+void cats_kv8_append_op(const at::Tensor& k, const at::Tensor& v, const at::Tensor& start, const c10::optional<at::Tensor>& count, at::Tensor& k8,
+                        at::Tensor& v8, at::Tensor& k_scale, at::Tensor& v_scale, at::Tensor& k_tail, at::Tensor& v_tail) {
+  const Kv8 c = check_kv8(k, k8, v8, k_scale, v_scale, k_tail, v_tail, "cats_kv8_append");
+  TORCH_CHECK(k.size(2) == c.heads && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(),
+              "flash_gemv.cats_kv8_append: k and v must be alike, (B, T, kv_heads, D)");
+  int ss = 0, cs = 0;
+  const int64_t* sp = words_of(start, k, c.B, "start", "cats_kv8_append", ss);
+  const int64_t* cp = count.has_value() && count->defined() ? words_of(*count, k, c.B, "count", "cats_kv8_append", cs) : nullptr;
+  if (k.numel() == 0) return;
+  const c10::DeviceGuard guard(k.device());
+  const at::Tensor kk = tokens_of(k), vv = tokens_of(v);
+  check_status(cats_kv8_append(kk.data_ptr(), Strides(kk).s, vv.data_ptr(), Strides(vv).s, sp, ss, cp, cs, k8.data_ptr(), v8.data_ptr(),
+                               k_scale.data_ptr<float>(), v_scale.data_ptr<float>(), k_tail.data_ptr(), v_tail.data_ptr(), (int)c.B, (int)k.size(1),
+                               (int)c.heads, (int)c.D, (int)c.blocks, dtype_code(k), current_stream(k)),
+               "cats_kv8_append");
+}
+
+at::Tensor cats_kv8_attention_op(const at::Tensor& q, const at::Tensor& start, const c10::optional<at::Tensor>& count, const at::Tensor& k8,
+                                 const at::Tensor& v8, const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& k_tail,
+                                 const at::Tensor& v_tail, const double scale, const int64_t window) {
+  const Kv8 c = check_kv8(q, k8, v8, k_scale, v_scale, k_tail, v_tail, "cats_kv8_attention");
+  const int64_t T = q.size(1), heads = q.size(2);
+  TORCH_CHECK(c.heads >= 1 && heads % c.heads == 0, "flash_gemv.cats_kv8_attention: ", heads, " query heads over ", c.heads, " cached heads");
+  TORCH_CHECK(window >= 0 && window <= INT_MAX, "flash_gemv.cats_kv8_attention: window must be 0 (all keys) or a number of keys");
+  int ss = 0, cs = 0;
+  const int64_t* sp = words_of(start, q, c.B, "start", "cats_kv8_attention", ss);
+  const int64_t* cp = count.has_value() && count->defined() ? words_of(*count, q, c.B, "count", "cats_kv8_attention", cs) : nullptr;
+  const c10::DeviceGuard guard(q.device());
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  if (q.numel() == 0) return out;
+  const at::Tensor qq = tokens_of(q);
+  const size_t bytes = cats_kv8_attention_scratch_bytes((int)c.B, (int)T, (int)heads, (int)c.heads, (int)c.D, (int)c.blocks, (int)window);
+  at::Tensor scratch;
+  if (bytes) scratch = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  check_status(cats_kv8_attention(qq.data_ptr(), Strides(qq).s, sp, ss, cp, cs, k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr<float>(),
+                                  v_scale.data_ptr<float>(), k_tail.data_ptr(), v_tail.data_ptr(), (float)scale, (int)window, out.data_ptr(), (int)c.B,
+                                  (int)T, (int)heads, (int)c.heads, (int)c.D, (int)c.blocks, dtype_code(q), bytes ? scratch.data_ptr() : nullptr, bytes,
+                                  current_stream(q)),
+               "cats_kv8_attention");
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> cats_beam_select_op(const at::Tensor& logits, const at::Tensor& scores,
+                                                                               const c10::optional<at::Tensor>& finished, const int64_t eos,
+                                                                               const int64_t keep) {
+  TORCH_CHECK(logits.is_cuda(), "flash_gemv.cats_beam_select: logits must be on the GPU");
+  TORCH_CHECK(logits.dim() == 3, "flash_gemv.cats_beam_select: logits must be (groups, beams, V), got ", logits.sizes());
+  const int64_t G = logits.size(0), n = logits.size(1), V = logits.size(2), K = keep > 0 ? keep : n;
+  check_dev(scores, "scores");
+  TORCH_CHECK(scores.scalar_type() == at::kFloat && scores.dim() == 2 && scores.size(0) == G && scores.size(1) == n && scores.device() == logits.device(),
+              "flash_gemv.cats_beam_select: scores must be (groups, beams) of float on the device of the logits");
+  const bool ends = finished.has_value() && finished->defined();
+  if (ends) {
+    check_dev(*finished, "finished");
+    TORCH_CHECK(finished->scalar_type() == at::kBool && finished->sizes() == scores.sizes() && finished->device() == logits.device(),
+                "flash_gemv.cats_beam_select: finished must be (groups, beams) of bool on the device of the logits");
+    TORCH_CHECK(eos >= 0, "flash_gemv.cats_beam_select: beams that have finished need eos");
+  }
+  TORCH_CHECK(n >= 1 && n <= CATS_MAX_BEAMS && K <= CATS_MAX_BEAMS && V >= 1 && K <= n * V, "flash_gemv.cats_beam_select: 1..", CATS_MAX_BEAMS,
+              " beams, and no more than there are continuations");
+  TORCH_CHECK(eos < V && V <= 1 << 30, "flash_gemv.cats_beam_select: eos ", eos, " is no word of ", V);
+  TORCH_CHECK(keep >= 0, "flash_gemv.cats_beam_select: keep must be 0 (as many as there are beams) or a number of beams");
+  const c10::DeviceGuard guard(logits.device());
+  auto out = [&](at::ScalarType type) { return at::empty({G, K}, logits.options().dtype(type)); };
+  at::Tensor best = out(at::kFloat), parents = out(at::kLong), tokens = out(at::kLong), done = out(at::kBool);
+  if (G == 0) return {best, parents, tokens, done};
+  TORCH_CHECK(G <= 65535 / n, "flash_gemv.cats_beam_select: at most 65535 beams in all");
+  // rows that follow one another at one distance are read where they are (the last position of (rows, T, V) logits, say)
+  const bool rows = logits.stride(2) == 1 && (G == 1 || n == 1 || logits.stride(0) == n * logits.stride(1));
+  const at::Tensor x = rows ? logits : logits.contiguous();
+  const int64_t pitch = n > 1 ? x.stride(1) : x.stride(0);
+  const size_t bytes = cats_beam_scratch_bytes((int)G, (int)n, (int)V, (int)K);
+  at::Tensor scratch = at::empty({(int64_t)bytes}, logits.options().dtype(at::kByte));
+  check_status(cats_beam_select(x.data_ptr(), G * n > 1 ? pitch : 0, scores.data_ptr<float>(), ends ? (const uint8_t*)finished->data_ptr() : nullptr, eos,
+                                best.data_ptr<float>(), parents.data_ptr<int64_t>(), tokens.data_ptr<int64_t>(), (uint8_t*)done.data_ptr(), (int)G, (int)n,
+                                (int)V, (int)K, dtype_code(x), scratch.data_ptr(), bytes, current_stream(logits)),
+               "cats_beam_select");
+  return {best, parents, tokens, done};
+}
+
+void cats_cache_reorder_op(const at::TensorList caches, const at::IntArrayRef slots, const at::Tensor& parents, const c10::optional<at::Tensor>& lengths) {
+  check_dev(parents, "parents");
+  TORCH_CHECK(parents.scalar_type() == at::kLong && parents.dim() == 2, "flash_gemv.cats_cache_reorder: parents must be (groups, beams) of int64");
+  const int64_t G = parents.size(0), n = parents.size(1);
+  TORCH_CHECK(n >= 1 && n <= CATS_MAX_BEAMS && G <= 65535, "flash_gemv.cats_cache_reorder: 1..", CATS_MAX_BEAMS, " beams a group");
+  TORCH_CHECK(caches.size() == slots.size() && !caches.empty(), "flash_gemv.cats_cache_reorder: one number of slots for each cache");
+  int step = 0;
+  const int64_t* lp = lengths.has_value() && lengths->defined() ? words_of(*lengths, parents, G * n, "lengths", "cats_cache_reorder", step) : nullptr;
+  std::vector<cats_cache_t> list;
+  for (size_t i = 0; i < caches.size(); i++) {
+    const at::Tensor& c = caches[i];
+    check_dev(c, "a cache");
+    TORCH_CHECK(c.dim() >= 3 && c.size(0) == G * n && c.device() == parents.device(), "flash_gemv.cats_cache_reorder: a cache must be (groups * beams, heads, entries, ...) on the device of the parents, got ", c.sizes());
+    TORCH_CHECK(slots[i] >= 0 && slots[i] <= INT_MAX && (slots[i] == 0 || lp), "flash_gemv.cats_cache_reorder: slots are 0 (all entries) or the tokens an entry holds, which need lengths");
+    if (c.numel() == 0) continue;
+    TORCH_CHECK(c.size(1) <= INT_MAX && c.size(2) <= INT_MAX, "flash_gemv.cats_cache_reorder: too large");
+    cats_cache_t d;
+    d.data = c.data_ptr();
+    d.entry_bytes = c.numel() / (c.size(0) * c.size(1) * c.size(2)) * (int64_t)c.element_size();
+    d.heads = (int)c.size(1);
+    d.entries = (int)c.size(2);
+    d.slots = (int)slots[i];
+    TORCH_CHECK(d.entry_bytes % 4 == 0, "flash_gemv.cats_cache_reorder: entries of a multiple of 4 bytes, got ", d.entry_bytes);
+    list.push_back(d);
+  }
+  if (list.empty() || G == 0) return;
+  const c10::DeviceGuard guard(parents.device());
+  check_status(cats_cache_reorder(list.data(), (int)list.size(), parents.data_ptr<int64_t>(), lp, step, (int)G, (int)n, current_stream(parents)),
+               "cats_cache_reorder");
+}
+
 }  // namespace
 
 TORCH_LIBRARY(flash_gemv, m) {
@@ -603,4 +765,10 @@ TORCH_LIBRARY(flash_gemv, m) {
   m.def("cats_silu_mask_mul", cats_silu_mask_mul_op);
   m.def("cats_prompt_mlp", cats_prompt_mlp_op);
   m.def("cats_attention_step", cats_attention_step_op);
+  // a cache in 8 bits, beam search
+  m.def("cats_kv8_append(Tensor k, Tensor v, Tensor start, Tensor? count, Tensor(a!) k8, Tensor(b!) v8, Tensor(c!) k_scale, Tensor(d!) v_scale, "
+        "Tensor(e!) k_tail, Tensor(f!) v_tail) -> ()", cats_kv8_append_op);
+  m.def("cats_kv8_attention", cats_kv8_attention_op);
+  m.def("cats_beam_select", cats_beam_select_op);
+  m.def("cats_cache_reorder(Tensor(a!)[] caches, int[] slots, Tensor parents, Tensor? lengths) -> ()", cats_cache_reorder_op);
 }

@@ -246,6 +246,63 @@ int cats_attention_step(const void* h, const void* x, const void* norm_weight, f
                         const int64_t* position, float* q_scratch, void* attn_scratch, void* out, int B, int H, int heads,
                         int max_len, int dtype, void* stream);
 
+/* ---- a cache of keys and values in 8 bits (fp16 / bf16 models) ----
+ * A row has `blocks` blocks of 64 tokens.  A block that is complete is held as e4m3 numbers, with one power of two as scale for a head's keys
+ * and one for its values: the smallest s with max |x| <= 448 s over the block's finite values (at least 2^-60; 1 for zeros); each value is x / s,
+ * rounded to nearest even, NaN if it is not finite.  The block that holds a row's last token, complete or not, is read as it was given.
+ *   k8 (B, kv_heads, blocks, 64, D)   v8 (B, kv_heads, blocks, D, 64)   e4m3, one byte a number
+ *   k_scale, v_scale (B, kv_heads, blocks) float       k_tail (B, kv_heads, 64, D)   v_tail (B, kv_heads, D, 64) in dtype, slot = position % 64
+ * D is 32, 64, 128 or 256.  k, v and q: strides of a row, a token and a head, in elements, multiples of 8; the elements of a head side by side.
+ * start, count: device words, one for each row (step 1) or one for all (step 0).  Row b has min(max(count, 0), T) new tokens (count NULL: T), at
+ * positions start .. start + count - 1.  Both calls may be captured; nothing is kept between calls. */
+#define CATS_KV8_MAX_BLOCKS (1 << 24)
+
+/* Stores the new tokens: quantises the blocks that they complete and leaves the last block in the tails.  What a row holds already has to end at
+ * start (a block's tokens before start are taken from the tails).  So the cache is the same whatever pieces the tokens come in.  A row whose
+ * tokens do not lie within its blocks is left as it is. */
+int cats_kv8_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, const int64_t* start, int start_step,
+                    const int64_t* count, int count_step, void* k8, void* v8, float* k_scale, float* v_scale, void* k_tail, void* v_tail, int B,
+                    int T, int kv_heads, int D, int blocks, int dtype, void* stream);
+
+/* out[b, i, h] = softmax(scale * q[b, i, h] . K^T) . V over the keys at positions p - window + 1 .. p (window 0: 0 .. p), p = start + i, of cached
+ * head h / (heads / kv_heads), for new tokens that cats_kv8_append has stored.  Rows i >= count are zeros; a row whose tokens do not lie within
+ * its blocks is NaN.  A query that sees a key or an element of a value that is not finite is NaN (in that element).  out (B, T, heads, D) in
+ * dtype, 16-byte aligned.  scale > 0.  scratch: 16-byte aligned, at least cats_kv8_attention_scratch_bytes() on the device of the call
+ * (which may be 0), nothing in it needs to be set.  The reference's attention is that of the models it patches
+ * (experiments/models/sparse_mistral/sparse_silu.py:756-832), over a cache in the model's type. */
+size_t cats_kv8_attention_scratch_bytes(int B, int T, int heads, int kv_heads, int D, int blocks, int window);
+int cats_kv8_attention(const void* q, const int64_t* q_strides, const int64_t* start, int start_step, const int64_t* count, int count_step,
+                       const void* k8, const void* v8, const float* k_scale, const float* v_scale, const void* k_tail, const void* v_tail,
+                       float scale, int window, void* out, int B, int T, int heads, int kv_heads, int D, int blocks, int dtype, void* scratch,
+                       size_t scratch_bytes, void* stream);
+
+/* ---- beam search ---- */
+#define CATS_MAX_BEAMS 16
+
+/* The best `keep` continuations of each group of beams:  total(b, v) = scores[b] + logits[b, v] - log sum exp(logits[b, :]), in descending
+ * order, equal ones by the lowest b * V + v.  logits (groups, beams, V) in dtype (fp32 too), rows row_stride elements apart; scores (groups, beams)
+ * float.  finished (groups, beams) bytes, optional: a beam that has finished goes on only as (b, eos) with its score.  Totals that are not finite
+ * count as -infinity (so beams with a score of -infinity take no part).  Outputs (groups, keep): scores, parents (b), tokens (v), and whether a
+ * beam has finished (its parent had, or v is eos; eos < 0: none).  Beams are ordered by their logits within a row and by totals in 64 bits between
+ * rows.  keep <= beams * V; both up to CATS_MAX_BEAMS.  scratch: 16-byte aligned, at least cats_beam_scratch_bytes(), nothing in it needs to be set. */
+size_t cats_beam_scratch_bytes(int groups, int beams, int V, int keep);
+int cats_beam_select(const void* logits, int64_t row_stride, const float* scores, const uint8_t* finished, int64_t eos, float* scores_out,
+                     int64_t* parents_out, int64_t* tokens_out, uint8_t* finished_out, int groups, int beams, int V, int keep, int dtype,
+                     void* scratch, size_t scratch_bytes, void* stream);
+
+/* Caches moved to the beams that go on, in place: row g * beams + j becomes what row g * beams + parents[g][j] was, in the entries that are live,
+ * for each of the n caches.  A cache is (groups * beams, heads, entries) of entry_bytes (a multiple of 4; 16 is faster, on 16-byte boundaries);
+ * an entry holds `slots` tokens, and ceil(length / slots) of them are live (slots 0: all are), length being lengths[row of the parent] (step 1) or
+ * lengths[0] (step 0).  What is not live stays as it is, and so does a beam whose parent is not within its group.  The caches may not overlap.
+ * The array of descriptions is read before the call returns. */
+typedef struct {
+  void* data;
+  int64_t entry_bytes;
+  int heads, entries, slots;
+} cats_cache_t;
+int cats_cache_reorder(const cats_cache_t* caches, int n, const int64_t* parents, const int64_t* lengths, int lengths_step, int groups,
+                       int beams, void* stream);
+
 /* z = SiLU(gate) * up over n elements, 0 where |SiLU(gate)| <= threshold; a NaN is kept.  What stands between the matrix products of a
  * prompt in the reference's dense branch (experiments/models/sparse_silu/ugly_utils.py:895-904), with its roundings. */
 int cats_silu_mask_mul(const void* gate, const void* up, void* z, size_t n, int dtype, float threshold, void* stream);

@@ -1,0 +1,312 @@
+"""The cache in 8 bits: what is stored, to the bit, and attention over it, against plain implementations in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from tests import cache_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def _args(cache):
+    return [cache[f] for f in ref.FIELDS]
+
+
+def _words(v):
+    return None if v is None else torch.tensor(v, device="cuda")
+
+
+def _append(cache, k, v, start, count=None):
+    import flash_gemv
+
+    flash_gemv.cats_kv8_append(k, v, _words(start), _words(count), *_args(cache))
+
+
+def _attention(cache, q, start, count=None, scale=None, window=0):
+    import flash_gemv
+
+    return flash_gemv.cats_kv8_attention(q, _words(start), _words(count), *_args(cache), q.shape[-1] ** -0.5 if scale is None else scale, window)
+
+
+def _tokens(g, B, T, heads, D, dtype, spread=0.5):
+    return (torch.randn(B, T, heads, D, generator=g) * torch.exp(spread * torch.randn(heads, D, generator=g))).to(dtype)
+
+
+def _filled(g, B, heads, blocks, D, dtype, lengths):
+    """A cache on the CPU that holds `lengths` tokens a row, NaN behind them."""
+    cache = ref.new_cache(B, heads, blocks, D, dtype)
+    T = max(lengths)
+    return ref.append(cache, _tokens(g, B, T, heads, D, dtype), _tokens(g, B, T, heads, D, dtype), [0] * B, lengths)
+
+
+# ---- storing ----
+
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("pieces", [
+    [[1, 1]], [[63, 64]], [[65, 1], [1, 64], [1, 1]], [[130, 200], [62, 56], [1, 1], [64, 64]], [[0, 5], [-3, 59], [1, 0]], [[256, 1]]])
+def test_append_in_pieces(D, dtype, pieces):
+    """Row by row: blocks that are completed, blocks that are not, tokens that a piece of one row has and another's has not, counts of 0 and
+    below; every byte that is not written stays."""
+    g = torch.Generator().manual_seed(D + len(pieces))
+    B, heads, blocks = 2, 3, 5
+    want = ref.new_cache(B, heads, blocks, D, dtype)
+    got = ref.to(want, "cuda")
+    at = [0, 0]
+    for counts in pieces:
+        T = max(max(counts), 1)
+        k, v = _tokens(g, B, T, heads, D, dtype), _tokens(g, B, T, heads, D, dtype)
+        want = ref.append(want, k, v, at, counts)
+        _append(got, k.cuda(), v.cuda(), at, counts)
+        for f in ref.FIELDS:
+            assert ref.same(got[f], want[f]), (f, counts)
+        at = [a + max(c, 0) for a, c in zip(at, counts)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_append_gives_the_same_whatever_the_pieces(dtype):
+    g = torch.Generator().manual_seed(1)
+    k, v = _tokens(g, 1, 300, 2, 64, dtype).cuda(), _tokens(g, 1, 300, 2, 64, dtype).cuda()
+    caches = []
+    for step in (300, 1, 37, 64, 128):
+        c = ref.new_cache(1, 2, 5, 64, dtype, fill=0.0, device="cuda")
+        for at in range(0, 300, step):
+            _append(c, k[:, at:at + step], v[:, at:at + step], [at])
+        caches.append(c)
+    last = 300 // 64 * 64
+    for c in caches[1:]:
+        for f in ref.FIELDS:
+            a, b = c[f].cpu().float(), caches[0][f].cpu().float()
+            if f == "k_tail":
+                a, b = a[:, :, : 300 - last], b[:, :, : 300 - last]
+            if f == "v_tail":
+                a, b = a[..., : 300 - last], b[..., : 300 - last]
+            assert torch.equal(a, b), f
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_append_values_at_the_edges(dtype):
+    """Zeros, the largest and the smallest numbers, maxima on a power of two and on 448 times one, one step above it, ties between two
+    e4m3 numbers, infinities and NaN."""
+    tiny, big = torch.finfo(dtype).smallest_normal, torch.finfo(dtype).max
+    above = 448 * (1 + torch.finfo(dtype).eps)
+    rows = [torch.zeros(64, 64), torch.full((64, 64), big), torch.full((64, 64), tiny), torch.linspace(-448, 448, 64 * 64).view(64, 64),
+            torch.linspace(-1, 1, 64 * 64).view(64, 64) * above, torch.linspace(0, 2, 64 * 64).view(64, 64), torch.arange(64 * 64).view(64, 64) / 16.0 % 36]
+    odd = torch.randn(64, 64, generator=torch.Generator().manual_seed(3))
+    odd[3, 5], odd[9, 5], odd[63, 63] = math.inf, -math.inf, math.nan
+    rows += [odd, torch.full((64, 64), math.nan), torch.full((64, 64), tiny / 8), torch.full((64, 64), 2.0 ** -62)]
+    k = torch.stack(rows).to(dtype)[:, :, None].contiguous()  # (rows, 64, 1, 64)
+    v = -k.flip(0)
+    want = ref.append(ref.new_cache(len(rows), 1, 2, 64, dtype), k, v, [0] * len(rows), None)
+    got = ref.new_cache(len(rows), 1, 2, 64, dtype, device="cuda")
+    _append(got, k.cuda(), v.cuda(), [0])
+    for f in ref.FIELDS:
+        assert ref.same(got[f], want[f]), f
+
+
+def test_append_outside_the_cache_leaves_it():
+    g = torch.Generator().manual_seed(2)
+    k = _tokens(g, 4, 3, 1, 64, F16).cuda()
+    c = ref.new_cache(4, 1, 1, 64, F16, fill=1.0, device="cuda")
+    before = {f: t.clone() for f, t in c.items()}
+    _append(c, k, k, [-1, 62, 64, 1 << 40])
+    for f in ref.FIELDS:
+        assert ref.same(c[f], before[f]), f
+    _append(c, k, k, [61])  # just inside
+    assert ref.same(c["k_tail"][:, 0, 61:], k[:, :, 0])
+
+
+def test_append_strides():
+    """Tokens as a projection leaves them, heads in front of tokens, every second head, and elements that no vector reads."""
+    g = torch.Generator().manual_seed(4)
+    base = _tokens(g, 2, 70, 6, 64, BF16).cuda()
+    want = ref.append(ref.new_cache(2, 3, 2, 64, BF16), base[:, :, ::2].cpu(), base[:, :, 1::2].cpu(), [0, 0], None)
+    fronted = base.transpose(1, 2).contiguous().transpose(1, 2)
+    odd = torch.empty(2, 70, 6, 65, dtype=BF16, device="cuda")
+    odd[..., 1:] = base
+    reversed_elements = base.flip(-1).contiguous()
+    for x in (base, fronted, odd[..., 1:], torch.empty(2, 70, 6, 128, dtype=BF16, device="cuda")[..., ::2].copy_(base)):
+        c = ref.new_cache(2, 3, 2, 64, BF16, device="cuda")
+        _append(c, x[:, :, ::2], x[:, :, 1::2], [0])
+        for f in ref.FIELDS:
+            assert ref.same(c[f], want[f]), f
+    assert not torch.equal(reversed_elements, base)
+
+
+# ---- attention ----
+
+def _check(B, T, heads, kv, D, dtype, lengths, blocks, window=0, count=None, seed=0, scale=None):
+    """lengths: tokens of each row with the new ones."""
+    g = torch.Generator().manual_seed(seed + D + T)
+    cache = _filled(g, B, kv, blocks, D, dtype, lengths)
+    q = (torch.randn(B, T, heads, D, generator=g) * 1.5).to(dtype)
+    n = [T] * B if count is None else [min(max(c, 0), T) for c in count]
+    start = [a - c for a, c in zip(lengths, n)]
+    out = _attention(ref.to(cache, "cuda"), q.cuda(), start, count, scale, window)
+    want, bound = ref.attention(cache, q, start, count, D ** -0.5 if scale is None else scale, window)
+    assert out.dtype == dtype and out.shape == q.shape
+    worst = float(((out.cpu().double() - want).abs() / bound.clamp_min(1e-30)).nan_to_num().max())
+    assert ref.within(out, want, bound), worst
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("length", [1, 2, 63, 64, 65, 128, 129, 300])
+def test_attention_of_one_token(D, length, dtype):
+    _check(1, 1, 2, 2, D, dtype, [length], 6)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,kv", [(1, 1), (4, 1), (6, 2), (7, 1), (8, 1), (16, 1), (17, 1), (34, 2)])
+def test_attention_of_grouped_heads(heads, kv, dtype):
+    _check(2, 1, heads, kv, 64, dtype, [200, 77], 4)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("T,heads,kv,lengths,window", [
+    (2, 3, 1, [2, 65], 0), (5, 14, 2, [130, 66], 0), (5, 14, 2, [130, 260], 70), (16, 1, 1, [16, 79], 0), (17, 1, 1, [64, 100], 0), (33, 2, 1, [33, 150], 20),
+    (64, 1, 1, [64, 192], 0), (100, 3, 3, [100, 228], 64), (130, 2, 1, [130, 300], 1), (3, 4, 4, [300, 129], 129), (1, 4, 2, [300, 257], 128), (1, 4, 2, [300, 257], 1),
+    (1, 4, 2, [300, 257], 1000)])
+def test_attention_of_several_tokens(T, heads, kv, lengths, window, dtype):
+    """Queries of one call that see different keys, in the tail, in the block before it and across windows."""
+    _check(2, T, heads, kv, 64, dtype, lengths, 5, window)
+
+
+@pytest.mark.parametrize("T,count,lengths", [(5, [5, 2, 0, -4], [130, 64, 70, 65]), (40, [40, 1, 17, 99], [140, 65, 128, 192]), (1, [1, 0, 1, 2], [64, 10, 1, 130])])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_of_ragged_rows(T, count, lengths, D):
+    """Rows of a padded batch: those behind a row's count are zeros."""
+    _check(4, T, 4, 2, D, BF16, lengths, 4, count=count)
+
+
+@pytest.mark.parametrize("dtype,D,length,heads,kv", [(F16, 128, 5000, 4, 1), (BF16, 64, 20000, 2, 2), (F16, 256, 2500, 1, 1), (BF16, 32, 9001, 3, 1)])
+def test_attention_over_long_caches(dtype, D, length, heads, kv):
+    """Many splits of a row's cache, some rows with one, and room behind them that holds NaN."""
+    _check(2, 1, heads, kv, D, dtype, [length, 70], length // 64 + 40)
+
+
+def test_attention_of_a_draft_over_a_long_cache():
+    _check(1, 6, 8, 2, 64, BF16, [6000], 120, window=5000)
+
+
+@pytest.mark.parametrize("scale", [1e-4, 3.0, 40.0])
+def test_attention_scales(scale):
+    """Weights that are all alike and weights of which one is left."""
+    _check(1, 3, 2, 1, 64, F16, [200], 4, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_blocks_of_very_different_sizes(dtype):
+    """The scales of the blocks lie 2^20 apart, keys' the one way and values' the other."""
+    g = torch.Generator().manual_seed(9)
+    size = torch.tensor([1.0, 2.0 ** -10, 2.0 ** 8, 2.0 ** -12, 1.0]).repeat_interleave(64)[:290, None, None]
+    k, v = (_tokens(g, 1, 290, 1, 64, torch.float32) * size).to(dtype), (_tokens(g, 1, 290, 1, 64, torch.float32) / size.clamp_min(2.0 ** -7)).to(dtype)
+    q = (torch.randn(1, 1, 2, 64, generator=g) * 0.01).to(dtype)
+    cache = ref.append(ref.new_cache(1, 1, 5, 64, dtype), k, v, [0], None)
+    out = _attention(ref.to(cache, "cuda"), q.cuda(), [289])
+    want, bound = ref.attention(cache, q, [289], None, 0.125)
+    assert ref.within(out, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("T,bad_at", [(1, 10), (1, 199), (70, 10), (70, 140), (70, 150), (70, 199), (20, 150)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_attention_values_that_are_not_finite(T, bad_at, value, dtype):
+    """They reach the queries that see them, in their own element (values) or all (keys), and no other query; in a complete block (200 tokens: up
+    to 191) and in the tail."""
+    g = torch.Generator().manual_seed(7)
+    k, v = _tokens(g, 1, 200, 2, 64, dtype), _tokens(g, 1, 200, 2, 64, dtype)
+    v[0, bad_at, 0, 17] = value
+    k[0, bad_at, 1, 5] = value
+    q = torch.randn(1, T, 4, 64, generator=g).to(dtype)
+    for window in (0, 45):
+        cache = ref.append(ref.new_cache(1, 2, 4, 64, dtype), k, v, [0], None)
+        out = _attention(ref.to(cache, "cuda"), q.cuda(), [200 - T], window=window)
+        want, bound = ref.attention(cache, q, [200 - T], None, 0.125, window)
+        assert ref.within(out, want, bound), window
+
+
+def test_attention_outside_the_cache_is_nan():
+    g = torch.Generator().manual_seed(2)
+    cache = ref.to(_filled(g, 3, 1, 2, 64, F16, [100, 100, 100]), "cuda")
+    q = torch.randn(3, 2, 1, 64, generator=g).half()
+    out = _attention(cache, q.cuda(), [127, -1, 98], [2, 1, 2]).cpu()
+    assert out[0].isnan().all() and out[1, 0].isnan().all() and (out[1, 1] == 0).all() and not out[2].isnan().any()
+
+
+def test_attention_strides_and_one_start_for_all():
+    g = torch.Generator().manual_seed(12)
+    cache = _filled(g, 3, 2, 3, 64, BF16, [150] * 3)
+    q = torch.randn(3, 4, 8, 64, generator=g).bfloat16()
+    want, bound = ref.attention(cache, q[:, :, ::2], [146] * 3, None, 0.125)
+    on = ref.to(cache, "cuda")
+    odd = torch.empty(3, 4, 8, 65, dtype=BF16, device="cuda")
+    odd[..., 1:] = q.cuda()
+    for x in (q.cuda(), q.transpose(1, 2).contiguous().cuda().transpose(1, 2), odd[..., 1:]):
+        assert ref.within(_attention(on, x[:, :, ::2], [146]), want, bound)
+    one = _attention(on, q[:1, :1].cuda().expand(3, 4, 8, 64)[:, :, ::2], [146])  # a stride of nothing
+    want, bound = ref.attention(cache, q[:1, :1].expand(3, 4, 8, 64)[:, :, ::2], [146] * 3, None, 0.125)
+    assert ref.within(one, want, bound)
+
+
+def test_empty_calls():
+    import flash_gemv
+
+    c = ref.new_cache(2, 1, 1, 64, F16, fill=0.0, device="cuda")
+    z = torch.empty(2, 0, 1, 64, dtype=F16, device="cuda")
+    flash_gemv.cats_kv8_append(z, z, _words([0]), None, *_args(c))
+    assert flash_gemv.cats_kv8_attention(z, _words([0]), None, *_args(c), 0.125).shape == (2, 0, 1, 64)
+
+
+def test_steps_on_another_stream_and_in_a_graph():
+    """A row that grows over the end of a block, eagerly on a stream of its own and replayed from a graph, with other work between."""
+    import flash_gemv
+
+    g = torch.Generator().manual_seed(5)
+    k, v, q = (_tokens(g, 2, 140, n, 64, F16).cuda() for n in (2, 2, 4))
+    states = []
+    for graph in (False, True):
+        c = ref.new_cache(2, 2, 40, 64, F16, fill=0.0, device="cuda")
+        _append(c, k[:, :120], v[:, :120], [0])
+        kk, vv, qq, at = k[:, 0:1].clone(), v[:, 0:1].clone(), q[:, 0:1].clone(), torch.tensor([120], device="cuda")
+        outs = []
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            def step():
+                flash_gemv.cats_kv8_append(kk, vv, at, None, *_args(c))
+                return flash_gemv.cats_kv8_attention(qq, at, None, *_args(c), 0.125)
+
+            if graph:
+                captured = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(captured, stream=side):
+                    out = step()
+            for p in range(120, 140):
+                kk.copy_(k[:, p:p + 1]), vv.copy_(v[:, p:p + 1]), qq.copy_(q[:, p:p + 1]), at.fill_(p)
+                if graph:
+                    captured.replay()
+                else:
+                    out = step()
+                outs.append(out.clone())
+                (qq @ qq.transpose(2, 3).contiguous()).sum()
+        side.synchronize()
+        states.append((outs, c))
+    for a, b in zip(*(s[0] for s in states)):
+        assert torch.equal(a, b)
+    for f in ref.FIELDS:
+        assert ref.same(states[0][1][f], states[1][1][f])
+    cpu = {f: t.cpu() for f, t in states[0][1].items()}
+    want, bound = ref.attention(cpu, q[:, 139:140].cpu(), [139, 139], None, 0.125)
+    assert ref.within(states[0][0][-1], want, bound)
+
+
+def test_results_do_not_change_from_call_to_call():
+    g = torch.Generator().manual_seed(6)
+    c = ref.to(_filled(g, 2, 2, 60, 64, BF16, [3500, 900]), "cuda")
+    q = torch.randn(2, 1, 8, 64, generator=g).bfloat16().cuda()
+    first = _attention(c, q, [3499, 899])
+    for _ in range(5):
+        assert torch.equal(_attention(c, q, [3499, 899]), first)
