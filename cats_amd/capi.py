@@ -25,7 +25,7 @@ SYMBOLS = (
     "cats_mlp_rowmajor_down", "cats_mlp_norm_residual", "cats_up_down", "cats_set_tuning", "cats_mlp_stage", "cats_mlp_noalloc", "cats_up_index", "cats_down_index",
     "cats_probe_read", "cats_mlp_norm_residual_norm", "cats_linear", "cats_attention_step", "cats_mlp_gate_cols", "cats_silu_mask_mul",
     "cats_prompt_scratch_bytes", "cats_prompt_mlp", "cats_prompt_plan", "cats_kv8_append", "cats_kv8_attention_scratch_bytes",
-    "cats_kv8_attention", "cats_beam_scratch_bytes", "cats_beam_select", "cats_cache_reorder",
+    "cats_kv8_attention", "cats_kv8_attention_step_scratch_bytes", "cats_kv8_attention_step", "cats_beam_scratch_bytes", "cats_beam_select", "cats_cache_reorder",
 )
 
 
@@ -83,6 +83,9 @@ def lib() -> ctypes.CDLL:
             L.cats_kv8_attention_scratch_bytes.argtypes = [i32] * 7; L.cats_kv8_attention_scratch_bytes.restype = sz
             L.cats_kv8_attention.argtypes = [vp, vp, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, f32, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, sz, vp]
             L.cats_kv8_attention.restype = i32
+            L.cats_kv8_attention_step_scratch_bytes.argtypes = [i32] * 4; L.cats_kv8_attention_step_scratch_bytes.restype = sz
+            L.cats_kv8_attention_step.argtypes = [vp, vp, vp, f32, *[vp] * 14, i32, i32, i32, i32, i32, i32, vp, sz, vp]
+            L.cats_kv8_attention_step.restype = i32
             L.cats_beam_scratch_bytes.argtypes = [i32] * 4; L.cats_beam_scratch_bytes.restype = sz
             L.cats_beam_select.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, sz, vp]; L.cats_beam_select.restype = i32
             L.cats_cache_reorder.argtypes = [vp, i32, vp, vp, i32, i32, i32, vp]; L.cats_cache_reorder.restype = i32

@@ -9,7 +9,7 @@
 #include <unordered_map>
 
 #include "cats_gemv.h"
-#include "cats_launch.h"
+#include "cats_launch_cache.h"
 
 // Built-in scratch of cats_mlp_noalloc: the per-workgroup partial sums and active counts of the single-pass kernel and of small layers'.
 // Every GPU the library runs on holds its own copy of this array, at its own address, until the process ends.
@@ -50,6 +50,8 @@ template <> hipError_t launch_prompt<F16>(bool, const PromptPlan&, PromptArgs, h
 template <> hipError_t launch_prompt<BF16>(bool, const PromptPlan&, PromptArgs, hipStream_t);
 template <> hipError_t launch_prompt_sum<F16>(const PromptSumArgs&, hipStream_t);
 template <> hipError_t launch_prompt_sum<BF16>(const PromptSumArgs&, hipStream_t);
+template <> hipError_t launch_kv8_attn<F16>(int, const KvAttnPlan&, KvAttnArgs, hipStream_t);
+template <> hipError_t launch_kv8_attn<BF16>(int, const KvAttnPlan&, KvAttnArgs, hipStream_t);
 hipError_t ensure_dynamic_lds(const void* kern, size_t bytes) {
   if (bytes <= 48 * 1024) return hipSuccess;
   static std::mutex mu;
@@ -1615,6 +1617,65 @@ int cats_attention_step(const void* h, const void* x, const void* norm_weight, f
                                             : launch_attn<F32>(hd, B, t, (hipStream_t)stream);
   if (e != hipSuccess) return CATS_ERR_LAUNCH;
   return cats_linear(attn_scratch, nullptr, 0.f, wo, h, out, B, H, H, dtype, stream);
+}
+
+// scratch: q | what attention leaves | partial sums of attention's splits
+static size_t kv8_step_vec_bytes(int B, int H) { return ((size_t)B * H * 2 + 255) / 256 * 256; }
+
+size_t cats_kv8_attention_step_scratch_bytes(int B, int H, int heads, int blocks) {
+  if (B < 1 || B > kKernelBatch || H < 1 || heads < 1 || H % heads != 0) return 0;
+  return 2 * kv8_step_vec_bytes(B, H) + cats_kv8_attention_scratch_bytes(B, 1, heads, heads, H / heads, blocks, 0);
+}
+
+int cats_kv8_attention_step(const void* h, const void* x, const void* norm_weight, float eps, const void* wq, const void* wk, const void* wv,
+                            const void* wo, void* k8, void* v8, float* k_scale, float* v_scale, void* k_tail, void* v_tail, const void* cos_table,
+                            const void* sin_table, const int64_t* position, void* out, int B, int H, int heads, int blocks, int max_len, int dtype,
+                            void* scratch, size_t scratch_bytes, void* stream) {
+  if (dtype != CATS_F16 && dtype != CATS_BF16) return CATS_ERR_DTYPE;
+  if (int st = check_proj(B, H, H, dtype)) return st;
+  if (heads < 1 || H % heads != 0 || blocks < 1 || blocks > CATS_KV8_MAX_BLOCKS || max_len < 1 || max_len > blocks * kKvBlock) return CATS_ERR_SHAPE;
+  const int hd = H / heads;
+  if (hd != 32 && hd != 64 && hd != 128 && hd != 256) return CATS_ERR_SHAPE;
+  if (!h || !x || !wq || !wk || !wv || !wo || !k8 || !v8 || !k_scale || !v_scale || !k_tail || !v_tail || !cos_table || !sin_table || !position || !out)
+    return CATS_ERR_NULL;
+  for (const void* p : {x, norm_weight, wq, wk, wv, wo, (const void*)k8, (const void*)v8, (const void*)k_tail, (const void*)v_tail})
+    if (!aligned16(p)) return CATS_ERR_ALIGN;
+  if (!scratch || ((uintptr_t)scratch & 255u) || scratch_bytes < cats_kv8_attention_step_scratch_bytes(B, H, heads, blocks)) return CATS_ERR_WORKSPACE;
+  char* const att = (char*)scratch + kv8_step_vec_bytes(B, H);
+  ProjArgs a;
+  memset(&a, 0, sizeof(a));
+  fill_rows(a.r, x, wq, H, H, B, dtype);
+  a.r.norm_w = (const u32x4*)norm_weight;
+  a.r.norm_eps = eps;
+  a.wk = (const u32x4*)wk;
+  a.wv = (const u32x4*)wv;
+  a.q16 = scratch;
+  a.k_cache = k_tail;
+  a.v_cache = v_tail;
+  a.cos_t = cos_table;
+  a.sin_t = sin_table;
+  a.pos = position;
+  a.half = hd / 2;
+  a.heads = heads;
+  a.max_len = max_len;
+  if (int st = do_proj(kProjQkv, dtype, a, (hipStream_t)stream)) return st;
+  KvAttnArgs t;
+  t.q = (const uint16_t*)scratch;
+  t.q_row = H, t.q_tok = 0, t.q_head = hd;
+  t.out = (uint16_t*)att;
+  t.span = {position, nullptr, 0, 0, max_len};
+  t.c = {(uint8_t*)k8, (uint8_t*)v8, k_scale, v_scale, (uint16_t*)k_tail, (uint16_t*)v_tail, heads, blocks};
+  t.part = (float*)(att + kv8_step_vec_bytes(B, H));
+  t.scale = 1.44269504088896341f / sqrtf((float)hd);
+  t.T = 1;
+  t.group = 1;
+  t.window = 0;
+  t.pairs = B * heads;
+  KvAttnPlan plan = kv8_attn_plan(B, 1, heads, heads, blocks, 0);
+  plan.seal = true;
+  const hipError_t e = dtype == CATS_F16 ? launch_kv8_attn<F16>(hd, plan, t, (hipStream_t)stream) : launch_kv8_attn<BF16>(hd, plan, t, (hipStream_t)stream);
+  if (e != hipSuccess) return CATS_ERR_LAUNCH;
+  return cats_linear(att, nullptr, 0.f, wo, h, out, B, H, H, dtype, stream);
 }
 
 }  // extern "C"

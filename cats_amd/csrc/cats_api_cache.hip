@@ -57,16 +57,20 @@ int check_span(const int64_t* start, int start_step, const int64_t* count, int c
   return (start_step == 0 || start_step == 1) && (count_step == 0 || count_step == 1) ? CATS_OK : CATS_ERR_SHAPE;
 }
 
-KvAttnPlan attn_plan(int B, int T, int heads, int kv_heads, int blocks, int window) {
+}  // namespace
+
+KvAttnPlan kv8_attn_plan(int B, int T, int heads, int kv_heads, int blocks, int window) {
   const int cus = current_device_cus(), rows = T * (heads / kv_heads);
   const long long groups = (long long)B * kv_heads * ((rows + 15) / 16);
   // tiles that a workgroup's queries see at most
   const int tiles = window ? (int)min((long long)blocks, ((long long)window + 16 + 2 * kKvBlock) / kKvBlock) : blocks;
-  KvAttnPlan plan;
+  KvAttnPlan plan = {1, false};
   const long long want = (4ll * cus + groups - 1) / groups;
   plan.splits = (int)max(1ll, min(want, (long long)(tiles + 3) / 4));
   return plan;
 }
+
+namespace {
 
 bool attn_shape_ok(int T, int heads, int kv_heads) {
   return heads >= kv_heads && heads % kv_heads == 0 && (long long)T * (heads / kv_heads) <= 16ll * kMaxGrid;
@@ -96,7 +100,7 @@ int cats_kv8_append(const void* k, const int64_t* k_strides, const void* v, cons
   a.v = (const uint16_t*)v;
   a.k_row = k_strides[0], a.k_tok = k_strides[1], a.k_head = k_strides[2];
   a.v_row = v_strides[0], a.v_tok = v_strides[1], a.v_head = v_strides[2];
-  a.span = {start, count, start_step, count_step};
+  a.span = {start, count, start_step, count_step, blocks * kKvBlock};
   a.T = T;
   const hipError_t e = dtype == CATS_F16 ? launch_kv8_append<F16>(D, a, B, (hipStream_t)stream) : launch_kv8_append<BF16>(D, a, B, (hipStream_t)stream);
   return e == hipSuccess ? CATS_OK : CATS_ERR_LAUNCH;
@@ -104,7 +108,7 @@ int cats_kv8_append(const void* k, const int64_t* k_strides, const void* v, cons
 
 size_t cats_kv8_attention_scratch_bytes(int B, int T, int heads, int kv_heads, int D, int blocks, int window) {
   if (check_cache(B, T, kv_heads, D, blocks, CATS_F16) || !attn_shape_ok(T, heads, kv_heads) || window < 0) return 0;
-  return attn_bytes(attn_plan(B, T, heads, kv_heads, blocks, window), B, T, heads, kv_heads, D);
+  return attn_bytes(kv8_attn_plan(B, T, heads, kv_heads, blocks, window), B, T, heads, kv_heads, D);
 }
 
 int cats_kv8_attention(const void* q, const int64_t* q_strides, const int64_t* start, int start_step, const int64_t* count, int count_step,
@@ -119,13 +123,13 @@ int cats_kv8_attention(const void* q, const int64_t* q_strides, const int64_t* s
   if (!aligned(out, 16)) return CATS_ERR_ALIGN;
   KvAttnArgs a;
   if (int st = fill_cache(a.c, (void*)k8, (void*)v8, (float*)k_scale, (float*)v_scale, (void*)k_tail, (void*)v_tail, kv_heads, blocks)) return st;
-  const KvAttnPlan plan = attn_plan(B, T, heads, kv_heads, blocks, window);
+  const KvAttnPlan plan = kv8_attn_plan(B, T, heads, kv_heads, blocks, window);
   const size_t bytes = attn_bytes(plan, B, T, heads, kv_heads, D);
   if (bytes && (!scratch || !aligned(scratch, 16) || scratch_bytes < bytes)) return CATS_ERR_WORKSPACE;
   a.q = (const uint16_t*)q;
   a.q_row = q_strides[0], a.q_tok = q_strides[1], a.q_head = q_strides[2];
   a.out = (uint16_t*)out;
-  a.span = {start, count, start_step, count_step};
+  a.span = {start, count, start_step, count_step, blocks * kKvBlock};
   a.part = (float*)scratch;
   a.scale = 1.44269504088896341f * scale;
   a.T = T;

@@ -34,7 +34,26 @@ struct ProjArgs {
   int half;              // head_dim / 2
   int heads;
   int max_len;
+  void* q16;             // a cache in 8 bits: the rotated q in dtype instead of q_out, and the caches are its tails, k (nb, heads, 64, head_dim)
+                         // and v (nb, heads, head_dim, 64), slot = position % 64
 };
+
+// Where row `row` of a q, k or v product (which 0, 1, 2) goes.
+template <class DT>
+__device__ __forceinline__ void proj_store_qkv(const ProjArgs& a, int which, int b, int row, int hd, long long pos, bool pos_ok, float u) {
+  typedef typename DT::st st;
+  if (which == 0) {
+    if (a.q16) ((st*)a.q16)[(size_t)b * a.r.N + row] = DT::fromf(u);
+    else a.q_out[(size_t)b * a.r.N + row] = u;
+  } else if (pos_ok) {
+    const int head = row / hd, e = row - head * hd;
+    const size_t pair = (size_t)b * a.heads + head;
+    st* cache = (st*)(which == 1 ? a.k_cache : a.v_cache);
+    if (!a.q16) cache[(pair * a.max_len + (size_t)pos) * hd + e] = DT::fromf(u);
+    else if (which == 1) cache[(pair * 64 + (pos & 63)) * hd + e] = DT::fromf(u);
+    else cache[(pair * hd + e) * 64 + (pos & 63)] = DT::fromf(u);
+  }
+}
 
 // R rows per wave.  For kProjQkv they are two, the elements of a head that the rotary embedding mixes, d and d + head_dim / 2,
 // so it is applied to the two sums where they are; the wave's number counts these pairs over the three matrices.
@@ -125,14 +144,7 @@ void proj_kernel(ProjArgs a) {
     for (int r = 0; r < R; r++)
 #pragma unroll
       for (int b = 0; b < B; b++)
-        if (b < p.nb) {
-          if (which == 0) a.q_out[(size_t)b * p.N + row[r]] = g[r][b];
-          else if (pos_ok) {
-            const int head = row[r] / (2 * a.half), e = row[r] - head * 2 * a.half;
-            st* cache = (st*)(which == 1 ? a.k_cache : a.v_cache);
-            cache[(((size_t)b * a.heads + head) * a.max_len + (size_t)pos) * 2 * a.half + e] = DT::fromf(g[r][b]);
-          }
-        }
+        if (b < p.nb) proj_store_qkv<DT>(a, which, b, row[r], 2 * a.half, pos, pos_ok, g[r][b]);
   } else {
     st* out = (st*)p.zt_out;
 #pragma unroll

@@ -37,11 +37,12 @@ struct KvSpan {
   const int64_t* count;  // nullptr: all T
   int start_step;        // 0: one start for all rows
   int count_step;
+  int limit;             // positions lie below it
 };
-__device__ __forceinline__ bool kv_span(const KvSpan& s, int b, int T, int blocks, int& start, int& n) {
+__device__ __forceinline__ bool kv_span(const KvSpan& s, int b, int T, int& start, int& n) {
   const long long a = s.start[(size_t)b * s.start_step], c = s.count ? s.count[(size_t)b * s.count_step] : T;
   n = (int)(c < 0 ? 0 : c > T ? T : c);
-  const bool ok = a >= 0 && a <= (long long)blocks * kKvBlock - n;
+  const bool ok = a >= 0 && a <= (long long)s.limit - n;
   start = ok ? (int)a : 0;
   return ok;
 }
@@ -79,6 +80,85 @@ __device__ __forceinline__ float kv_scale_of(float amax) {
 }
 __device__ __forceinline__ float kv_code_of(float x, float inv) { return fmaf(x, 0.f, x * inv); }  // NaN where x is not finite
 
+// Elements d0 .. of a token in the tails.
+template <class DT, int D, int NV>
+__device__ __forceinline__ void kv_tail_token(const uint16_t* kt, const uint16_t* vt, int tok, int d0, u32x4 (&kx)[NV], u32x4 (&vx)[NV]) {
+#pragma unroll
+  for (int i = 0; i < NV; i++) kx[i] = ((const u32x4*)(kt + tok * D + d0))[i];
+#pragma unroll
+  for (int i = 0; i < NV; i++)
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      vx[i][e] = vt[(d0 + 8 * i + 2 * e) * kKvBlock + tok] | (uint32_t)vt[(d0 + 8 * i + 2 * e + 1) * kKvBlock + tok] << 16;
+}
+
+// Quantises block `blk` of a (row, cached head) pair.  256 threads: thread 4 t + i holds elements i D / 4 .. of token t, NV vectors of its key and value.
+template <int D>
+struct KvStage {
+  uint32_t most[2][4];
+  uint8_t v[D][kKvBlock + 4];
+};
+template <class DT, int D, int NV>
+__device__ __forceinline__ void kv_quantise(const KvCache& c, size_t pair, int blk, const u32x4 (&kx)[NV], const u32x4 (&vx)[NV], KvStage<D>& stage) {
+  const int tid = threadIdx.x, tok = tid / 4, d0 = tid % 4 * (D / 4);
+  // magnitudes of 16-bit floats are ordered as integers
+  auto most = [](const u32x4 (&x)[NV]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const uint32_t w = x[i][e], lo = w & 0x7fffu, hi = w >> 16 & 0x7fffu;
+        m = max(m, max(lo < Kv<DT>::kExp ? lo : 0u, hi < Kv<DT>::kExp ? hi : 0u));
+      }
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, kWave));
+    return m;
+  };
+  const uint32_t mk = most(kx), mv = most(vx);
+  if (tid % kWave == 0) {
+    stage.most[0][tid / kWave] = mk;
+    stage.most[1][tid / kWave] = mv;
+  }
+  __syncthreads();
+  auto scale_of = [&](int i) {
+    return kv_scale_of(DT::tof((uint16_t)max(max(stage.most[i][0], stage.most[i][1]), max(stage.most[i][2], stage.most[i][3]))));
+  };
+  const float ks = scale_of(0), vs = scale_of(1);
+  const size_t block = pair * c.blocks + blk;
+  if (tid == 0) {
+    c.ks[block] = ks;
+    c.vs[block] = vs;
+  }
+  auto codes = [](u32x4 x, float inv) {  // of eight values
+    uint32_t out[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const uint32_t a = x[2 * i], b = x[2 * i + 1];
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(kv_code_of(DT::tof((uint16_t)a), inv), kv_code_of(DT::tof((uint16_t)(a >> 16)), inv), 0, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(kv_code_of(DT::tof((uint16_t)b), inv), kv_code_of(DT::tof((uint16_t)(b >> 16)), inv), w, true);
+      out[i] = (uint32_t)w;
+    }
+    return u32x2{out[0], out[1]};
+  };
+  const float ki = 1.f / ks, vi = 1.f / vs;  // powers of two
+  u32x2* k8 = (u32x2*)(c.k8 + block * kKvBlock * D + tok * D + d0);
+#pragma unroll
+  for (int i = 0; i < NV; i++) k8[i] = codes(kx[i], ki);
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const u32x2 w = codes(vx[i], vi);
+#pragma unroll
+    for (int e = 0; e < 8; e++) stage.v[d0 + 8 * i + e][tok] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
+  }
+  __syncthreads();
+  u32x4* v8 = (u32x4*)(c.v8 + block * kKvBlock * D);
+  for (int i = tid; i < D * 4; i += 256) {
+    const uint32_t* s = (const uint32_t*)&stage.v[i / 4][i % 4 * 16];
+    v8[i] = u32x4{s[0], s[1], s[2], s[3]};
+  }
+}
+
 struct KvAppendArgs {
   const uint16_t* k;  // (B, T, heads, D) in elements: strides of a row, a token and a head
   const uint16_t* v;
@@ -96,7 +176,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(KvAppendArgs p) {
   constexpr int E = D / 4, NV = E / 8;  // elements and vectors of a token that one of its four threads holds
   const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
   int start, n;
-  if (!kv_span(p.span, b, p.T, p.c.blocks, start, n) || n == 0) return;
+  if (!kv_span(p.span, b, p.T, start, n) || n == 0) return;
   const int end = start + n, last = (end - 1) / kKvBlock, blk = start / kKvBlock + blockIdx.x;
   if (blk > last) return;
   const size_t pair = (size_t)b * p.c.heads + h;
@@ -105,8 +185,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(KvAppendArgs p) {
   const uint16_t* k = p.k + b * p.k_row + h * p.k_head;
   const uint16_t* v = p.v + b * p.v_row + h * p.v_head;
 
-  __shared__ uint32_t s_max[2][4];
-  __shared__ uint8_t s_v[D][kKvBlock + 4];
+  __shared__ KvStage<D> stage;
   if ((blk + 1) * kKvBlock <= end) {
     const int tok = tid / 4, d0 = tid % 4 * E, at = blk * kKvBlock + tok - start;
     u32x4 kx[NV], vx[NV];
@@ -116,70 +195,9 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(KvAppendArgs p) {
 #pragma unroll
       for (int i = 0; i < NV; i++) vx[i] = load_stream((const u32x4*)(v + at * p.v_tok + d0) + i);
     } else {
-#pragma unroll
-      for (int i = 0; i < NV; i++) kx[i] = ((const u32x4*)(kt + tok * D + d0))[i];
-#pragma unroll
-      for (int i = 0; i < NV; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          vx[i][e] = vt[(d0 + 8 * i + 2 * e) * kKvBlock + tok] | (uint32_t)vt[(d0 + 8 * i + 2 * e + 1) * kKvBlock + tok] << 16;
+      kv_tail_token<DT, D>(kt, vt, tok, d0, kx, vx);
     }
-    // magnitudes of 16-bit floats are ordered as integers
-    auto most = [](const u32x4 (&x)[NV]) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < NV; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const uint32_t w = x[i][e], lo = w & 0x7fffu, hi = w >> 16 & 0x7fffu;
-          m = max(m, max(lo < Kv<DT>::kExp ? lo : 0u, hi < Kv<DT>::kExp ? hi : 0u));
-        }
-#pragma unroll
-      for (int o = 1; o < kWave; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, kWave));
-      return m;
-    };
-    const uint32_t mk = most(kx), mv = most(vx);
-    if (tid % kWave == 0) {
-      s_max[0][tid / kWave] = mk;
-      s_max[1][tid / kWave] = mv;
-    }
-    __syncthreads();
-    auto scale_of = [&](int i) {
-      return kv_scale_of(DT::tof((uint16_t)max(max(s_max[i][0], s_max[i][1]), max(s_max[i][2], s_max[i][3]))));
-    };
-    const float ks = scale_of(0), vs = scale_of(1);
-    const size_t block = pair * p.c.blocks + blk;
-    if (tid == 0) {
-      p.c.ks[block] = ks;
-      p.c.vs[block] = vs;
-    }
-    auto codes = [](u32x4 x, float inv) {  // of eight values
-      uint32_t out[2];
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const uint32_t a = x[2 * i], c = x[2 * i + 1];
-        int w = __builtin_amdgcn_cvt_pk_fp8_f32(kv_code_of(DT::tof((uint16_t)a), inv), kv_code_of(DT::tof((uint16_t)(a >> 16)), inv), 0, false);
-        w = __builtin_amdgcn_cvt_pk_fp8_f32(kv_code_of(DT::tof((uint16_t)c), inv), kv_code_of(DT::tof((uint16_t)(c >> 16)), inv), w, true);
-        out[i] = (uint32_t)w;
-      }
-      return u32x2{out[0], out[1]};
-    };
-    const float ki = 1.f / ks, vi = 1.f / vs;  // powers of two
-    u32x2* k8 = (u32x2*)(p.c.k8 + block * kKvBlock * D + tok * D + d0);
-#pragma unroll
-    for (int i = 0; i < NV; i++) k8[i] = codes(kx[i], ki);
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const u32x2 w = codes(vx[i], vi);
-#pragma unroll
-      for (int e = 0; e < 8; e++) s_v[d0 + 8 * i + e][tok] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
-    }
-    __syncthreads();
-    u32x4* v8 = (u32x4*)(p.c.v8 + block * kKvBlock * D);
-    for (int i = tid; i < D * 4; i += 256) {
-      const uint32_t* s = (const uint32_t*)&s_v[i / 4][i % 4 * 16];
-      v8[i] = u32x4{s[0], s[1], s[2], s[3]};
-    }
+    kv_quantise<DT, D>(p.c, pair, blk, kx, vx, stage);
   }
   if (blockIdx.x != 0) return;
   __syncthreads();  // what the tail held has been read
@@ -271,9 +289,11 @@ __device__ __forceinline__ uint32_t kv_fix16(uint32_t& w) {
 // row (V) or of whole lines (K).  The numbers become 16-bit operands (two an instruction), the blocks' scales go into the
 // exponent: with w = s * ks * scale + log2(vs), weights are 2^(w - max w) <= 1, O sums them times the codes, and the sum of
 // weights adds them divided by vs.
+// SEAL: the tokens are in the tails and nowhere else yet.  One workgroup a pair more quantises the block that they complete; nobody reads that block
+// in this launch.
 // A masked weight is 0, but 0 times a NaN is not: where a tile is seen in part, numbers of V that are not finite are taken out and the
 // rows that see one are set to NaN.
-template <class DT, int D>
+template <class DT, int D, bool SEAL>
 __global__ __launch_bounds__(256) void kv8_attn_step_kernel(KvAttnArgs p) {
   constexpr int W = 4, ROWS = 16, C = D / 64, NU = D / 16, NK = D >= 64 ? C : 1;
   typedef Kv<DT> F;
@@ -282,7 +302,17 @@ __global__ __launch_bounds__(256) void kv8_attn_step_kernel(KvAttnArgs p) {
   const int b = pair / p.c.heads;
   int start, n;
   KvTiles t;
-  const bool ok = kv_span(p.span, b, p.T, p.c.blocks, start, n);
+  const bool ok = kv_span(p.span, b, p.T, start, n);
+  if constexpr (SEAL) {
+    if (split == p.splits) {
+      __shared__ KvStage<D> stage;
+      if (!ok || (start + n) % kKvBlock != 0 || n == 0 || blockIdx.z != 0) return;
+      u32x4 kx[D / 32], vx[D / 32];
+      kv_tail_token<DT, D>(p.c.kt + (size_t)pair * kKvBlock * D, p.c.vt + (size_t)pair * kKvBlock * D, threadIdx.x / 4, threadIdx.x % 4 * (D / 4), kx, vx);
+      kv_quantise<DT, D>(p.c, pair, (start + n) / kKvBlock - 1, kx, vx, stage);
+      return;
+    }
+  }
   if (!kv_tiles<ROWS, W>(p, r0, start, n, t) || !ok) {
     if (split == 0) kv_fill_rows<DT>(p, pair, r0, ROWS, n, ok, D, threadIdx.x, 256);
     return;
@@ -497,7 +527,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(KvAttnArgs p) {
   const int pair = blockIdx.x, rows = p.T * p.group, j0 = blockIdx.y * 16;
   int start, n;
   KvTiles t;
-  if (!kv_span(p.span, pair / p.c.heads, p.T, p.c.blocks, start, n) || !kv_tiles<ROWS, UNIT>(p, j0 / ROWS * ROWS, start, n, t) || t.active == 1) return;
+  if (!kv_span(p.span, pair / p.c.heads, p.T, start, n) || !kv_tiles<ROWS, UNIT>(p, j0 / ROWS * ROWS, start, n, t) || t.active == 1) return;
   const float* ml = p.part + (size_t)p.pairs * p.splits * rows * D;
   for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
     const int r = j0 + i / (D / 4), d = i % (D / 4) * 4;

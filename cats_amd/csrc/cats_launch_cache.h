@@ -10,7 +10,9 @@ namespace cats {
 // The cache in 8 bits (cats_kv8.h), 16-bit types.  launch_kv8_attn fills in what the plan decides.
 struct KvAttnPlan {
   int splits;  // of a row's cache
+  bool seal;   // the new tokens are in the tails only: quantise the blocks they complete
 };
+KvAttnPlan kv8_attn_plan(int B, int T, int heads, int kv_heads, int blocks, int window);
 template <class DT>
 hipError_t launch_kv8_append(int D, const KvAppendArgs& a, int B, hipStream_t stream);
 template <class DT>

@@ -104,10 +104,7 @@ __global__ __launch_bounds__(kMmaThreads) void proj_mma_kernel(ProjArgs a) {
         const int d = row % hd;
         u = rj < 4 ? u * s_cs[d] - other * s_cs[hd + d] : u * s_cs[d] + other * s_cs[hd + d];
       }
-      if (rb < p.nb) {
-        if (which == 0) a.q_out[(size_t)rb * p.N + row] = u;
-        else if (pos_ok) ((st*)(which == 1 ? a.k_cache : a.v_cache))[(((size_t)rb * a.heads + row / hd) * a.max_len + (size_t)pos) * hd + row % hd] = DT::fromf(u);
-      }
+      if (rb < p.nb) proj_store_qkv<DT>(a, which, rb, row, hd, pos, pos_ok, u);
     } else if (rb < p.nb && row < p.N) {
       ((st*)p.zt_out)[(size_t)rb * p.N + row] = DT::fromf(MODE == kProjAdd ? u + res : u);
     }

@@ -663,6 +663,49 @@ at::Tensor cats_kv8_attention_op(const at::Tensor& q, const at::Tensor& start, c
   return out;
 }
 
+// cats_attention_step over a cache in 8 bits.
+at::Tensor cats_kv8_attention_step_op(const at::Tensor& h, const at::Tensor& x, const c10::optional<at::Tensor>& norm_weight, const double eps,
+                                      const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& wv, const at::Tensor& wo, at::Tensor& k8,
+                                      at::Tensor& v8, at::Tensor& k_scale, at::Tensor& v_scale, at::Tensor& k_tail, at::Tensor& v_tail,
+                                      const at::Tensor& cos_table, const at::Tensor& sin_table, const at::Tensor& position) {
+  check_dev(h, "h");
+  check_dev(x, "x");
+  const int B = batch_rows(h, "cats_kv8_attention_step");
+  const int64_t H = h.size(-1);
+  TORCH_CHECK(x.sizes() == h.sizes() && x.scalar_type() == h.scalar_type() && x.device() == h.device(), "flash_gemv.cats_kv8_attention_step: x must be like h");
+  for (const at::Tensor* w : {&wq, &wk, &wv, &wo}) check_weight(*w, h, H, H, "a projection");
+  const bool norm = norm_weight.has_value() && norm_weight->defined();
+  if (norm) {
+    check_dev(*norm_weight, "norm_weight");
+    TORCH_CHECK(norm_weight->scalar_type() == h.scalar_type() && norm_weight->numel() == H && norm_weight->device() == h.device(),
+                "flash_gemv.cats_kv8_attention_step: norm_weight must be a (H,) tensor of h's dtype on h's device");
+  }
+  TORCH_CHECK(k8.dim() == 5 && k8.size(1) * k8.size(4) == H, "flash_gemv.cats_kv8_attention_step: k8 must be (B, heads, blocks, 64, head_dim), got ", k8.sizes());
+  const int64_t heads = k8.size(1), hd = k8.size(4);
+  const Kv8 c = check_kv8(h.view({B, 1, heads, hd}), k8, v8, k_scale, v_scale, k_tail, v_tail, "cats_kv8_attention_step");
+  const int64_t max_len = cos_table.size(0);
+  for (const at::Tensor* t : {&cos_table, &sin_table}) {
+    check_dev(*t, "a rotary table");
+    TORCH_CHECK(t->dim() == 2 && t->size(0) == max_len && t->size(1) == hd && t->scalar_type() == h.scalar_type() && t->device() == h.device(),
+                "flash_gemv.cats_kv8_attention_step: the rotary tables must be (max_len, head_dim) in h's dtype");
+  }
+  TORCH_CHECK(max_len <= c.blocks * 64, "flash_gemv.cats_kv8_attention_step: a cache of ", c.blocks, " blocks does not hold ", max_len, " tokens");
+  check_dev(position, "position");
+  TORCH_CHECK(position.scalar_type() == at::kLong && position.numel() == 1 && position.device() == h.device(),
+              "flash_gemv.cats_kv8_attention_step: position must be one int64 on h's device");
+  const c10::DeviceGuard guard(h.device());
+  at::Tensor out = at::empty_like(h);
+  const size_t bytes = cats_kv8_attention_step_scratch_bytes(B, (int)H, (int)heads, (int)c.blocks);
+  at::Tensor scratch = at::empty({(int64_t)bytes}, h.options().dtype(at::kByte));
+  check_status(cats_kv8_attention_step(h.data_ptr(), x.data_ptr(), norm ? norm_weight->data_ptr() : nullptr, (float)eps, wq.data_ptr(), wk.data_ptr(),
+                                       wv.data_ptr(), wo.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
+                                       k_tail.data_ptr(), v_tail.data_ptr(), cos_table.data_ptr(), sin_table.data_ptr(), position.data_ptr<int64_t>(),
+                                       out.data_ptr(), B, (int)H, (int)heads, (int)c.blocks, (int)max_len, dtype_code(h), scratch.data_ptr(), bytes,
+                                       current_stream(h)),
+               "cats_kv8_attention_step");
+  return out;
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> cats_beam_select_op(const at::Tensor& logits, const at::Tensor& scores,
                                                                                const c10::optional<at::Tensor>& finished, const int64_t eos,
                                                                                const int64_t keep) {
@@ -769,6 +812,9 @@ TORCH_LIBRARY(flash_gemv, m) {
   m.def("cats_kv8_append(Tensor k, Tensor v, Tensor start, Tensor? count, Tensor(a!) k8, Tensor(b!) v8, Tensor(c!) k_scale, Tensor(d!) v_scale, "
         "Tensor(e!) k_tail, Tensor(f!) v_tail) -> ()", cats_kv8_append_op);
   m.def("cats_kv8_attention", cats_kv8_attention_op);
+  m.def("cats_kv8_attention_step(Tensor h, Tensor x, Tensor? norm_weight, float eps, Tensor wq, Tensor wk, Tensor wv, Tensor wo, Tensor(a!) k8, "
+        "Tensor(b!) v8, Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor(e!) k_tail, Tensor(f!) v_tail, Tensor cos_table, Tensor sin_table, "
+        "Tensor position) -> Tensor", cats_kv8_attention_step_op);
   m.def("cats_beam_select", cats_beam_select_op);
   m.def("cats_cache_reorder(Tensor(a!)[] caches, int[] slots, Tensor parents, Tensor? lengths) -> ()", cats_cache_reorder_op);
 }

@@ -9,7 +9,7 @@ its tree spells out: decoder layer order ``h += attn(input_layernorm(h)); h += m
 Outside the MLP every mode runs the same code -- stock PyTorch-ROCm ops for a prompt, the projection and attention kernels of
 ``cats_decode.h`` for one new token per row (``LlamaDecoder._takes_step``) -- so dense-vs-CATS differences isolate the MLP path.
 The decode step is shape-static (fixed-size KV cache, position kept on the device) so it can be replayed from a
-HIP graph.
+HIP graph.  The cache may be one in 8 bits (``DecoderConfig.kv_cache``), and ``generate_beams`` searches with several hypotheses a prompt.
 """
 from __future__ import annotations
 
@@ -21,6 +21,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .kv8 import Kv8Cache
 from .mlp import CatsMLP, _bare, _nothing_watches, _plain
 
 
@@ -34,6 +35,7 @@ class DecoderConfig:
     rms_eps: float = 1e-5
     rope_theta: float = 10000.0
     max_len: int = 512
+    kv_cache: str = "dtype"  # "e4m3": a cache in 8 bits (cats_amd.kv8), for 16-bit models on the GPU
 
     @property
     def head_dim(self):
@@ -66,14 +68,37 @@ class Attention(nn.Module):
         self.q_proj, self.k_proj, self.v_proj, self.o_proj = (nn.Linear(Hd, Hd, **kw) for _ in range(4))
         self.k_cache = None
         self.v_cache = None
+        self.kv8 = None
 
     def reset_cache(self, batch, dtype, device):
         c = self.cfg
+        if c.kv_cache == "e4m3":
+            self.k_cache = self.v_cache = None
+            self.kv8 = Kv8Cache(batch, c.num_heads, c.max_len, c.head_dim, dtype, device)
+            return
+        if c.kv_cache != "dtype":
+            raise ValueError(f"kv_cache is 'dtype' or 'e4m3', not {c.kv_cache!r}")
+        self.kv8 = None
         self.k_cache = torch.zeros(batch, c.num_heads, c.max_len, c.head_dim, dtype=dtype, device=device)
         self.v_cache = torch.zeros_like(self.k_cache)
 
+    def caches(self):
+        """([tensors of (rows, heads, entries, ...)], [tokens an entry of each holds]), as flash_gemv.cats_cache_reorder takes them."""
+        if self.kv8 is not None:
+            return self.kv8.tensors(), list(Kv8Cache.SLOTS)
+        return [self.k_cache, self.v_cache], [1, 1]
+
+    def repeat_cache(self, times):
+        """Each row of the cache `times` times, for as many beams."""
+        holder, names = (self.kv8, Kv8Cache.FIELDS) if self.kv8 is not None else (self, ("k_cache", "v_cache"))
+        for name in names:
+            t = getattr(holder, name)
+            t = t.view(torch.uint8) if t.element_size() == 1 else t
+            setattr(holder, name, t.repeat_interleave(times, 0).view(getattr(holder, name).dtype))
+
     def forward(self, h, cos, sin, positions, mask):
-        """h (B, q, H); cos/sin (q, head_dim); positions (q,) int64 cache slots; mask (q, max_len) additive."""
+        """h (B, q, H); cos/sin (q, head_dim); positions (q,) int64 cache slots; mask (q, max_len) additive.  A cache in 8 bits takes positions that
+        follow one another and what it holds, and masks by them."""
         c = self.cfg
         B, q, _ = h.shape
         shp = (B, q, c.num_heads, c.head_dim)
@@ -82,6 +107,12 @@ class Attention(nn.Module):
         vh = self.v_proj(h).view(shp).transpose(1, 2)
         qh = qh * cos + rotate_half(qh) * sin
         kh = kh * cos + rotate_half(kh) * sin
+        if self.kv8 is not None:
+            if torch.is_grad_enabled() and any(t.requires_grad for t in (qh, kh, vh)):
+                raise RuntimeError("attention over a cache in 8 bits has no gradient: run the model under torch.no_grad()")
+            start = positions[:1]
+            self.kv8.append(kh.transpose(1, 2), vh.transpose(1, 2), start)
+            return self.o_proj(self.kv8.attend(qh.transpose(1, 2), start).reshape(B, q, c.hidden_size))
         self.k_cache.index_copy_(2, positions, kh)
         self.v_cache.index_copy_(2, positions, vh)
         att = torch.matmul(qh, self.k_cache.transpose(2, 3)) / math.sqrt(c.head_dim) + mask
@@ -118,13 +149,18 @@ class DecoderLayer(nn.Module):
     def _bare_for(self, dtype, device, tables, batch):
         """Whether the kernels of a decode step may stand for this layer's input norm and attention."""
         at, n = self.self_attn, self.input_layernorm
-        if not (_bare(self, DecoderLayer) and _bare(at, Attention) and _bare(n, RMSNorm) and at.k_cache is not None):
+        if not (_bare(self, DecoderLayer) and _bare(at, Attention) and _bare(n, RMSNorm) and (at.k_cache is not None or at.kv8 is not None)):
             return False
         H = at.cfg.hidden_size
         lin = (at.q_proj, at.k_proj, at.v_proj, at.o_proj)
         if not all(_bare(m, nn.Linear) and m.bias is None and m.weight.shape == (H, H) for m in lin) or n.weight.shape != (H,):
             return False
         shape = (batch, at.cfg.num_heads, *tables[0].shape)
+        if at.kv8 is not None:
+            c = at.kv8
+            return (all(_plain(m.weight, dtype, device) for m in lin) and _plain(n.weight, dtype, device) and c.k_tail.dtype == dtype
+                    and c.k_tail.shape == (batch, at.cfg.num_heads, 64, at.cfg.head_dim) and c.blocks * 64 >= at.cfg.max_len
+                    and all(t.device == device for t in c.tensors()))
         return (all(_plain(t, dtype, device) for t in (*(m.weight for m in lin), n.weight, at.k_cache, at.v_cache))
                 and at.k_cache.shape == shape and at.v_cache.shape == shape and at.cfg.max_len == shape[2])
 
@@ -133,6 +169,11 @@ class DecoderLayer(nn.Module):
         import flash_gemv  # noqa: F401  (raises if the HIP op library is missing)
 
         at, n = self.self_attn, self.input_layernorm
+        if at.kv8 is not None:
+            h = torch.ops.flash_gemv.cats_kv8_attention_step(h, h if normed is None else normed, n.weight if normed is None else None, n.eps,
+                                                             at.q_proj.weight, at.k_proj.weight, at.v_proj.weight, at.o_proj.weight,
+                                                             *at.kv8.tensors(), cos_table, sin_table, positions)
+            return self._mlp_tail(h, next_norm)
         h = torch.ops.flash_gemv.cats_attention_step(h, h if normed is None else normed, n.weight if normed is None else None, n.eps,
                                                      at.q_proj.weight, at.k_proj.weight, at.v_proj.weight, at.o_proj.weight,
                                                      at.k_cache, at.v_cache, cos_table, sin_table, positions)
@@ -172,9 +213,11 @@ class LlamaDecoder(nn.Module):
         if self._takes_step(h, positions):
             return self._forward_step(h, positions)
         cos, sin = self.cos_table[positions], self.sin_table[positions]
-        slots = torch.arange(cfg.max_len, device=tokens.device)
-        mask = torch.zeros(positions.numel(), cfg.max_len, dtype=self.dtype, device=tokens.device)
-        mask.masked_fill_(slots[None, :] > positions[:, None], float("-inf"))
+        mask = None
+        if cfg.kv_cache == "dtype":
+            slots = torch.arange(cfg.max_len, device=tokens.device)
+            mask = torch.zeros(positions.numel(), cfg.max_len, dtype=self.dtype, device=tokens.device)
+            mask.masked_fill_(slots[None, :] > positions[:, None], float("-inf"))
         normed = None
         for i, layer in enumerate(self.layers):
             next_norm = self.layers[i + 1].input_layernorm if i + 1 < len(self.layers) else self.norm
@@ -270,6 +313,24 @@ class LlamaDecoder(nn.Module):
             acts[i] = None
         return thresholds
 
+    def _captured(self, step, state):
+        """step() as a HIP graph.  The two steps spent on capture are taken back: `state` and the caches are as they were."""
+        kept = [*state, *(t for l in self.layers for t in l.self_attn.caches()[0])]
+        snap = [t.clone() for t in kept]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()                                                       # warm-up on the capture stream (allocations)
+            side.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        for t, s in zip(kept, snap):
+            t.copy_(s)
+        return graph
+
     @torch.no_grad()
     def generate_greedy(self, prompt, gen_len: int, use_graph: bool = True):
         """Greedy decode; returns (tokens (gen_len,), seconds for tokens 2..gen_len).  The first generated token
@@ -293,26 +354,7 @@ class LlamaDecoder(nn.Module):
             pos.add_(1)
             step_idx.add_(1)
 
-        graph = None
-        if use_graph:
-            snap = [t.clone() for t in (tok, pos, step_idx, out)]
-            caches = [(l.self_attn.k_cache.clone(), l.self_attn.v_cache.clone()) for l in self.layers]
-            side = torch.cuda.Stream()
-            side.wait_stream(torch.cuda.current_stream())
-            with torch.cuda.stream(side):
-                step()                                                   # warm-up on the capture stream (allocations)
-                side.synchronize()
-                graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(graph, stream=side):
-                    step()
-            torch.cuda.current_stream().wait_stream(side)
-            torch.cuda.synchronize()
-            for t, s in zip((tok, pos, step_idx, out), snap):            # rewind the two steps spent on capture
-                t.copy_(s)
-            for l, (k, v) in zip(self.layers, caches):
-                l.self_attn.k_cache.copy_(k)
-                l.self_attn.v_cache.copy_(v)
-            del caches
+        graph = self._captured(step, (tok, pos, step_idx, out)) if use_graph else None
         torch.cuda.synchronize()
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record()
@@ -325,6 +367,54 @@ class LlamaDecoder(nn.Module):
         torch.cuda.synchronize()
         return out.clone(), e0.elapsed_time(e1) * 1e-3
 
+
+    @torch.no_grad()
+    def generate_beams(self, prompt, beams: int, gen_len: int, eos: int = -1, use_graph: bool = True):
+        """Beam search from prompt (groups, P), the groups' prompts of one length: the `beams` best continuations of gen_len tokens of each that the
+        search finds, by the sum of their tokens' log-probabilities.  Returns (tokens (groups, beams, gen_len), scores (groups, beams) float), best
+        first.  A beam that has met eos goes on as eos at no cost.  Selection, the moving of caches and the history stay on the GPU."""
+        import flash_gemv
+
+        dev, (G, P) = prompt.device, prompt.shape
+        if not (1 <= beams <= 16 and gen_len >= 1 and P >= 1 and P + gen_len <= self.cfg.max_len):
+            raise ValueError("1..16 beams, and a prompt and as many tokens as the cache has room for")
+        self.reset_cache(G)
+        logits = self.forward(prompt, torch.arange(P, device=dev))[:, -1:]
+        finish = lambda d: d if eos >= 0 else None
+        scores, _, tokens, done = flash_gemv.cats_beam_select(logits, torch.zeros(G, 1, device=dev), None, eos, beams)
+        for layer in self.layers:
+            layer.self_attn.repeat_cache(beams)
+        # parents and tokens of every step; the best beams' words are traced back at the end
+        parents_at = torch.zeros(gen_len, G, beams, dtype=torch.int64, device=dev)
+        tokens_at = torch.zeros_like(parents_at)
+        tokens_at[0] = tokens
+        pos = torch.full((1,), P, dtype=torch.int64, device=dev)
+        at = torch.ones(1, dtype=torch.int64, device=dev)
+        caches, slots = [], []
+        for layer in self.layers:
+            c, s = layer.self_attn.caches()
+            caches += c
+            slots += s
+
+        def step():
+            lg = self.forward(tokens.view(-1, 1), pos)[:, -1].unflatten(0, (G, beams))
+            best, parents, words, ended = flash_gemv.cats_beam_select(lg, scores, finish(done), eos)
+            pos.add_(1)
+            flash_gemv.cats_cache_reorder(caches, slots, parents, pos)
+            parents_at.index_copy_(0, at, parents[None])
+            tokens_at.index_copy_(0, at, words[None])
+            at.add_(1)
+            scores.copy_(best), tokens.copy_(words), done.copy_(ended)
+
+        graph = self._captured(step, (tokens, scores, done, pos, at, parents_at, tokens_at)) if use_graph and gen_len > 1 else None
+        for _ in range(gen_len - 1):
+            step() if graph is None else graph.replay()
+        out = torch.empty(G, beams, gen_len, dtype=torch.int64, device=dev)
+        beam = torch.arange(beams, device=dev).expand(G, beams)
+        for i in range(gen_len - 1, -1, -1):
+            out[:, :, i] = tokens_at[i].gather(1, beam)
+            beam = parents_at[i].gather(1, beam)
+        return out, scores
 
     @torch.no_grad()
     def decode_forced(self, prompt, forced):

@@ -276,6 +276,16 @@ int cats_kv8_attention(const void* q, const int64_t* q_strides, const int64_t* s
                        float scale, int window, void* out, int B, int T, int heads, int kv_heads, int D, int blocks, int dtype, void* scratch,
                        size_t scratch_bytes, void* stream);
 
+/* cats_attention_step over such a cache, with as many cached heads as query heads: k and v of the new token go to the tails, and the block that
+ * it completes is quantised beside attention.  q is rounded to dtype before the products.  Limits on B and H are those of cats_linear; position lies
+ * in [0, max_len), max_len <= 64 * blocks, and what the cache holds ends at it; elsewhere nothing is stored and out is NaN.  Three launches, four
+ * where the cache is long enough to be split.  scratch: 256-byte aligned, at least cats_kv8_attention_step_scratch_bytes(), nothing in it needs to be set. */
+size_t cats_kv8_attention_step_scratch_bytes(int B, int H, int heads, int blocks);
+int cats_kv8_attention_step(const void* h, const void* x, const void* norm_weight, float eps, const void* wq, const void* wk, const void* wv,
+                            const void* wo, void* k8, void* v8, float* k_scale, float* v_scale, void* k_tail, void* v_tail, const void* cos_table,
+                            const void* sin_table, const int64_t* position, void* out, int B, int H, int heads, int blocks, int max_len, int dtype,
+                            void* scratch, size_t scratch_bytes, void* stream);
+
 /* ---- beam search ---- */
 #define CATS_MAX_BEAMS 16
 
