@@ -57,16 +57,19 @@ int check_span(const int64_t* start, int start_step, const int64_t* count, int c
   return (start_step == 0 || start_step == 1) && (count_step == 0 || count_step == 1) ? CATS_OK : CATS_ERR_SHAPE;
 }
 
+constexpr int kStepRows = 64;  // rows of queries a cached head up to which they are taken 16 at a time
+
 }  // namespace
 
 KvAttnPlan kv8_attn_plan(int B, int T, int heads, int kv_heads, int blocks, int window) {
   const int cus = current_device_cus(), rows = T * (heads / kv_heads);
-  const long long groups = (long long)B * kv_heads * ((rows + 15) / 16);
+  KvAttnPlan plan = {rows > kStepRows, 1, false};
+  const int per = plan.prompt ? kKvPromptRows : 16, unit = plan.prompt ? kKvPromptUnit : 4;
+  const long long groups = (long long)B * kv_heads * ((rows + per - 1) / per);
   // tiles that a workgroup's queries see at most
-  const int tiles = window ? (int)min((long long)blocks, ((long long)window + 16 + 2 * kKvBlock) / kKvBlock) : blocks;
-  KvAttnPlan plan = {1, false};
-  const long long want = (4ll * cus + groups - 1) / groups;
-  plan.splits = (int)max(1ll, min(want, (long long)(tiles + 3) / 4));
+  const int tiles = window ? (int)min((long long)blocks, ((long long)window + per + 2 * kKvBlock) / kKvBlock) : blocks;
+  const long long want = ((plan.prompt ? 2ll : 4ll) * cus + groups - 1) / groups;
+  plan.splits = (int)max(1ll, min(want, (long long)(tiles + unit - 1) / unit));
   return plan;
 }
 

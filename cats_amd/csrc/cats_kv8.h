@@ -521,6 +521,287 @@ __global__ __launch_bounds__(256) void kv8_attn_step_kernel(KvAttnArgs p) {
   }
 }
 
+// Many new tokens: 128 rows of queries a workgroup, 32 a wave, all of whose waves share the tiles of 64 keys, which come through LDS in 8 bits,
+// the next one's loads in flight over this one's products.  The same steps as above with v_mfma_f32_32x32x16:
+//   S^T   tile u, row 8 a + 4 h + i of the result: token 32 u + 16 h + 4 a + i, in lanes of half h = lane / 32; columns are queries
+//   O^T   operand of step (u, v): tokens 32 u + 16 h + 8 v .. + 7, again those whose weights the lane has
+// Rows of LDS are 16-byte pieces, exchanged within a row so that any 16 lanes in order find the 64 banks once each.
+// Workgroups with the most keys start first.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <class DT> struct Mma32;
+template <> struct Mma32<F16> {
+  static __device__ __forceinline__ f32x16 run(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Mma32<BF16> {
+  static __device__ __forceinline__ f32x16 run(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+// Which piece of token t's row of K is exchanged with piece 0: of the lanes that read together, tokens differ in bits 0, 1, 4 and 2.
+template <int D>
+__device__ __forceinline__ int kv_swap_k(int t) {
+  if (D == 256) return (t & 3) | (t >> 4 & 1) << 2 | (t >> 2 & 1) << 3;
+  if (D == 128) return (t >> 1 & 1) | (t >> 4 & 1) << 1 | (t >> 2 & 1) << 2;
+  if (D == 64) return (t >> 4 & 1) | (t >> 2 & 1) << 1;
+  return t >> 4 & 1;
+}
+__device__ __forceinline__ int kv_swap_v(int d) { return d >> 2 & 3; }
+
+constexpr int kKvPromptRows = 128, kKvPromptUnit = 8;  // rows of a workgroup; tiles that make a split worth while
+template <class DT, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(KvAttnArgs p) {
+  constexpr int ROWS = kKvPromptRows, C = D / 32, NW = D / 32, PK = D / 16, NL = D * kKvBlock / 16 / 256 > 0 ? D * kKvBlock / 16 / 256 : 1;
+  constexpr int kVecs = D * kKvBlock / 16;  // of a tile's keys, and of its values
+  typedef Kv<DT> F;
+  __shared__ u32x4 s_kv[2][2][kVecs];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, m = lane & 31, h = lane >> 5;
+  const int pair = blockIdx.x, r0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * ROWS, split = blockIdx.z, rows = p.T * p.group;
+  const int b = pair / p.c.heads;
+  int start, n;
+  KvTiles t;
+  const bool ok = kv_span(p.span, b, p.T, start, n);
+  if (!kv_tiles<ROWS, kKvPromptUnit>(p, r0, start, n, t) || !ok) {
+    if (split == 0) kv_fill_rows<DT>(p, pair, r0, ROWS, n, ok, D, tid, 256);
+    return;
+  }
+  if (split >= t.active) return;
+
+  const int mine = r0 + 32 * wave + m, row = min(mine, rows - 1), pos = start + min(row / p.group, n - 1);
+  const int first = p.window ? pos - p.window : -1;  // the query sees first + 1 .. pos
+  // the wave's own keys
+  const int lo_pos = start + min((r0 + 32 * wave) / p.group, n - 1), hi_pos = start + min((r0 + 32 * wave + 31) / p.group, n - 1);
+  u32x4 qf[C][2];
+  {
+    const uint16_t* q = p.q + b * p.q_row + (row / p.group) * p.q_tok + ((pair - b * p.c.heads) * p.group + row % p.group) * p.q_head;
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int v = 0; v < 2; v++) qf[c][v] = *(const u32x4*)(q + 32 * c + 16 * h + 8 * v);
+  }
+  const u32x4* k8 = (const u32x4*)p.c.k8 + (size_t)pair * p.c.blocks * kVecs;
+  const u32x4* v8 = (const u32x4*)p.c.v8 + (size_t)pair * p.c.blocks * kVecs;
+  const float* kscale = p.c.ks + (size_t)pair * p.c.blocks;
+  const float* vscale = p.c.vs + (size_t)pair * p.c.blocks;
+
+  u32x4 kn[NL], vn[NL];
+  auto fetch = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < NL; i++)
+      if (kVecs >= 256 || tid < kVecs) {
+        kn[i] = k8[(size_t)tile * kVecs + i * 256 + tid];
+        vn[i] = v8[(size_t)tile * kVecs + i * 256 + tid];
+      }
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < NL; i++)
+      if (kVecs >= 256 || tid < kVecs) {
+        const int at = i * 256 + tid, tok = at / PK, d = at / 4;
+        s_kv[buf][0][tok * PK + ((at % PK) ^ kv_swap_k<D>(tok))] = kn[i];
+        s_kv[buf][1][d * 4 + ((at % 4) ^ kv_swap_v(d))] = vn[i];
+      }
+  };
+
+  float top = -FLT_MAX, sum = 0.f;
+  f32x16 o[NW];
+#pragma unroll
+  for (int w = 0; w < NW; w++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) o[w][e] = 0.f;
+  const int ktok = 16 * (m >> 2 & 1) + 4 * (m >> 3) + (m & 3);  // token of this lane's row of K in tile 0; 32 more in tile 1
+
+  // weights of a tile from its scores; returns them as operands
+  auto weigh = [&](f32x16 (&s)[2], float ks, float vs, u32x4 (&pf)[2][2]) {
+    const float sc = p.scale * ks, lv = __builtin_amdgcn_logf(vs);
+    float mx = s[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[u][e]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+    const float now = fmaxf(top, fmaf(mx, sc, lv)), off = lv + F::HEAD - now;
+    if (__any(now > top)) {
+      const float keep = __builtin_amdgcn_exp2f(top - now);
+      sum *= keep;
+#pragma unroll
+      for (int w = 0; w < NW; w++) o[w] *= keep;
+      top = now;
+    }
+    float add = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        s[u][e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], sc, off));
+        add += s[u][e];
+      }
+#pragma unroll
+      for (int v = 0; v < 2; v++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) pf[u][v][e] = DT::pack(s[u][8 * v + 2 * e], s[u][8 * v + 2 * e + 1]);
+    }
+    sum = fmaf(add, __builtin_amdgcn_rcpf(vs), sum);
+  };
+  auto seen = [&](int key) { return key <= pos && key > first; };
+  auto mask = [&](f32x16 (&s)[2], int tile) {
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[u][e] = seen(tile * kKvBlock + 32 * u + 16 * h + e) ? s[u][e] : -INFINITY;
+  };
+  // O of elements 32 w .. with numbers of V that are not finite taken out of the operands a; bad has 1 in their places
+  auto add_part = [&](int w, int tile, u32x4 (&a)[2][2], u32x4 (&bad)[2][2], u32x4 (&pf)[2][2]) {
+    f32x16 z;
+#pragma unroll
+    for (int e = 0; e < 16; e++) z[e] = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int v = 0; v < 2; v++) {
+        u32x4 one;
+        const int key = tile * kKvBlock + 32 * u + 16 * h + 8 * v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) one[e] = (seen(key + 2 * e) ? F::kOne : 0u) | (seen(key + 2 * e + 1) ? F::kOne << 16 : 0u);
+        o[w] = Mma32<DT>::run(a[u][v], pf[u][v], o[w]);
+        z = Mma32<DT>::run(bad[u][v], one, z);
+      }
+#pragma unroll
+    for (int e = 0; e < 16; e++) o[w][e] = z[e] > 0.f ? NAN : o[w][e];
+  };
+
+  const int end8 = min(t.tile_hi, t.last - 1);  // last tile in 8 bits
+  int tile = t.tile_lo + split, buf = 0;
+  if (tile <= end8) {
+    fetch(tile);
+    store(0);
+  }
+  lds_barrier();
+  for (; tile <= end8; tile += t.active, buf ^= 1) {
+    const bool more = tile + t.active <= end8;
+    if (more) fetch(tile + t.active);
+    const int key0 = tile * kKvBlock;
+    if (key0 <= hi_pos && !(p.window && key0 + kKvBlock - 1 <= lo_pos - p.window)) {  // some query of the wave sees some key
+      const bool part = key0 + kKvBlock - 1 > lo_pos || (p.window && key0 <= hi_pos - p.window);
+      f32x16 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[u][e] = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const int tok = ktok + 32 * u;
+          const u32x4 kk = s_kv[buf][0][tok * PK + ((2 * c + h) ^ kv_swap_k<D>(tok))];
+          s[u] = Mma32<DT>::run(kv_wide<DT>(kk[0], kk[1]), qf[c][0], s[u]);
+          s[u] = Mma32<DT>::run(kv_wide<DT>(kk[2], kk[3]), qf[c][1], s[u]);
+        }
+      if (part) mask(s, tile);
+      u32x4 pf[2][2];
+      weigh(s, kscale[tile], vscale[tile], pf);
+#pragma unroll
+      for (int w = 0; w < NW; w++) {
+        const int d = 32 * w + m;
+        u32x4 vv[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) vv[u] = s_kv[buf][1][d * 4 + ((2 * u + h) ^ kv_swap_v(d))];
+        if (!part) {
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            o[w] = Mma32<DT>::run(kv_wide<DT>(vv[u][0], vv[u][1]), pf[u][0], o[w]);
+            o[w] = Mma32<DT>::run(kv_wide<DT>(vv[u][2], vv[u][3]), pf[u][1], o[w]);
+          }
+        } else {
+          u32x4 a[2][2], bad[2][2];
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+              uint32_t w0 = vv[u][2 * v], w1 = vv[u][2 * v + 1];
+              const uint32_t b0 = kv_fix8(w0), b1 = kv_fix8(w1);
+              a[u][v] = kv_wide<DT>(w0, w1);
+              bad[u][v] = kv_wide<DT>(b0, b1);
+            }
+          add_part(w, tile, a, bad, pf);
+        }
+      }
+    }
+    if (more) store(buf ^ 1);
+    lds_barrier();
+  }
+  // the tail, by the split whose turn it would be, from memory: one tile of the last rows only
+  if (t.tile_hi == t.last && (t.last - t.tile_lo) % t.active == split && t.last * kKvBlock <= hi_pos) {
+    const uint16_t* kt = p.c.kt + (size_t)pair * kKvBlock * D;
+    const uint16_t* vt = p.c.vt + (size_t)pair * kKvBlock * D;
+    f32x16 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[u][e] = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int v = 0; v < 2; v++) s[u] = Mma32<DT>::run(*(const u32x4*)(kt + (ktok + 32 * u) * D + 32 * c + 16 * h + 8 * v), qf[c][v], s[u]);
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[u][e] = fmaf(s[u][e], 0.f, s[u][e]);  // a key that is not finite makes the score NaN, as in e4m3
+    }
+    mask(s, t.last);
+    u32x4 pf[2][2];
+    weigh(s, 1.f, 1.f, pf);
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+      u32x4 a[2][2], bad[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int v = 0; v < 2; v++) {
+          a[u][v] = *(const u32x4*)(vt + (32 * w + m) * kKvBlock + 32 * u + 16 * h + 8 * v);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            uint32_t x = a[u][v][e];
+            bad[u][v][e] = kv_fix16<DT>(x);
+            a[u][v][e] = x;
+          }
+        }
+      add_part(w, t.last, a, bad, pf);
+    }
+  }
+  sum += __shfl_xor(sum, 32, kWave);
+  if (mine >= rows) return;
+  if (t.active == 1) {
+    const bool dead = mine / p.group >= n;
+    const float f = 1.f / sum;
+    uint16_t* out = kv_out_row(p, pair, mine, D);
+#pragma unroll
+    for (int w = 0; w < NW; w++)
+#pragma unroll
+      for (int a = 0; a < 4; a++) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = dead ? 0.f : o[w][4 * a + e] * f;
+        *(u32x2*)(out + 32 * w + 8 * a + 4 * h) = u32x2{DT::pack(x[0], x[1]), DT::pack(x[2], x[3])};
+      }
+  } else {
+    const size_t at = ((size_t)pair * p.splits + split) * rows + mine;
+#pragma unroll
+    for (int w = 0; w < NW; w++)
+#pragma unroll
+      for (int a = 0; a < 4; a++) {
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = o[w][4 * a + e];
+        *(f32x4*)(p.part + at * D + 32 * w + 8 * a + 4 * h) = x;
+      }
+    if (h == 0) {
+      float* ml = p.part + (size_t)p.pairs * p.splits * rows * D + 2 * at;
+      ml[0] = top;
+      ml[1] = sum;
+    }
+  }
+}
+
 // The splits' results, in a fixed order.  A workgroup per (pair, 16 rows); rows whose cache was one split's are done already.
 template <class DT, int D, int ROWS, int UNIT>
 __global__ __launch_bounds__(256) void kv8_join_kernel(KvAttnArgs p) {

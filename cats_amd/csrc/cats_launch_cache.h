@@ -9,6 +9,7 @@ namespace cats {
 
 // The cache in 8 bits (cats_kv8.h), 16-bit types.  launch_kv8_attn fills in what the plan decides.
 struct KvAttnPlan {
+  bool prompt; // 128 rows a workgroup
   int splits;  // of a row's cache
   bool seal;   // the new tokens are in the tails only: quantise the blocks they complete
 };

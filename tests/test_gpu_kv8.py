@@ -175,6 +175,21 @@ def test_attention_of_several_tokens(T, heads, kv, lengths, window, dtype):
     _check(2, T, heads, kv, 64, dtype, lengths, 5, window)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("T,heads,kv,lengths,window", [(150, 3, 1, [150, 400], 0), (150, 3, 1, [400, 192], 77), (129, 2, 2, [129, 193], 0), (21, 7, 1, [21, 300], 0), (65, 1, 1, [65, 128], 0)])
+def test_attention_of_prompts(T, heads, kv, lengths, window, D, dtype):
+    """Many rows a workgroup: tiles of rows that end inside a token's heads, waves without a row, rows that end in the tail and before it."""
+    _check(2, T, heads, kv, D, dtype, lengths, 8, window)
+
+
+@pytest.mark.parametrize("dtype,D,T,lengths,window,count", [
+    (F16, 128, 40, [4000, 100], 0, [40, 40]), (BF16, 64, 70, [6000, 3000], 2500, [70, 3]), (BF16, 256, 33, [1700, 1600], 0, [0, 33]), (F16, 32, 90, [3000, 2999], 64, [90, 90])])
+def test_attention_of_pieces_behind_long_caches(dtype, D, T, lengths, window, count):
+    """Many rows and a cache in splits, of which a short row, a window or an empty row leaves some without a tile."""
+    _check(2, T, 2, 1, D, dtype, lengths, max(lengths) // 64 + 3, window, count)
+
+
 @pytest.mark.parametrize("T,count,lengths", [(5, [5, 2, 0, -4], [130, 64, 70, 65]), (40, [40, 1, 17, 99], [140, 65, 128, 192]), (1, [1, 0, 1, 2], [64, 10, 1, 130])])
 @pytest.mark.parametrize("D", [64, 128])
 def test_attention_of_ragged_rows(T, count, lengths, D):
