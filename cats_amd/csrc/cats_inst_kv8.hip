@@ -36,13 +36,15 @@ struct KvLaunch {
       const dim3 grid(a.pairs, (rows + kKvPromptRows - 1) / kKvPromptRows, a.splits);
       hipError_t e = launch_kernel(kv8_attn_prompt_kernel<DT, D>, grid, dim3(256), 0, stream, a);
       if (e == hipSuccess && a.splits > 1)
-        e = launch_kernel(kv8_join_kernel<DT, D, kKvPromptRows, kKvPromptUnit>, dim3(a.pairs, (rows + 15) / 16), dim3(256), 0, stream, a);
+        e = launch_kernel(kv8_join_kernel<DT, D, kKvPromptRows, kKvPromptUnit>, dim3(a.pairs * rows), dim3(256), 0, stream, a);
       return e;
     }
-    auto kern = plan.seal ? kv8_attn_step_kernel<DT, D, true> : kv8_attn_step_kernel<DT, D, false>;
+    auto kern = plan.seal                   ? kv8_attn_step_kernel<DT, D, false, true>
+                : a.T > 1 || a.window ? kv8_attn_step_kernel<DT, D, true, false>
+                                      : kv8_attn_step_kernel<DT, D, false, false>;
     hipError_t e = launch_kernel(kern, dim3(a.pairs, a.splits + plan.seal, (rows + 15) / 16), dim3(256), 0, stream, a);
     if (e == hipSuccess && a.splits > 1)
-      e = launch_kernel(kv8_join_kernel<DT, D, 16, 4>, dim3(a.pairs, (rows + 15) / 16), dim3(256), 0, stream, a);
+      e = launch_kernel(kv8_join_kernel<DT, D, 16, kKvStepWaves>, dim3(a.pairs * rows), dim3(256), 0, stream, a);
     return e;
   }
   static hipError_t attn(int D, const KvAttnPlan& plan, const KvAttnArgs& a, hipStream_t stream) {

@@ -281,23 +281,30 @@ __device__ __forceinline__ uint32_t kv_fix16(uint32_t& w) {
   return m * Kv<DT>::kOne;
 }
 
-// One new token, or a few: ROWS = 16 rows of queries, the cache split over workgroups and over the four waves of each, the waves' results
-// joined in LDS and the workgroups' by kv8_join_kernel.  Each wave takes 64 tokens at a time:
-//   S^T = K . Q^T   tile t, row 4 g + i of the 16x16 result: token 16 g + 4 t + i, in lanes of group g = lane / 16; columns are queries
+// One new token, or a few: 16 rows of queries, the cache split over workgroups and over the four waves of each, the waves' results joined in LDS
+// and the workgroups' by kv8_join_kernel.  Each wave takes 64 tokens at a time:
+//   S^T = K . Q^T   tile i, row 4 g + e of the 16x16 result: token 16 g + 4 i + e, in lanes of group g = lane / 16; columns are queries
 //   O^T += V^T . P  the weights of lane group g are those of tokens 16 g .. + 15 in order: what the lane has to supply as operand
 // so weights go from one product into the other without leaving their lane, and every load of the cache is 16 bytes a lane of 1 KiB in a
-// row (V) or of whole lines (K).  The numbers become 16-bit operands (two an instruction), the blocks' scales go into the
-// exponent: with w = s * ks * scale + log2(vs), weights are 2^(w - max w) <= 1, O sums them times the codes, and the sum of
-// weights adds them divided by vs.
+// row (V) or of whole lines (K).  The next tile's keys are asked for when this one's have been used, and so are its values.  The numbers become
+// 16-bit operands (two an instruction), the blocks' scales go into the exponent: with w = s * ks * scale + log2(vs), weights are
+// 2^(w - max w) <= 1, O sums them times the codes, and the sum of weights adds them divided by vs.
+// The tail is four times sixteen tokens, for a wave each: tile `wave` of the four, and one product over sixteen tokens.
+// A masked weight is 0, but 0 times a NaN is not: where keys are masked, numbers of V that are not finite are taken out and the
+// queries that see one are set to NaN.
+// MASK: queries that see different keys, or a window.  One token without a window sees all of every tile but the tail.
 // SEAL: the tokens are in the tails and nowhere else yet.  One workgroup a pair more quantises the block that they complete; nobody reads that block
 // in this launch.
-// A masked weight is 0, but 0 times a NaN is not: where a tile is seen in part, numbers of V that are not finite are taken out and the
-// rows that see one are set to NaN.
-template <class DT, int D, bool SEAL>
-__global__ __launch_bounds__(256) void kv8_attn_step_kernel(KvAttnArgs p) {
-  constexpr int W = 4, ROWS = 16, C = D / 64, NU = D / 16, NK = D >= 64 ? C : 1;
+constexpr int kKvStepWaves = 4;
+// Waves a SIMD, as far as registers allow.
+constexpr int kv_step_waves(int D, bool mask) { return D == 256 ? 1 : D == 128 ? (mask ? 2 : 3) : D == 64 && mask ? 3 : 4; }
+template <class DT, int D, bool MASK, bool SEAL>
+__global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_kernel(KvAttnArgs p) {
+  constexpr bool AHEAD = D < 256 || !MASK;  // the next tile's keys over this one's values: registers
+  constexpr int W = kKvStepWaves, ROWS = 16, NU = D / 16, NK = D >= 64 ? D / 64 : 1, NV = D >= 64 ? 2 : 1;
   typedef Kv<DT> F;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & (kWave - 1), m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pair = blockIdx.x, split = blockIdx.y, r0 = blockIdx.z * ROWS, rows = p.T * p.group;
   const int b = pair / p.c.heads;
   int start, n;
@@ -321,160 +328,206 @@ __global__ __launch_bounds__(256) void kv8_attn_step_kernel(KvAttnArgs p) {
 
   // queries: operand of step (c, v) is elements 64 c + 16 g + 8 v .. + 7 (of 32 elements: 8 g .. + 7)
   const int row = min(r0 + m, rows - 1), tok = min(row / p.group, n - 1), pos = start + tok;
-  const uint16_t* q = p.q + b * p.q_row + (row / p.group) * p.q_tok + ((pair - b * p.c.heads) * p.group + row % p.group) * p.q_head;
-  u32x4 qf[NK][2];
+  const int first = MASK && p.window ? pos - p.window : -1;  // the query sees first + 1 .. pos
+  const int d0 = D >= 64 ? 16 * g : 8 * g;
+  u32x4 qf[NK][NV];
+  {
+    const uint16_t* q = p.q + b * p.q_row + (row / p.group) * p.q_tok + ((pair - b * p.c.heads) * p.group + row % p.group) * p.q_head;
 #pragma unroll
-  for (int c = 0; c < NK; c++)
+    for (int c = 0; c < NK; c++)
 #pragma unroll
-    for (int v = 0; v < (D >= 64 ? 2 : 1); v++) qf[c][v] = *(const u32x4*)(q + (D >= 64 ? 64 * c + 16 * g + 8 * v : 8 * g));
-
-  const size_t kv = (size_t)pair;
-  const uint8_t* k8 = p.c.k8 + kv * p.c.blocks * kKvBlock * D;
-  const uint8_t* v8 = p.c.v8 + kv * p.c.blocks * kKvBlock * D;
+      for (int v = 0; v < NV; v++) qf[c][v] = *(const u32x4*)(q + 64 * c + d0 + 8 * v);
+  }
   const int ktok = 16 * (m >> 2) + (m & 3);  // token of this lane's row of K in tile 0; 4 more in each of the next
+  const uint8_t* k8 = p.c.k8 + (size_t)pair * p.c.blocks * kKvBlock * D + ktok * D + d0;
+  const uint8_t* v8 = p.c.v8 + (size_t)pair * p.c.blocks * kKvBlock * D + m * kKvBlock + 16 * g;
+  const float* kscale = p.c.ks + (size_t)pair * p.c.blocks;
+  const float* vscale = p.c.vs + (size_t)pair * p.c.blocks;
+
+  u32x4 kk[4][NK], vv[NU];
+  auto fetch_k = [&](int tile) {
+    const uint8_t* k = k8 + (size_t)tile * kKvBlock * D;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int c = 0; c < NK; c++) {
+        if constexpr (D >= 64) {
+          kk[i][c] = load_stream((const u32x4*)(k + 4 * i * D + 64 * c));
+        } else {
+          const u32x2 w = *(const u32x2*)(k + 4 * i * D);
+          kk[i][c] = u32x4{w[0], w[1], 0u, 0u};
+        }
+      }
+  };
+  auto fetch_v = [&](int tile) {
+    const uint8_t* v = v8 + (size_t)tile * kKvBlock * D;
+#pragma unroll
+    for (int u = 0; u < NU; u++) vv[u] = load_stream((const u32x4*)(v + 16 * u * kKvBlock));
+  };
+  const int step = t.active * W, end8 = min(t.tile_hi, t.last - 1);  // last tile in 8 bits
+  int tile = t.tile_lo + split * W + wave;
 
   float top = -FLT_MAX, sum = 0.f;
   f32x4 o[NU];
 #pragma unroll
   for (int u = 0; u < NU; u++) o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  for (int tile = t.tile_lo + split * W + wave; tile <= t.tile_hi; tile += t.active * W) {
-    const bool tail = tile == t.last;
-    const int key0 = tile * kKvBlock + 16 * g;  // of this lane's weights
-    const bool part = tail || tile * kKvBlock + kKvBlock - 1 > t.pos_lo || (p.window && tile * kKvBlock <= t.pos_hi - p.window);
-    f32x4 s[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    u32x4 vv[NU];
-    float ks = 1.f, vs = 1.f;
-    if (!tail) {
-      const uint8_t* kb = k8 + (size_t)tile * kKvBlock * D;
-      const uint8_t* vb = v8 + (size_t)tile * kKvBlock * D;
-      ks = p.c.ks[kv * p.c.blocks + tile];
-      vs = p.c.vs[kv * p.c.blocks + tile];
-      if constexpr (D >= 64) {
-        u32x4 kk[4][NK];
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-          for (int c = 0; c < NK; c++) kk[i][c] = load_stream((const u32x4*)(kb + (ktok + 4 * i) * D + 64 * c + 16 * g));
-#pragma unroll
-        for (int u = 0; u < NU; u++) vv[u] = load_stream((const u32x4*)(vb + (16 * u + m) * kKvBlock + 16 * g));
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-          for (int c = 0; c < NK; c++) {
-            s[i] = Mma<DT>::run(kv_wide<DT>(kk[i][c][0], kk[i][c][1]), qf[c][0], s[i]);
-            s[i] = Mma<DT>::run(kv_wide<DT>(kk[i][c][2], kk[i][c][3]), qf[c][1], s[i]);
-          }
-      } else {
-        u32x2 kk[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) kk[i] = *(const u32x2*)(kb + (ktok + 4 * i) * D + 8 * g);
-#pragma unroll
-        for (int u = 0; u < NU; u++) vv[u] = load_stream((const u32x4*)(vb + (16 * u + m) * kKvBlock + 16 * g));
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[i] = Mma<DT>::run(kv_wide<DT>(kk[i][0], kk[i][1]), qf[0][0], s[i]);
-      }
-    } else {
-      const uint16_t* kb = p.c.kt + kv * kKvBlock * D;
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int c = 0; c < NK; c++)
-#pragma unroll
-          for (int v = 0; v < (D >= 64 ? 2 : 1); v++)
-            s[i] = Mma<DT>::run(*(const u32x4*)(kb + (ktok + 4 * i) * D + (D >= 64 ? 64 * c + 16 * g + 8 * v : 8 * g)), qf[c][v], s[i]);
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) s[i][e] = fmaf(s[i][e], 0.f, s[i][e]);  // a key that is not finite makes the score NaN, as in e4m3
-    }
-    if (part) {
-      const int first = p.window ? pos - p.window : -1;  // the query sees first + 1 .. pos
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int key = key0 + 4 * i + e;
-          s[i][e] = key <= pos && key > first ? s[i][e] : -INFINITY;
-        }
-    }
+  auto seen = [&](int key) { return key <= pos && (!MASK || key > first); };
+  // weights of this lane's N x 4 scores, in place; the lanes of a query agree on their largest
+  auto weigh = [&](f32x4* s, int N, float ks, float vs) {
     const float sc = p.scale * ks, lv = __builtin_amdgcn_logf(vs);
     float mx = s[0][0];
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < N; i++)
 #pragma unroll
       for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[i][e]);
     mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
     mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-    const float now = fmaxf(top, fmaf(mx, sc, lv)), keep = __builtin_amdgcn_exp2f(top - now), off = lv + F::HEAD - now;
-    top = now;
+    const float now = fmaxf(top, fmaf(mx, sc, lv)), off = lv + F::HEAD - now;
+    if (__any(now > top)) {
+      const float keep = __builtin_amdgcn_exp2f(top - now);
+      sum *= keep;
+#pragma unroll
+      for (int u = 0; u < NU; u++) o[u] *= keep;
+      top = now;
+    }
     float add = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < N; i++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], sc, off));
         add += s[i][e];
       }
-    sum = fmaf(sum, keep, add * __builtin_amdgcn_rcpf(vs));
-    u32x4 pf[2];  // the weights, rounded to the type the products take: half a step each, independent of one another
+    sum = fmaf(add, __builtin_amdgcn_rcpf(vs), sum);
+  };
+
+  if (tile <= end8) {
+    fetch_k(tile);
+    fetch_v(tile);
+    for (;;) {
+      const float ks = kscale[tile], vs = vscale[tile];
+      f32x4 s[4];
 #pragma unroll
-    for (int v = 0; v < 2; v++)
-      pf[v] = u32x4{DT::pack(s[2 * v][0], s[2 * v][1]), DT::pack(s[2 * v][2], s[2 * v][3]), DT::pack(s[2 * v + 1][0], s[2 * v + 1][1]),
-                    DT::pack(s[2 * v + 1][2], s[2 * v + 1][3])};
+      for (int i = 0; i < 4; i++) {
+        __builtin_amdgcn_sched_barrier(0);
+        s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < NU; u++) o[u] *= keep;
-    if (!part) {
+        for (int c = 0; c < NK; c++)
+#pragma unroll
+          for (int v = 0; v < NV; v++) s[i] = Mma<DT>::run(kv_wide<DT>(kk[i][c][2 * v], kk[i][c][2 * v + 1]), qf[c][v], s[i]);
+      }
+      const bool more = tile + step <= end8;
+      __builtin_amdgcn_sched_barrier(0);
+      if (AHEAD && more) fetch_k(tile + step);
+      __builtin_amdgcn_sched_barrier(0);
+      const int key0 = tile * kKvBlock + 16 * g;  // of this lane's weights
+      const bool part = MASK && (tile * kKvBlock + kKvBlock - 1 > t.pos_lo || (p.window && tile * kKvBlock <= t.pos_hi - p.window));
+      if (part) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[i][e] = seen(key0 + 4 * i + e) ? s[i][e] : -INFINITY;
+      }
+      weigh(s, 4, ks, vs);
+      u32x4 pf[2];  // the weights, rounded to the type the products take: half a step each, independent of one another
+#pragma unroll
+      for (int v = 0; v < 2; v++)
+        pf[v] = u32x4{DT::pack(s[2 * v][0], s[2 * v][1]), DT::pack(s[2 * v][2], s[2 * v][3]), DT::pack(s[2 * v + 1][0], s[2 * v + 1][1]),
+                      DT::pack(s[2 * v + 1][2], s[2 * v + 1][3])};
+      if (part) {
+        uint32_t some = 0;
+#pragma unroll
+        for (int u = 0; u < NU; u++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            uint32_t w = vv[u][e];
+            some |= kv_fix8(w);
+          }
+        if (__any(some != 0)) {
+          auto one = [&](int j) { return seen(key0 + j) ? F::kOne : 0u; };
+          u32x4 sees[2];
+#pragma unroll
+          for (int v = 0; v < 2; v++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) sees[v][e] = one(8 * v + 2 * e) | one(8 * v + 2 * e + 1) << 16;
+#pragma unroll
+          for (int u = 0; u < NU; u++) {
+            f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+              uint32_t w0 = vv[u][2 * v], w1 = vv[u][2 * v + 1];
+              const uint32_t b0 = kv_fix8(w0), b1 = kv_fix8(w1);
+              vv[u][2 * v] = w0;
+              vv[u][2 * v + 1] = w1;
+              z = Mma<DT>::run(kv_wide<DT>(b0, b1), sees[v], z);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[u][e] = z[e] > 0.f ? NAN : o[u][e];
+            __builtin_amdgcn_sched_barrier(0);  // one after the other: rare, and registers are short
+          }
+        }
+      }
 #pragma unroll
       for (int u = 0; u < NU; u++) {
+        if (u % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // operands of four products at a time
         o[u] = Mma<DT>::run(kv_wide<DT>(vv[u][0], vv[u][1]), pf[0], o[u]);
         o[u] = Mma<DT>::run(kv_wide<DT>(vv[u][2], vv[u][3]), pf[1], o[u]);
       }
-    } else {
-      u32x4 seen[2];  // 1 where the query sees the key
-      const int first = p.window ? pos - p.window : -1;
-      auto one = [&](int j) { return key0 + j <= pos && key0 + j > first ? Kv<DT>::kOne : 0u; };
+      __builtin_amdgcn_sched_barrier(0);
+      if (!more) break;
+      tile += step;
+      if (!AHEAD) fetch_k(tile);
+      fetch_v(tile);
+    }
+  }
+
+  // the tail, by the split whose turn it would be
+  if (t.tile_hi == t.last && (t.last - t.tile_lo) / W % t.active == split) {
+    const uint16_t* kt = p.c.kt + (size_t)pair * kKvBlock * D + (ktok + 4 * wave) * D + d0;
+    const uint16_t* vt = p.c.vt + (size_t)pair * kKvBlock * D + m * kKvBlock + 16 * g + 4 * wave;
+    u32x4 kq[NK][NV];
+    u32x2 vq[NU];
 #pragma unroll
-      for (int v = 0; v < 2; v++)
+    for (int c = 0; c < NK; c++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) seen[v][e] = one(8 * v + 2 * e) | one(8 * v + 2 * e + 1) << 16;
-      const uint16_t* vb = p.c.vt + kv * kKvBlock * D;
+      for (int v = 0; v < NV; v++) kq[c][v] = *(const u32x4*)(kt + 64 * c + 8 * v);
+#pragma unroll
+    for (int u = 0; u < NU; u++) vq[u] = *(const u32x2*)(vt + 16 * u * kKvBlock);
+    f32x4 s[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int c = 0; c < NK; c++)
+#pragma unroll
+      for (int v = 0; v < NV; v++) s[0] = Mma<DT>::run(kq[c][v], qf[c][v], s[0]);
+    const int key = t.last * kKvBlock + 16 * g + 4 * wave;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float x = fmaf(s[0][e], 0.f, s[0][e]);  // a key that is not finite makes the score NaN, as in e4m3
+      s[0][e] = seen(key + e) ? x : -INFINITY;
+    }
+    weigh(s, 1, 1.f, 1.f);
+    const u32x2 pf = u32x2{DT::pack(s[0][0], s[0][1]), DT::pack(s[0][2], s[0][3])};
+    uint32_t some = 0;
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+      uint32_t x = vq[u][0], y = vq[u][1];
+      some |= kv_fix16<DT>(x) | kv_fix16<DT>(y);
+      o[u] = DownMma<DT>::run(u32x2{x, y}, pf, o[u]);
+    }
+    if (__any(some != 0)) {
+      auto one = [&](int j) { return seen(key + j) ? F::kOne : 0u; };
+      const u32x2 sees = u32x2{one(0) | one(1) << 16, one(2) | one(3) << 16};
 #pragma unroll
       for (int u = 0; u < NU; u++) {
-        u32x4 a[2], bad[2];
-        if (tail) {
-#pragma unroll
-          for (int v = 0; v < 2; v++) {
-            a[v] = *(const u32x4*)(vb + (16 * u + m) * kKvBlock + 16 * g + 8 * v);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              uint32_t w = a[v][e];
-              bad[v][e] = kv_fix16<DT>(w);
-              a[v][e] = w;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int v = 0; v < 2; v++) {
-            uint32_t w0 = vv[u][2 * v], w1 = vv[u][2 * v + 1];
-            const uint32_t b0 = kv_fix8(w0), b1 = kv_fix8(w1);
-            a[v] = kv_wide<DT>(w0, w1);
-            bad[v] = kv_wide<DT>(b0, b1);
-          }
-        }
-        f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int v = 0; v < 2; v++) {
-          o[u] = Mma<DT>::run(a[v], pf[v], o[u]);
-          z = Mma<DT>::run(bad[v], seen[v], z);
-        }
+        uint32_t x = vq[u][0], y = vq[u][1];
+        const u32x2 bad = u32x2{kv_fix16<DT>(x), kv_fix16<DT>(y)};
+        const f32x4 z = DownMma<DT>::run(bad, sees, f32x4{0.f, 0.f, 0.f, 0.f});
+        __builtin_amdgcn_sched_barrier(0);  // one after the other: rare, and registers are short
 #pragma unroll
         for (int e = 0; e < 4; e++) o[u][e] = z[e] > 0.f ? NAN : o[u][e];
       }
     }
   }
+
   sum += __shfl_xor(sum, 16, kWave);
   sum += __shfl_xor(sum, 32, kWave);
 
@@ -802,35 +855,56 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   }
 }
 
-// The splits' results, in a fixed order.  A workgroup per (pair, 16 rows); rows whose cache was one split's are done already.
+// The splits' results, in a fixed order.  A workgroup per (pair, row): as many groups of D / 4 lanes as fit take every so manieth split, and LDS joins
+// the groups.  Rows whose cache was one split's are done already.  ROWS and UNIT are the attention kernel's.
 template <class DT, int D, int ROWS, int UNIT>
 __global__ __launch_bounds__(256) void kv8_join_kernel(KvAttnArgs p) {
-  const int pair = blockIdx.x, rows = p.T * p.group, j0 = blockIdx.y * 16;
+  constexpr int L = D / 4, G = 256 / L;
+  __shared__ __align__(16) float s_o[G][D];
+  __shared__ float s_top[G], s_sum[G];
+  const int rows = p.T * p.group, pair = blockIdx.x / rows, r = blockIdx.x - pair * rows, grp = threadIdx.x / L, d = threadIdx.x % L * 4;
   int start, n;
   KvTiles t;
-  if (!kv_span(p.span, pair / p.c.heads, p.T, start, n) || !kv_tiles<ROWS, UNIT>(p, j0 / ROWS * ROWS, start, n, t) || t.active == 1) return;
-  const float* ml = p.part + (size_t)p.pairs * p.splits * rows * D;
-  for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
-    const int r = j0 + i / (D / 4), d = i % (D / 4) * 4;
-    if (r >= rows) return;
-    const size_t at = (size_t)pair * p.splits * rows + r;
-    float most = -FLT_MAX;
-    for (int s = 0; s < t.active; s++) most = fmaxf(most, ml[2 * (at + (size_t)s * rows)]);
-    f32x4 num = f32x4{0.f, 0.f, 0.f, 0.f};
-    float den = 0.f;
-    for (int s = 0; s < t.active; s++) {
-      const size_t a = at + (size_t)s * rows;
-      const float f = __builtin_amdgcn_exp2f(ml[2 * a] - most);
-      const f32x4 x = *(const f32x4*)(p.part + a * D + d);
+  if (!kv_span(p.span, pair / p.c.heads, p.T, start, n) || !kv_tiles<ROWS, UNIT>(p, r / ROWS * ROWS, start, n, t) || t.active == 1) return;
+  const size_t at = (size_t)pair * p.splits * rows + r;
+  const float* ml = p.part + (size_t)p.pairs * p.splits * rows * D + 2 * at;
+  const float* part = p.part + at * D + d;
+  float top = -FLT_MAX, den = 0.f;
+  f32x4 num = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = grp; s < t.active; s += G) {
+    const float mx = ml[2 * (size_t)s * rows], sm = ml[2 * (size_t)s * rows + 1];
+    const f32x4 x = *(const f32x4*)(part + (size_t)s * rows * D);
+    const float now = fmaxf(top, mx), keep = __builtin_amdgcn_exp2f(top - now), f = __builtin_amdgcn_exp2f(mx - now);
 #pragma unroll
-      for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e]);
-      den = fmaf(f, ml[2 * a + 1], den);
-    }
-    const bool dead = r / p.group >= n;
-#pragma unroll
-    for (int e = 0; e < 4; e++) num[e] = dead ? 0.f : num[e] / den;
-    *(u32x2*)(kv_out_row(p, pair, r, D) + d) = u32x2{DT::pack(num[0], num[1]), DT::pack(num[2], num[3])};
+    for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e] * keep);
+    den = fmaf(f, sm, den * keep);
+    top = now;
   }
+  *(f32x4*)&s_o[grp][d] = num;
+  if (d == 0) {
+    s_top[grp] = top;
+    s_sum[grp] = den;
+  }
+  __syncthreads();
+  if (grp != 0) return;
+  float most = s_top[0];
+#pragma unroll
+  for (int i = 1; i < G; i++) most = fmaxf(most, s_top[i]);
+  num = f32x4{0.f, 0.f, 0.f, 0.f};
+  den = 0.f;
+#pragma unroll
+  for (int i = 0; i < G; i++) {
+    const float f = __builtin_amdgcn_exp2f(s_top[i] - most);
+    const f32x4 x = *(const f32x4*)&s_o[i][d];
+#pragma unroll
+    for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e]);
+    den = fmaf(f, s_sum[i], den);
+  }
+  const bool dead = r / p.group >= n;
+#pragma unroll
+  for (int e = 0; e < 4; e++) num[e] = dead ? 0.f : num[e] / den;
+  *(u32x2*)(kv_out_row(p, pair, r, D) + d) = u32x2{DT::pack(num[0], num[1]), DT::pack(num[2], num[3])};
 }
 
 }  // namespace cats
