@@ -157,7 +157,7 @@ BeamPlan beam_plan(int groups, int beams, int V) {
   const long long small = ((long long)V + 4 * kWave * 8 - 1) / (4 * kWave * 8);
   p.per_lane = small * groups * beams <= 4ll * current_device_cus() ? 8 : 32;
   const int per = 4 * kWave * p.per_lane;
-  p.pieces = (V - 1) / per + 1;
+  p.pieces = (V + 7 - 1) / per + 1;  // a row may start up to seven elements behind a vector's start
   return p;
 }
 bool beam_ok(int groups, int beams, int V, int keep) {
@@ -199,8 +199,8 @@ int cats_beam_select(const void* logits, int64_t row_stride, const float* scores
   a.tokens_out = tokens_out;
   a.finished_out = finished_out;
   a.ml = (float*)scratch;
-  a.keys = (uint32_t*)(a.ml + 2 * n);
-  a.ids = (int*)(a.keys + n * keep);
+  a.vals = a.ml + 2 * n;
+  a.ids = (int*)(a.vals + n * keep);
   a.beams = beams;
   a.V = V;
   a.keep = keep;

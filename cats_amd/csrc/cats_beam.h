@@ -15,6 +15,7 @@ constexpr int kBeamMax = 16;  // beams of a group, before and after
 // gathered (some more than `keep`) and ranked by comparing each with all; only where ties make that more than 64 are the best taken one by
 // one.  The workgroup's four waves are joined.  beam_join_kernel: a workgroup per group, a wave per beam joins its row's pieces in the same way, and
 // the beams' candidates are ranked by their totals in 64 bits: the order has to be that of the sums, which differ in their last bits only.
+// A row with a NaN or +infinity has no finite total at all, so neither has to be found among the best.
 
 struct BeamArgs {
   const void* logits;     // rows of V, row_stride elements apart
@@ -27,99 +28,151 @@ struct BeamArgs {
   int64_t* tokens_out;
   uint8_t* finished_out;
   float* ml;              // [row][piece][2] maximum and sum of exponentials
-  uint32_t* keys;         // [row][piece][keep]
-  int* ids;
+  float* vals;            // [row][piece][keep], in order
+  int* ids;               // -1: none
   int beams, V, keep, pieces;
 };
 
-// Floats ordered as unsigned integers; NaN as -infinity, -0 as 0.  0 is below them all.
-__device__ __forceinline__ uint32_t beam_key(float x) {
-  const uint32_t b = __float_as_uint(x != x ? -INFINITY : x + 0.f);
-  return b >> 31 ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float beam_value(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
-
 template <int CTRL>
-__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
-  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true));
+__device__ __forceinline__ float dpp_get(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) { return fmaxf(v, dpp_get<CTRL>(v)); }
 // Largest over the 64 lanes, the same in all; the steps of wave_sum.
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+__device__ __forceinline__ float wave_max(float v) {
   v = dpp_max<0xB1>(v);
   v = dpp_max<0x4E>(v);
   v = dpp_max<0x141>(v);
   v = dpp_max<0x140>(v);
-  const uint32_t a = __builtin_amdgcn_readlane((int)v, 0), b = __builtin_amdgcn_readlane((int)v, 16), c = __builtin_amdgcn_readlane((int)v, 32),
-                 d = __builtin_amdgcn_readlane((int)v, 48);
-  return max(max(a, b), max(c, d));
+  const int i = __float_as_int(v);
+  return fmaxf(fmaxf(__int_as_float(__builtin_amdgcn_readlane(i, 0)), __int_as_float(__builtin_amdgcn_readlane(i, 16))),
+               fmaxf(__int_as_float(__builtin_amdgcn_readlane(i, 32)), __int_as_float(__builtin_amdgcn_readlane(i, 48))));
+}
+// The k-th largest of the 64 lanes' values, k in 1..16, the same in all.  Rows of 16 lanes are sorted in descending order (a bitonic sort whose every
+// merge starts with a mirrored exchange); of two sorted rows, the larger of each lane and its mirrored one are the 16 largest, in bitonic order.
+// Some 60 instructions, where taking the largest k times is 30 each.
+__device__ __forceinline__ float wave_kth(float v, int k, int lane) {
+  auto order = [&](float other, int bit) {  // the lower lane of a pair keeps the larger value
+    const float hi = fmaxf(v, other), lo = fminf(v, other);
+    v = lane & bit ? lo : hi;
+  };
+  auto merge = [&]() {  // of a bitonic row
+    order(dpp_get<0x128>(v), 8);
+    order(dpp_get<0x1B>(dpp_get<0x141>(v)), 4);
+    order(dpp_get<0x4E>(v), 2);
+    order(dpp_get<0xB1>(v), 1);
+  };
+  order(dpp_get<0xB1>(v), 1);
+  order(dpp_get<0x1B>(v), 2);
+  order(dpp_get<0xB1>(v), 1);
+  order(dpp_get<0x141>(v), 4);
+  order(dpp_get<0x4E>(v), 2);
+  order(dpp_get<0xB1>(v), 1);
+  order(dpp_get<0x140>(v), 8);
+  order(dpp_get<0x1B>(dpp_get<0x141>(v)), 4);
+  order(dpp_get<0x4E>(v), 2);
+  order(dpp_get<0xB1>(v), 1);
+  v = fmaxf(v, __shfl_xor(v, 31, kWave));
+  merge();
+  v = fmaxf(v, __shfl_xor(v, 47, kWave));
+  merge();
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k - 1));
+}
+// Floats ordered as unsigned integers, -0 as 0.
+__device__ __forceinline__ uint32_t beam_key(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) v = min(v, __shfl_xor(v, o, kWave));
+  return v;
+}
+// LDS of this wave alone: what its lanes have written is there for all of them.
+__device__ __forceinline__ void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
+  __builtin_amdgcn_wave_barrier();
 }
 
 struct BeamList {  // in LDS, of a wave
-  uint32_t key[kWave];
+  float val[kWave];
   int id[kWave];
 };
 
-// Writes the best `keep` of the wave's keys to `best`, in order, ids ascending among equal keys; 0 behind the last.  A key of 0 is no entry.
-template <int E>
-__device__ __forceinline__ void wave_best(uint32_t (&key)[E], const int (&id)[E], int keep, int lane, BeamList& list, BeamList& best) {
-  uint32_t mine = 0;
+// Writes the best `keep` of the wave's values to `best`, in order, lower ids first among equal ones, ids of -1 behind the last.  id(i) is that of
+// x[i], -1 for no entry (and x[i] = -infinity).  The lowest 32 ids of the wave, or all, are within the first FRONT values of the first `lanes` lanes.
+template <int FRONT, int E, class Id>
+__device__ __forceinline__ void wave_best(const float (&x)[E], Id id, int lanes, int keep, int lane, BeamList& list, BeamList& best) {
+  float bound = -INFINITY;
+  if constexpr (E > 1) {  // one value a lane fits the list as it is
+    float mine = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < E; i++) mine = max(mine, key[i]);
-  uint32_t bound = 0, rest = mine;
-  for (int k = 0; k < keep; k++) {
-    bound = wave_max(rest);
-    const uint64_t at = __ballot(rest == bound);
-    if (lane == (int)__builtin_ctzll(at)) rest = 0;
+    for (int i = 0; i < E; i++) mine = fmaxf(mine, x[i]);
+    bound = wave_kth(mine, keep, lane);
   }
-  bound = max(bound, 1u);
   int count = 0;
-#pragma unroll
-  for (int i = 0; i < E; i++) {
-    const bool in = key[i] >= bound;
+  auto take = [&](bool in, int i) {
     const uint64_t b = __ballot(in);
     const int at = count + ballot_rank(b);
     if (in && at < kWave) {
-      list.key[at] = key[i];
-      list.id[at] = id[i];
+      list.val[at] = x[i];
+      list.id[at] = id(i);
     }
     count += __popcll(b);
+  };
+  const bool low = bound == -INFINITY;  // less than `keep` lanes have more than that, or there is one value a lane
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    const bool in = low ? x[i] > bound : x[i] >= bound;
+    if (__any(in)) take(in, i);
   }
-  if (lane < keep) best.key[lane] = 0;
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
-  __builtin_amdgcn_wave_barrier();
+  if (low && count < keep) {  // then values of -infinity are among the best, those with the lowest ids
+#pragma unroll
+    for (int i = 0; i < FRONT; i++) take(lane < lanes && x[i] == -INFINITY && id(i) >= 0, i);
+  }
+  if (lane < keep) best.id[lane] = -1;
+  wave_lds_sync();
   if (count <= kWave) {
-    const uint32_t k = lane < count ? list.key[lane] : 0u;
-    const int v = lane < count ? list.id[lane] : INT32_MAX;
+    const float v = lane < count ? list.val[lane] : 0.f;
+    const int n = lane < count ? list.id[lane] : 0;
+    const uint32_t hi = beam_key(v), lo = ~(uint32_t)n;  // larger is better
+    const uint64_t mine = (uint64_t)hi << 32 | lo;
     int rank = 0;
     for (int j = 0; j < count; j++) {
-      const uint32_t kj = __builtin_amdgcn_readlane((int)k, j);
-      const int vj = __builtin_amdgcn_readlane(v, j);
-      rank += kj > k || (kj == k && vj < v);
+      const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, j);
+      rank += other > mine;
     }
     if (lane < count && rank < keep) {
-      best.key[rank] = k;
-      best.id[rank] = v;
+      best.val[rank] = v;
+      best.id[rank] = n;
     }
   } else {
+    uint64_t gone = 0;  // of this lane's values
+    static_assert(E <= 64, "a bit each");
     for (int k = 0; k < keep; k++) {
-      uint32_t top = 0;
+      float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < E; i++) top = max(top, key[i]);
+      for (int i = 0; i < E; i++) top = gone >> i & 1 ? top : fmaxf(top, x[i]);
       top = wave_max(top);
-      uint32_t first = 0;  // of ids, turned round
+      int first = INT32_MAX, which = 0;
 #pragma unroll
-      for (int i = 0; i < E; i++) first = key[i] == top ? max(first, ~(uint32_t)id[i]) : first;
-      const int which = (int)~wave_max(first);
-#pragma unroll
-      for (int i = 0; i < E; i++) key[i] = id[i] == which ? 0u : key[i];
+      for (int i = 0; i < E; i++) {
+        const int n = id(i);
+        const bool in = !(gone >> i & 1) && n >= 0 && x[i] == top && n < first;
+        first = in ? n : first;
+        which = in ? i : which;
+      }
+      const int lowest = wave_min(first);
+      if (lowest == INT32_MAX) break;
+      if (first == lowest) gone |= (uint64_t)1 << which;
       if (lane == 0) {
-        best.key[k] = top;
-        best.id[k] = which;
+        best.val[k] = top;
+        best.id[k] = lowest;
       }
     }
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
-  __builtin_amdgcn_wave_barrier();
+  wave_lds_sync();
 }
 
 template <class DT, int E>
@@ -131,53 +184,50 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(BeamArgs p) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, row = blockIdx.y, piece = blockIdx.x;
   if (p.finished && p.finished[row]) return;
   const st* x = (const st*)p.logits + row * p.row_stride;
-  const int first = (piece * W + wave) * kWave * E;  // the wave's elements, in vectors of VEC that go round the lanes
-  uint32_t key[E];
-  int id[E];
+  // the wave's elements, in vectors of VEC that go round the lanes; vectors are those of memory, so a row may start inside its first
+  const int first = (piece * W + wave) * kWave * E - (int)(((uintptr_t)x & 15u) / sizeof(st));
   float val[E];
-  const bool whole = first + kWave * E <= p.V && ((uintptr_t)x & 15u) == 0;
+  auto id = [&](int i) {
+    const int at = first + (i / VEC * kWave + lane) * VEC + i % VEC;
+    return at >= 0 && at < p.V ? at : -1;
+  };
+  if (first >= 0 && first + kWave * E <= p.V) {
+    u32x4 w[E / VEC];
 #pragma unroll
-  for (int i = 0; i < E / VEC; i++) {
-    const int at = first + (i * kWave + lane) * VEC;
-    if (whole) {
-      const u32x4 w = load_stream((const u32x4*)(x + at));
+    for (int i = 0; i < E / VEC; i++) w[i] = load_stream((const u32x4*)(x + first + (i * kWave + lane) * VEC));
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
-        if constexpr (VEC == 4) val[i * VEC + e] = __uint_as_float(w[e]);
-        else val[i * VEC + e] = DT::tof((st)(w[e / 2] >> (16 * (e & 1))));
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; e++) val[i * VEC + e] = at + e < p.V ? DT::tof(x[at + e]) : 0.f;
+    for (int i = 0; i < E; i++) {
+      const uint32_t c = w[i / VEC][i % VEC * 4 / VEC];
+      if constexpr (VEC == 4) val[i] = __uint_as_float(c);
+      else val[i] = DT::tof((st)(c >> (16 * (i & 1))));
     }
+  } else {
+    st w[E];
 #pragma unroll
-    for (int e = 0; e < VEC; e++) {
-      id[i * VEC + e] = at + e;
-      key[i * VEC + e] = at + e < p.V ? beam_key(val[i * VEC + e]) : 0u;
-    }
+    for (int i = 0; i < E; i++) w[i] = x[max(id(i), 0)];
+#pragma unroll
+    for (int i = 0; i < E; i++) val[i] = id(i) >= 0 ? DT::tof(w[i]) : -INFINITY;
   }
-  uint32_t top = 0;
+  float m = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < E; i++) top = max(top, key[i]);
-  top = wave_max(top);
-  const float m = top ? beam_value(top) : -INFINITY, base = m == -INFINITY ? 0.f : m;
+  for (int i = 0; i < E; i++) m = fmaxf(m, val[i]);
+  m = wave_max(m);
+  // exp of a difference that is rounded once: within 2^-24 of |x - m|, as the difference itself is
+  const float base = m == -INFINITY ? 0.f : m;
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < E; i++) sum += key[i] ? expf(val[i] - base) : 0.f;
+  for (int i = 0; i < E; i++) sum += __builtin_amdgcn_exp2f((val[i] - base) * 1.44269504088896341f);
   sum = wave_sum(sum);
-  wave_best<E>(key, id, p.keep, lane, s_list[wave], s_best[wave]);
+  wave_best<VEC>(val, id, 32 / VEC, p.keep, lane, s_list[wave], s_best[wave]);
   if (lane == 0) {
     s_ml[wave][0] = m;
     s_ml[wave][1] = sum;
   }
   __syncthreads();
   if (wave != 0) return;
-  uint32_t k1[1] = {0};
-  int i1[1] = {0};
-  if (lane < W * p.keep) {
-    k1[0] = s_best[lane / p.keep].key[lane % p.keep];
-    i1[0] = s_best[lane / p.keep].id[lane % p.keep];
-  }
+  const int from = lane / p.keep, which = lane - from * p.keep;
+  const int n = from < W ? s_best[from < W ? from : 0].id[which] : -1;
+  const float v1[1] = {n >= 0 ? s_best[from].val[which] : -INFINITY};
   float mm = s_ml[0][0];
 #pragma unroll
   for (int w = 1; w < W; w++) mm = fmaxf(mm, s_ml[w][0]);
@@ -186,10 +236,10 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(BeamArgs p) {
 #pragma unroll
   for (int w = 0; w < W; w++) ss += s_ml[w][0] == -INFINITY ? s_ml[w][1] : s_ml[w][1] * expf(s_ml[w][0] - bb);
   __builtin_amdgcn_wave_barrier();
-  wave_best<1>(k1, i1, p.keep, lane, s_list[0], s_best[0]);
+  wave_best<1>(v1, [&](int) { return n; }, kWave, p.keep, lane, s_list[0], s_best[0]);
   const size_t out = (size_t)row * p.pieces + piece;
   if (lane < p.keep) {
-    p.keys[out * p.keep + lane] = s_best[0].key[lane];
+    p.vals[out * p.keep + lane] = s_best[0].val[lane];
     p.ids[out * p.keep + lane] = s_best[0].id[lane];
   }
   if (lane == 0) {
@@ -198,77 +248,136 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(BeamArgs p) {
   }
 }
 
-// Candidates of a row come in pieces of `keep`; a wave takes 64 at a time beside the best it has.
+// Doubles ordered as unsigned integers, -0 as 0.  0 is below them all.
+__device__ __forceinline__ uint64_t beam_key(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
+  return b >> 63 ? ~b : b | 1ull << 63;
+}
+
+// Candidates of a row come in pieces of `keep`; a wave takes 512 at a time beside the best it has.  What the beams offer is in order for each of them
+// (total, then id), so of equal totals the earlier offer is the better one.  Few of them are ranked in 64 bits: those whose totals, rounded to
+// float, which keeps their order, are not below the keep-th best of the lanes'.
 template <int N>
 __global__ __launch_bounds__(N* kWave) void beam_join_kernel(BeamArgs p) {
   __shared__ BeamList s_list[N], s_best[N];
   __shared__ double s_total[N * N];
-  __shared__ long long s_flat[N * N];
+  __shared__ int s_token[N * N];  // -1: no offer
   const int lane = threadIdx.x & (kWave - 1), b = threadIdx.x >> 6, group = blockIdx.x, row = group * p.beams + b;
   const double kNone = -(double)INFINITY;
   if (b < p.beams) {
     const bool done = p.finished && p.finished[row];
     const float score = p.scores[row];
     double total = kNone;
-    long long token = lane;  // where nothing is finite, the lowest ones
+    int token = lane < p.V ? lane : -1;  // where nothing is finite, the lowest ones
     if (done) {
-      token = lane == 0 ? p.eos : lane - 1 < p.eos ? lane - 1 : lane;  // behind eos what no finished beam does, at -infinity
-      if (token >= p.V) token = -1;
-      if (lane == 0 && fabsf(score) < INFINITY) total = score;
+      if (fabsf(score) < INFINITY) {
+        token = lane == 0 ? (int)p.eos : lane - 1 < p.eos ? lane - 1 : lane;  // behind eos what no finished beam does, at -infinity
+        if (token >= p.V) token = -1;
+        if (lane == 0) total = score;
+      }
     } else {
       const float* ml = p.ml + (size_t)row * p.pieces * 2;
-      uint32_t top = 0;
-      for (int i = lane; i < p.pieces; i += kWave) top = max(top, beam_key(ml[2 * i]));
-      const float m = beam_value(wave_max(top)), base = m == -INFINITY ? 0.f : m;
+      const size_t at = (size_t)row * p.pieces * p.keep;
+      const int n = p.pieces * p.keep;
+      constexpr int E = 8;
+      float val[E + 1];
+      int id[E + 1];
+      auto fetch = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+          const int j = i0 + i * kWave + lane;
+          const int k = p.ids[at + min(j, n - 1)];
+          const float v = p.vals[at + min(j, n - 1)];
+          id[i] = j < n ? k : -1;
+          val[i] = id[i] >= 0 ? v : -INFINITY;
+        }
+      };
+      float m = lane < p.pieces ? ml[2 * lane] : -INFINITY;
+      fetch(0);
+      for (int i = lane + kWave; i < p.pieces; i += kWave) m = fmaxf(m, ml[2 * i]);
+      m = wave_max(m);
+      const float base = m == -INFINITY ? 0.f : m;
       double sum = 0.0;
       for (int i = lane; i < p.pieces; i += kWave)
         sum += ml[2 * i] == -INFINITY ? (double)ml[2 * i + 1] : (double)ml[2 * i + 1] * exp((double)ml[2 * i] - base);
 #pragma unroll
       for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
       const double lse = (double)base + log(sum);
-      const bool fine = fabsf(score) < INFINITY && fabs(lse) < (double)INFINITY;
-      if (fine) {
-        const size_t at = (size_t)row * p.pieces * p.keep;
-        const int n = p.pieces * p.keep;
-        uint32_t key[2] = {0, 0};
-        int id[2] = {0, 0};
-        for (int i0 = 0; i0 < n; i0 += kWave) {
-          key[0] = i0 + lane < n ? p.keys[at + i0 + lane] : 0u;
-          id[0] = key[0] ? p.ids[at + i0 + lane] : 0;
-          const uint32_t have = key[1];
-          if (i0 == 0 || wave_max(key[0]) >= wave_max(lane == p.keep - 1 ? have : 0u)) {
-            wave_best<2>(key, id, p.keep, lane, s_list[b], s_best[b]);
-            key[1] = lane < p.keep ? s_best[b].key[lane] : 0u;
-            id[1] = key[1] ? s_best[b].id[lane] : 0;
-          }
+      if (fabsf(score) < INFINITY && fabs(lse) < (double)INFINITY) {
+        val[E] = -INFINITY;
+        id[E] = -1;
+        for (int i0 = 0; i0 < n; i0 += E * kWave) {
+          if (i0) fetch(i0);
+          wave_best<E + 1>(val, [&](int i) { return id[i]; }, kWave, p.keep, lane, s_list[b], s_best[b]);
+          id[E] = lane < p.keep ? s_best[b].id[lane] : -1;
+          val[E] = id[E] >= 0 ? s_best[b].val[lane] : -INFINITY;
         }
-        token = key[1] ? id[1] : -1;
-        const double x = (double)score + ((double)beam_value(key[1]) - lse);
-        if (key[1] && fabs(x) < (double)INFINITY) total = x;
-      } else if (lane >= p.V) {
-        token = -1;
+        token = id[E];
+        const double x = (double)score + ((double)val[E] - lse);
+        if (token >= 0 && fabs(x) < (double)INFINITY) total = x;
       }
     }
     if (lane < p.keep) {
       s_total[b * p.keep + lane] = total;
-      s_flat[b * p.keep + lane] = token < 0 ? -1 : (long long)b * p.V + token;
+      s_token[b * p.keep + lane] = token;
     }
   }
   __syncthreads();
+  if (b != 0) return;
   const int n = p.beams * p.keep;
-  if (threadIdx.x >= n) return;
-  const double mine = s_total[threadIdx.x];
-  const long long flat = s_flat[threadIdx.x];
-  if (flat < 0) return;
-  int rank = 0;
-  for (int j = 0; j < n; j++) rank += s_flat[j] >= 0 && (s_total[j] > mine || (s_total[j] == mine && s_flat[j] < flat));
-  if (rank >= p.keep) return;
-  const int out = group * p.keep + rank, parent = threadIdx.x / p.keep;
-  const long long token = flat - (long long)parent * p.V;
-  p.scores_out[out] = (float)mine;
-  p.parents_out[out] = parent;
-  p.tokens_out[out] = token;
-  p.finished_out[out] = token == p.eos || (p.finished && p.finished[group * p.beams + parent]);
+  constexpr int E = N * N / kWave;
+  uint64_t key[E];
+  float most = -INFINITY, near[E];
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    const int c = i * kWave + lane;
+    const bool in = c < n && s_token[c] >= 0;
+    const double t = in ? s_total[c] : kNone;
+    key[i] = in ? beam_key(t) : 0;
+    near[i] = (float)t;
+    most = fmaxf(most, near[i]);
+  }
+  const float bound = wave_kth(most, p.keep, lane);
+  int count = 0;
+  int* const list = s_list[0].id;
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    const bool in = key[i] && near[i] >= bound;  // all of them where the bound is -infinity
+    const uint64_t at = __ballot(in);
+    const int j = count + ballot_rank(at);
+    if (in && j < kWave) list[j] = i * kWave + lane;
+    count += __popcll(at);
+  }
+  wave_lds_sync();
+  auto give = [&](int c, int rank) {
+    if (rank >= p.keep) return;
+    const int out = group * p.keep + rank, parent = c / p.keep, token = s_token[c];
+    p.scores_out[out] = (float)s_total[c];
+    p.parents_out[out] = parent;
+    p.tokens_out[out] = token;
+    p.finished_out[out] = token == p.eos || (p.finished && p.finished[group * p.beams + parent]);
+  };
+  if (count <= kWave) {
+    const int c = lane < count ? list[lane] : 0;  // the list is in order
+    const uint64_t mine = beam_key(s_total[c]);
+    int rank = 0;
+    for (int j = 0; j < count; j++) {
+      const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
+      rank += other > mine || (other == mine && j < lane);
+    }
+    if (lane < count) give(c, rank);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+      const int c = i * kWave + lane;
+      int rank = 0;
+      for (int j = 0; j < n; j++) {
+        const uint64_t other = s_token[j] >= 0 ? beam_key(s_total[j]) : 0;
+        rank += other > key[i] || (other == key[i] && j < c);
+      }
+      if (key[i]) give(c, rank);
+    }
+  }
 }
 
 // ---- reordering --------------------------------------------------------------------------------------------------------------------

@@ -29,23 +29,26 @@ struct KvLaunch {
     }
     return hipErrorInvalidValue;
   }
+  // A workgroup a row from five splits on
+  template <int D, int ROWS, int UNIT>
+  static hipError_t join(const KvAttnArgs& a, hipStream_t stream) {
+    const int items = a.pairs * a.T * a.group, per = 256 / (D / 4);
+    if (a.splits > 4) return launch_kernel(kv8_join_kernel<DT, D, ROWS, UNIT, true>, dim3(items), dim3(256), 0, stream, a);
+    return launch_kernel(kv8_join_kernel<DT, D, ROWS, UNIT, false>, dim3((items + per - 1) / per), dim3(256), 0, stream, a);
+  }
   template <int D>
   static hipError_t attn_d(const KvAttnPlan& plan, const KvAttnArgs& a, hipStream_t stream) {
     const int rows = a.T * a.group;
     if (plan.prompt) {
       const dim3 grid(a.pairs, (rows + kKvPromptRows - 1) / kKvPromptRows, a.splits);
       hipError_t e = launch_kernel(kv8_attn_prompt_kernel<DT, D>, grid, dim3(256), 0, stream, a);
-      if (e == hipSuccess && a.splits > 1)
-        e = launch_kernel(kv8_join_kernel<DT, D, kKvPromptRows, kKvPromptUnit>, dim3(a.pairs * rows), dim3(256), 0, stream, a);
-      return e;
+      return e == hipSuccess && a.splits > 1 ? join<D, kKvPromptRows, kKvPromptUnit>(a, stream) : e;
     }
     auto kern = plan.seal                   ? kv8_attn_step_kernel<DT, D, false, true>
                 : a.T > 1 || a.window ? kv8_attn_step_kernel<DT, D, true, false>
                                       : kv8_attn_step_kernel<DT, D, false, false>;
     hipError_t e = launch_kernel(kern, dim3(a.pairs, a.splits + plan.seal, (rows + 15) / 16), dim3(256), 0, stream, a);
-    if (e == hipSuccess && a.splits > 1)
-      e = launch_kernel(kv8_join_kernel<DT, D, 16, kKvStepWaves>, dim3(a.pairs * rows), dim3(256), 0, stream, a);
-    return e;
+    return e == hipSuccess && a.splits > 1 ? join<D, 16, kKvStepWaves>(a, stream) : e;
   }
   static hipError_t attn(int D, const KvAttnPlan& plan, const KvAttnArgs& a, hipStream_t stream) {
     switch (D) {

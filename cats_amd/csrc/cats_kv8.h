@@ -855,14 +855,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   }
 }
 
-// The splits' results, in a fixed order.  A workgroup per (pair, row): as many groups of D / 4 lanes as fit take every so manieth split, and LDS joins
-// the groups.  Rows whose cache was one split's are done already.  ROWS and UNIT are the attention kernel's.
-template <class DT, int D, int ROWS, int UNIT>
+// The splits' results, in a fixed order.  ALONE: a workgroup per (pair, row), whose groups of D / 4 lanes take every so manieth split and are
+// joined in LDS.  Otherwise, for few splits, a row per group.  Rows whose cache was one split's are done already.  ROWS and UNIT are the
+// attention kernel's.
+template <class DT, int D, int ROWS, int UNIT, bool ALONE>
 __global__ __launch_bounds__(256) void kv8_join_kernel(KvAttnArgs p) {
   constexpr int L = D / 4, G = 256 / L;
-  __shared__ __align__(16) float s_o[G][D];
-  __shared__ float s_top[G], s_sum[G];
-  const int rows = p.T * p.group, pair = blockIdx.x / rows, r = blockIdx.x - pair * rows, grp = threadIdx.x / L, d = threadIdx.x % L * 4;
+  const int grp = threadIdx.x / L, d = threadIdx.x % L * 4;
+  const int rows = p.T * p.group, item = ALONE ? blockIdx.x : blockIdx.x * G + grp, pair = item / rows, r = item - pair * rows;
+  if (pair >= p.pairs) return;
   int start, n;
   KvTiles t;
   if (!kv_span(p.span, pair / p.c.heads, p.T, start, n) || !kv_tiles<ROWS, UNIT>(p, r / ROWS * ROWS, start, n, t) || t.active == 1) return;
@@ -872,7 +873,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(KvAttnArgs p) {
   float top = -FLT_MAX, den = 0.f;
   f32x4 num = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = grp; s < t.active; s += G) {
+  for (int s = ALONE ? grp : 0; s < t.active; s += ALONE ? G : 1) {
     const float mx = ml[2 * (size_t)s * rows], sm = ml[2 * (size_t)s * rows + 1];
     const f32x4 x = *(const f32x4*)(part + (size_t)s * rows * D);
     const float now = fmaxf(top, mx), keep = __builtin_amdgcn_exp2f(top - now), f = __builtin_amdgcn_exp2f(mx - now);
@@ -881,25 +882,29 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(KvAttnArgs p) {
     den = fmaf(f, sm, den * keep);
     top = now;
   }
-  *(f32x4*)&s_o[grp][d] = num;
-  if (d == 0) {
-    s_top[grp] = top;
-    s_sum[grp] = den;
-  }
-  __syncthreads();
-  if (grp != 0) return;
-  float most = s_top[0];
+  if constexpr (ALONE) {
+    __shared__ __align__(16) float s_o[G][D];
+    __shared__ float s_top[G], s_sum[G];
+    *(f32x4*)&s_o[grp][d] = num;
+    if (d == 0) {
+      s_top[grp] = top;
+      s_sum[grp] = den;
+    }
+    __syncthreads();
+    if (grp != 0) return;
+    float most = s_top[0];
 #pragma unroll
-  for (int i = 1; i < G; i++) most = fmaxf(most, s_top[i]);
-  num = f32x4{0.f, 0.f, 0.f, 0.f};
-  den = 0.f;
+    for (int i = 1; i < G; i++) most = fmaxf(most, s_top[i]);
+    num = f32x4{0.f, 0.f, 0.f, 0.f};
+    den = 0.f;
 #pragma unroll
-  for (int i = 0; i < G; i++) {
-    const float f = __builtin_amdgcn_exp2f(s_top[i] - most);
-    const f32x4 x = *(const f32x4*)&s_o[i][d];
+    for (int i = 0; i < G; i++) {
+      const float f = __builtin_amdgcn_exp2f(s_top[i] - most);
+      const f32x4 x = *(const f32x4*)&s_o[i][d];
 #pragma unroll
-    for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e]);
-    den = fmaf(f, s_sum[i], den);
+      for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e]);
+      den = fmaf(f, s_sum[i], den);
+    }
   }
   const bool dead = r / p.group >= n;
 #pragma unroll
