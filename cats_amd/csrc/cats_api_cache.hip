@@ -63,13 +63,14 @@ constexpr int kStepRows = 64;  // rows of queries a cached head up to which they
 
 KvAttnPlan kv8_attn_plan(int B, int T, int heads, int kv_heads, int blocks, int window) {
   const int cus = current_device_cus(), rows = T * (heads / kv_heads);
-  KvAttnPlan plan = {rows > kStepRows, 1, false};
+  KvAttnPlan plan = {rows > kStepRows, 1, false, false};
   const int per = plan.prompt ? kKvPromptRows : 16, unit = plan.prompt ? kKvPromptUnit : 4;
   const long long groups = (long long)B * kv_heads * ((rows + per - 1) / per);
   // tiles that a workgroup's queries see at most
   const int tiles = window ? (int)min((long long)blocks, ((long long)window + per + 2 * kKvBlock) / kKvBlock) : blocks;
   const long long want = ((plan.prompt ? 2ll : 4ll) * cus + groups - 1) / groups;
   plan.splits = (int)max(1ll, min(want, (long long)(tiles + unit - 1) / unit));
+  plan.fold = groups * plan.splits <= 2ll * cus;
   return plan;
 }
 

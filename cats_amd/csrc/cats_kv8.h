@@ -13,6 +13,8 @@
 #pragma once
 #include <float.h>
 
+#include <type_traits>
+
 #include "cats_down_mma.h"
 #include "cats_rows_mma.h"
 
@@ -228,6 +230,7 @@ struct KvAttnArgs {
   int T, group;       // group: query heads of a cached head
   int window;         // keys that a query sees, at most; 0: all
   int pairs, splits;  // pairs: rows x cached heads
+  int fold;           // kv8_attn_prompt_kernel: all workgroups start together
 };
 
 // Row r of a (row, cached head) pair is head r % group of token r / group: the queries of a step that share a cached head are one
@@ -267,18 +270,47 @@ __device__ __forceinline__ void kv_fill_rows(const KvAttnArgs& p, int pair, int 
   }
 }
 
-// Sets numbers that are not finite to 0 and says where they were: `ones` has 1 (e4m3 or the type itself) there and 0 elsewhere.
-__device__ __forceinline__ uint32_t kv_fix8(uint32_t& w) {
-  const uint32_t m = (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-  w &= ~(m * 0xffu);
-  return m * 0x38u;
+// A masked weight is 0, but 0 times a NaN is not.  So where keys are masked, numbers of V that are not finite are set to 0, and at the end, if there
+// were any, the queries that see one are set to NaN: products of those places (1, and 0 elsewhere) and of what a query sees count them.
+__device__ __forceinline__ uint32_t kv_nan8(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7; }  // bit 0 of each byte
+template <class DT>
+__device__ __forceinline__ uint32_t kv_nan16(uint32_t w) {  // bit 0 of each half
+  return ((w & Kv<DT>::kExp) == Kv<DT>::kExp ? 1u : 0u) | ((w >> 16 & Kv<DT>::kExp) == Kv<DT>::kExp ? 0x10000u : 0u);
+}
+// Sets them to 0; not 0 if there were any.
+__device__ __forceinline__ uint32_t kv_fix8(u32x4& x) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const uint32_t w = x[e], n = kv_nan8(w);
+    x[e] = w & ~(n * 0xffu);
+    any |= n;
+  }
+  return any;
+}
+template <class DT, class V>
+__device__ __forceinline__ uint32_t kv_fix16(V& x) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int e = 0; e < (int)(sizeof(V) / 4); e++) {
+    const uint32_t w = x[e], n = kv_nan16<DT>(w);
+    x[e] = w & ~(n * 0xffffu);
+    any |= n;
+  }
+  return any;
+}
+// Eight numbers' places as an operand.
+template <class DT>
+__device__ __forceinline__ u32x4 kv_bad8(const uint8_t* at) {
+  const u32x2 w = *(const u32x2*)at;
+  return kv_wide<DT>(kv_nan8(w[0]) * 0x38u, kv_nan8(w[1]) * 0x38u);  // 1 in e4m3
 }
 template <class DT>
-__device__ __forceinline__ uint32_t kv_fix16(uint32_t& w) {
-  const uint32_t lo = (w & Kv<DT>::kExp) == Kv<DT>::kExp ? 1u : 0u, hi = (w >> 16 & Kv<DT>::kExp) == Kv<DT>::kExp ? 0x10000u : 0u;
-  const uint32_t m = lo | hi;
-  w &= ~(m * 0xffffu);
-  return m * Kv<DT>::kOne;
+__device__ __forceinline__ u32x4 kv_bad16(const uint16_t* at) {
+  u32x4 w = *(const u32x4*)at;
+#pragma unroll
+  for (int e = 0; e < 4; e++) w[e] = kv_nan16<DT>(w[e]) * Kv<DT>::kOne;
+  return w;
 }
 
 // One new token, or a few: 16 rows of queries, the cache split over workgroups and over the four waves of each, the waves' results joined in LDS
@@ -290,8 +322,6 @@ __device__ __forceinline__ uint32_t kv_fix16(uint32_t& w) {
 // 16-bit operands (two an instruction), the blocks' scales go into the exponent: with w = s * ks * scale + log2(vs), weights are
 // 2^(w - max w) <= 1, O sums them times the codes, and the sum of weights adds them divided by vs.
 // The tail is four times sixteen tokens, for a wave each: tile `wave` of the four, and one product over sixteen tokens.
-// A masked weight is 0, but 0 times a NaN is not: where keys are masked, numbers of V that are not finite are taken out and the
-// queries that see one are set to NaN.
 // MASK: queries that see different keys, or a window.  One token without a window sees all of every tile but the tail.
 // SEAL: the tokens are in the tails and nowhere else yet.  One workgroup a pair more quantises the block that they complete; nobody reads that block
 // in this launch.
@@ -368,6 +398,7 @@ __global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_ker
   int tile = t.tile_lo + split * W + wave;
 
   float top = -FLT_MAX, sum = 0.f;
+  uint32_t some = 0;  // whether a tile that is seen in part had numbers of V that are not finite
   f32x4 o[NU];
 #pragma unroll
   for (int u = 0; u < NU; u++) o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -399,8 +430,12 @@ __global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_ker
         add += s[i][e];
       }
     sum = fmaf(add, __builtin_amdgcn_rcpf(vs), sum);
+    asm volatile("" : "+v"(sum));  // here: the weights' registers are wanted
   };
 
+  auto part_tile = [&](int at) {  // whether some query does not see all of it
+    return at * kKvBlock + kKvBlock - 1 > t.pos_lo || (p.window && at * kKvBlock <= t.pos_hi - p.window);
+  };
   if (tile <= end8) {
     fetch_k(tile);
     fetch_v(tile);
@@ -421,7 +456,7 @@ __global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_ker
       if (AHEAD && more) fetch_k(tile + step);
       __builtin_amdgcn_sched_barrier(0);
       const int key0 = tile * kKvBlock + 16 * g;  // of this lane's weights
-      const bool part = MASK && (tile * kKvBlock + kKvBlock - 1 > t.pos_lo || (p.window && tile * kKvBlock <= t.pos_hi - p.window));
+      const bool part = MASK && part_tile(tile);
       if (part) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -435,37 +470,8 @@ __global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_ker
         pf[v] = u32x4{DT::pack(s[2 * v][0], s[2 * v][1]), DT::pack(s[2 * v][2], s[2 * v][3]), DT::pack(s[2 * v + 1][0], s[2 * v + 1][1]),
                       DT::pack(s[2 * v + 1][2], s[2 * v + 1][3])};
       if (part) {
-        uint32_t some = 0;
 #pragma unroll
-        for (int u = 0; u < NU; u++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            uint32_t w = vv[u][e];
-            some |= kv_fix8(w);
-          }
-        if (__any(some != 0)) {
-          auto one = [&](int j) { return seen(key0 + j) ? F::kOne : 0u; };
-          u32x4 sees[2];
-#pragma unroll
-          for (int v = 0; v < 2; v++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) sees[v][e] = one(8 * v + 2 * e) | one(8 * v + 2 * e + 1) << 16;
-#pragma unroll
-          for (int u = 0; u < NU; u++) {
-            f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int v = 0; v < 2; v++) {
-              uint32_t w0 = vv[u][2 * v], w1 = vv[u][2 * v + 1];
-              const uint32_t b0 = kv_fix8(w0), b1 = kv_fix8(w1);
-              vv[u][2 * v] = w0;
-              vv[u][2 * v + 1] = w1;
-              z = Mma<DT>::run(kv_wide<DT>(b0, b1), sees[v], z);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[u][e] = z[e] > 0.f ? NAN : o[u][e];
-            __builtin_amdgcn_sched_barrier(0);  // one after the other: rare, and registers are short
-          }
-        }
+        for (int u = 0; u < NU; u++) some |= kv_fix8(vv[u]);
       }
 #pragma unroll
       for (int u = 0; u < NU; u++) {
@@ -482,7 +488,8 @@ __global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_ker
   }
 
   // the tail, by the split whose turn it would be
-  if (t.tile_hi == t.last && (t.last - t.tile_lo) / W % t.active == split) {
+  const bool tail = t.tile_hi == t.last && (t.last - t.tile_lo) / W % t.active == split;
+  if (tail) {
     const uint16_t* kt = p.c.kt + (size_t)pair * kKvBlock * D + (ktok + 4 * wave) * D + d0;
     const uint16_t* vt = p.c.vt + (size_t)pair * kKvBlock * D + m * kKvBlock + 16 * g + 4 * wave;
     u32x4 kq[NK][NV];
@@ -506,28 +513,34 @@ __global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_ker
     }
     weigh(s, 1, 1.f, 1.f);
     const u32x2 pf = u32x2{DT::pack(s[0][0], s[0][1]), DT::pack(s[0][2], s[0][3])};
-    uint32_t some = 0;
 #pragma unroll
     for (int u = 0; u < NU; u++) {
-      uint32_t x = vq[u][0], y = vq[u][1];
-      some |= kv_fix16<DT>(x) | kv_fix16<DT>(y);
-      o[u] = DownMma<DT>::run(u32x2{x, y}, pf, o[u]);
+      some |= kv_fix16<DT>(vq[u]);
+      o[u] = DownMma<DT>::run(vq[u], pf, o[u]);
     }
-    if (__any(some != 0)) {
-      auto one = [&](int j) { return seen(key + j) ? F::kOne : 0u; };
-      const u32x2 sees = u32x2{one(0) | one(1) << 16, one(2) | one(3) << 16};
+  }
+  if (__any(some != 0)) {  // the queries that see a number that is not finite
+    auto spoil = [&](int tile, auto load) {
 #pragma unroll
       for (int u = 0; u < NU; u++) {
-        uint32_t x = vq[u][0], y = vq[u][1];
-        const u32x2 bad = u32x2{kv_fix16<DT>(x), kv_fix16<DT>(y)};
-        const f32x4 z = DownMma<DT>::run(bad, sees, f32x4{0.f, 0.f, 0.f, 0.f});
-        __builtin_amdgcn_sched_barrier(0);  // one after the other: rare, and registers are short
+        f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < 2; v++) {
+          const int key = tile * kKvBlock + 16 * g + 8 * v;
+          u32x4 one;
+#pragma unroll
+          for (int e = 0; e < 4; e++) one[e] = (seen(key + 2 * e) ? F::kOne : 0u) | (seen(key + 2 * e + 1) ? F::kOne << 16 : 0u);
+          z = Mma<DT>::run(load(16 * u + m, 16 * g + 8 * v), one, z);
+        }
 #pragma unroll
         for (int e = 0; e < 4; e++) o[u][e] = z[e] > 0.f ? NAN : o[u][e];
       }
-    }
+    };
+    if constexpr (MASK)
+      for (tile = t.tile_lo + split * W + wave; tile <= end8; tile += step)
+        if (part_tile(tile)) spoil(tile, [&](int d, int key) { return kv_bad8<DT>(p.c.v8 + ((size_t)pair * p.c.blocks + tile) * kKvBlock * D + d * kKvBlock + key); });
+    if (tail) spoil(t.last, [&](int d, int key) { return kv_bad16<DT>(p.c.vt + ((size_t)pair * D + d) * kKvBlock + key); });
   }
-
   sum += __shfl_xor(sum, 16, kWave);
   sum += __shfl_xor(sum, 32, kWave);
 
@@ -609,8 +622,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   constexpr int kVecs = D * kKvBlock / 16;  // of a tile's keys, and of its values
   typedef Kv<DT> F;
   __shared__ u32x4 s_kv[2][2][kVecs];
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6, m = lane & 31, h = lane >> 5;
-  const int pair = blockIdx.x, r0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * ROWS, split = blockIdx.z, rows = p.T * p.group;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 31, h = lane >> 5;
+  // workgroups with the most keys first; the second half of those that start together the other way round, so that a CU's two come out even
+  const int ny = gridDim.y, y = blockIdx.y, half = (ny + 1) / 2;
+  const int r0 = (p.fold && y >= half ? y - half : ny - 1 - y) * ROWS;
+  const int pair = blockIdx.x, split = blockIdx.z, rows = p.T * p.group;
   const int b = pair / p.c.heads;
   int start, n;
   KvTiles t;
@@ -658,11 +674,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   };
 
   float top = -FLT_MAX, sum = 0.f;
+  uint32_t some = 0;  // whether a tile that is seen in part had numbers of V that are not finite
   f32x16 o[NW];
+  auto zeros = [] {
+    f32x16 z;
 #pragma unroll
-  for (int w = 0; w < NW; w++)
+    for (int e = 0; e < 16; e++) z[e] = 0.f;
+    return z;
+  };
 #pragma unroll
-    for (int e = 0; e < 16; e++) o[w][e] = 0.f;
+  for (int w = 0; w < NW; w++) o[w] = zeros();
   const int ktok = 16 * (m >> 2 & 1) + 4 * (m >> 3) + (m & 3);  // token of this lane's row of K in tile 0; 32 more in tile 1
 
   // weights of a tile from its scores; returns them as operands
@@ -674,14 +695,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
 #pragma unroll
       for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[u][e]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-    const float now = fmaxf(top, fmaf(mx, sc, lv)), off = lv + F::HEAD - now;
-    if (__any(now > top)) {
-      const float keep = __builtin_amdgcn_exp2f(top - now);
-      sum *= keep;
+    const float now = fmaxf(top, fmaf(mx, sc, lv)), off = lv + F::HEAD - now, keep = __builtin_amdgcn_exp2f(top - now);
+    sum *= keep;
 #pragma unroll
-      for (int w = 0; w < NW; w++) o[w] *= keep;
-      top = now;
-    }
+    for (int w = 0; w < NW; w++) o[w] *= keep;
+    top = now;
     float add = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -696,6 +714,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
         for (int e = 0; e < 4; e++) pf[u][v][e] = DT::pack(s[u][8 * v + 2 * e], s[u][8 * v + 2 * e + 1]);
     }
     sum = fmaf(add, __builtin_amdgcn_rcpf(vs), sum);
+    asm volatile("" : "+v"(sum));  // here: the weights' registers are wanted
   };
   auto seen = [&](int key) { return key <= pos && key > first; };
   auto mask = [&](f32x16 (&s)[2], int tile) {
@@ -704,26 +723,42 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
 #pragma unroll
       for (int e = 0; e < 16; e++) s[u][e] = seen(tile * kKvBlock + 32 * u + 16 * h + e) ? s[u][e] : -INFINITY;
   };
-  // O of elements 32 w .. with numbers of V that are not finite taken out of the operands a; bad has 1 in their places
-  auto add_part = [&](int w, int tile, u32x4 (&a)[2][2], u32x4 (&bad)[2][2], u32x4 (&pf)[2][2]) {
-    f32x16 z;
+  // one tile of 64 keys from LDS; PART: some query of the wave does not see all of them
+  auto take = [&](auto PART, int tile, int buf) {
+    f32x16 s[2] = {zeros(), zeros()};
 #pragma unroll
-    for (int e = 0; e < 16; e++) z[e] = 0.f;
+    for (int c = 0; c < C; c++)
 #pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-      for (int v = 0; v < 2; v++) {
-        u32x4 one;
-        const int key = tile * kKvBlock + 32 * u + 16 * h + 8 * v;
-#pragma unroll
-        for (int e = 0; e < 4; e++) one[e] = (seen(key + 2 * e) ? F::kOne : 0u) | (seen(key + 2 * e + 1) ? F::kOne << 16 : 0u);
-        o[w] = Mma32<DT>::run(a[u][v], pf[u][v], o[w]);
-        z = Mma32<DT>::run(bad[u][v], one, z);
+      for (int u = 0; u < 2; u++) {
+        const int tok = ktok + 32 * u;
+        const u32x4 kk = s_kv[buf][0][tok * PK + ((2 * c + h) ^ kv_swap_k<D>(tok))];
+        s[u] = Mma32<DT>::run(kv_wide<DT>(kk[0], kk[1]), qf[c][0], s[u]);
+        s[u] = Mma32<DT>::run(kv_wide<DT>(kk[2], kk[3]), qf[c][1], s[u]);
       }
+    if constexpr (PART) mask(s, tile);
+    u32x4 pf[2][2];
+    weigh(s, kscale[tile], vscale[tile], pf);
+    auto values = [&](int w, int u) {
+      const int d = 32 * w + m;
+      return s_kv[buf][1][d * 4 + ((2 * u + h) ^ kv_swap_v(d))];
+    };
 #pragma unroll
-    for (int e = 0; e < 16; e++) o[w][e] = z[e] > 0.f ? NAN : o[w][e];
+    for (int w = 0; w < NW; w++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        u32x4 vv = values(w, u);
+        if constexpr (PART) some |= kv_fix8(vv);
+        o[w] = Mma32<DT>::run(kv_wide<DT>(vv[0], vv[1]), pf[u][0], o[w]);
+        o[w] = Mma32<DT>::run(kv_wide<DT>(vv[2], vv[3]), pf[u][1], o[w]);
+      }
   };
 
+  auto whole_tile = [&](int tile) {  // whether all queries of the wave see all of it
+    return tile * kKvBlock + kKvBlock - 1 <= lo_pos && !(p.window && tile * kKvBlock <= hi_pos - p.window);
+  };
+  auto seen_tile = [&](int tile) {  // whether some query of the wave sees some of it
+    return tile * kKvBlock <= hi_pos && !(p.window && tile * kKvBlock + kKvBlock - 1 <= lo_pos - p.window);
+  };
   const int end8 = min(t.tile_hi, t.last - 1);  // last tile in 8 bits
   int tile = t.tile_lo + split, buf = 0;
   if (tile <= end8) {
@@ -731,68 +766,28 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
     store(0);
   }
   lds_barrier();
-  for (; tile <= end8; tile += t.active, buf ^= 1) {
-    const bool more = tile + t.active <= end8;
-    if (more) fetch(tile + t.active);
-    const int key0 = tile * kKvBlock;
-    if (key0 <= hi_pos && !(p.window && key0 + kKvBlock - 1 <= lo_pos - p.window)) {  // some query of the wave sees some key
-      const bool part = key0 + kKvBlock - 1 > lo_pos || (p.window && key0 <= hi_pos - p.window);
-      f32x16 s[2];
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) s[u][e] = 0.f;
-#pragma unroll
-      for (int c = 0; c < C; c++)
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-          const int tok = ktok + 32 * u;
-          const u32x4 kk = s_kv[buf][0][tok * PK + ((2 * c + h) ^ kv_swap_k<D>(tok))];
-          s[u] = Mma32<DT>::run(kv_wide<DT>(kk[0], kk[1]), qf[c][0], s[u]);
-          s[u] = Mma32<DT>::run(kv_wide<DT>(kk[2], kk[3]), qf[c][1], s[u]);
-        }
-      if (part) mask(s, tile);
-      u32x4 pf[2][2];
-      weigh(s, kscale[tile], vscale[tile], pf);
-#pragma unroll
-      for (int w = 0; w < NW; w++) {
-        const int d = 32 * w + m;
-        u32x4 vv[2];
-#pragma unroll
-        for (int u = 0; u < 2; u++) vv[u] = s_kv[buf][1][d * 4 + ((2 * u + h) ^ kv_swap_v(d))];
-        if (!part) {
-#pragma unroll
-          for (int u = 0; u < 2; u++) {
-            o[w] = Mma32<DT>::run(kv_wide<DT>(vv[u][0], vv[u][1]), pf[u][0], o[w]);
-            o[w] = Mma32<DT>::run(kv_wide<DT>(vv[u][2], vv[u][3]), pf[u][1], o[w]);
-          }
-        } else {
-          u32x4 a[2][2], bad[2][2];
-#pragma unroll
-          for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int v = 0; v < 2; v++) {
-              uint32_t w0 = vv[u][2 * v], w1 = vv[u][2 * v + 1];
-              const uint32_t b0 = kv_fix8(w0), b1 = kv_fix8(w1);
-              a[u][v] = kv_wide<DT>(w0, w1);
-              bad[u][v] = kv_wide<DT>(b0, b1);
-            }
-          add_part(w, tile, a, bad, pf);
-        }
-      }
+  auto run = [&](auto PART, int to) {
+    for (; tile <= to; tile += t.active, buf ^= 1) {
+      const bool more = tile + t.active <= end8;
+      if (more) fetch(tile + t.active);
+      if (!PART || seen_tile(tile)) take(PART, tile, buf);
+      if (more) store(buf ^ 1);
+      lds_barrier();
     }
-    if (more) store(buf ^ 1);
-    lds_barrier();
-  }
+  };
+  // tiles that a window cuts, tiles that all of the workgroup's queries see, tiles that hold some of their own keys
+  const int cut = p.window && t.pos_hi >= p.window ? (t.pos_hi - p.window) / kKvBlock : -1, own = (t.pos_lo + 1) / kKvBlock;  // last and first of them
+  run(std::true_type(), min(cut, end8));
+  run(std::false_type(), min(own - 1, end8));
+  run(std::true_type(), end8);
   // the tail, by the split whose turn it would be, from memory: one tile of the last rows only
-  if (t.tile_hi == t.last && (t.last - t.tile_lo) % t.active == split && t.last * kKvBlock <= hi_pos) {
+  const bool tail = t.tile_hi == t.last && (t.last - t.tile_lo) % t.active == split && t.last * kKvBlock <= hi_pos;
+  if (tail) {
     const uint16_t* kt = p.c.kt + (size_t)pair * kKvBlock * D;
     const uint16_t* vt = p.c.vt + (size_t)pair * kKvBlock * D;
-    f32x16 s[2];
+    f32x16 s[2] = {zeros(), zeros()};
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-#pragma unroll
-      for (int e = 0; e < 16; e++) s[u][e] = 0.f;
 #pragma unroll
       for (int c = 0; c < C; c++)
 #pragma unroll
@@ -805,21 +800,40 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
     weigh(s, 1.f, 1.f, pf);
 #pragma unroll
     for (int w = 0; w < NW; w++) {
-      u32x4 a[2][2], bad[2][2];
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll
         for (int v = 0; v < 2; v++) {
-          a[u][v] = *(const u32x4*)(vt + (32 * w + m) * kKvBlock + 32 * u + 16 * h + 8 * v);
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            uint32_t x = a[u][v][e];
-            bad[u][v][e] = kv_fix16<DT>(x);
-            a[u][v][e] = x;
-          }
+          u32x4 x = *(const u32x4*)(vt + (32 * w + m) * kKvBlock + 32 * u + 16 * h + 8 * v);
+          some |= kv_fix16<DT>(x);
+          o[w] = Mma32<DT>::run(x, pf[u][v], o[w]);
         }
-      add_part(w, t.last, a, bad, pf);
+      __builtin_amdgcn_sched_barrier(0);
     }
+  }
+  if (__any(some != 0)) {  // the queries that see a number that is not finite
+    auto spoil = [&](int tile, auto load) {
+#pragma unroll
+      for (int w = 0; w < NW; w++) {
+        f32x16 z = zeros();
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int v = 0; v < 2; v++) {
+            const int key = tile * kKvBlock + 32 * u + 16 * h + 8 * v;
+            u32x4 one;
+#pragma unroll
+            for (int e = 0; e < 4; e++) one[e] = (seen(key + 2 * e) ? F::kOne : 0u) | (seen(key + 2 * e + 1) ? F::kOne << 16 : 0u);
+            z = Mma32<DT>::run(load(32 * w + m, 32 * u + 16 * h + 8 * v), one, z);
+          }
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[w][e] = z[e] > 0.f ? NAN : o[w][e];
+      }
+    };
+    for (tile = t.tile_lo + split; tile <= end8; tile += t.active)
+      if (seen_tile(tile) && !whole_tile(tile))
+        spoil(tile, [&](int d, int key) { return kv_bad8<DT>((const uint8_t*)(v8 + (size_t)tile * kVecs) + d * kKvBlock + key); });
+    if (tail) spoil(t.last, [&](int d, int key) { return kv_bad16<DT>(p.c.vt + ((size_t)pair * D + d) * kKvBlock + key); });
   }
   sum += __shfl_xor(sum, 32, kWave);
   if (mine >= rows) return;

@@ -11,6 +11,7 @@ namespace cats {
 struct KvAttnPlan {
   bool prompt; // 128 rows a workgroup
   int splits;  // of a row's cache
+  bool fold;   // prompt: all workgroups start together
   bool seal;   // the new tokens are in the tails only: quantise the blocks they complete
 };
 KvAttnPlan kv8_attn_plan(int B, int T, int heads, int kv_heads, int blocks, int window);
