@@ -54,13 +54,13 @@ __device__ __forceinline__ bool kv_span(const KvSpan& s, int b, int T, int& star
 template <class DT> struct Kv;
 template <> struct Kv<F16> {
   static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
-  static constexpr float HEAD = 15.f;
+  static constexpr float HEAD = 15.f, SLACK = 8.f;
   template <bool HI>
   static __device__ __forceinline__ uint32_t cvt(uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI)); }
 };
 template <> struct Kv<BF16> {
   static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u;
-  static constexpr float HEAD = 0.f;
+  static constexpr float HEAD = 0.f, SLACK = 8.f;
   template <bool HI>
   static __device__ __forceinline__ uint32_t cvt(uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI)); }
 };
@@ -695,11 +695,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
 #pragma unroll
       for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[u][e]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-    const float now = fmaxf(top, fmaf(mx, sc, lv)), off = lv + F::HEAD - now, keep = __builtin_amdgcn_exp2f(top - now);
-    sum *= keep;
+    const float now = fmaxf(top, fmaf(mx, sc, lv));
+    if (__any(now > top + F::SLACK)) {
+      const float keep = __builtin_amdgcn_exp2f(top - now);
+      sum *= keep;
 #pragma unroll
-    for (int w = 0; w < NW; w++) o[w] *= keep;
-    top = now;
+      for (int w = 0; w < NW; w++) o[w] *= keep;
+      top = now;
+    }
+    const float off = lv + F::HEAD - F::SLACK - top;
     float add = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
