@@ -655,7 +655,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   const float* vscale = p.c.vs + (size_t)pair * p.c.blocks;
 
   u32x4 kn[NL], vn[NL];
+  float ksn = 1.f, vsn = 1.f, ks = 1.f, vs = 1.f;  // scales of the tile that is fetched and of the one in LDS
   auto fetch = [&](int tile) {
+    ksn = kscale[tile];
+    vsn = vscale[tile];
 #pragma unroll
     for (int i = 0; i < NL; i++)
       if (kVecs >= 256 || tid < kVecs) {
@@ -664,6 +667,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
       }
   };
   auto store = [&](int buf) {
+    ks = ksn;
+    vs = vsn;
 #pragma unroll
     for (int i = 0; i < NL; i++)
       if (kVecs >= 256 || tid < kVecs) {
@@ -741,7 +746,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
       }
     if constexpr (PART) mask(s, tile);
     u32x4 pf[2][2];
-    weigh(s, kscale[tile], vscale[tile], pf);
+    weigh(s, ks, vs, pf);
     auto values = [&](int w, int u) {
       const int d = 32 * w + m;
       return s_kv[buf][1][d * 4 + ((2 * u + h) ^ kv_swap_v(d))];
