@@ -313,6 +313,16 @@ __device__ __forceinline__ u32x4 kv_bad16(const uint16_t* at) {
   return w;
 }
 
+// Largest over the lanes that agree modulo 32, and modulo 16, in all of them: the halves of a wave, and its rows, change places.
+__device__ __forceinline__ float max_mod32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_mod16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return max_mod32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+
 // One new token, or a few: 16 rows of queries, the cache split over workgroups and over the four waves of each, the waves' results joined in LDS
 // and the workgroups' by kv8_join_kernel.  Each wave takes 64 tokens at a time:
 //   S^T = K . Q^T   tile i, row 4 g + e of the 16x16 result: token 16 g + 4 i + e, in lanes of group g = lane / 16; columns are queries
@@ -411,8 +421,7 @@ __global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_ker
     for (int i = 0; i < N; i++)
 #pragma unroll
       for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[i][e]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+    mx = max_mod16(mx);
     const float now = fmaxf(top, fmaf(mx, sc, lv)), off = lv + F::HEAD - now;
     if (__any(now > top)) {
       const float keep = __builtin_amdgcn_exp2f(top - now);
@@ -699,7 +708,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
     for (int u = 0; u < 2; u++)
 #pragma unroll
       for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[u][e]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+    mx = max_mod32(mx);
     const float now = fmaxf(top, fmaf(mx, sc, lv));
     if (__any(now > top + F::SLACK)) {
       const float keep = __builtin_amdgcn_exp2f(top - now);
@@ -734,28 +743,43 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   };
   // one tile of 64 keys from LDS; PART: some query of the wave does not see all of them
   auto take = [&](auto PART, int tile, int buf) {
+    // All of a tile's keys are asked for at once, and its values before the weights are computed: what LDS takes to answer is as long as eight
+    // products each time.
     f32x16 s[2] = {zeros(), zeros()};
+    u32x4 x[2 * NW];  // C is NW
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         const int tok = ktok + 32 * u;
-        const u32x4 kk = s_kv[buf][0][tok * PK + ((2 * c + h) ^ kv_swap_k<D>(tok))];
+        x[2 * c + u] = s_kv[buf][0][tok * PK + ((2 * c + h) ^ kv_swap_k<D>(tok))];
+      }
+    if (D <= 128) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const u32x4 kk = x[2 * c + u];
         s[u] = Mma32<DT>::run(kv_wide<DT>(kk[0], kk[1]), qf[c][0], s[u]);
         s[u] = Mma32<DT>::run(kv_wide<DT>(kk[2], kk[3]), qf[c][1], s[u]);
       }
-    if constexpr (PART) mask(s, tile);
-    u32x4 pf[2][2];
-    weigh(s, ks, vs, pf);
-    auto values = [&](int w, int u) {
-      const int d = 32 * w + m;
-      return s_kv[buf][1][d * 4 + ((2 * u + h) ^ kv_swap_v(d))];
-    };
+    if (D <= 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int w = 0; w < NW; w++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        u32x4 vv = values(w, u);
+        const int d = 32 * w + m;
+        x[2 * w + u] = s_kv[buf][1][d * 4 + ((2 * u + h) ^ kv_swap_v(d))];
+      }
+    if (D <= 128) __builtin_amdgcn_sched_barrier(0);
+    if constexpr (PART) mask(s, tile);
+    u32x4 pf[2][2];
+    weigh(s, ks, vs, pf);
+#pragma unroll
+    for (int w = 0; w < NW; w++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        u32x4 vv = x[2 * w + u];
         if constexpr (PART) some |= kv_fix8(vv);
         o[w] = Mma32<DT>::run(kv_wide<DT>(vv[0], vv[1]), pf[u][0], o[w]);
         o[w] = Mma32<DT>::run(kv_wide<DT>(vv[2], vv[3]), pf[u][1], o[w]);
