@@ -596,8 +596,9 @@ __global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_ker
   }
 }
 
-// Many new tokens: 128 rows of queries a workgroup, 32 a wave, all of whose waves share the tiles of 64 keys, which come through LDS in 8 bits,
-// the next one's loads in flight over this one's products.  The same steps as above with v_mfma_f32_32x32x16:
+// Many new tokens: 64 rows of queries a workgroup and two tiles of 64 keys at a time, a wave for each 32 rows and tile; what the two halves of the keys
+// give is joined in LDS at the end.  The tiles come into LDS in 8 bits, straight from memory, the next two while the weights of these are computed.
+// The same steps as above with v_mfma_f32_32x32x16:
 //   S^T   tile u, row 8 a + 4 h + i of the result: token 32 u + 16 h + 4 a + i, in lanes of half h = lane / 32; columns are queries
 //   O^T   operand of step (u, v): tokens 32 u + 16 h + 8 v .. + 7, again those whose weights the lane has
 // Rows of LDS are 16-byte pieces, exchanged within a row so that any 16 lanes in order find the 64 banks once each.
@@ -624,14 +625,15 @@ __device__ __forceinline__ int kv_swap_k(int t) {
 }
 __device__ __forceinline__ int kv_swap_v(int d) { return d >> 2 & 3; }
 
-constexpr int kKvPromptRows = 128, kKvPromptUnit = 8;  // rows of a workgroup; tiles that make a split worth while
+constexpr int kKvPromptRows = 64, kKvPromptUnit = 8;  // rows of a workgroup; tiles that make a split worth while
 template <class DT, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(KvAttnArgs p) {
-  constexpr int ROWS = kKvPromptRows, C = D / 32, NW = D / 32, PK = D / 16, NL = D * kKvBlock / 16 / 256 > 0 ? D * kKvBlock / 16 / 256 : 1;
+  constexpr int ROWS = kKvPromptRows, C = D / 32, NW = D / 32, PK = D / 16;
   constexpr int kVecs = D * kKvBlock / 16;  // of a tile's keys, and of its values
   typedef Kv<DT> F;
-  __shared__ u32x4 s_kv[2][2][kVecs];
+  __shared__ u32x4 s_kv[2][2][2][kVecs];  // [buffer][tile][keys, values]
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 31, h = lane >> 5;
+  const int rw = wave & 1, kh = wave >> 1;  // the wave's rows and its tile of two
   // workgroups with the most keys first; the second half of those that start together the other way round, so that a CU's two come out even
   const int ny = gridDim.y, y = blockIdx.y, half = (ny + 1) / 2;
   const int r0 = (p.fold && y >= half ? y - half : ny - 1 - y) * ROWS;
@@ -646,10 +648,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   }
   if (split >= t.active) return;
 
-  const int mine = r0 + 32 * wave + m, row = min(mine, rows - 1), pos = start + min(row / p.group, n - 1);
+  const int mine = r0 + 32 * rw + m, row = min(mine, rows - 1), pos = start + min(row / p.group, n - 1);
   const int first = p.window ? pos - p.window : -1;  // the query sees first + 1 .. pos
   // the wave's own keys
-  const int lo_pos = start + min((r0 + 32 * wave) / p.group, n - 1), hi_pos = start + min((r0 + 32 * wave + 31) / p.group, n - 1);
+  const int lo_pos = start + min((r0 + 32 * rw) / p.group, n - 1), hi_pos = start + min((r0 + 32 * rw + 31) / p.group, n - 1);
   u32x4 qf[C][2];
   {
     const uint16_t* q = p.q + b * p.q_row + (row / p.group) * p.q_tok + ((pair - b * p.c.heads) * p.group + row % p.group) * p.q_head;
@@ -663,28 +665,27 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   const float* kscale = p.c.ks + (size_t)pair * p.c.blocks;
   const float* vscale = p.c.vs + (size_t)pair * p.c.blocks;
 
-  u32x4 kn[NL], vn[NL];
-  float ksn = 1.f, vsn = 1.f, ks = 1.f, vs = 1.f;  // scales of the tile that is fetched and of the one in LDS
-  auto fetch = [&](int tile) {
-    ksn = kscale[tile];
-    vsn = vscale[tile];
+  // A wave brings half of the rows of keys and of values of its tile, 1 KiB at a time: lane l of load j writes piece 64 j + l and reads what belongs
+  // there.  What is exchanged goes by bits of the row, so load j differs from load 0 by constants.
+  const int end8 = min(t.tile_hi, t.last - 1);  // last tile in 8 bits; behind it the last one comes again
+  float ks = 1.f, vs = 1.f, ks1 = 1.f, vs1 = 1.f;  // scales of the wave's tile and of the next one
+  auto bring = [&](int tile, int buf) {
+    const int at = min(tile + kh, end8);
+    ks1 = kscale[at];
+    vs1 = vscale[at];
+    const u32x4* kf = k8 + (size_t)at * kVecs + rw * (kVecs / 2);
+    const u32x4* vf = v8 + (size_t)at * kVecs + rw * (kVecs / 2);
+    u32x4* to = s_kv[buf][kh][0] + rw * (kVecs / 2);
+    int l = lane;
+    asm volatile("" : "+v"(l));  // addresses are computed here each time: kept over the loop they would cost the registers that tiles need
+    const int kq = (l % PK) ^ kv_swap_k<D>(l / PK), kl = l / PK * PK, vl = l / 4 * 4 + ((l % 4) ^ kv_swap_v(l / 4));
 #pragma unroll
-    for (int i = 0; i < NL; i++)
-      if (kVecs >= 256 || tid < kVecs) {
-        kn[i] = k8[(size_t)tile * kVecs + i * 256 + tid];
-        vn[i] = v8[(size_t)tile * kVecs + i * 256 + tid];
-      }
-  };
-  auto store = [&](int buf) {
-    ks = ksn;
-    vs = vsn;
-#pragma unroll
-    for (int i = 0; i < NL; i++)
-      if (kVecs >= 256 || tid < kVecs) {
-        const int at = i * 256 + tid, tok = at / PK, d = at / 4;
-        s_kv[buf][0][tok * PK + ((at % PK) ^ kv_swap_k<D>(tok))] = kn[i];
-        s_kv[buf][1][d * 4 + ((at % 4) ^ kv_swap_v(d))] = vn[i];
-      }
+    for (int j = 0; j < kVecs / 2 / kWave; j++) {
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kf + j * kWave + (kl + (kq ^ kv_swap_k<D>(j * kWave / PK)))),
+                                       (__attribute__((address_space(3))) void*)(to + j * kWave), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vf + j * kWave + vl),
+                                       (__attribute__((address_space(3))) void*)(to + kVecs + j * kWave), 16, 0, 0);
+    }
   };
 
   float top = -FLT_MAX, sum = 0.f;
@@ -742,79 +743,85 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
       for (int e = 0; e < 16; e++) s[u][e] = seen(tile * kKvBlock + 32 * u + 16 * h + e) ? s[u][e] : -INFINITY;
   };
   // one tile of 64 keys from LDS; PART: some query of the wave does not see all of them
-  auto take = [&](auto PART, int tile, int buf) {
+  auto take = [&](auto PART, int tile, int buf, auto behind) {
     // All of a tile's keys are asked for at once, and its values before the weights are computed: what LDS takes to answer is as long as eight
-    // products each time.
+    // products each time.  (Heads of 256 elements do not have the registers.)
+    constexpr bool ASK = D <= 128;
     f32x16 s[2] = {zeros(), zeros()};
-    u32x4 x[2 * NW];  // C is NW
+    int kt = ktok, vd = m;  // as in bring
+    asm volatile("" : "+v"(kt), "+v"(vd));
+    auto keys = [&](int c, int u) { return s_kv[buf][kh][0][(kt + 32 * u) * PK + ((2 * c + h) ^ kv_swap_k<D>(kt))]; };
+    auto values = [&](int w, int u) { return s_kv[buf][kh][1][(32 * w + vd) * 4 + ((2 * u + h) ^ kv_swap_v(vd))]; };
+    u32x4 x[ASK ? 2 * NW : 1];  // C is NW
+    if constexpr (ASK) {
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) x[2 * c + u] = keys(c, u);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        const int tok = ktok + 32 * u;
-        x[2 * c + u] = s_kv[buf][0][tok * PK + ((2 * c + h) ^ kv_swap_k<D>(tok))];
-      }
-    if (D <= 128) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int c = 0; c < C; c++)
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const u32x4 kk = x[2 * c + u];
+        const u32x4 kk = ASK ? x[ASK ? 2 * c + u : 0] : keys(c, u);
         s[u] = Mma32<DT>::run(kv_wide<DT>(kk[0], kk[1]), qf[c][0], s[u]);
         s[u] = Mma32<DT>::run(kv_wide<DT>(kk[2], kk[3]), qf[c][1], s[u]);
       }
-    if (D <= 128) __builtin_amdgcn_sched_barrier(0);
+    if constexpr (ASK) {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int w = 0; w < NW; w++)
+      for (int w = 0; w < NW; w++)
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const int d = 32 * w + m;
-        x[2 * w + u] = s_kv[buf][1][d * 4 + ((2 * u + h) ^ kv_swap_v(d))];
-      }
-    if (D <= 128) __builtin_amdgcn_sched_barrier(0);
+        for (int u = 0; u < 2; u++) x[2 * w + u] = values(w, u);
+      __builtin_amdgcn_sched_barrier(0);
+      behind();
+    }
+    __builtin_amdgcn_s_setprio(0);
     if constexpr (PART) mask(s, tile);
     u32x4 pf[2][2];
     weigh(s, ks, vs, pf);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int w = 0; w < NW; w++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        u32x4 vv = x[2 * w + u];
+        u32x4 vv = ASK ? x[ASK ? 2 * w + u : 0] : values(w, u);
         if constexpr (PART) some |= kv_fix8(vv);
         o[w] = Mma32<DT>::run(kv_wide<DT>(vv[0], vv[1]), pf[u][0], o[w]);
         o[w] = Mma32<DT>::run(kv_wide<DT>(vv[2], vv[3]), pf[u][1], o[w]);
       }
+    if constexpr (!ASK) behind();
   };
 
-  auto whole_tile = [&](int tile) {  // whether all queries of the wave see all of it
-    return tile * kKvBlock + kKvBlock - 1 <= lo_pos && !(p.window && tile * kKvBlock <= hi_pos - p.window);
-  };
   auto seen_tile = [&](int tile) {  // whether some query of the wave sees some of it
     return tile * kKvBlock <= hi_pos && !(p.window && tile * kKvBlock + kKvBlock - 1 <= lo_pos - p.window);
   };
-  const int end8 = min(t.tile_hi, t.last - 1);  // last tile in 8 bits
-  int tile = t.tile_lo + split, buf = 0;
-  if (tile <= end8) {
-    fetch(tile);
-    store(0);
-  }
+  const int step = 2 * t.active;
+  int tile = t.tile_lo + 2 * split, buf = 0;  // the first of the two
+  if (t.tile_lo <= end8) bring(tile, 0);
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): in LDS
+  ks = ks1, vs = vs1;
   lds_barrier();
   auto run = [&](auto PART, int to) {
-    for (; tile <= to; tile += t.active, buf ^= 1) {
-      const bool more = tile + t.active <= end8;
-      if (more) fetch(tile + t.active);
-      if (!PART || seen_tile(tile)) take(PART, tile, buf);
-      if (more) store(buf ^ 1);
+    for (; tile <= to; tile += step, buf ^= 1) {
+      const int at = tile + kh;
+      // After the last read of this buffer's other half: a read of LDS behind these loads would wait for them.
+      auto behind = [&] { bring(tile + step, buf ^ 1); };
+      if (!PART || (at <= end8 && seen_tile(at))) take(PART, at, buf, behind);
+      else behind();
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+      ks = ks1, vs = vs1;
       lds_barrier();
     }
   };
   // tiles that a window cuts, tiles that all of the workgroup's queries see, tiles that hold some of their own keys
   const int cut = p.window && t.pos_hi >= p.window ? (t.pos_hi - p.window) / kKvBlock : -1, own = (t.pos_lo + 1) / kKvBlock;  // last and first of them
   run(std::true_type(), min(cut, end8));
-  run(std::false_type(), min(own - 1, end8));
+  run(std::false_type(), min(own - 2, end8 - 1));
   run(std::true_type(), end8);
   // the tail, by the split whose turn it would be, from memory: one tile of the last rows only
-  const bool tail = t.tile_hi == t.last && (t.last - t.tile_lo) % t.active == split && t.last * kKvBlock <= hi_pos;
+  const bool tail = t.tile_hi == t.last && (t.last - t.tile_lo) / 2 % t.active == split && (t.last - t.tile_lo) % 2 == kh && t.last * kKvBlock <= hi_pos;
   if (tail) {
     const uint16_t* kt = p.c.kt + (size_t)pair * kKvBlock * D;
     const uint16_t* vt = p.c.vt + (size_t)pair * kKvBlock * D;
@@ -863,12 +870,40 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
         for (int e = 0; e < 16; e++) o[w][e] = z[e] > 0.f ? NAN : o[w][e];
       }
     };
-    for (tile = t.tile_lo + split; tile <= end8; tile += t.active)
-      if (seen_tile(tile) && !whole_tile(tile))
+    for (tile = t.tile_lo + 2 * split + kh; tile <= end8; tile += step)
+      if (seen_tile(tile))
         spoil(tile, [&](int d, int key) { return kv_bad8<DT>((const uint8_t*)(v8 + (size_t)tile * kVecs) + d * kKvBlock + key); });
     if (tail) spoil(t.last, [&](int d, int key) { return kv_bad16<DT>(p.c.vt + ((size_t)pair * D + d) * kKvBlock + key); });
   }
   sum += __shfl_xor(sum, 32, kWave);
+  // the other half of the keys
+  __shared__ float s_top[2][32], s_sum[2][32];
+  f32x4* s_o = (f32x4*)s_kv[rw][0][0];  // all tiles have been read: [D / 8][lane] of each wave
+  if (kh == 1) {
+#pragma unroll
+    for (int w = 0; w < NW; w++)
+#pragma unroll
+      for (int a = 0; a < 4; a++) s_o[(4 * w + a) * kWave + lane] = f32x4{o[w][4 * a], o[w][4 * a + 1], o[w][4 * a + 2], o[w][4 * a + 3]};
+    if (h == 0) {
+      s_top[rw][m] = top;
+      s_sum[rw][m] = sum;
+    }
+  }
+  lds_barrier();
+  if (kh == 1) return;
+  {
+    const float other = s_top[rw][m], now = fmaxf(top, other), f = __builtin_amdgcn_exp2f(top - now), g = __builtin_amdgcn_exp2f(other - now);
+    sum = fmaf(g, s_sum[rw][m], f * sum);
+    top = now;
+#pragma unroll
+    for (int w = 0; w < NW; w++)
+#pragma unroll
+      for (int a = 0; a < 4; a++) {
+        const f32x4 x = s_o[(4 * w + a) * kWave + lane];
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[w][4 * a + e] = fmaf(g, x[e], f * o[w][4 * a + e]);
+      }
+  }
   if (mine >= rows) return;
   if (t.active == 1) {
     const bool dead = mine / p.group >= n;
