@@ -12,6 +12,7 @@
 // v_mfma_f32_16x16x32 and of 32x32x16, where 64 tokens of one element are 16 bytes of each of four lanes.
 #pragma once
 #include <float.h>
+#include <limits.h>
 
 #include <type_traits>
 
@@ -737,10 +738,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   };
   auto seen = [&](int key) { return key <= pos && key > first; };
   auto mask = [&](f32x16 (&s)[2], int tile) {
+    const int most = pos - tile * kKvBlock - 16 * h;  // of 32 u + e
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
-      for (int e = 0; e < 16; e++) s[u][e] = seen(tile * kKvBlock + 32 * u + 16 * h + e) ? s[u][e] : -INFINITY;
+      for (int e = 0; e < 16; e++) s[u][e] = 32 * u + e <= most ? s[u][e] : -INFINITY;
+    if (p.window) {
+      const int least = most - p.window;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[u][e] = 32 * u + e > least ? s[u][e] : -INFINITY;
+    }
   };
   // one tile of 64 keys from LDS; PART: some query of the wave does not see all of them
   auto take = [&](auto PART, int tile, int buf, auto behind) {
@@ -778,7 +787,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
       behind();
     }
     __builtin_amdgcn_s_setprio(0);
-    if constexpr (PART) mask(s, tile);
+    if constexpr (PART) {
+      mask(s, tile);
+      if constexpr (ASK) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * NW; i++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) bad |= (x[i][e] & 0x7f7f7f7fu) + 0x01010101u;
+        if (__any((bad & 0x80808080u) != 0)) {
+          some = 1;
+#pragma unroll
+          for (int i = 0; i < 2 * NW; i++) kv_fix8(x[i]);
+        }
+      }
+    }
     u32x4 pf[2][2];
     weigh(s, ks, vs, pf);
     __builtin_amdgcn_s_setprio(1);
@@ -787,7 +810,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         u32x4 vv = ASK ? x[ASK ? 2 * w + u : 0] : values(w, u);
-        if constexpr (PART) some |= kv_fix8(vv);
+        if constexpr (PART && !ASK) some |= kv_fix8(vv);
         o[w] = Mma32<DT>::run(kv_wide<DT>(vv[0], vv[1]), pf[u][0], o[w]);
         o[w] = Mma32<DT>::run(kv_wide<DT>(vv[2], vv[3]), pf[u][1], o[w]);
       }
@@ -805,11 +828,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   lds_barrier();
   auto run = [&](auto PART, int to) {
     for (; tile <= to; tile += step, buf ^= 1) {
-      const int at = tile + kh;
-      // After the last read of this buffer's other half: a read of LDS behind these loads would wait for them.
-      auto behind = [&] { bring(tile + step, buf ^ 1); };
-      if (!PART || (at <= end8 && seen_tile(at))) take(PART, at, buf, behind);
-      else behind();
+      // Behind the last read of this buffer: a read of LDS behind these loads would wait for them.  A second tile behind the last one has no key
+      // that is seen: it is the last one again.
+      take(PART, tile + kh <= end8 ? tile + kh : INT_MAX / kKvBlock, buf, [&] { bring(tile + step, buf ^ 1); });
       __builtin_amdgcn_s_waitcnt(0x0f70);
       ks = ks1, vs = vs1;
       lds_barrier();
