@@ -275,8 +275,9 @@ __device__ __forceinline__ void kv_fill_rows(const KvAttnArgs& p, int pair, int 
 // were any, the queries that see one are set to NaN: products of those places (1, and 0 elsewhere) and of what a query sees count them.
 __device__ __forceinline__ uint32_t kv_nan8(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7; }  // bit 0 of each byte
 template <class DT>
-__device__ __forceinline__ uint32_t kv_nan16(uint32_t w) {  // bit 0 of each half
-  return ((w & Kv<DT>::kExp) == Kv<DT>::kExp ? 1u : 0u) | ((w >> 16 & Kv<DT>::kExp) == Kv<DT>::kExp ? 0x10000u : 0u);
+__device__ __forceinline__ uint32_t kv_nan16(uint32_t w) {  // bit 0 of each half: an exponent of ones carries into the sign's place
+  constexpr uint32_t E = Kv<DT>::kExp * 0x10001u, L = (Kv<DT>::kExp & -Kv<DT>::kExp) * 0x10001u;
+  return ((w & E) + L) >> 15 & 0x10001u;
 }
 // Sets them to 0; not 0 if there were any.
 __device__ __forceinline__ uint32_t kv_fix8(u32x4& x) {
@@ -856,6 +857,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
 #pragma unroll
       for (int e = 0; e < 16; e++) s[u][e] = fmaf(s[u][e], 0.f, s[u][e]);  // a key that is not finite makes the score NaN, as in e4m3
     }
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 x[NW][2][2];
+#pragma unroll
+    for (int w = 0; w < NW; w++)
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int v = 0; v < 2; v++) x[w][u][v] = *(const u32x4*)(vt + (32 * w + m) * kKvBlock + 32 * u + 16 * h + 8 * v);
+    __builtin_amdgcn_sched_barrier(0);
     mask(s, t.last);
     u32x4 pf[2][2];
     weigh(s, 1.f, 1.f, pf);
@@ -865,9 +875,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
       for (int u = 0; u < 2; u++)
 #pragma unroll
         for (int v = 0; v < 2; v++) {
-          u32x4 x = *(const u32x4*)(vt + (32 * w + m) * kKvBlock + 32 * u + 16 * h + 8 * v);
-          some |= kv_fix16<DT>(x);
-          o[w] = Mma32<DT>::run(x, pf[u][v], o[w]);
+          some |= kv_fix16<DT>(x[w][u][v]);
+          o[w] = Mma32<DT>::run(x[w][u][v], pf[u][v], o[w]);
         }
       __builtin_amdgcn_sched_barrier(0);
     }
