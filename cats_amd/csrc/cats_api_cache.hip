@@ -57,20 +57,28 @@ int check_span(const int64_t* start, int start_step, const int64_t* count, int c
   return (start_step == 0 || start_step == 1) && (count_step == 0 || count_step == 1) ? CATS_OK : CATS_ERR_SHAPE;
 }
 
-constexpr int kStepRows = 64;  // rows of queries a cached head up to which they are taken 16 at a time
+// Which kernel, and how many splits of a row's cache.  Up to 16 rows of queries a cached head are one operand of the step's kernel; more of them are
+// several of its workgroups, each of which reads the cache, or the prompt's kernel.  That one pays for LDS and for few splits of short caches, so
+// the line is drawn by the work, (row, cached head) pairs x 16 rows x tiles of the cache.  Step / prompt in us, heads of 128 elements, bf16:
+//   8 pairs, 64 rows, 20 tiles 12.0 / 17.2     8, 128, 20 14.2 / 17.7     8, 64, 59 14.3 / 16.0     8, 128, 59 17.7 / 17.5     8, 256, 59 25.3 / 20.3
+//   64 pairs, 24 rows, 79 tiles 32.7 / 24.0    64, 64, 79 51.8 / 30.9     32, 64, 2 7.7 / 8.3       32, 256, 5 13.7 / 11.5     32, 512, 10 17.8 / 18.6
+// Both are to have two workgroups a CU (the step's with four: 64 rows of 8 heads at 1000 tokens 26.3 against 23.1, 16 rows of 32 at 2000 49.2
+// against 45.7, one row of 8 at 3000 tokens the same).  A cache of up to 16 tiles is not split: the second launch costs more (one row, 32 heads,
+// 8 cached, 300 tokens 9.5 with, 6.7 without; 16 rows of 32 at 600 tokens 23.2 and 18.8; one row at 600 tokens 9.5 and 9.0).
+constexpr int kStepRows = 16, kStepWork = 3000, kStepAlone = 16;
 
 }  // namespace
 
 KvAttnPlan kv8_attn_plan(int B, int T, int heads, int kv_heads, int blocks, int window) {
   const int cus = current_device_cus(), rows = T * (heads / kv_heads);
-  KvAttnPlan plan = {rows > kStepRows, 1, false, false};
-  const int per = plan.prompt ? kKvPromptRows : 16, unit = plan.prompt ? kKvPromptUnit : 4;
-  const long long groups = (long long)B * kv_heads * ((rows + per - 1) / per);
   // tiles that a workgroup's queries see at most
-  const int tiles = window ? (int)min((long long)blocks, ((long long)window + per + 2 * kKvBlock) / kKvBlock) : blocks;
-  const long long want = ((plan.prompt ? 2ll : 4ll) * cus + groups - 1) / groups;
-  plan.splits = (int)max(1ll, min(want, (long long)(tiles + unit - 1) / unit));
-  plan.fold = groups * plan.splits <= 2ll * cus;
+  const int tiles = window ? (int)min((long long)blocks, ((long long)window + kKvPromptRows + 2 * kKvBlock) / kKvBlock) : blocks;
+  const long long pairs = (long long)B * kv_heads, step_groups = pairs * ((rows + 15) / 16);
+  KvAttnPlan plan = {rows > kStepRows && step_groups * tiles > kStepWork, 1, false};
+  const int unit = plan.prompt ? kKvPromptUnit : kKvStepWaves;
+  const long long groups = plan.prompt ? pairs * ((rows + kKvPromptRows - 1) / kKvPromptRows) : step_groups;
+  const long long want = (2ll * cus + groups - 1) / groups;
+  if (plan.prompt || tiles > kStepAlone) plan.splits = (int)max(1ll, min(want, (long long)(tiles + unit - 1) / unit));
   return plan;
 }
 

@@ -76,7 +76,6 @@ hipError_t launch_kv8_append<CATS_DT>(int D, const KvAppendArgs& a, int B, hipSt
 template <>
 hipError_t launch_kv8_attn<CATS_DT>(int D, const KvAttnPlan& plan, KvAttnArgs a, hipStream_t stream) {
   a.splits = plan.splits;
-  a.fold = plan.fold;
   return KvLaunch<CATS_DT>::attn(D, plan, a, stream);
 }
 

@@ -231,7 +231,6 @@ struct KvAttnArgs {
   int T, group;       // group: query heads of a cached head
   int window;         // keys that a query sees, at most; 0: all
   int pairs, splits;  // pairs: rows x cached heads
-  int fold;           // kv8_attn_prompt_kernel: all workgroups start together
 };
 
 // Row r of a (row, cached head) pair is head r % group of token r / group: the queries of a step that share a cached head are one
@@ -636,10 +635,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   __shared__ u32x4 s_kv[2][2][2][kVecs];  // [buffer][tile][keys, values]
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 31, h = lane >> 5;
   const int rw = wave & 1, kh = wave >> 1;  // the wave's rows and its tile of two
-  // workgroups with the most keys first; the second half of those that start together the other way round, so that a CU's two come out even
-  const int ny = gridDim.y, y = blockIdx.y, half = (ny + 1) / 2;
-  const int r0 = (p.fold && y >= half ? y - half : ny - 1 - y) * ROWS;
-  const int pair = blockIdx.x, split = blockIdx.z, rows = p.T * p.group;
+  const int pair = blockIdx.x, r0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * ROWS, split = blockIdx.z, rows = p.T * p.group;
   const int b = pair / p.c.heads;
   int start, n;
   KvTiles t;

@@ -9,9 +9,8 @@ namespace cats {
 
 // The cache in 8 bits (cats_kv8.h), 16-bit types.  launch_kv8_attn fills in what the plan decides.
 struct KvAttnPlan {
-  bool prompt; // 128 rows a workgroup
+  bool prompt; // kv8_attn_prompt_kernel
   int splits;  // of a row's cache
-  bool fold;   // prompt: all workgroups start together
   bool seal;   // the new tokens are in the tails only: quantise the blocks they complete
 };
 KvAttnPlan kv8_attn_plan(int B, int T, int heads, int kv_heads, int blocks, int window);
