@@ -71,6 +71,13 @@ __device__ __forceinline__ u32x4 kv_wide(uint32_t a, uint32_t b) {
   return u32x4{Kv<DT>::template cvt<false>(a), Kv<DT>::template cvt<true>(a), Kv<DT>::template cvt<false>(b), Kv<DT>::template cvt<true>(b)};
 }
 
+// Places of numbers that are not finite.
+template <class DT>
+__device__ __forceinline__ uint32_t kv_nan16(uint32_t w) {  // bit 0 of each half: an exponent of ones carries into the sign's place
+  constexpr uint32_t E = Kv<DT>::kExp * 0x10001u, L = (Kv<DT>::kExp & -Kv<DT>::kExp) * 0x10001u;
+  return ((w & E) + L) >> 15 & 0x10001u;
+}
+
 // ---- storing ----------------------------------------------------------------------------------------------------------------------
 
 // The smallest power of two with amax <= 448 * scale, between 2^-60 and 2^120 (values below 2^-70 become 0); 1 for a block of zeros.
@@ -81,83 +88,114 @@ __device__ __forceinline__ float kv_scale_of(float amax) {
   e = e < -60 ? -60 : e;
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
-__device__ __forceinline__ float kv_code_of(float x, float inv) { return fmaf(x, 0.f, x * inv); }  // NaN where x is not finite
 
-// Elements d0 .. of a token in the tails.
-template <class DT, int D, int NV>
-__device__ __forceinline__ void kv_tail_token(const uint16_t* kt, const uint16_t* vt, int tok, int d0, u32x4 (&kx)[NV], u32x4 (&vx)[NV]) {
-#pragma unroll
-  for (int i = 0; i < NV; i++) kx[i] = ((const u32x4*)(kt + tok * D + d0))[i];
-#pragma unroll
-  for (int i = 0; i < NV; i++)
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      vx[i][e] = vt[(d0 + 8 * i + 2 * e) * kKvBlock + tok] | (uint32_t)vt[(d0 + 8 * i + 2 * e + 1) * kKvBlock + tok] << 16;
-}
-
-// Quantises block `blk` of a (row, cached head) pair.  256 threads: thread 4 t + i holds elements i D / 4 .. of token t, NV vectors of its key and value.
+// A block on its way into e4m3: 256 threads.  Of the keys thread 4 t + i holds elements i D / 4 .. of token t.  Of the values a thread holds four
+// tokens of eight elements, which become one dword for each element; LDS turns them round.
+template <int D>
+struct KvBlockRegs {
+  static constexpr int NK = D / 32, NV = D > 128 ? D / 128 : 1;
+  u32x4 k[NK];
+  u32x4 v[NV][4];
+  static __device__ __forceinline__ int k_token() { return threadIdx.x / 4; }
+  static __device__ __forceinline__ int k_first() { return threadIdx.x % 4 * (D / 4); }
+  // item i of the thread: tokens 4 v_four .. + 3 of elements v_first .. + 7
+  static __device__ __forceinline__ bool v_on(int i) { return (int)threadIdx.x + 256 * i < 2 * D; }
+  static __device__ __forceinline__ int v_four(int i) { return (threadIdx.x + 256 * i) / (D / 8); }
+  static __device__ __forceinline__ int v_first(int i) { return (threadIdx.x + 256 * i) % (D / 8) * 8; }
+};
 template <int D>
 struct KvStage {
   uint32_t most[2][4];
-  uint8_t v[D][kKvBlock + 4];
+  uint32_t v[D][kKvBlock / 4 + 1];
 };
-template <class DT, int D, int NV>
-__device__ __forceinline__ void kv_quantise(const KvCache& c, size_t pair, int blk, const u32x4 (&kx)[NV], const u32x4 (&vx)[NV], KvStage<D>& stage) {
-  const int tid = threadIdx.x, tok = tid / 4, d0 = tid % 4 * (D / 4);
+// What the tails hold.
+template <int D>
+__device__ __forceinline__ void kv_from_tails(KvBlockRegs<D>& r, const uint16_t* kt, const uint16_t* vt) {
+#pragma unroll
+  for (int i = 0; i < r.NK; i++) r.k[i] = ((const u32x4*)(kt + r.k_token() * D + r.k_first()))[i];
+#pragma unroll
+  for (int i = 0; i < r.NV; i++)
+    if (r.v_on(i)) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const u32x2 lo = *(const u32x2*)(vt + (r.v_first(i) + e) * kKvBlock + 4 * r.v_four(i));
+        const u32x2 hi = *(const u32x2*)(vt + (r.v_first(i) + e + 1) * kKvBlock + 4 * r.v_four(i));
+#pragma unroll
+        for (int j = 0; j < 4; j++) r.v[i][j][e / 2] = (lo[j / 2] >> (16 * (j & 1)) & 0xffffu) | (hi[j / 2] >> (16 * (j & 1)) << 16);
+      }
+    }
+}
+// Quantises block `blk` of a (row, cached head) pair.
+template <class DT, int D>
+__device__ __forceinline__ void kv_quantise(const KvCache& c, size_t pair, int blk, KvBlockRegs<D>& r, KvStage<D>& stage) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  const int tid = threadIdx.x;
   // magnitudes of 16-bit floats are ordered as integers
-  auto most = [](const u32x4 (&x)[NV]) {
-    uint32_t m = 0;
+  auto larger = [](uint32_t m, uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, w & 0x7fff7fffu))); };
+  auto finite = [](uint32_t w) { return w & ~(kv_nan16<DT>(w) * 0xffffu); };
+  auto most = [&](bool all) {  // of keys in the first, of values in the second; all: also of what is not finite
+    uint32_t m[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < NV; i++)
+    for (int i = 0; i < r.NK; i++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const uint32_t w = x[i][e], lo = w & 0x7fffu, hi = w >> 16 & 0x7fffu;
-        m = max(m, max(lo < Kv<DT>::kExp ? lo : 0u, hi < Kv<DT>::kExp ? hi : 0u));
+      for (int e = 0; e < 4; e++) m[0] = larger(m[0], all ? r.k[i][e] : finite(r.k[i][e]));
+#pragma unroll
+    for (int i = 0; i < r.NV; i++)
+      if (r.v_on(i)) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) m[1] = larger(m[1], all ? r.v[i][j][e] : finite(r.v[i][j][e]));
       }
 #pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, kWave));
-    return m;
+    for (int a = 0; a < 2; a++) {
+      m[a] = max(m[a] & 0xffffu, m[a] >> 16);
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) m[a] = max(m[a], (uint32_t)__shfl_xor((int)m[a], o, kWave));
+      if (tid % kWave == 0) stage.most[a][tid / kWave] = m[a];
+    }
+    __syncthreads();
   };
-  const uint32_t mk = most(kx), mv = most(vx);
-  if (tid % kWave == 0) {
-    stage.most[0][tid / kWave] = mk;
-    stage.most[1][tid / kWave] = mv;
+  auto of_all = [&](int a) { return max(max(stage.most[a][0], stage.most[a][1]), max(stage.most[a][2], stage.most[a][3])); };
+  most(true);
+  const bool odd = max(of_all(0), of_all(1)) >= Kv<DT>::kExp;  // numbers that are not finite: rare
+  if (odd) {
+    __syncthreads();
+    most(false);
   }
-  __syncthreads();
-  auto scale_of = [&](int i) {
-    return kv_scale_of(DT::tof((uint16_t)max(max(stage.most[i][0], stage.most[i][1]), max(stage.most[i][2], stage.most[i][3]))));
-  };
-  const float ks = scale_of(0), vs = scale_of(1);
+  const float ks = kv_scale_of(DT::tof((uint16_t)of_all(0))), vs = kv_scale_of(DT::tof((uint16_t)of_all(1)));
   const size_t block = pair * c.blocks + blk;
   if (tid == 0) {
     c.ks[block] = ks;
     c.vs[block] = vs;
   }
-  auto codes = [](u32x4 x, float inv) {  // of eight values
-    uint32_t out[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const uint32_t a = x[2 * i], b = x[2 * i + 1];
-      int w = __builtin_amdgcn_cvt_pk_fp8_f32(kv_code_of(DT::tof((uint16_t)a), inv), kv_code_of(DT::tof((uint16_t)(a >> 16)), inv), 0, false);
-      w = __builtin_amdgcn_cvt_pk_fp8_f32(kv_code_of(DT::tof((uint16_t)b), inv), kv_code_of(DT::tof((uint16_t)(b >> 16)), inv), w, true);
-      out[i] = (uint32_t)w;
-    }
-    return u32x2{out[0], out[1]};
-  };
   const float ki = 1.f / ks, vi = 1.f / vs;  // powers of two
-  u32x2* k8 = (u32x2*)(c.k8 + block * kKvBlock * D + tok * D + d0);
+  auto four = [&](float a, float b, float x, float y) {  // in e4m3; NaN where a number is not finite
+    if (odd) a = fmaf(a, 0.f, a), b = fmaf(b, 0.f, b), x = fmaf(x, 0.f, x), y = fmaf(y, 0.f, y);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, y, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
+  };
+  auto lo = [](uint32_t w) { return DT::tof((uint16_t)w); };
+  auto hi = [](uint32_t w) { return DT::tof((uint16_t)(w >> 16)); };
+  u32x2* k8 = (u32x2*)(c.k8 + block * kKvBlock * D + r.k_token() * D + r.k_first());
 #pragma unroll
-  for (int i = 0; i < NV; i++) k8[i] = codes(kx[i], ki);
-#pragma unroll
-  for (int i = 0; i < NV; i++) {
-    const u32x2 w = codes(vx[i], vi);
-#pragma unroll
-    for (int e = 0; e < 8; e++) stage.v[d0 + 8 * i + e][tok] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
+  for (int i = 0; i < r.NK; i++) {
+    const u32x4 x = r.k[i];
+    k8[i] = u32x2{four(lo(x[0]) * ki, hi(x[0]) * ki, lo(x[1]) * ki, hi(x[1]) * ki), four(lo(x[2]) * ki, hi(x[2]) * ki, lo(x[3]) * ki, hi(x[3]) * ki)};
   }
+#pragma unroll
+  for (int i = 0; i < r.NV; i++)
+    if (r.v_on(i)) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const uint32_t w0 = r.v[i][0][e], w1 = r.v[i][1][e], w2 = r.v[i][2][e], w3 = r.v[i][3][e];
+        stage.v[r.v_first(i) + 2 * e][r.v_four(i)] = four(lo(w0) * vi, lo(w1) * vi, lo(w2) * vi, lo(w3) * vi);
+        stage.v[r.v_first(i) + 2 * e + 1][r.v_four(i)] = four(hi(w0) * vi, hi(w1) * vi, hi(w2) * vi, hi(w3) * vi);
+      }
+    }
   __syncthreads();
   u32x4* v8 = (u32x4*)(c.v8 + block * kKvBlock * D);
   for (int i = tid; i < D * 4; i += 256) {
-    const uint32_t* s = (const uint32_t*)&stage.v[i / 4][i % 4 * 16];
+    const uint32_t* s = &stage.v[i / 4][i % 4 * 4];
     v8[i] = u32x4{s[0], s[1], s[2], s[3]};
   }
 }
@@ -176,7 +214,6 @@ struct KvAppendArgs {
 // Bound by memory: 2 bytes of a value read and one written.
 template <class DT, int D>
 __global__ __launch_bounds__(256) void kv8_append_kernel(KvAppendArgs p) {
-  constexpr int E = D / 4, NV = E / 8;  // elements and vectors of a token that one of its four threads holds
   const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
   int start, n;
   if (!kv_span(p.span, b, p.T, start, n) || n == 0) return;
@@ -190,17 +227,21 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(KvAppendArgs p) {
 
   __shared__ KvStage<D> stage;
   if ((blk + 1) * kKvBlock <= end) {
-    const int tok = tid / 4, d0 = tid % 4 * E, at = blk * kKvBlock + tok - start;
-    u32x4 kx[NV], vx[NV];
-    if (at >= 0) {
+    KvBlockRegs<D> r;
+    const int first = blk * kKvBlock - start;  // the new token that is the block's token 0
+    if (first < 0) kv_from_tails<D>(r, kt, vt);
+    if (first + r.k_token() >= 0) {
 #pragma unroll
-      for (int i = 0; i < NV; i++) kx[i] = load_stream((const u32x4*)(k + at * p.k_tok + d0) + i);
-#pragma unroll
-      for (int i = 0; i < NV; i++) vx[i] = load_stream((const u32x4*)(v + at * p.v_tok + d0) + i);
-    } else {
-      kv_tail_token<DT, D>(kt, vt, tok, d0, kx, vx);
+      for (int i = 0; i < r.NK; i++) r.k[i] = load_stream((const u32x4*)(k + (first + r.k_token()) * p.k_tok + r.k_first()) + i);
     }
-    kv_quantise<DT, D>(p.c, pair, blk, kx, vx, stage);
+#pragma unroll
+    for (int i = 0; i < r.NV; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int t = first + 4 * r.v_four(i) + j;
+        if (r.v_on(i) && t >= 0) r.v[i][j] = load_stream((const u32x4*)(v + t * p.v_tok + r.v_first(i)));
+      }
+    kv_quantise<DT, D>(p.c, pair, blk, r, stage);
   }
   if (blockIdx.x != 0) return;
   __syncthreads();  // what the tail held has been read
@@ -273,11 +314,6 @@ __device__ __forceinline__ void kv_fill_rows(const KvAttnArgs& p, int pair, int 
 // A masked weight is 0, but 0 times a NaN is not.  So where keys are masked, numbers of V that are not finite are set to 0, and at the end, if there
 // were any, the queries that see one are set to NaN: products of those places (1, and 0 elsewhere) and of what a query sees count them.
 __device__ __forceinline__ uint32_t kv_nan8(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7; }  // bit 0 of each byte
-template <class DT>
-__device__ __forceinline__ uint32_t kv_nan16(uint32_t w) {  // bit 0 of each half: an exponent of ones carries into the sign's place
-  constexpr uint32_t E = Kv<DT>::kExp * 0x10001u, L = (Kv<DT>::kExp & -Kv<DT>::kExp) * 0x10001u;
-  return ((w & E) + L) >> 15 & 0x10001u;
-}
 // Sets them to 0; not 0 if there were any.
 __device__ __forceinline__ uint32_t kv_fix8(u32x4& x) {
   uint32_t any = 0;
@@ -355,9 +391,9 @@ __global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_ker
     if (split == p.splits) {
       __shared__ KvStage<D> stage;
       if (!ok || (start + n) % kKvBlock != 0 || n == 0 || blockIdx.z != 0) return;
-      u32x4 kx[D / 32], vx[D / 32];
-      kv_tail_token<DT, D>(p.c.kt + (size_t)pair * kKvBlock * D, p.c.vt + (size_t)pair * kKvBlock * D, threadIdx.x / 4, threadIdx.x % 4 * (D / 4), kx, vx);
-      kv_quantise<DT, D>(p.c, pair, (start + n) / kKvBlock - 1, kx, vx, stage);
+      KvBlockRegs<D> r;
+      kv_from_tails<D>(r, p.c.kt + (size_t)pair * kKvBlock * D, p.c.vt + (size_t)pair * kKvBlock * D);
+      kv_quantise<DT, D>(p.c, pair, (start + n) / kKvBlock - 1, r, stage);
       return;
     }
   }
