@@ -1632,6 +1632,7 @@ int cats_kv8_attention_step(const void* h, const void* x, const void* norm_weigh
                             const void* sin_table, const int64_t* position, void* out, int B, int H, int heads, int blocks, int max_len, int dtype,
                             void* scratch, size_t scratch_bytes, void* stream) {
   if (dtype != CATS_F16 && dtype != CATS_BF16) return CATS_ERR_DTYPE;
+  if (B > kKernelBatch) return CATS_ERR_BATCH;
   if (int st = check_proj(B, H, H, dtype)) return st;
   if (heads < 1 || H % heads != 0 || blocks < 1 || blocks > CATS_KV8_MAX_BLOCKS || max_len < 1 || max_len > blocks * kKvBlock) return CATS_ERR_SHAPE;
   const int hd = H / heads;

@@ -84,6 +84,9 @@ KvAttnPlan kv8_attn_plan(int B, int T, int heads, int kv_heads, int blocks, int 
 
 namespace {
 
+// A window that no cache of so many blocks exceeds is none.
+int window_of(int window, int blocks) { return window >= (long long)blocks * kKvBlock ? 0 : window; }
+
 bool attn_shape_ok(int T, int heads, int kv_heads) {
   return heads >= kv_heads && heads % kv_heads == 0 && (long long)T * (heads / kv_heads) <= 16ll * kMaxGrid;
 }
@@ -120,7 +123,7 @@ int cats_kv8_append(const void* k, const int64_t* k_strides, const void* v, cons
 
 size_t cats_kv8_attention_scratch_bytes(int B, int T, int heads, int kv_heads, int D, int blocks, int window) {
   if (check_cache(B, T, kv_heads, D, blocks, CATS_F16) || !attn_shape_ok(T, heads, kv_heads) || window < 0) return 0;
-  return attn_bytes(kv8_attn_plan(B, T, heads, kv_heads, blocks, window), B, T, heads, kv_heads, D);
+  return attn_bytes(kv8_attn_plan(B, T, heads, kv_heads, blocks, window_of(window, blocks)), B, T, heads, kv_heads, D);
 }
 
 int cats_kv8_attention(const void* q, const int64_t* q_strides, const int64_t* start, int start_step, const int64_t* count, int count_step,
@@ -133,6 +136,7 @@ int cats_kv8_attention(const void* q, const int64_t* q_strides, const int64_t* s
   if (int st = check_span(start, start_step, count, count_step)) return st;
   if (!out) return CATS_ERR_NULL;
   if (!aligned(out, 16)) return CATS_ERR_ALIGN;
+  window = window_of(window, blocks);
   KvAttnArgs a;
   if (int st = fill_cache(a.c, (void*)k8, (void*)v8, (float*)k_scale, (float*)v_scale, (void*)k_tail, (void*)v_tail, kv_heads, blocks)) return st;
   const KvAttnPlan plan = kv8_attn_plan(B, T, heads, kv_heads, blocks, window);

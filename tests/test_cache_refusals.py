@@ -72,6 +72,17 @@ def test_attention_scratch(L):
 
 
 @pytest.mark.parametrize("change,status", [
+    (dict(), 6), (dict(scratch=_p(8), bytes=1 << 30), 6), (dict(dtype=2), 1), (dict(B=0), 4), (dict(B=9), 4), (dict(H=8192 * 9, heads=576), 2), (dict(heads=3), 2), (dict(heads=8), 2),
+    (dict(blocks=0), 2), (dict(max_len=129), 2), (dict(max_len=0), 2), (dict(h=None), 5), (dict(wo=None), 5), (dict(v_tail=None), 5), (dict(position=None), 5), (dict(x=_p(8)), 3),
+    (dict(wk=_p(8)), 3), (dict(v8=_p(4)), 3)])
+def test_step_refuses(L, change, status):
+    a = dict(h=_p(), x=_p(), norm=None, eps=1e-5, wq=_p(), wk=_p(), wv=_p(), wo=_p(), k8=_p(), v8=_p(), k_scale=_p(), v_scale=_p(), k_tail=_p(), v_tail=_p(), cos=_p(),
+             sin=_p(), position=_p(), out=_p(), B=1, H=128, heads=2, blocks=2, max_len=128, dtype=0, scratch=None, bytes=0)
+    a.update(change)
+    assert L.cats_kv8_attention_step(*a.values(), None) == status
+
+
+@pytest.mark.parametrize("change,status", [
     (dict(), 6), (dict(dtype=3), 1), (dict(beams=17), 2), (dict(keep=17), 2), (dict(keep=0), 2), (dict(groups=0), 2), (dict(V=0), 2), (dict(beams=1, V=2, keep=3), 2),
     (dict(eos=100), 2), (dict(finished=_p(), eos=-1), 2), (dict(stride=-1), 2), (dict(groups=65536, beams=1), 2), (dict(logits=None), 5), (dict(parents=None), 5),
     (dict(finished_out=None), 5), (dict(logits=_p(1)), 3), (dict(dtype=2, logits=_p(2)), 3), (dict(scores=_p(2)), 3), (dict(tokens=_p(4)), 3), (dict(scratch=_p(8), bytes=1 << 30), 6)])

@@ -206,3 +206,22 @@ def test_a_step_in_a_graph():
         results.append(seen)
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+def test_what_the_operators_refuse():
+    import flash_gemv
+
+    x, s = torch.zeros(2, 3, 50, device="cuda"), torch.zeros(2, 3, device="cuda")
+    done = torch.zeros(2, 3, dtype=torch.bool, device="cuda")
+    flash_gemv.cats_beam_select(x, s, done, 4)
+    for args in ((x[0], s), (x.double(), s), (x, s.double()), (x, s[:1]), (x, s.cpu()), (x, s, done[:1], 4), (x, s, done.int(), 4), (x, s, done), (x, s, None, 50),
+                 (x, s, None, -1, 17), (x, s, None, -1, -1), (x[:, :1, :2], s[:, :1].contiguous(), None, -1, 3), (torch.zeros(1, 17, 50, device="cuda"), torch.zeros(1, 17, device="cuda"))):
+        with pytest.raises(RuntimeError):
+            flash_gemv.cats_beam_select(*args)
+    c, p, n = torch.zeros(6, 2, 5, 4, device="cuda"), torch.zeros(2, 3, dtype=torch.int64, device="cuda"), torch.tensor([3], device="cuda")
+    flash_gemv.cats_cache_reorder([c], [1], p, n)
+    for args in (([c], [1], p), ([c], [1, 1], p, n), ([], [], p, n), ([c], [-1], p, n), ([c[:5]], [1], p, n), ([c[0]], [1], p, n), ([c], [1], p.int(), n),
+                 ([c], [1], p[0], n), ([c], [1], p, n.int()), ([c], [1], p, torch.zeros(2, dtype=torch.int64, device="cuda")), ([c.transpose(1, 2)], [1], p, n),
+                 ([c.to(torch.uint8)[..., :3].contiguous()], [1], p, n), ([c.cpu()], [1], p, n), ([c], [1], p.cpu(), n)):
+        with pytest.raises(RuntimeError):
+            flash_gemv.cats_cache_reorder(*args)

@@ -244,6 +244,122 @@ def test_attention_values_that_are_not_finite(T, bad_at, value, dtype):
         assert ref.within(out, want, bound), window
 
 
+@pytest.mark.parametrize("T", [1, 5, 70])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_attention_of_queries_that_are_not_finite(T, value):
+    """They spoil their own outputs alone."""
+    g = torch.Generator().manual_seed(8)
+    cache = _filled(g, 1, 1, 5, 64, F16, [300])
+    q = torch.randn(1, T, 2, 64, generator=g).half()
+    q[0, T - 1, 1, 9] = value
+    out = _attention(ref.to(cache, "cuda"), q.cuda(), [300 - T])
+    want, bound = ref.attention(cache, q, [300 - T], None, 0.125)
+    assert ref.within(out, want, bound) and out[0, T - 1, 1].isnan().all()
+
+
+@pytest.mark.parametrize("T", [1, 3, 70])
+@pytest.mark.parametrize("window", [319, 320, 321, 2 ** 31 - 1])
+def test_attention_windows_as_long_as_the_cache(T, window):
+    """319 of the 320 tokens that five blocks hold, and windows that hide nothing."""
+    _check(2, T, 2, 1, 64, BF16, [320, 100], 5, window)
+
+
+def test_attention_tails_behind_the_last_token_hold_anything():
+    """Infinities and the largest numbers where the tails have not been written."""
+    g = torch.Generator().manual_seed(13)
+    cache = _filled(g, 1, 1, 3, 128, F16, [140])
+    q = torch.randn(1, 80, 1, 128, generator=g).half()
+    want, bound = ref.attention(cache, q, [60], None, 0.1)
+    for value in (math.inf, -math.inf, 65504.0):
+        c = {f: t.clone() for f, t in cache.items()}
+        c["k_tail"][:, :, 12:], c["v_tail"][..., 12:] = value, value
+        c = ref.to(c, "cuda")
+        assert ref.within(_attention(c, q.cuda(), [60], scale=0.1), want, bound)
+        assert ref.within(_attention(c, q[:, 79:].cuda(), [139], scale=0.1), want[:, 79:], bound[:, 79:])
+
+
+def test_two_streams_at_once():
+    """Calls of two caches of one shape side by side: nothing is shared."""
+    g = torch.Generator().manual_seed(14)
+    caches = [ref.to(_filled(g, 1, 2, 60, 64, BF16, [3000]), "cuda") for _ in range(2)]
+    q = [torch.randn(1, 1, 8, 64, generator=g).bfloat16().cuda() for _ in range(2)]
+    alone = [_attention(c, x, [2999]) for c, x in zip(caches, q)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    start = _words([2999])
+    import flash_gemv
+
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(flash_gemv.cats_kv8_attention(q[i], start, None, *_args(caches[i]), 0.125))
+    torch.cuda.synchronize()
+    for a, o in zip(alone, outs):
+        assert all(torch.equal(a, x) for x in o)
+
+
+def test_prompt_in_a_graph():
+    """A captured prompt, replayed on other tokens and another start, with splits and without."""
+    import flash_gemv
+
+    g = torch.Generator().manual_seed(15)
+    for lengths in ([70, 200], [4000, 4000]):
+        cache = ref.to(_filled(g, 2, 1, 70, 64, F16, lengths), "cuda")
+        q, start, count = torch.zeros(2, 70, 2, 64, dtype=F16, device="cuda"), torch.tensor([0, 0], device="cuda"), torch.tensor([70], device="cuda")
+        call = lambda: flash_gemv.cats_kv8_attention(q, start, count, *_args(cache), 0.125)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = call()
+        torch.cuda.current_stream().wait_stream(side)
+        for n in (70, 65, 70):
+            q.copy_(torch.randn(2, 70, 2, 64, generator=g).half())
+            start.copy_(torch.tensor([x - n for x in lengths]))
+            count.fill_(n)
+            graph.replay()
+            got = out.clone()
+            assert torch.equal(got, call()) and not got[:, :n].isnan().any()
+            (q.float() ** 2).sum()
+
+
+def test_what_the_operators_refuse():
+    """Types, shapes and devices that do not belong together, before anything is launched."""
+    import flash_gemv
+
+    c = ref.new_cache(2, 2, 3, 128, F16, fill=0.0, device="cuda")
+    x, at = torch.zeros(2, 1, 2, 128, dtype=F16, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    append = lambda k=x, v=x, start=at, count=None, **o: flash_gemv.cats_kv8_append(k, v, start, count, *(o.get(f, c[f]) for f in ref.FIELDS))
+    attend = lambda q=x, start=at, count=None, scale=0.1, window=0, **o: flash_gemv.cats_kv8_attention(q, start, count, *(o.get(f, c[f]) for f in ref.FIELDS), scale, window)
+    append(), attend()
+    three = torch.zeros(3, dtype=torch.int64, device="cuda")
+    for call in (append, attend):
+        for wrong in (dict(start=at.int()), dict(start=at.cpu()), dict(start=three), dict(count=three), dict(k8=c["k8"].view(torch.uint8)), dict(v8=c["k8"]),
+                      dict(k_scale=c["k_scale"].double()), dict(v_scale=c["v_scale"][:, :, :2]), dict(k_tail=c["k_tail"].bfloat16()), dict(v_tail=c["k_tail"]),
+                      dict(k8=c["k8"][:, :, :2])):
+            with pytest.raises(RuntimeError):
+                call(**wrong)
+    for wrong in (x.float(), x[0], x[..., :32], x.double(), x[:1], x.cpu()):
+        with pytest.raises(RuntimeError):
+            append(wrong, wrong)
+        with pytest.raises(RuntimeError):
+            attend(wrong)
+    with pytest.raises(RuntimeError):
+        append(x, x.bfloat16())
+    with pytest.raises(RuntimeError):
+        append(x[:, :, :1], x[:, :, :1])
+    with pytest.raises(RuntimeError):
+        attend(torch.zeros(2, 1, 3, 128, dtype=F16, device="cuda"))
+    for wrong in (dict(window=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=1e39)):
+        with pytest.raises(RuntimeError):
+            attend(**wrong)
+    long = torch.zeros(2, 193, 2, 128, dtype=F16, device="cuda")  # more tokens than the cache has room for
+    with pytest.raises(RuntimeError):
+        append(long, long)
+
+
 def test_attention_outside_the_cache_is_nan():
     g = torch.Generator().manual_seed(2)
     cache = ref.to(_filled(g, 3, 1, 2, 64, F16, [100, 100, 100]), "cuda")
