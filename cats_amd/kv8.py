@@ -35,7 +35,7 @@ class Kv8Cache:
         # zeros in e4m3 by way of bytes: 0 is 0
         self.k8 = zeros(*shape, BLOCK, head_dim, dtype=torch.uint8).view(torch.float8_e4m3fn)
         self.v8 = zeros(*shape, head_dim, BLOCK, dtype=torch.uint8).view(torch.float8_e4m3fn)
-        self.k_scale, self.v_scale = zeros(*shape, dtype=torch.float32), zeros(*shape, dtype=torch.float32)
+        self.k_scale, self.v_scale = (torch.ones(shape, dtype=torch.float32, device=device) for _ in range(2))  # tokens that were never stored are zeros
         self.k_tail = zeros(rows, kv_heads, BLOCK, head_dim, dtype=dtype)
         self.v_tail = zeros(rows, kv_heads, head_dim, BLOCK, dtype=dtype)
 
