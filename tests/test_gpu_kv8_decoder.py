@@ -97,6 +97,7 @@ def test_decoder_with_a_cache_in_8_bits(dtype):
             h.remove()
         for l, s in zip(m.layers, seen):
             at, cache = l.self_attn, ref.new_cache(2, 4, 4, 64, dtype, fill=0.0)
+            cache["k_scale"].fill_(1.0), cache["v_scale"].fill_(1.0)  # as a new cache has them
             for (a, b), x, out in zip(pieces, s["x"], s["out"]):
                 cos, sin = m.cos_table[a:b], m.sin_table[a:b]
                 q, k, v = (p(x).view(2, b - a, 4, 64).transpose(1, 2) for p in (at.q_proj, at.k_proj, at.v_proj))
@@ -107,6 +108,15 @@ def test_decoder_with_a_cache_in_8_bits(dtype):
                 assert ref.within(out.view(2, b - a, 4, 64), want, bound), (a, b)
             for f, t in zip(ref.FIELDS, at.kv8.tensors()):
                 assert ref.same(t, cache[f]), f
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_tokens_that_were_never_stored_are_zeros(T):
+    from cats_amd.kv8 import Kv8Cache
+
+    c = Kv8Cache(2, 1, 256, 64, F16)
+    q = _randn(torch.Generator().manual_seed(3), 2, T, 4, 64, dtype=F16).cuda()
+    assert (c.attend(q, torch.tensor([200, 7], device="cuda")) == 0).all()
 
 
 def test_greedy_with_a_cache_in_8_bits_replays_its_graph():
