@@ -10,10 +10,10 @@ constexpr int kBeamMax = 16;  // beams of a group, before and after
 //   total(b, v) = score[b] + logit[b][v] - log(sum over v of exp(logit[b][v]));   the best `keep` of a group, ties to the lowest b * V + v
 // A beam that has finished goes on only as (b, eos) with its score.  Totals that are not finite count as -infinity.
 //
-// beam_rows_kernel: one pass over the logits.  A wave holds 64 E of them in registers and leaves their maximum, the sum of exponentials and
-// the best `keep`.  For those: the keep-th best of the lanes' best values bounds what can be among them, so what is not below it is
-// gathered (some more than `keep`) and ranked by comparing each with all; only where ties make that more than 64 are the best taken one by
-// one.  The workgroup's four waves are joined.  beam_join_kernel: a workgroup per group, a wave per beam joins its row's pieces in the same way, and
+// beam_rows_kernel: one pass over the logits.  A workgroup holds 256 E of them in registers and leaves their maximum, the sum of exponentials and
+// the best `keep`.  For those: of the 64 sets of values that lane l of each wave holds, the keep-th best of their best values bounds what can be
+// among them, so what is not below it is gathered (some more than `keep`) and ranked by comparing each with all; only where ties make that
+// more than 64 are each wave's best taken one by one and joined.  beam_join_kernel: a workgroup per group, a wave per beam joins its row's pieces in the same way, and
 // the beams' candidates are ranked by their totals in 64 bits: the order has to be that of the sums, which differ in their last bits only.
 // A row with a NaN or +infinity has no finite total at all, so neither has to be found among the best.
 
@@ -100,10 +100,65 @@ struct BeamList {  // in LDS, of a wave
   int id[kWave];
 };
 
+// Writes the best `keep` of the `count` <= 64 pairs that the lanes hold to `best`, in order, lower ids first among equal values.
+__device__ __forceinline__ void wave_rank(float v, int n, int count, int keep, int lane, BeamList& best) {
+  const uint32_t hi = beam_key(v), lo = ~(uint32_t)n;  // larger is better
+  const uint64_t mine = (uint64_t)hi << 32 | lo;
+  int rank = 0;
+  for (int j = 0; j < count; j++) {
+    const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, j);
+    rank += other > mine;
+  }
+  if (lane < count && rank < keep) {
+    best.val[rank] = v;
+    best.id[rank] = n;
+  }
+}
+// The same of any number of values, taken one by one: for those with many equal ones.  `own` is what id() computes from, hidden from the compiler
+// in every round: E ids kept for this would take the registers that let more waves wait for memory.
+template <int E, class Id>
+__device__ __forceinline__ void wave_pick(const float (&x)[E], Id id, int& own, int keep, int lane, BeamList& best) {
+  uint64_t gone = 0;  // of this lane's values
+  static_assert(E <= 64, "a bit each");
+  for (int k = 0; k < keep; k++) {
+    asm volatile("" : "+v"(own));
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < E; i++) top = gone >> i & 1 ? top : fmaxf(top, x[i]);
+    top = wave_max(top);
+    int first = INT32_MAX, which = 0;
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+      const int n = id(i);
+      const bool in = !(gone >> i & 1) && n >= 0 && x[i] == top && n < first;
+      first = in ? n : first;
+      which = in ? i : which;
+    }
+    const int lowest = wave_min(first);
+    if (lowest == INT32_MAX) break;
+    if (first == lowest) gone |= (uint64_t)1 << which;
+    if (lane == 0) {
+      best.val[k] = top;
+      best.id[k] = lowest;
+    }
+  }
+}
+// Appends a value of each lane that is `in` to the list, as far as it has room; the count goes on.
+__device__ __forceinline__ void wave_take(bool in, float v, int n, int& count, BeamList& list) {
+  const uint64_t b = __ballot(in);
+  const int at = count + ballot_rank(b);
+  if (in && at < kWave) {
+    list.val[at] = v;
+    list.id[at] = n;
+  }
+  count += __popcll(b);
+}
+
 // Writes the best `keep` of the wave's values to `best`, in order, lower ids first among equal ones, ids of -1 behind the last.  id(i) is that of
-// x[i], -1 for no entry (and x[i] = -infinity).  The lowest 32 ids of the wave, or all, are within the first FRONT values of the first `lanes` lanes.
+// x[i], -1 for no entry (and x[i] = -infinity).  The lowest 32 ids of the wave,
+// or all, are within the first FRONT values.
 template <int FRONT, int E, class Id>
-__device__ __forceinline__ void wave_best(const float (&x)[E], Id id, int lanes, int keep, int lane, BeamList& list, BeamList& best) {
+__device__ __forceinline__ void wave_best(const float (&x)[E], Id id, int keep, int lane, BeamList& list, BeamList& best) {
   float bound = -INFINITY;
   if constexpr (E > 1) {  // one value a lane fits the list as it is
     float mine = -INFINITY;
@@ -112,89 +167,46 @@ __device__ __forceinline__ void wave_best(const float (&x)[E], Id id, int lanes,
     bound = wave_kth(mine, keep, lane);
   }
   int count = 0;
-  auto take = [&](bool in, int i) {
-    const uint64_t b = __ballot(in);
-    const int at = count + ballot_rank(b);
-    if (in && at < kWave) {
-      list.val[at] = x[i];
-      list.id[at] = id(i);
-    }
-    count += __popcll(b);
-  };
   const bool low = bound == -INFINITY;  // less than `keep` lanes have more than that, or there is one value a lane
 #pragma unroll
   for (int i = 0; i < E; i++) {
     const bool in = low ? x[i] > bound : x[i] >= bound;
-    if (__any(in)) take(in, i);
+    if (__any(in)) wave_take(in, x[i], id(i), count, list);
   }
   if (low && count < keep) {  // then values of -infinity are among the best, those with the lowest ids
 #pragma unroll
-    for (int i = 0; i < FRONT; i++) take(lane < lanes && x[i] == -INFINITY && id(i) >= 0, i);
+    for (int i = 0; i < FRONT; i++) wave_take(x[i] == -INFINITY && id(i) >= 0, x[i], id(i), count, list);
   }
   if (lane < keep) best.id[lane] = -1;
   wave_lds_sync();
-  if (count <= kWave) {
-    const float v = lane < count ? list.val[lane] : 0.f;
-    const int n = lane < count ? list.id[lane] : 0;
-    const uint32_t hi = beam_key(v), lo = ~(uint32_t)n;  // larger is better
-    const uint64_t mine = (uint64_t)hi << 32 | lo;
-    int rank = 0;
-    for (int j = 0; j < count; j++) {
-      const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, j);
-      rank += other > mine;
-    }
-    if (lane < count && rank < keep) {
-      best.val[rank] = v;
-      best.id[rank] = n;
-    }
-  } else {
-    uint64_t gone = 0;  // of this lane's values
-    static_assert(E <= 64, "a bit each");
-    for (int k = 0; k < keep; k++) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < E; i++) top = gone >> i & 1 ? top : fmaxf(top, x[i]);
-      top = wave_max(top);
-      int first = INT32_MAX, which = 0;
-#pragma unroll
-      for (int i = 0; i < E; i++) {
-        const int n = id(i);
-        const bool in = !(gone >> i & 1) && n >= 0 && x[i] == top && n < first;
-        first = in ? n : first;
-        which = in ? i : which;
-      }
-      const int lowest = wave_min(first);
-      if (lowest == INT32_MAX) break;
-      if (first == lowest) gone |= (uint64_t)1 << which;
-      if (lane == 0) {
-        best.val[k] = top;
-        best.id[k] = lowest;
-      }
-    }
-  }
+  int none = 0;
+  if (count <= kWave) wave_rank(lane < count ? list.val[lane] : 0.f, lane < count ? list.id[lane] : 0, count, keep, lane, best);
+  else wave_pick(x, id, none, keep, lane, best);
   wave_lds_sync();
 }
 
 template <class DT, int E>
-__global__ __launch_bounds__(256) void beam_rows_kernel(BeamArgs p) {
+__global__ __launch_bounds__(256, 6) void beam_rows_kernel(BeamArgs p) {
   typedef typename DT::st st;
-  constexpr int VEC = DT::VEC, W = 4;
+  constexpr int VEC = DT::VEC, W = 4, G = E / VEC;
   __shared__ BeamList s_list[W], s_best[W];
-  __shared__ float s_ml[W][2];
+  __shared__ float s_max[W][kWave], s_sum[W];
+  __shared__ int s_count[W];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, row = blockIdx.y, piece = blockIdx.x;
   if (p.finished && p.finished[row]) return;
   const st* x = (const st*)p.logits + row * p.row_stride;
   // the wave's elements, in vectors of VEC that go round the lanes; vectors are those of memory, so a row may start inside its first
   const int first = (piece * W + wave) * kWave * E - (int)(((uintptr_t)x & 15u) / sizeof(st));
   float val[E];
+  int own = first + lane * VEC;
   auto id = [&](int i) {
-    const int at = first + (i / VEC * kWave + lane) * VEC + i % VEC;
+    const int at = own + i / VEC * kWave * VEC + i % VEC;
     return at >= 0 && at < p.V ? at : -1;
   };
   if (first >= 0 && first + kWave * E <= p.V) {
-    u32x4 w[E / VEC];
+    u32x4 w[G];
 #pragma unroll
-    for (int i = 0; i < E / VEC; i++) w[i] = load_stream((const u32x4*)(x + first + (i * kWave + lane) * VEC));
+    for (int i = 0; i < G; i++) w[i] = load_stream((const u32x4*)(x + first + (i * kWave + lane) * VEC));
 #pragma unroll
     for (int i = 0; i < E; i++) {
       const uint32_t c = w[i / VEC][i % VEC * 4 / VEC];
@@ -208,43 +220,91 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(BeamArgs p) {
 #pragma unroll
     for (int i = 0; i < E; i++) val[i] = id(i) >= 0 ? DT::tof(w[i]) : -INFINITY;
   }
-  float m = -INFINITY;
+  float top[G], most = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < E; i++) m = fmaxf(m, val[i]);
-  m = wave_max(m);
+  for (int g = 0; g < G; g++) {
+    top[g] = val[g * VEC];
+#pragma unroll
+    for (int i = 1; i < VEC; i++) top[g] = fmaxf(top[g], val[g * VEC + i]);
+    most = fmaxf(most, top[g]);
+  }
+  s_max[wave][lane] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; w++) most = fmaxf(most, s_max[w][lane]);
+  const float m = wave_max(most), bound = wave_kth(most, p.keep, lane);
   // exp of a difference that is rounded once: within 2^-24 of |x - m|, as the difference itself is
   const float base = m == -INFINITY ? 0.f : m;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < E; i++) sum += __builtin_amdgcn_exp2f((val[i] - base) * 1.44269504088896341f);
   sum = wave_sum(sum);
-  wave_best<VEC>(val, id, 32 / VEC, p.keep, lane, s_list[wave], s_best[wave]);
+  const bool low = bound == -INFINITY;  // less than `keep` of the 64 have more than that
+  int count = 0;
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    if (!__any(top[g] >= bound)) continue;
+#pragma unroll
+    for (int i = g * VEC; i < (g + 1) * VEC; i++) {
+      const bool in = low ? val[i] > bound : val[i] >= bound;
+      if (__any(in)) wave_take(in, val[i], id(i), count, s_list[wave]);
+    }
+  }
   if (lane == 0) {
-    s_ml[wave][0] = m;
-    s_ml[wave][1] = sum;
+    s_count[wave] = count;
+    s_sum[wave] = sum;
   }
   __syncthreads();
-  if (wave != 0) return;
-  const int from = lane / p.keep, which = lane - from * p.keep;
-  const int n = from < W ? s_best[from < W ? from : 0].id[which] : -1;
-  const float v1[1] = {n >= 0 ? s_best[from].val[which] : -INFINITY};
-  float mm = s_ml[0][0];
+  int counts[W], all = 0;
 #pragma unroll
-  for (int w = 1; w < W; w++) mm = fmaxf(mm, s_ml[w][0]);
-  const float bb = mm == -INFINITY ? 0.f : mm;
-  float ss = 0.f;
+  for (int w = 0; w < W; w++) all += counts[w] = s_count[w];
+  float v = -INFINITY;
+  int n = -1;
+  if (all <= kWave) {
+    if (wave != 0) return;
+    if (low && all < p.keep) {  // then values of -infinity are among the best, those with the lowest ids: in the first lanes' first vectors
 #pragma unroll
-  for (int w = 0; w < W; w++) ss += s_ml[w][0] == -INFINITY ? s_ml[w][1] : s_ml[w][1] * expf(s_ml[w][0] - bb);
-  __builtin_amdgcn_wave_barrier();
-  wave_best<1>(v1, [&](int) { return n; }, kWave, p.keep, lane, s_list[0], s_best[0]);
+      for (int i = 0; i < VEC; i++) wave_take(lane < 32 / VEC && val[i] == -INFINITY && id(i) >= 0, val[i], id(i), counts[0], s_list[0]);
+      all = counts[0] + counts[1] + counts[2] + counts[3];
+    }
+    if (lane < p.keep) s_best[0].id[lane] = -1;
+    wave_lds_sync();
+    int w = 0, at = lane;
+#pragma unroll
+    for (int i = 0; i < W - 1; i++) {
+      const bool on = w == i && at >= counts[i];
+      at -= on ? counts[i] : 0;
+      w += on;
+    }
+    if (lane < all) v = s_list[w].val[at], n = s_list[w].id[at];
+  } else {
+    BeamList& best = s_best[wave];
+    if (lane < p.keep) best.id[lane] = -1;
+    wave_lds_sync();
+    if (count <= kWave) wave_rank(lane < count ? s_list[wave].val[lane] : 0.f, lane < count ? s_list[wave].id[lane] : 0, count, p.keep, lane, best);
+    else wave_pick(val, id, own, p.keep, lane, best);
+    __syncthreads();
+    if (wave != 0) return;
+    const int from = lane / p.keep, which = lane - from * p.keep;
+    v = from < W ? s_best[from < W ? from : 0].val[which] : 0.f;
+    n = from < W ? s_best[from < W ? from : 0].id[which] : -1;
+    wave_lds_sync();
+    all = 0;
+    wave_take(n >= 0, v, n, all, s_list[0]);
+    if (lane < p.keep) s_best[0].id[lane] = -1;
+    wave_lds_sync();
+    if (lane < all) v = s_list[0].val[lane], n = s_list[0].id[lane];
+  }
+  wave_rank(v, n, all, p.keep, lane, s_best[0]);
+  wave_lds_sync();
   const size_t out = (size_t)row * p.pieces + piece;
   if (lane < p.keep) {
     p.vals[out * p.keep + lane] = s_best[0].val[lane];
     p.ids[out * p.keep + lane] = s_best[0].id[lane];
   }
   if (lane == 0) {
-    p.ml[2 * out] = mm;
-    p.ml[2 * out + 1] = ss;
+    p.ml[2 * out] = m;
+    p.ml[2 * out + 1] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
   }
 }
 
@@ -262,11 +322,30 @@ __global__ __launch_bounds__(N* kWave) void beam_join_kernel(BeamArgs p) {
   __shared__ BeamList s_list[N], s_best[N];
   __shared__ double s_total[N * N];
   __shared__ int s_token[N * N];  // -1: no offer
+  __shared__ bool s_done[N];
   const int lane = threadIdx.x & (kWave - 1), b = threadIdx.x >> 6, group = blockIdx.x, row = group * p.beams + b;
   const double kNone = -(double)INFINITY;
   if (b < p.beams) {
+    // Everything is asked for at once, also of a beam that has finished: what beam_rows_kernel left out is room of the workspace all the same.
+    const float* ml = p.ml + (size_t)row * p.pieces * 2;
+    const size_t at = (size_t)row * p.pieces * p.keep;
+    const int n = p.pieces * p.keep;
+    constexpr int E = 8;
+    float val[E + 1];
+    int id[E + 1];
+    auto fetch = [&](int i0) {
+#pragma unroll
+      for (int i = 0; i < E; i++) {
+        const int j = i0 + i * kWave + lane;
+        const int k = p.ids[at + min(j, n - 1)];
+        const float v = p.vals[at + min(j, n - 1)];
+        id[i] = j < n ? k : -1;
+        val[i] = id[i] >= 0 ? v : -INFINITY;
+      }
+    };
     const bool done = p.finished && p.finished[row];
-    const float score = p.scores[row];
+    const float score = p.scores[row], m0 = ml[2 * min(lane, p.pieces - 1)], l0 = ml[2 * min(lane, p.pieces - 1) + 1];
+    fetch(0);
     double total = kNone;
     int token = lane < p.V ? lane : -1;  // where nothing is finite, the lowest ones
     if (done) {
@@ -276,30 +355,15 @@ __global__ __launch_bounds__(N* kWave) void beam_join_kernel(BeamArgs p) {
         if (lane == 0) total = score;
       }
     } else {
-      const float* ml = p.ml + (size_t)row * p.pieces * 2;
-      const size_t at = (size_t)row * p.pieces * p.keep;
-      const int n = p.pieces * p.keep;
-      constexpr int E = 8;
-      float val[E + 1];
-      int id[E + 1];
-      auto fetch = [&](int i0) {
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-          const int j = i0 + i * kWave + lane;
-          const int k = p.ids[at + min(j, n - 1)];
-          const float v = p.vals[at + min(j, n - 1)];
-          id[i] = j < n ? k : -1;
-          val[i] = id[i] >= 0 ? v : -INFINITY;
-        }
-      };
-      float m = lane < p.pieces ? ml[2 * lane] : -INFINITY;
-      fetch(0);
+      float m = m0;
       for (int i = lane + kWave; i < p.pieces; i += kWave) m = fmaxf(m, ml[2 * i]);
       m = wave_max(m);
       const float base = m == -INFINITY ? 0.f : m;
       double sum = 0.0;
-      for (int i = lane; i < p.pieces; i += kWave)
-        sum += ml[2 * i] == -INFINITY ? (double)ml[2 * i + 1] : (double)ml[2 * i + 1] * exp((double)ml[2 * i] - base);
+      for (int i = lane; i < p.pieces; i += kWave) {
+        const float mi = i == lane ? m0 : ml[2 * i], li = i == lane ? l0 : ml[2 * i + 1];
+        sum += mi == -INFINITY ? (double)li : (double)li * exp((double)mi - base);
+      }
 #pragma unroll
       for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
       const double lse = (double)base + log(sum);
@@ -308,7 +372,7 @@ __global__ __launch_bounds__(N* kWave) void beam_join_kernel(BeamArgs p) {
         id[E] = -1;
         for (int i0 = 0; i0 < n; i0 += E * kWave) {
           if (i0) fetch(i0);
-          wave_best<E + 1>(val, [&](int i) { return id[i]; }, kWave, p.keep, lane, s_list[b], s_best[b]);
+          wave_best<E + 1>(val, [&](int i) { return id[i]; }, p.keep, lane, s_list[b], s_best[b]);
           id[E] = lane < p.keep ? s_best[b].id[lane] : -1;
           val[E] = id[E] >= 0 ? s_best[b].val[lane] : -INFINITY;
         }
@@ -321,6 +385,7 @@ __global__ __launch_bounds__(N* kWave) void beam_join_kernel(BeamArgs p) {
       s_total[b * p.keep + lane] = total;
       s_token[b * p.keep + lane] = token;
     }
+    if (lane == 0) s_done[b] = done;
   }
   __syncthreads();
   if (b != 0) return;
@@ -355,7 +420,7 @@ __global__ __launch_bounds__(N* kWave) void beam_join_kernel(BeamArgs p) {
     p.scores_out[out] = (float)s_total[c];
     p.parents_out[out] = parent;
     p.tokens_out[out] = token;
-    p.finished_out[out] = token == p.eos || (p.finished && p.finished[group * p.beams + parent]);
+    p.finished_out[out] = token == p.eos || s_done[parent];
   };
   if (count <= kWave) {
     const int c = lane < count ? list[lane] : 0;  // the list is in order
