@@ -131,7 +131,7 @@ int cats_kv8_attention(const void* q, const int64_t* q_strides, const int64_t* s
                        float scale, int window, void* out, int B, int T, int heads, int kv_heads, int D, int blocks, int dtype, void* scratch,
                        size_t scratch_bytes, void* stream) {
   if (int st = check_cache(B, T, kv_heads, D, blocks, dtype)) return st;
-  if (!attn_shape_ok(T, heads, kv_heads) || window < 0 || !(scale > 0.f) || !(scale <= FLT_MAX)) return CATS_ERR_SHAPE;
+  if (!attn_shape_ok(T, heads, kv_heads) || window < 0 || !(scale >= 0x1p-64f && scale <= 0x1p64f)) return CATS_ERR_SHAPE;
   if (int st = check_strides(q, q_strides)) return st;
   if (int st = check_span(start, start_step, count, count_step)) return st;
   if (!out) return CATS_ERR_NULL;

@@ -777,7 +777,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
 #pragma unroll
       for (int e = 0; e < 16; e++) s[u][e] = 32 * u + e <= most ? s[u][e] : -INFINITY;
     if (p.window) {
-      const int least = most - p.window;
+      const int least = max(most, -kKvBlock) - p.window;  // a tile that is none has most near INT_MIN
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll

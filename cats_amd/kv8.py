@@ -9,6 +9,9 @@ kept as it was given.  So a token is rounded once, and a cache holds the same wh
     out = cache.attend(q, start)           # q (rows, T, heads, head_dim), causal; the same start and count
     cache.reorder(parents, start + T)      # beam search: rows become what their parents were
 
+A row ends where the last call left it.  Tokens are taken back by a smaller start, as far as the start of the block that holds the last one, or
+to the start of any block: tokens of an earlier block are there as e4m3 only, and the rest of that block has to be given again.
+
 For fp16 and bf16 on the GPU, heads of 32, 64, 128 or 256 elements, without gradients.
 """
 from __future__ import annotations

@@ -155,13 +155,15 @@ def cats_kv8_append(k, v, start, count, k8, v8, k_scale, v_scale, k_tail, v_tail
     """Store new tokens in a cache in 8 bits (``cats_amd.kv8.Kv8Cache`` holds one; the format is in ``include/cats_gemv.h``).
 
     k, v (B, T, kv_heads, D) half or bfloat16, any strides; start, count int64 on the GPU, one for all rows or one each (count None: all T): row b's
-    first ``count`` tokens go to positions ``start ..``, where what it holds already ends."""
+    first ``count`` tokens go to positions ``start ..``, where what it holds already ends.  A smaller start takes tokens back, as far as the start of the block of 64 that holds the
+    last one, or to the start of any block."""
     torch.ops.flash_gemv.cats_kv8_append(k, v, start, count, k8, v8, k_scale, v_scale, k_tail, v_tail)
 
 
 def cats_kv8_attention(q, start, count, k8, v8, k_scale, v_scale, k_tail, v_tail, scale, window=0):
     """Causal attention of the tokens that cats_kv8_append has stored: q (B, T, heads, D), heads a multiple of the cache's, over the positions up to
-    each token's own, at most ``window`` of them (0: all).  Returns (B, T, heads, D); rows behind ``count`` are zeros.  Serving only: no gradient."""
+    each token's own, at most ``window`` of them (0: all); ``scale`` lies in 2^-64 .. 2^64.
+    Returns (B, T, heads, D); rows behind ``count`` are zeros.  Serving only: no gradient."""
     return torch.ops.flash_gemv.cats_kv8_attention(q, start, count, k8, v8, k_scale, v_scale, k_tail, v_tail, scale, window)
 
 

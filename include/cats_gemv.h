@@ -258,8 +258,9 @@ int cats_attention_step(const void* h, const void* x, const void* norm_weight, f
 #define CATS_KV8_MAX_BLOCKS (1 << 24)
 
 /* Stores the new tokens: quantises the blocks that they complete and leaves the last block in the tails.  What a row holds already has to end at
- * start (a block's tokens before start are taken from the tails).  So the cache is the same whatever pieces the tokens come in.  A row whose
- * tokens do not lie within its blocks is left as it is. */
+ * start (a block's tokens before start are taken from the tails).  So the cache is the same whatever pieces the tokens come in.  Tokens may be taken
+ * back by a smaller start, as far as the start of the block that holds the last one, or to the start of any block; what an earlier block held in
+ * the type is gone.  A row whose tokens do not lie within its blocks is left as it is. */
 int cats_kv8_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, const int64_t* start, int start_step,
                     const int64_t* count, int count_step, void* k8, void* v8, float* k_scale, float* v_scale, void* k_tail, void* v_tail, int B,
                     int T, int kv_heads, int D, int blocks, int dtype, void* stream);
@@ -267,7 +268,7 @@ int cats_kv8_append(const void* k, const int64_t* k_strides, const void* v, cons
 /* out[b, i, h] = softmax(scale * q[b, i, h] . K^T) . V over the keys at positions p - window + 1 .. p (window 0: 0 .. p), p = start + i, of cached
  * head h / (heads / kv_heads), for new tokens that cats_kv8_append has stored.  Rows i >= count are zeros; a row whose tokens do not lie within
  * its blocks is NaN.  A query that sees a key or an element of a value that is not finite is NaN (in that element).  out (B, T, heads, D) in
- * dtype, 16-byte aligned.  scale > 0.  scratch: 16-byte aligned, at least cats_kv8_attention_scratch_bytes() on the device of the call
+ * dtype, 16-byte aligned.  scale lies in 2^-64 .. 2^64.  scratch: 16-byte aligned, at least cats_kv8_attention_scratch_bytes() on the device of the call
  * (which may be 0), nothing in it needs to be set.  The reference's attention is that of the models it patches
  * (experiments/models/sparse_mistral/sparse_silu.py:756-832), over a cache in the model's type. */
 size_t cats_kv8_attention_scratch_bytes(int B, int T, int heads, int kv_heads, int D, int blocks, int window);

@@ -58,7 +58,7 @@ def test_strides_that_no_vector_reads(L, strides):
 
 @pytest.mark.parametrize("change,status", [
     (dict(), 6), (dict(scratch=_p(), bytes=64), 6), (dict(dtype=2), 1), (dict(B=0), 4), (dict(heads=3, kv=2), 2), (dict(heads=1, kv=2), 2), (dict(window=-1), 2),
-    (dict(scale=0.0), 2), (dict(scale=-1.0), 2), (dict(scale=float("nan")), 2), (dict(scale=float("inf")), 2), (dict(q=None), 5), (dict(out=None), 5), (dict(out=_p(8)), 3),
+    (dict(scale=2.0 ** -65), 2), (dict(scale=2.0 ** 65), 2), (dict(scale=0.0), 2), (dict(scale=-1.0), 2), (dict(scale=float("nan")), 2), (dict(scale=float("inf")), 2), (dict(q=None), 5), (dict(out=None), 5), (dict(out=_p(8)), 3),
     (dict(q=_p(2)), 3), (dict(T=4000 * 64 + 1), 2), (dict(T=100000, heads=64), 2), (dict(k8=None), 5)])
 def test_attention_refuses(L, change, status):
     """The plain call ends at its scratch, which a cache of 4000 blocks needs."""

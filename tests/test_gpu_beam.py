@@ -54,6 +54,25 @@ def test_ties_go_to_the_lowest(V, dtype):
     _check(up.flip(-1).contiguous(), torch.tensor([[0.0, -0.3]]))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,V", [(1, 2000), (256, 8100), (256, 20001)])
+def test_more_candidates_than_are_gathered(rows, V, dtype):
+    """Equal best values spread over the waves of a workgroup, or in one of them, and few words left side by side, in both sizes of a piece."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(rows // min(rows, 16), min(rows, 16), V, generator=g).to(dtype)
+    s = -torch.arange(min(rows, 16)).float().expand(x.shape[:2]).contiguous()
+    spread = x.clone()
+    spread[..., torch.randperm(min(V, 8000), generator=g)[:100]] = 10.0
+    _check(spread, s)
+    one = x.clone()
+    one[..., 300:400] = 10.0
+    one[..., torch.randperm(V, generator=g)[:3]] = 11.0
+    _check(one, s)
+    left = torch.full_like(x, -math.inf)
+    left[..., 200:300] = x[..., 200:300]
+    _check(left, s)
+
+
 @pytest.mark.parametrize("V", [40, 9000])
 def test_select_at_the_start_and_where_words_are_masked(V):
     """Beams that take no part yet, words at -infinity and at the type's lowest value, fewer words left than beams, rows with a NaN or +infinity."""

@@ -87,6 +87,20 @@ def test_append_gives_the_same_whatever_the_pieces(dtype):
             assert torch.equal(a, b), f
 
 
+@pytest.mark.parametrize("start", [128, 129, 150, 64, 0])
+def test_tokens_taken_back(start):
+    """150 tokens, of which those from `start` on are replaced: within the last block, and from the start of an earlier one."""
+    g = torch.Generator().manual_seed(start)
+    k, v, k2, v2, q = (_tokens(g, 1, 150, n, 64, F16) for n in (2, 2, 2, 2, 4))
+    c = ref.new_cache(1, 2, 4, 64, F16, device="cuda")
+    _append(c, k.cuda(), v.cuda(), [0])
+    _append(c, k2[:, :40].cuda(), v2[:, :40].cuda(), [start])
+    both = [torch.cat((a[:, :start], b[:, :40]), 1) for a, b in ((k, k2), (v, v2))]
+    want = ref.append(ref.new_cache(1, 2, 4, 64, F16), *both, [0], None)
+    out = _attention(c, q[:, :40].cuda(), [start])
+    assert ref.within(out, *ref.attention(want, q[:, :40], [start], None, 0.125))
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_append_values_at_the_edges(dtype):
     """Zeros, the largest and the smallest numbers, maxima on a power of two and on 448 times one, one step above it, ties between two
@@ -211,6 +225,19 @@ def test_attention_of_a_draft_over_a_long_cache():
 def test_attention_scales(scale):
     """Weights that are all alike and weights of which one is left."""
     _check(1, 3, 2, 1, 64, F16, [200], 4, scale=scale)
+
+
+@pytest.mark.parametrize("T", [3, 70])
+@pytest.mark.parametrize("scale", [2.0 ** -64, 2.0 ** 64])
+def test_attention_scales_at_the_limits(scale, T):
+    """Keys of the smallest block scale: masked weights are 0 all the same."""
+    g = torch.Generator().manual_seed(T)
+    k, v, q = _tokens(g, 1, 200, 1, 64, BF16) * 2.0 ** -58, _tokens(g, 1, 200, 1, 64, BF16), _tokens(g, 1, T, 2, 64, BF16)
+    cache = ref.append(ref.new_cache(1, 1, 4, 64, BF16), k, v, [0], None)
+    assert cache["k_scale"][0, 0, 0] == 2.0 ** -60
+    out = _attention(ref.to(cache, "cuda"), q.cuda(), [200 - T], scale=scale, window=90)
+    want, bound = ref.attention(cache, q, [200 - T], None, scale, 90)
+    assert out.isfinite().all() and ref.within(out, want, bound)
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
