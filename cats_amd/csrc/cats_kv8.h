@@ -482,9 +482,47 @@ __global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_ker
   auto part_tile = [&](int at) {  // whether some query does not see all of it
     return at * kKvBlock + kKvBlock - 1 > t.pos_lo || (p.window && at * kKvBlock <= t.pos_hi - p.window);
   };
+  // the tail, by the split whose turn it would be: its loads go ahead of the first tile's, whose way from memory hides what the tail takes
+  const bool tail = t.tile_hi == t.last && (t.last - t.tile_lo) / W % t.active == split;
+  u32x4 kq[NK][NV];
+  u32x2 vq[NU];
+  if (tail) {
+    const uint16_t* kt = p.c.kt + (size_t)pair * kKvBlock * D + (ktok + 4 * wave) * D + d0;
+    const uint16_t* vt = p.c.vt + (size_t)pair * kKvBlock * D + m * kKvBlock + 16 * g + 4 * wave;
+#pragma unroll
+    for (int c = 0; c < NK; c++)
+#pragma unroll
+      for (int v = 0; v < NV; v++) kq[c][v] = *(const u32x4*)(kt + 64 * c + 8 * v);
+#pragma unroll
+    for (int u = 0; u < NU; u++) vq[u] = *(const u32x2*)(vt + 16 * u * kKvBlock);
+  }
+  __builtin_amdgcn_sched_barrier(0);
   if (tile <= end8) {
     fetch_k(tile);
     fetch_v(tile);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  if (tail) {
+    f32x4 s[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int c = 0; c < NK; c++)
+#pragma unroll
+      for (int v = 0; v < NV; v++) s[0] = Mma<DT>::run(kq[c][v], qf[c][v], s[0]);
+    const int key = t.last * kKvBlock + 16 * g + 4 * wave;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float x = fmaf(s[0][e], 0.f, s[0][e]);  // a key that is not finite makes the score NaN, as in e4m3
+      s[0][e] = seen(key + e) ? x : -INFINITY;
+    }
+    weigh(s, 1, 1.f, 1.f);
+    const u32x2 pf = u32x2{DT::pack(s[0][0], s[0][1]), DT::pack(s[0][2], s[0][3])};
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+      some |= kv_fix16<DT>(vq[u]);
+      o[u] = DownMma<DT>::run(vq[u], pf, o[u]);
+    }
+  }
+  if (tile <= end8) {
     for (;;) {
       const float ks = kscale[tile], vs = vscale[tile];
       f32x4 s[4];
@@ -533,38 +571,6 @@ __global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_ker
     }
   }
 
-  // the tail, by the split whose turn it would be
-  const bool tail = t.tile_hi == t.last && (t.last - t.tile_lo) / W % t.active == split;
-  if (tail) {
-    const uint16_t* kt = p.c.kt + (size_t)pair * kKvBlock * D + (ktok + 4 * wave) * D + d0;
-    const uint16_t* vt = p.c.vt + (size_t)pair * kKvBlock * D + m * kKvBlock + 16 * g + 4 * wave;
-    u32x4 kq[NK][NV];
-    u32x2 vq[NU];
-#pragma unroll
-    for (int c = 0; c < NK; c++)
-#pragma unroll
-      for (int v = 0; v < NV; v++) kq[c][v] = *(const u32x4*)(kt + 64 * c + 8 * v);
-#pragma unroll
-    for (int u = 0; u < NU; u++) vq[u] = *(const u32x2*)(vt + 16 * u * kKvBlock);
-    f32x4 s[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-    for (int c = 0; c < NK; c++)
-#pragma unroll
-      for (int v = 0; v < NV; v++) s[0] = Mma<DT>::run(kq[c][v], qf[c][v], s[0]);
-    const int key = t.last * kKvBlock + 16 * g + 4 * wave;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float x = fmaf(s[0][e], 0.f, s[0][e]);  // a key that is not finite makes the score NaN, as in e4m3
-      s[0][e] = seen(key + e) ? x : -INFINITY;
-    }
-    weigh(s, 1, 1.f, 1.f);
-    const u32x2 pf = u32x2{DT::pack(s[0][0], s[0][1]), DT::pack(s[0][2], s[0][3])};
-#pragma unroll
-    for (int u = 0; u < NU; u++) {
-      some |= kv_fix16<DT>(vq[u]);
-      o[u] = DownMma<DT>::run(vq[u], pf, o[u]);
-    }
-  }
   if (__any(some != 0)) {  // the queries that see a number that is not finite
     auto spoil = [&](int tile, auto load) {
 #pragma unroll
