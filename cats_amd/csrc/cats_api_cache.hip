@@ -165,10 +165,15 @@ namespace {
 struct BeamPlan {
   int per_lane, pieces;
 };
-BeamPlan beam_plan(int groups, int beams, int V) {
+// Eight elements a lane where that is up to four workgroups a CU and leaves the second launch 256 candidates a row at most, else 32.  Both launches, 8 / 32,
+// in us, logits of 16 bits, keep = beams:
+//   4 beams, 32000 words 9.2 / 10.2     8 x 4, 32000 9.8 / 10.6     4 x 8, 50257 11.9 / 12.3     8, 64000 10.5 / 11.6
+//   8 x 4, 64000 11.0 / 10.8            4 x 16, 32000 17.2 / 15.9   16 x 8, 32000 14.6 / 13.8    8 x 8, 128000 (fp32) 18.7 / 16.2
+//   8, 128000 (504 candidates) 11.3 / 11.9     16, 50257 (400) 17.9 / 15.9     16, 128000 (1008) 30.6 / 17.3
+BeamPlan beam_plan(int groups, int beams, int V, int keep) {
   BeamPlan p;
   const long long small = ((long long)V + 4 * kWave * 8 - 1) / (4 * kWave * 8);
-  p.per_lane = small * groups * beams <= 4ll * current_device_cus() ? 8 : 32;
+  p.per_lane = small * groups * beams <= 4ll * current_device_cus() && small * keep <= 256 ? 8 : 32;
   const int per = 4 * kWave * p.per_lane;
   p.pieces = (V + 7 - 1) / per + 1;  // a row may start up to seven elements behind a vector's start
   return p;
@@ -187,7 +192,7 @@ size_t beam_bytes(const BeamPlan& p, int groups, int beams, int keep) {
 extern "C" {
 
 size_t cats_beam_scratch_bytes(int groups, int beams, int V, int keep) {
-  return beam_ok(groups, beams, V, keep) ? beam_bytes(beam_plan(groups, beams, V), groups, beams, keep) : 0;
+  return beam_ok(groups, beams, V, keep) ? beam_bytes(beam_plan(groups, beams, V, keep), groups, beams, keep) : 0;
 }
 
 int cats_beam_select(const void* logits, int64_t row_stride, const float* scores, const uint8_t* finished, int64_t eos, float* scores_out,
@@ -198,7 +203,7 @@ int cats_beam_select(const void* logits, int64_t row_stride, const float* scores
   if (!logits || !scores || !scores_out || !parents_out || !tokens_out || !finished_out) return CATS_ERR_NULL;
   const size_t esz = dtype == CATS_F32 ? 4 : 2;
   if (!aligned(logits, esz) || !aligned(scores, 4) || !aligned(scores_out, 4) || !aligned(parents_out, 8) || !aligned(tokens_out, 8)) return CATS_ERR_ALIGN;
-  const BeamPlan plan = beam_plan(groups, beams, V);
+  const BeamPlan plan = beam_plan(groups, beams, V, keep);
   const size_t n = (size_t)groups * beams * plan.pieces;
   if (!scratch || !aligned(scratch, 16) || scratch_bytes < beam_bytes(plan, groups, beams, keep)) return CATS_ERR_WORKSPACE;
   BeamArgs a;

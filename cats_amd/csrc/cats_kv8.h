@@ -51,7 +51,8 @@ __device__ __forceinline__ bool kv_span(const KvSpan& s, int b, int T, int& star
 }
 
 // What differs between the two types.  HEAD: attention's weights are held as 2^HEAD times themselves, so that in fp16 the normal numbers
-// reach down to 2^-29 of the largest weight.
+// reach down to 2^-29 of the largest weight.  SLACK: by how many powers of two weights may pass 2^HEAD's part before kv8_attn_prompt_kernel scales its
+// sums again; they start that much lower (8 against 0: a prompt of 2048 tokens 58.8 / 61.3 us, heads of 256 behind 3300 tokens 70.9 / 73.7).
 template <class DT> struct Kv;
 template <> struct Kv<F16> {
   static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
@@ -211,7 +212,8 @@ struct KvAppendArgs {
 
 // Workgroup (i, head, row) quantises block start / 64 + i if these tokens complete it; the first one also stores the tail.  It is the only one that
 // reads the tail (the tokens of the first block that were there before) and the only one that writes it, behind a barrier.
-// Bound by memory: 2 bytes of a value read and one written.
+// Bound by memory, 2 bytes of a value read and one written: 8 prompts of 2048 tokens, 32 heads of 128, 93 us, 4.3 TB/s where a copy reaches 4.9 (with
+// the values turned round a byte at a time in LDS 107).  A token each for 64 rows of 8 heads is the launch, 6.6 us.
 template <class DT, int D>
 __global__ __launch_bounds__(256) void kv8_append_kernel(KvAppendArgs p) {
   const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
@@ -369,14 +371,17 @@ __device__ __forceinline__ float max_mod16(float v) {
 // 16-bit operands (two an instruction), the blocks' scales go into the exponent: with w = s * ks * scale + log2(vs), weights are
 // 2^(w - max w) <= 1, O sums them times the codes, and the sum of weights adds them divided by vs.
 // The tail is four times sixteen tokens, for a wave each: tile `wave` of the four, and one product over sixteen tokens.
+// Bound by the cache's bytes where it is long: one row of 131072 tokens, 8 heads of 128 for 32, 43 us, 6.2 TB/s where a read stream reaches 7.1, and 4.6
+// for the join.  16 rows of 2048 to 4096 tokens take 22.8 us where the bytes take 14.5: four tiles a wave do not hide the way of the first and what
+// the end costs.  100 tokens are the launch and three trips to memory one behind the other (positions, keys and values, the output), 6 us.
 // MASK: queries that see different keys, or a window.  One token without a window sees all of every tile but the tail.
 // SEAL: the tokens are in the tails and nowhere else yet.  One workgroup a pair more quantises the block that they complete; nobody reads that block
 // in this launch.
 constexpr int kKvStepWaves = 4;
 // Waves a SIMD, as far as registers allow.
-constexpr int kv_step_waves(int D, bool mask) { return D == 256 ? 1 : D == 128 ? (mask ? 2 : 3) : D == 64 && mask ? 3 : 4; }
+constexpr int kv_step_waves(int D) { return D == 256 ? 1 : D == 128 ? 3 : 4; }
 template <class DT, int D, bool MASK, bool SEAL>
-__global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_kernel(KvAttnArgs p) {
+__global__ __launch_bounds__(256, kv_step_waves(D)) void kv8_attn_step_kernel(KvAttnArgs p) {
   constexpr bool AHEAD = D < 256 || !MASK;  // the next tile's keys over this one's values: registers
   constexpr int W = kKvStepWaves, ROWS = 16, NU = D / 16, NK = D >= 64 ? D / 64 : 1, NV = D >= 64 ? 2 : 1;
   typedef Kv<DT> F;
@@ -646,6 +651,10 @@ __global__ __launch_bounds__(256, kv_step_waves(D, MASK)) void kv8_attn_step_ker
 //   O^T   operand of step (u, v): tokens 32 u + 16 h + 8 v .. + 7, again those whose weights the lane has
 // Rows of LDS are 16-byte pieces, exchanged within a row so that any 16 lanes in order find the 64 banks once each.
 // Workgroups with the most keys start first.
+// Bound by what a SIMD issues: a tile is 64 products a wave (1024 cycles of the matrix cores with heads of 128) and some 330 other instructions, of which 128
+// turn e4m3 into operands and 64 are exponentials, and the two overlap only in part (alone 1189 and 1169 cycles, together 1570).  A prompt of 2048
+// tokens, 32 heads of 128, takes 50 us, 680 TFLOP/s of what is seen; two pieces of 512 behind 7680 tokens 123 us, 840 (a large product 1125 to 1180).
+// 128 rows a workgroup need the registers of one wave a SIMD and were slower.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <class DT> struct Mma32;
 template <> struct Mma32<F16> {
@@ -825,6 +834,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
       __builtin_amdgcn_sched_barrier(0);
       behind();
     }
+    // The other wave's products before this one's weights: two pieces of 512 behind 7680 tokens 146 us, without 151; a prompt of 2048 58.8 and 57.3.
     __builtin_amdgcn_s_setprio(0);
     if constexpr (PART) {
       mask(s, tile);
@@ -1005,8 +1015,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   }
 }
 
-// The splits' results, in a fixed order.  ALONE: a workgroup per (pair, row), whose groups of D / 4 lanes take every so manieth split and are
-// joined in LDS.  Otherwise, for few splits, a row per group.  Rows whose cache was one split's are done already.  ROWS and UNIT are the
+// The splits' results, in a fixed order: 4 us, the launch and two trips to memory.  ALONE: a workgroup per (pair, row), whose groups of D / 4 lanes take
+// every so manieth split and are joined in LDS.  Otherwise, for few splits, a row per group.  Rows whose cache was one split's are done already.  ROWS and UNIT are the
 // attention kernel's.
 template <class DT, int D, int ROWS, int UNIT, bool ALONE>
 __global__ __launch_bounds__(256) void kv8_join_kernel(KvAttnArgs p) {
