@@ -316,7 +316,8 @@ __device__ __forceinline__ uint64_t beam_key(double x) {
   return b >> 63 ? ~b : b | 1ull << 63;
 }
 
-// Candidates of a row come in pieces of `keep`; a wave takes 512 at a time beside the best it has.  What the beams offer is in order for each of them
+// Candidates of a row come in pieces of `keep`; a wave takes 256 at a time beside the best it has (512: 16 beams of 32000 words 15.3 us, 14.7; of 200000
+// 27.0, 25.9).  What the beams offer is in order for each of them
 // (total, then id), so of equal totals the earlier offer is the better one.  Few of them are ranked in 64 bits: those whose totals, rounded to
 // float, which keeps their order, are not below the keep-th best of the lanes'.
 template <int N>
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(N* kWave) void beam_join_kernel(BeamArgs p) {
     const float* ml = p.ml + (size_t)row * p.pieces * 2;
     const size_t at = (size_t)row * p.pieces * p.keep;
     const int n = p.pieces * p.keep;
-    constexpr int E = 8;
+    constexpr int E = 4;
     float val[E + 1];
     int id[E + 1];
     auto fetch = [&](int i0) {
