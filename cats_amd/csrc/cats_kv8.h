@@ -715,7 +715,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   const float* vscale = p.c.vs + (size_t)pair * p.c.blocks;
 
   // A wave brings half of the rows of keys and of values of its tile, 1 KiB at a time: lane l of load j writes piece 64 j + l and reads what belongs
-  // there.  What is exchanged goes by bits of the row, so load j differs from load 0 by constants.
+  // there.  What is exchanged goes by bits of the row, so load j differs from load 0 by constants, and reads of LDS differ by constants too: four
+  // offsets in bytes are kept over the loop, hidden from the compiler, which would keep every address that follows from them.
+  unsigned k_from = (lane / PK * PK + ((lane % PK) ^ kv_swap_k<D>(lane / PK))) * 16, v_from = (lane / 4 * 4 + ((lane % 4) ^ kv_swap_v(lane / 4))) * 16;
+  const int ktok = 16 * (m >> 2 & 1) + 4 * (m >> 3) + (m & 3);  // token of this lane's row of K in tile 0; 32 more in tile 1
+  unsigned k_at = (ktok * PK + (h ^ kv_swap_k<D>(ktok))) * 16, v_at = (m * 4 + (h ^ kv_swap_v(m))) * 16;
+  asm volatile("" : "+v"(k_from), "+v"(v_from), "+v"(k_at), "+v"(v_at));
   const int end8 = min(t.tile_hi, t.last - 1);  // last tile in 8 bits; behind it the last one comes again
   float ks = 1.f, vs = 1.f, ks1 = 1.f, vs1 = 1.f;  // scales of the wave's tile and of the next one
   auto bring = [&](int tile, int buf) {
@@ -725,14 +730,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
     const u32x4* kf = k8 + (size_t)at * kVecs + rw * (kVecs / 2);
     const u32x4* vf = v8 + (size_t)at * kVecs + rw * (kVecs / 2);
     u32x4* to = s_kv[buf][kh][0] + rw * (kVecs / 2);
-    int l = lane;
-    asm volatile("" : "+v"(l));  // addresses are computed here each time: kept over the loop they would cost the registers that tiles need
-    const int kq = (l % PK) ^ kv_swap_k<D>(l / PK), kl = l / PK * PK, vl = l / 4 * 4 + ((l % 4) ^ kv_swap_v(l / 4));
 #pragma unroll
     for (int j = 0; j < kVecs / 2 / kWave; j++) {
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kf + j * kWave + (kl + (kq ^ kv_swap_k<D>(j * kWave / PK)))),
+      const char *kj = (const char*)(kf + j * kWave), *vj = (const char*)(vf + j * kWave);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kj + (size_t)(k_from ^ (16u * kv_swap_k<D>(j * kWave / PK)))),
                                        (__attribute__((address_space(3))) void*)(to + j * kWave), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vf + j * kWave + vl),
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vj + (size_t)v_from),
                                        (__attribute__((address_space(3))) void*)(to + kVecs + j * kWave), 16, 0, 0);
     }
   };
@@ -748,7 +751,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   };
 #pragma unroll
   for (int w = 0; w < NW; w++) o[w] = zeros();
-  const int ktok = 16 * (m >> 2 & 1) + 4 * (m >> 3) + (m & 3);  // token of this lane's row of K in tile 0; 32 more in tile 1
 
   // weights of a tile from its scores; returns them as operands
   auto weigh = [&](f32x16 (&s)[2], float ks, float vs, u32x4 (&pf)[2][2]) {
@@ -805,10 +807,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
     // products each time.  (Heads of 256 elements do not have the registers.)
     constexpr bool ASK = D <= 128;
     f32x16 s[2] = {zeros(), zeros()};
-    int kt = ktok, vd = m;  // as in bring
-    asm volatile("" : "+v"(kt), "+v"(vd));
-    auto keys = [&](int c, int u) { return s_kv[buf][kh][0][(kt + 32 * u) * PK + ((2 * c + h) ^ kv_swap_k<D>(kt))]; };
-    auto values = [&](int w, int u) { return s_kv[buf][kh][1][(32 * w + vd) * 4 + ((2 * u + h) ^ kv_swap_v(vd))]; };
+    const char* tile_kv = (const char*)s_kv[buf][kh][0];
+    auto keys = [&](int c, int u) { return *(const u32x4*)(tile_kv + (k_at ^ 32u * c) + 32 * u * PK * 16); };
+    auto values = [&](int w, int u) { return *(const u32x4*)(tile_kv + (v_at ^ 32u * u) + (kVecs + 32 * w * 4) * 16); };
     u32x4 x[ASK ? 2 * NW : 1];  // C is NW
     if constexpr (ASK) {
 #pragma unroll
