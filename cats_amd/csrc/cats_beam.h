@@ -485,7 +485,7 @@ __device__ __forceinline__ void reorder_units(const ReorderArgs& p, const Reorde
         long long e = c.entries;
         if (c.slots) {
           const long long len = p.lengths[(size_t)(group * p.beams + f) * p.lengths_step];
-          e = len <= 0 ? 0 : min(e, (len + c.slots - 1) / c.slots);
+          e = len <= 0 ? 0 : min(e, (len - 1) / c.slots + 1);
         }
         live[j] = e * c.entry_bytes / (long long)sizeof(U);
         most = max(most, live[j]);

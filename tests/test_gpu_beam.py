@@ -244,3 +244,34 @@ def test_what_the_operators_refuse():
                  ([c.to(torch.uint8)[..., :3].contiguous()], [1], p, n), ([c.cpu()], [1], p, n), ([c], [1], p.cpu(), n)):
         with pytest.raises(RuntimeError):
             flash_gemv.cats_cache_reorder(*args)
+
+
+def test_reorder_with_a_length_that_no_cache_has():
+    import flash_gemv
+
+    c = torch.arange(2 * 5 * 4, dtype=torch.int32).view(2, 1, 5, 4)
+    got = c.cuda()
+    flash_gemv.cats_cache_reorder([got], [64], torch.tensor([[1, 0]], device="cuda"), torch.tensor([2 ** 63 - 1], device="cuda"))
+    assert torch.equal(got.cpu(), c.flip(0))
+
+
+def test_offsets_beyond_32_bits():
+    """Logits whose rows lie 2^32 bytes apart, and a row of a cache of more than 2^32 bytes."""
+    import flash_gemv
+
+    g = torch.Generator().manual_seed(6)
+    x, s = torch.randn(1, 3, 1000, generator=g).half(), -torch.rand(1, 3, generator=g)
+    far = torch.empty(2 ** 32 + 2000, dtype=F16, device="cuda").as_strided((1, 3, 1000), (0, 2 ** 31 + 8, 1))
+    far.copy_(x)
+    _check(x, s)
+    for a, b in zip(flash_gemv.cats_beam_select(far, s.cuda()), flash_gemv.cats_beam_select(x.cuda(), s.cuda())):
+        assert torch.equal(a, b)
+    del far
+    torch.cuda.empty_cache()
+    entries = 2 ** 28 + 1000
+    c = torch.zeros(2, 1, entries, 4, dtype=torch.int32, device="cuda")
+    last = torch.randint(1, 1 << 30, (2, 1, 2000, 4), generator=g, dtype=torch.int32)
+    c[:, :, -2000:] = last.cuda()
+    flash_gemv.cats_cache_reorder([c], [1], torch.tensor([[1, 0]], device="cuda"), torch.tensor([entries - 3], device="cuda"))
+    assert torch.equal(c[:, :, -2000:-3].cpu(), last.flip(0)[:, :, :-3]) and torch.equal(c[:, :, -3:].cpu(), last[:, :, -3:])
+    assert int(c[:, :, :-2000].max()) == 0

@@ -468,3 +468,23 @@ def test_results_do_not_change_from_call_to_call():
     first = _attention(c, q, [3499, 899])
     for _ in range(5):
         assert torch.equal(_attention(c, q, [3499, 899]), first)
+
+
+def test_offsets_beyond_32_bits():
+    """A cache of more than 2^32 bytes of keys and of values, its last tokens, by the step's and the prompt's kernel."""
+    from cats_amd.kv8 import Kv8Cache
+
+    g = torch.Generator().manual_seed(12)
+    blocks, behind = 70000, 192  # zeros in front of the new tokens, as many as the window reaches back
+    c = Kv8Cache(1, 8, blocks * 64, 128, BF16)
+    small = ref.new_cache(1, 8, 20, 128, BF16, fill=0.0)
+    small["k_scale"].fill_(1.0), small["v_scale"].fill_(1.0)
+    start = blocks * 64 - 1024
+    for T, at in ((700, 0), (1, 700)):
+        k, v, q = (_tokens(g, 1, T, n, 128, BF16) for n in (8, 8, 16))
+        small = ref.append(small, k, v, [behind + at], None)
+        c.append(k.cuda(), v.cuda(), _words([start + at]))
+        out = c.attend(q.cuda(), _words([start + at]), window=150)
+        assert ref.within(out, *ref.attention(small, q, [behind + at], None, 128 ** -0.5, 150))
+    assert torch.equal(c.k8[0, :, start // 64:start // 64 + 10].cpu().float(), small["k8"][0, :, 3:13].float())
+    assert torch.equal(c.v8[0, :, start // 64:start // 64 + 10].cpu().float(), small["v8"][0, :, 3:13].float())
