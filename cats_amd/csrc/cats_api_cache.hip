@@ -59,13 +59,16 @@ int check_span(const int64_t* start, int start_step, const int64_t* count, int c
 
 // Which kernel, and how many splits of a row's cache.  Up to 16 rows of queries a cached head are one operand of the step's kernel; more of them are
 // several of its workgroups, each of which reads the cache, or the prompt's kernel.  That one pays for LDS and for few splits of short caches, so
-// the line is drawn by the work, (row, cached head) pairs x 16 rows x tiles of the cache.  Step / prompt in us, heads of 128 elements, bf16:
-//   8 pairs, 64 rows, 20 tiles 12.0 / 17.2     8, 128, 20 14.2 / 17.7     8, 64, 59 14.3 / 16.0     8, 128, 59 17.7 / 17.5     8, 256, 59 25.3 / 20.3
-//   64 pairs, 24 rows, 79 tiles 32.7 / 24.0    64, 64, 79 51.8 / 30.9     32, 64, 2 7.7 / 8.3       32, 256, 5 13.7 / 11.5     32, 512, 10 17.8 / 18.6
-// Both are to have two workgroups a CU (the step's with four: 64 rows of 8 heads at 1000 tokens 26.3 against 23.1, 16 rows of 32 at 2000 49.2
-// against 45.7, one row of 8 at 3000 tokens the same).  A cache of up to 16 tiles is not split: the second launch costs more (one row, 32 heads,
-// 8 cached, 300 tokens 9.5 with, 6.7 without; 16 rows of 32 at 600 tokens 23.2 and 18.8; one row at 600 tokens 9.5 and 9.0).
-constexpr int kStepRows = 16, kStepWork = 3000, kStepAlone = 16;
+// the line is drawn by the work, (row, cached head) pairs x 16 rows x tiles of the cache.  Step / prompt in us, heads of 128, bf16:
+//   8 pairs, 256 rows, 20 tiles (2560) 15.5 / 17.8     8, 128, 59 (3776) 18.2 / 20.2     8, 192, 59 (5664) 21.4 / 20.8     8, 256, 59 (7552) 20.2 / 21.0
+//   128, 32, 10 (2560) 10.4 / 13.6     8, 1024, 5 (2560) 9.4 / 11.4     8, 2048, 10 (10240) 16.2 / 14.1     64, 24, 79 (10112) 27.7 / 22.3
+// A second launch costs more than it gives for short caches, up to 16 tiles for the step's kernel (one row, 32 heads, 8 cached, 300 tokens 9.5 with,
+// 6.7 without; 16 rows of 32 at 600 tokens 23.2 and 18.8; one row at 600 tokens 9.5 and 9.0), up to 32 for the prompt's (512 tokens of 32 heads
+// over 8, 10 tiles, 17.6 with two splits, 14.0 with one; 256 behind 768, 20 tiles, 21.3 and 18.3; 256 behind 1144, 28 tiles, 24.1 and 21.3).  Beyond that
+// the step's is to have two workgroups a CU (with four: 64 rows of 8 heads at 1000 tokens 26.3 against 23.1, 16 rows of 32 at 2000 49.2 against
+// 45.7, one row of 8 at 3000 tokens the same), the prompt's one, and 16 tiles a split (two a CU and 8 tiles: 512 behind 3584 54.0, 48.1; 128
+// behind 3172 32.4, 24.9; 100 behind 7900 39.8, 37.0).
+constexpr int kStepRows = 16, kStepWork = 5000, kStepAlone = 16, kPromptAlone = 32;
 
 }  // namespace
 
@@ -77,8 +80,8 @@ KvAttnPlan kv8_attn_plan(int B, int T, int heads, int kv_heads, int blocks, int 
   KvAttnPlan plan = {rows > kStepRows && step_groups * tiles > kStepWork, 1, false};
   const int unit = plan.prompt ? kKvPromptUnit : kKvStepWaves;
   const long long groups = plan.prompt ? pairs * ((rows + kKvPromptRows - 1) / kKvPromptRows) : step_groups;
-  const long long want = (2ll * cus + groups - 1) / groups;
-  if (plan.prompt || tiles > kStepAlone) plan.splits = (int)max(1ll, min(want, (long long)(tiles + unit - 1) / unit));
+  const long long want = ((plan.prompt ? 1ll : 2ll) * cus + groups - 1) / groups;
+  if (tiles > (plan.prompt ? kPromptAlone : kStepAlone)) plan.splits = (int)max(1ll, min(want, (long long)(tiles + unit - 1) / unit));
   return plan;
 }
 

@@ -678,7 +678,7 @@ __device__ __forceinline__ int kv_swap_k(int t) {
 }
 __device__ __forceinline__ int kv_swap_v(int d) { return d >> 2 & 3; }
 
-constexpr int kKvPromptRows = 64, kKvPromptUnit = 8;  // rows of a workgroup; tiles that make a split worth while
+constexpr int kKvPromptRows = 64, kKvPromptUnit = 16;  // rows of a workgroup; tiles that make a split worth while
 template <class DT, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(KvAttnArgs p) {
   constexpr int ROWS = kKvPromptRows, C = D / 32, NW = D / 32, PK = D / 16;
