@@ -26,6 +26,7 @@ SYMBOLS = (
     "cats_probe_read", "cats_mlp_norm_residual_norm", "cats_linear", "cats_attention_step", "cats_mlp_gate_cols", "cats_silu_mask_mul",
     "cats_prompt_scratch_bytes", "cats_prompt_mlp", "cats_prompt_plan", "cats_kv8_append", "cats_kv8_attention_scratch_bytes",
     "cats_kv8_attention", "cats_kv8_attention_step_scratch_bytes", "cats_kv8_attention_step", "cats_beam_scratch_bytes", "cats_beam_select", "cats_cache_reorder",
+    "cats_kv8_attention_plan",
 )
 
 
@@ -81,6 +82,7 @@ def lib() -> ctypes.CDLL:
             L.cats_kv8_append.argtypes = [vp, vp, vp, vp, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]
             L.cats_kv8_append.restype = i32
             L.cats_kv8_attention_scratch_bytes.argtypes = [i32] * 7; L.cats_kv8_attention_scratch_bytes.restype = sz
+            L.cats_kv8_attention_plan.argtypes = [i32] * 7 + [vp]; L.cats_kv8_attention_plan.restype = i32
             L.cats_kv8_attention.argtypes = [vp, vp, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, f32, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, sz, vp]
             L.cats_kv8_attention.restype = i32
             L.cats_kv8_attention_step_scratch_bytes.argtypes = [i32] * 4; L.cats_kv8_attention_step_scratch_bytes.restype = sz
@@ -229,6 +231,13 @@ def prompt_plan(product, M, H, I):
     plan = (ctypes.c_int * 6)()
     check(lib().cats_prompt_plan(product, M, H, I, plan), "cats_prompt_plan")
     return tuple(plan)
+
+
+def kv8_attention_plan(B, T, heads, kv_heads, D, blocks, window=0):
+    """(whether cats_kv8_attention launches the kernel for many tokens, splits of a row's cache at most) on the current device."""
+    plan = (ctypes.c_int * 2)()
+    check(lib().cats_kv8_attention_plan(B, T, heads, kv_heads, D, blocks, window, plan), "cats_kv8_attention_plan")
+    return bool(plan[0]), plan[1]
 
 
 def up_down(x, a, wup, wdown_t, threshold, ws: Workspace):

@@ -129,6 +129,16 @@ size_t cats_kv8_attention_scratch_bytes(int B, int T, int heads, int kv_heads, i
   return attn_bytes(kv8_attn_plan(B, T, heads, kv_heads, blocks, window_of(window, blocks)), B, T, heads, kv_heads, D);
 }
 
+int cats_kv8_attention_plan(int B, int T, int heads, int kv_heads, int D, int blocks, int window, int* out) {
+  if (int st = check_cache(B, T, kv_heads, D, blocks, CATS_F16)) return st;
+  if (!attn_shape_ok(T, heads, kv_heads) || window < 0) return CATS_ERR_SHAPE;
+  if (!out) return CATS_ERR_NULL;
+  const KvAttnPlan plan = kv8_attn_plan(B, T, heads, kv_heads, blocks, window_of(window, blocks));
+  out[0] = plan.prompt;
+  out[1] = plan.splits;
+  return CATS_OK;
+}
+
 int cats_kv8_attention(const void* q, const int64_t* q_strides, const int64_t* start, int start_step, const int64_t* count, int count_step,
                        const void* k8, const void* v8, const float* k_scale, const float* v_scale, const void* k_tail, const void* v_tail,
                        float scale, int window, void* out, int B, int T, int heads, int kv_heads, int D, int blocks, int dtype, void* scratch,

@@ -277,6 +277,10 @@ int cats_kv8_attention(const void* q, const int64_t* q_strides, const int64_t* s
                        float scale, int window, void* out, int B, int T, int heads, int kv_heads, int D, int blocks, int dtype, void* scratch,
                        size_t scratch_bytes, void* stream);
 
+/* What cats_kv8_attention launches on the current device, for tests and profiles: plan[0] = 1 where it is the kernel for many tokens, else 0, plan[1] =
+ * splits of a row's cache at most.  Not in the reference. */
+int cats_kv8_attention_plan(int B, int T, int heads, int kv_heads, int D, int blocks, int window, int* plan);
+
 /* cats_attention_step over such a cache, with as many cached heads as query heads: k and v of the new token go to the tails, and the block that
  * it completes is quantised beside attention.  q is rounded to dtype before the products.  Limits on B and H are those of cats_linear; position lies
  * in [0, max_len), max_len <= 64 * blocks, and what the cache holds ends at it; elsewhere nothing is stored and out is NaN.  Three launches, four

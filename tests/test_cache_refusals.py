@@ -120,3 +120,14 @@ def test_operators_refuse_cpu_tensors():
                  lambda: flash_gemv.cats_beam_select(torch.zeros(1, 2, 9), torch.zeros(1, 2)), lambda: flash_gemv.cats_cache_reorder([x], [0], torch.zeros(1, 1, dtype=torch.int64))):
         with pytest.raises(RuntimeError, match="GPU"):
             call()
+
+
+def test_plan_refusals():
+    from cats_amd import capi
+
+    out = (ctypes.c_int * 2)()
+    plan = capi.lib().cats_kv8_attention_plan
+    assert plan(1, 1, 2, 1, 64, 4, 0, out) == 0 and out[0] == 0 and out[1] == 1
+    assert plan(1, 1, 2, 1, 64, 4, 0, None) == 5
+    for bad in ((1, 1, 3, 2, 64, 4, 0), (1, 1, 2, 1, 48, 4, 0), (1, 0, 2, 1, 64, 4, 0), (1, 1, 2, 1, 64, 4, -1), (1, 300, 2, 1, 64, 4, 0)):
+        assert plan(*bad, out) == 2

@@ -40,7 +40,7 @@ def test_select(G, n, V, keep, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
-@pytest.mark.parametrize("V", [3, 64, 3000, 40000])
+@pytest.mark.parametrize("V", [3, 64, 3000, 40000, 180000])
 def test_ties_go_to_the_lowest(V, dtype):
     """All logits equal, few values, zeros of both signs, and rows with the same score: more equal values than a wave gathers."""
     g = torch.Generator().manual_seed(V)
@@ -73,7 +73,7 @@ def test_more_candidates_than_are_gathered(rows, V, dtype):
     _check(left, s)
 
 
-@pytest.mark.parametrize("V", [40, 9000])
+@pytest.mark.parametrize("V", [40, 9000, 140000])
 def test_select_at_the_start_and_where_words_are_masked(V):
     """Beams that take no part yet, words at -infinity and at the type's lowest value, fewer words left than beams, rows with a NaN or +infinity."""
     g = torch.Generator().manual_seed(V)
@@ -94,7 +94,7 @@ def test_select_at_the_start_and_where_words_are_masked(V):
     _check(x, torch.tensor([[math.nan, 0.0, math.inf, -1.0], [none, none, none, none]]))
 
 
-@pytest.mark.parametrize("V,eos", [(50, 0), (50, 49), (50, 3), (20000, 2)])
+@pytest.mark.parametrize("V,eos", [(50, 0), (50, 49), (50, 3), (20000, 2), (140000, 100000)])
 def test_finished_beams_go_on_alone(V, eos):
     g = torch.Generator().manual_seed(V + eos)
     x = torch.randn(4, 4, V, generator=g).half()

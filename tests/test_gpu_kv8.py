@@ -472,6 +472,7 @@ def test_results_do_not_change_from_call_to_call():
 
 def test_offsets_beyond_32_bits():
     """A cache of more than 2^32 bytes of keys and of values, its last tokens, by the step's and the prompt's kernel."""
+    from cats_amd import capi
     from cats_amd.kv8 import Kv8Cache
 
     g = torch.Generator().manual_seed(12)
@@ -481,7 +482,8 @@ def test_offsets_beyond_32_bits():
     small["k_scale"].fill_(1.0), small["v_scale"].fill_(1.0)
     start = blocks * 64 - 1024
     for T, at in ((700, 0), (1, 700)):
-        k, v, q = (_tokens(g, 1, T, n, 128, BF16) for n in (8, 8, 16))
+        assert capi.kv8_attention_plan(1, T, 32, 8, 128, blocks, 150)[0] == (T > 1)
+        k, v, q = (_tokens(g, 1, T, n, 128, BF16) for n in (8, 8, 32))
         small = ref.append(small, k, v, [behind + at], None)
         c.append(k.cuda(), v.cuda(), _words([start + at]))
         out = c.attend(q.cuda(), _words([start + at]), window=150)
