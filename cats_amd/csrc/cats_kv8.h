@@ -653,8 +653,8 @@ __global__ __launch_bounds__(256, kv_step_waves(D)) void kv8_attn_step_kernel(Kv
 // Workgroups with the most keys start first.
 // Bound by what a SIMD issues: a tile is 32 products a wave (1024 cycles of the matrix cores with heads of 128) and some 300 other instructions, of which 128
 // turn e4m3 into operands and 32 are exponentials, and the two overlap only in part (a loop of each, alone 1189 and 1169 cycles, on one SIMD 1570); a third
-// wave a SIMD, which heads of 64 have room for, is worth 2 to 6 %.  A prompt of 2048 tokens, 32 heads of 128, takes 50 us, 690 TFLOP/s of what is
-// seen; two pieces of 512 behind 7680 tokens 119 us, 870 (a large product 1125 to 1180).
+// wave a SIMD, which heads of 64 have room for, is worth 2 to 6 %.  A prompt of 2048 tokens, 32 heads of 128, takes 49 us, 700 TFLOP/s of what is
+// seen; two pieces of 512 behind 7680 tokens 117 us, 890 (a large product 1125 to 1180).
 // 128 rows a workgroup need the registers of one wave a SIMD and were slower.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <class DT> struct Mma32;
