@@ -354,7 +354,7 @@ class LlamaDecoder(nn.Module):
             pos.add_(1)
             step_idx.add_(1)
 
-        graph = self._captured(step, (tok, pos, step_idx, out)) if use_graph else None
+        graph = self._captured(step, (tok, pos, step_idx, out)) if use_graph and gen_len > 1 else None  # one token has no step, and `out` no room for one
         torch.cuda.synchronize()
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record()

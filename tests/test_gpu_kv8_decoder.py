@@ -130,6 +130,16 @@ def test_greedy_with_a_cache_in_8_bits_replays_its_graph():
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
+@pytest.mark.parametrize("kv_cache", ["dtype", "e4m3"])
+def test_one_token_has_no_step_to_capture(kv_cache):
+    """The only token comes from the prompt: a step made for the capture alone would store its token behind the output."""
+    m = _model(F16, kv_cache, 40)
+    prompt = torch.randint(0, 120, (1, 39), generator=torch.Generator().manual_seed(4)).cuda()
+    eager, _ = m.generate_greedy(prompt, 1, use_graph=False)
+    graph, _ = m.generate_greedy(prompt, 1, use_graph=True)
+    assert eager.shape == (1,) and torch.equal(eager, graph)
+
+
 def _search(m, prompt, beams, gen_len, eos):
     """Beam search that computes every beam from its first token at every step."""
     G, P = prompt.shape
