@@ -362,6 +362,16 @@ __device__ __forceinline__ float max_mod16(float v) {
   return max_mod32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
 
+// A weight's exponent is s * sc - top.  Scores of 2^24 and more lie further apart than 1 in 32 bits, and then the product, rounded in `top` and not in
+// the fma, may exceed it by any power of two: the largest weight would overflow.  So where a query's largest score is far from 0, scores are
+// taken relative to the tile's largest, and that one's distance from the top, a difference of rounded products and not above 0 (or SLACK), is added.  Below
+// this bound the rest is at most 2^-7 of an exponent, what 32 bits hold of such a score.
+__device__ __forceinline__ bool kv_far(float top) { return fabsf(top) > 0x1p16f && top > -FLT_MAX; }
+__device__ __forceinline__ float kv_scaled(float s, float sc) {  // rounded, whatever it is added to
+#pragma clang fp contract(off)
+  return s * sc;
+}
+
 // One new token, or a few: 16 rows of queries, the cache split over workgroups and over the four waves of each, the waves' results joined in LDS
 // and the workgroups' by kv8_join_kernel.  Each wave takes 64 tokens at a time:
 //   S^T = K . Q^T   tile i, row 4 g + e of the 16x16 result: token 16 g + 4 i + e, in lanes of group g = lane / 16; columns are queries
@@ -450,6 +460,7 @@ __global__ __launch_bounds__(256, kv_step_waves(D)) void kv8_attn_step_kernel(Kv
   int tile = t.tile_lo + split * W + wave;
 
   float top = -FLT_MAX, sum = 0.f;
+  bool far = false;   // whether some query's scores are
   uint32_t some = 0;  // whether a tile that is seen in part had numbers of V that are not finite
   f32x4 o[NU];
 #pragma unroll
@@ -464,13 +475,23 @@ __global__ __launch_bounds__(256, kv_step_waves(D)) void kv8_attn_step_kernel(Kv
 #pragma unroll
       for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[i][e]);
     mx = max_mod16(mx);
-    const float now = fmaxf(top, fmaf(mx, sc, lv)), off = lv + F::HEAD - now;
+    const float at = kv_scaled(mx, sc), now = fmaxf(top, at + lv);
+    float off = lv + F::HEAD - now;
     if (__any(now > top)) {
       const float keep = __builtin_amdgcn_exp2f(top - now);
       sum *= keep;
 #pragma unroll
       for (int u = 0; u < NU; u++) o[u] *= keep;
       top = now;
+      far = __any(kv_far(top));
+    }
+    if (far) {
+      const float ref = fmaxf(mx, -FLT_MAX);
+      off = fminf(at - now + lv, 0.f) + F::HEAD;
+#pragma unroll
+      for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[i][e] -= ref;
     }
     float add = 0.f;
 #pragma unroll
@@ -742,6 +763,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   };
 
   float top = -FLT_MAX, sum = 0.f;
+  bool far = false;   // whether some query's scores are
   uint32_t some = 0;  // whether a tile that is seen in part had numbers of V that are not finite
   f32x16 o[NW];
   auto zeros = [] {
@@ -762,15 +784,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
 #pragma unroll
       for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[u][e]);
     mx = max_mod32(mx);
-    const float now = fmaxf(top, fmaf(mx, sc, lv));
+    const float at = kv_scaled(mx, sc), now = fmaxf(top, at + lv);
     if (__any(now > top + F::SLACK)) {
       const float keep = __builtin_amdgcn_exp2f(top - now);
       sum *= keep;
 #pragma unroll
       for (int w = 0; w < NW; w++) o[w] *= keep;
       top = now;
+      far = __any(kv_far(top));
     }
-    const float off = lv + F::HEAD - F::SLACK - top;
+    float off = lv + F::HEAD - F::SLACK - top;
+    if (far) {
+      const float ref = fmaxf(mx, -FLT_MAX);
+      off = fminf(at - top + lv, F::SLACK) + F::HEAD - F::SLACK;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[u][e] -= ref;
+    }
     float add = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
