@@ -548,50 +548,51 @@ __global__ __launch_bounds__(256, kv_step_waves(D)) void kv8_attn_step_kernel(Kv
       o[u] = DownMma<DT>::run(vq[u], pf, o[u]);
     }
   }
-  if (tile <= end8) {
-    for (;;) {
-      const float ks = kscale[tile], vs = vscale[tile];
-      f32x4 s[4];
+  // What the next tile would need is asked for under a condition and not behind a way out of the loop: with that (and heads of 32, MASK) this compiler took
+  // parts of vv for undefined and gave their registers to others.
+  while (tile <= end8) {
+    const float ks = kscale[tile], vs = vscale[tile];
+    f32x4 s[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        __builtin_amdgcn_sched_barrier(0);
-        s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < NK; c++)
-#pragma unroll
-          for (int v = 0; v < NV; v++) s[i] = Mma<DT>::run(kv_wide<DT>(kk[i][c][2 * v], kk[i][c][2 * v + 1]), qf[c][v], s[i]);
-      }
-      const bool more = tile + step <= end8;
+    for (int i = 0; i < 4; i++) {
       __builtin_amdgcn_sched_barrier(0);
-      if (AHEAD && more) fetch_k(tile + step);
-      __builtin_amdgcn_sched_barrier(0);
-      const int key0 = tile * kKvBlock + 16 * g;  // of this lane's weights
-      const bool part = MASK && part_tile(tile);
-      if (part) {
+      s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+      for (int c = 0; c < NK; c++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) s[i][e] = seen(key0 + 4 * i + e) ? s[i][e] : -INFINITY;
-      }
-      weigh(s, 4, ks, vs);
-      u32x4 pf[2];  // the weights, rounded to the type the products take: half a step each, independent of one another
+        for (int v = 0; v < NV; v++) s[i] = Mma<DT>::run(kv_wide<DT>(kk[i][c][2 * v], kk[i][c][2 * v + 1]), qf[c][v], s[i]);
+    }
+    const bool more = tile + step <= end8;
+    __builtin_amdgcn_sched_barrier(0);
+    if (AHEAD && more) fetch_k(tile + step);
+    __builtin_amdgcn_sched_barrier(0);
+    const int key0 = tile * kKvBlock + 16 * g;  // of this lane's weights
+    const bool part = MASK && part_tile(tile);
+    if (part) {
 #pragma unroll
-      for (int v = 0; v < 2; v++)
-        pf[v] = u32x4{DT::pack(s[2 * v][0], s[2 * v][1]), DT::pack(s[2 * v][2], s[2 * v][3]), DT::pack(s[2 * v + 1][0], s[2 * v + 1][1]),
-                      DT::pack(s[2 * v + 1][2], s[2 * v + 1][3])};
-      if (part) {
+      for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int u = 0; u < NU; u++) some |= kv_fix8(vv[u]);
-      }
+        for (int e = 0; e < 4; e++) s[i][e] = seen(key0 + 4 * i + e) ? s[i][e] : -INFINITY;
+    }
+    weigh(s, 4, ks, vs);
+    u32x4 pf[2];  // the weights, rounded to the type the products take: half a step each, independent of one another
 #pragma unroll
-      for (int u = 0; u < NU; u++) {
-        if (u % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // operands of four products at a time
-        o[u] = Mma<DT>::run(kv_wide<DT>(vv[u][0], vv[u][1]), pf[0], o[u]);
-        o[u] = Mma<DT>::run(kv_wide<DT>(vv[u][2], vv[u][3]), pf[1], o[u]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if (!more) break;
-      tile += step;
+    for (int v = 0; v < 2; v++)
+      pf[v] = u32x4{DT::pack(s[2 * v][0], s[2 * v][1]), DT::pack(s[2 * v][2], s[2 * v][3]), DT::pack(s[2 * v + 1][0], s[2 * v + 1][1]),
+                    DT::pack(s[2 * v + 1][2], s[2 * v + 1][3])};
+    if (part) {
+#pragma unroll
+      for (int u = 0; u < NU; u++) some |= kv_fix8(vv[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+      if (u % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // operands of four products at a time
+      o[u] = Mma<DT>::run(kv_wide<DT>(vv[u][0], vv[u][1]), pf[0], o[u]);
+      o[u] = Mma<DT>::run(kv_wide<DT>(vv[u][2], vv[u][3]), pf[1], o[u]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    tile += step;
+    if (more) {
       if (!AHEAD) fetch_k(tile);
       fetch_v(tile);
     }
