@@ -50,27 +50,34 @@ __device__ __forceinline__ bool kv_span(const KvSpan& s, int b, int T, int& star
   return ok;
 }
 
-// What differs between the two types.  HEAD: attention's weights are held as 2^HEAD times themselves, so that in fp16 the normal numbers
-// reach down to 2^-29 of the largest weight.  SLACK: by how many powers of two weights may pass 2^HEAD's part before kv8_attn_prompt_kernel scales its
-// sums again; they start that much lower (8 against 0: a prompt of 2048 tokens 58.8 / 61.3 us, heads of 256 behind 3300 tokens 70.9 / 73.7).
+// What differs between the two types.  HEAD: attention's weights are held as 2^HEAD times themselves: in fp16 the normal numbers reach down to 2^-29
+// of the largest weight, in bf16 2^32 values of the largest size add up within 32 bits.  SLACK: by how many powers of two weights may pass 2^HEAD's part before
+// kv8_attn_prompt_kernel scales its sums again; they start that much lower (8 against 0: a prompt of 2048 tokens 58.8 / 61.3 us, heads of 256 behind 3300 tokens
+// 70.9 / 73.7).
+// VMAX: e4m3 values become operands of the type as what they stand for, so sums have one unit, blocks and the tail alike, and weights are those of the softmax.
+// The conversion multiplies by a power of two; what is stored of an fp16 value is one of 16 bits again, but for 256 times a scale of 2^8, and every bf16 scale
+// reaches the products up to 2^73 a value.  What a scale has beyond VMAX goes into the weights of its block (kv_over).
 template <class DT> struct Kv;
 template <> struct Kv<F16> {
   static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
-  static constexpr float HEAD = 15.f, SLACK = 8.f;
+  static constexpr float HEAD = 15.f, SLACK = 8.f, VMAX = 0x1p7f;
   template <bool HI>
-  static __device__ __forceinline__ uint32_t cvt(uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI)); }
+  static __device__ __forceinline__ uint32_t cvt(uint32_t w, float scale) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI)); }
 };
 template <> struct Kv<BF16> {
   static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u;
-  static constexpr float HEAD = 0.f, SLACK = 8.f;
+  static constexpr float HEAD = -32.f, SLACK = 8.f, VMAX = 0x1p64f;
   template <bool HI>
-  static __device__ __forceinline__ uint32_t cvt(uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI)); }
+  static __device__ __forceinline__ uint32_t cvt(uint32_t w, float scale) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI)); }
 };
-// Eight e4m3 numbers as an operand of sixteen bits, exactly.
+// Eight e4m3 numbers times a power of two as an operand of sixteen bits, exactly.
 template <class DT>
-__device__ __forceinline__ u32x4 kv_wide(uint32_t a, uint32_t b) {
-  return u32x4{Kv<DT>::template cvt<false>(a), Kv<DT>::template cvt<true>(a), Kv<DT>::template cvt<false>(b), Kv<DT>::template cvt<true>(b)};
+__device__ __forceinline__ u32x4 kv_wide(uint32_t a, uint32_t b, float scale = 1.f) {
+  typedef Kv<DT> F;
+  return u32x4{F::template cvt<false>(a, scale), F::template cvt<true>(a, scale), F::template cvt<false>(b, scale), F::template cvt<true>(b, scale)};
 }
+template <class DT>
+__device__ __forceinline__ float kv_over(float vs) { return fmaxf(vs * (1.f / Kv<DT>::VMAX), 1.f); }
 
 // Places of numbers that are not finite.
 template <class DT>
@@ -378,8 +385,8 @@ __device__ __forceinline__ float kv_scaled(float s, float sc) {  // rounded, wha
 //   O^T += V^T . P  the weights of lane group g are those of tokens 16 g .. + 15 in order: what the lane has to supply as operand
 // so weights go from one product into the other without leaving their lane, and every load of the cache is 16 bytes a lane of 1 KiB in a
 // row (V) or of whole lines (K).  The next tile's keys are asked for when this one's have been used, and so are its values.  The numbers become
-// 16-bit operands (two an instruction), the blocks' scales go into the exponent: with w = s * ks * scale + log2(vs), weights are
-// 2^(w - max w) <= 1, O sums them times the codes, and the sum of weights adds them divided by vs.
+// 16-bit operands (two an instruction), the keys' scale goes into the exponent, the values' into the conversion: with w = s * ks * scale, weights are
+// 2^(HEAD + w - max w), O sums them times the values, and both are divided at the end.
 // The tail is four times sixteen tokens, for a wave each: tile `wave` of the four, and one product over sixteen tokens.
 // Bound by the cache's bytes where it is long: one row of 131072 tokens, 8 heads of 128 for 32, 43 us, 6.2 TB/s where a read stream reaches 7.1, and 4.6
 // for the join.  16 rows of 2048 to 4096 tokens take 22.8 us where the bytes take 14.5: four tiles a wave do not hide the way of the first and what
@@ -467,8 +474,8 @@ __global__ __launch_bounds__(256, kv_step_waves(D)) void kv8_attn_step_kernel(Kv
   for (int u = 0; u < NU; u++) o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto seen = [&](int key) { return key <= pos && (!MASK || key > first); };
   // weights of this lane's N x 4 scores, in place; the lanes of a query agree on their largest
-  auto weigh = [&](f32x4* s, int N, float ks, float vs) {
-    const float sc = p.scale * ks, lv = __builtin_amdgcn_logf(vs);
+  auto weigh = [&](f32x4* s, int N, float ks, float over) {
+    const float sc = p.scale * ks, lv = __builtin_amdgcn_logf(over);
     float mx = s[0][0];
 #pragma unroll
     for (int i = 0; i < N; i++)
@@ -501,7 +508,7 @@ __global__ __launch_bounds__(256, kv_step_waves(D)) void kv8_attn_step_kernel(Kv
         s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], sc, off));
         add += s[i][e];
       }
-    sum = fmaf(add, __builtin_amdgcn_rcpf(vs), sum);
+    sum = fmaf(add, __builtin_amdgcn_rcpf(over), sum);
     asm volatile("" : "+v"(sum));  // here: the weights' registers are wanted
   };
 
@@ -551,7 +558,7 @@ __global__ __launch_bounds__(256, kv_step_waves(D)) void kv8_attn_step_kernel(Kv
   // What the next tile would need is asked for under a condition and not behind a way out of the loop: with that (and heads of 32, MASK) this compiler took
   // parts of vv for undefined and gave their registers to others.
   while (tile <= end8) {
-    const float ks = kscale[tile], vs = vscale[tile];
+    const float ks = kscale[tile], vs = vscale[tile], vm = fminf(vs, F::VMAX);
     f32x4 s[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -574,7 +581,7 @@ __global__ __launch_bounds__(256, kv_step_waves(D)) void kv8_attn_step_kernel(Kv
 #pragma unroll
         for (int e = 0; e < 4; e++) s[i][e] = seen(key0 + 4 * i + e) ? s[i][e] : -INFINITY;
     }
-    weigh(s, 4, ks, vs);
+    weigh(s, 4, ks, kv_over<DT>(vs));
     u32x4 pf[2];  // the weights, rounded to the type the products take: half a step each, independent of one another
 #pragma unroll
     for (int v = 0; v < 2; v++)
@@ -587,8 +594,8 @@ __global__ __launch_bounds__(256, kv_step_waves(D)) void kv8_attn_step_kernel(Kv
 #pragma unroll
     for (int u = 0; u < NU; u++) {
       if (u % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // operands of four products at a time
-      o[u] = Mma<DT>::run(kv_wide<DT>(vv[u][0], vv[u][1]), pf[0], o[u]);
-      o[u] = Mma<DT>::run(kv_wide<DT>(vv[u][2], vv[u][3]), pf[1], o[u]);
+      o[u] = Mma<DT>::run(kv_wide<DT>(vv[u][0], vv[u][1], vm), pf[0], o[u]);
+      o[u] = Mma<DT>::run(kv_wide<DT>(vv[u][2], vv[u][3], vm), pf[1], o[u]);
     }
     __builtin_amdgcn_sched_barrier(0);
     tile += step;
@@ -777,8 +784,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
   for (int w = 0; w < NW; w++) o[w] = zeros();
 
   // weights of a tile from its scores; returns them as operands
-  auto weigh = [&](f32x16 (&s)[2], float ks, float vs, u32x4 (&pf)[2][2]) {
-    const float sc = p.scale * ks, lv = __builtin_amdgcn_logf(vs);
+  auto weigh = [&](f32x16 (&s)[2], float ks, float over, u32x4 (&pf)[2][2]) {
+    const float sc = p.scale * ks, lv = __builtin_amdgcn_logf(over);
     float mx = s[0][0];
 #pragma unroll
     for (int u = 0; u < 2; u++)
@@ -816,7 +823,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
 #pragma unroll
         for (int e = 0; e < 4; e++) pf[u][v][e] = DT::pack(s[u][8 * v + 2 * e], s[u][8 * v + 2 * e + 1]);
     }
-    sum = fmaf(add, __builtin_amdgcn_rcpf(vs), sum);
+    sum = fmaf(add, __builtin_amdgcn_rcpf(over), sum);
     asm volatile("" : "+v"(sum));  // here: the weights' registers are wanted
   };
   auto seen = [&](int key) { return key <= pos && key > first; };
@@ -886,14 +893,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
       }
     }
     u32x4 pf[2][2];
-    weigh(s, ks, vs, pf);
+    const float vm = fminf(vs, F::VMAX);
+    weigh(s, ks, kv_over<DT>(vs), pf);
     __builtin_amdgcn_s_setprio(1);
     if constexpr (ASK) {
       // Sums of different w in turn, and each operand made while the product before it runs: otherwise the products wait for theirs (a prompt of 2048
       // tokens 50.6, 49.6 us; two pieces of 512 behind 7680 119.7, 118.0; the same for the scores gains nothing).
       auto wide = [&](int i) {
         const u32x4 vv = x[2 * (i % NW) + i / (2 * NW)];
-        return i / NW & 1 ? kv_wide<DT>(vv[2], vv[3]) : kv_wide<DT>(vv[0], vv[1]);
+        return i / NW & 1 ? kv_wide<DT>(vv[2], vv[3], vm) : kv_wide<DT>(vv[0], vv[1], vm);
       };
       __builtin_amdgcn_sched_barrier(0);
       u32x4 operand = wide(0);
@@ -917,8 +925,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv8_attn_prompt_kernel(
         for (int u = 0; u < 2; u++) {
           u32x4 vv = values(w, u);
           if constexpr (PART) some |= kv_fix8(vv);
-          o[w] = Mma32<DT>::run(kv_wide<DT>(vv[0], vv[1]), pf[u][0], o[w]);
-          o[w] = Mma32<DT>::run(kv_wide<DT>(vv[2], vv[3]), pf[u][1], o[w]);
+          o[w] = Mma32<DT>::run(kv_wide<DT>(vv[0], vv[1], vm), pf[u][0], o[w]);
+          o[w] = Mma32<DT>::run(kv_wide<DT>(vv[2], vv[3], vm), pf[u][1], o[w]);
         }
       behind();
     }

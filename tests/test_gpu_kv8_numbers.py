@@ -85,3 +85,56 @@ def test_equal_scores_that_are_large_share_the_weight(dtype, scale, T, window):
         # half a step of each weight and of the output, 2^-20 for the sums and the division
         bound[0, i] = (ref.HALF[dtype] + 2.0 ** -20) * (x.mean(0).abs() + x.abs().mean(0)) + 2.0 ** -25 * (dtype == F16)
     assert ref.within(_call(cache, q, [300 - T], window, scale), want, bound)
+
+
+@pytest.mark.parametrize("T,blocks", [(1, 16), (5, 16), (70, ROOM)])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -13, 2.0 ** -17, 2.0 ** -19])
+def test_light_weights_of_small_values_count(size, T, blocks):
+    """A thousand tokens alike whose weights are 1.2 times 2^-13 of a key's in the tail: a seventh of the whole together, whatever the values' size and with
+    a block of zeros (whose scale is 1) among them.  fp16, where weights have the fewest bits; one split, so that waves have the tail and blocks."""
+    D, n = 64, 1010
+    g = torch.Generator().manual_seed(11)
+    k = torch.zeros(1, n, 1, D)
+    v = (1 + 0.2 * torch.randn(1, n, 1, D, generator=g)) * size
+    v[:, 640:704] = 0
+    q = torch.zeros(1, T, 2, D)
+    q[..., 0] = 1.0
+    k[0, n - T, 0, 0] = (13 * math.log(2) - math.log(1.2)) / 0.125
+    k, v, q = k.half(), v.half(), q.half()
+    cache = _room(k, v, blocks)
+    assert capi.kv8_attention_plan(1, T, 2, 1, D, blocks, 0)[0] or capi.kv8_attention_plan(1, T, 2, 1, D, blocks, 0)[1] == 1
+    want, bound = ref.attention(cache, q, [n - T], None, 0.125)
+    assert ref.within(_call(cache, q, [n - T]), want, bound)
+
+
+@pytest.mark.parametrize("T,window", [(1, 0), (5, 0), (70, 0)])
+@pytest.mark.parametrize("large,small", [(2.0 ** 100, 1.0), (2.0 ** 126, 1.0), (2.0 ** 126, 2.0 ** -40), (2.0 ** 126, 0.0), (2.0 ** 66, 2.0 ** 60)])
+def test_values_of_all_sizes_count_in_the_sum_of_weights(large, small, T, window):
+    """bf16 blocks whose scales lie up to 2^167 apart: the keys of the small values weigh as much as those of the large ones."""
+    g = torch.Generator().manual_seed(12)
+    k, v = _tokens(g, 1, 300, 1, 64, BF16), torch.randn(1, 300, 1, 64, generator=g).clamp(-1.9, 1.9) * small
+    v[:, 64:128] = torch.randn(1, 64, 1, 64, generator=g).clamp(-1.9, 1.9) * large
+    q = torch.randn(1, T, 2, 64, generator=g).bfloat16()
+    cache = _room(k, v.bfloat16())
+    want, bound = ref.attention(cache, q, [300 - T], None, 0.125)
+    out = _call(cache, q, [300 - T], window)
+    assert out.isfinite().all() and ref.within(out, want, bound)
+
+
+@pytest.mark.parametrize("T,window", [(1, 0), (5, 0), (70, 0)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("size", ["largest", "smallest"])
+def test_values_at_the_ends_of_the_type(dtype, size, T, window):
+    """Values up to the largest number, whose block rounds to 256 times its scale, and fp16's down to single steps of 2^-24; in blocks and in the tail."""
+    g = torch.Generator().manual_seed(13)
+    k, v = _tokens(g, 1, 300, 1, 64, dtype), torch.rand(1, 300, 1, 64, generator=g) * 2 - 1
+    if size == "largest":
+        v = v * torch.finfo(dtype).max
+        v[0, 3, 0, 9], v[0, 290, 0, 11] = torch.finfo(dtype).max, -torch.finfo(dtype).max
+    else:
+        v = torch.randint(-40, 41, v.shape, generator=g) * (2.0 ** -24 if dtype == F16 else 2.0 ** -62)
+        v[0, 64:128] = v[0, 64:128].sign() * (2.0 ** -24 if dtype == F16 else 2.0 ** -62)
+    q = torch.randn(1, T, 2, 64, generator=g).to(dtype)
+    cache = _room(k, v.to(dtype))
+    want, bound = ref.attention(cache, q, [300 - T], None, 0.125)
+    assert ref.within(_call(cache, q, [300 - T], window), want, bound)
