@@ -188,7 +188,7 @@ BeamPlan beam_plan(int groups, int beams, int V, int keep) {
   const long long small = ((long long)V + 4 * kWave * 8 - 1) / (4 * kWave * 8);
   p.per_lane = small * groups * beams <= 4ll * current_device_cus() && small * keep <= 256 ? 8 : 32;
   const int per = 4 * kWave * p.per_lane;
-  p.pieces = (V + 7 - 1) / per + 1;  // a row may start up to seven elements behind a vector's start
+  p.pieces = (V - 1) / per + 1;
   return p;
 }
 bool beam_ok(int groups, int beams, int V, int keep) {

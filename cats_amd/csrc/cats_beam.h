@@ -187,6 +187,8 @@ __device__ __forceinline__ void wave_best(const float (&x)[E], Id id, int keep, 
   wave_lds_sync();
 }
 
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // wherever an element starts
+
 template <class DT, int E>
 __global__ __launch_bounds__(256, 6) void beam_rows_kernel(BeamArgs p) {
   typedef typename DT::st st;
@@ -197,18 +199,19 @@ __global__ __launch_bounds__(256, 6) void beam_rows_kernel(BeamArgs p) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6, row = blockIdx.y, piece = blockIdx.x;
   if (p.finished && p.finished[row]) return;
   const st* x = (const st*)p.logits + row * p.row_stride;
-  // the wave's elements, in vectors of VEC that go round the lanes; vectors are those of memory, so a row may start inside its first
-  const int first = (piece * W + wave) * kWave * E - (int)(((uintptr_t)x & 15u) / sizeof(st));
+  // The wave's elements, in vectors of VEC that go round the lanes, wherever the row starts: which words are summed together goes by their ids alone, so rows
+  // that are the same have the same sums to the bit, and tie.
+  const int first = (piece * W + wave) * kWave * E;
   float val[E];
   int own = first + lane * VEC;
   auto id = [&](int i) {
     const int at = own + i / VEC * kWave * VEC + i % VEC;
-    return at >= 0 && at < p.V ? at : -1;
+    return at < p.V ? at : -1;
   };
-  if (first >= 0 && first + kWave * E <= p.V) {
+  if (first + kWave * E <= p.V) {
     u32x4 w[G];
 #pragma unroll
-    for (int i = 0; i < G; i++) w[i] = load_stream((const u32x4*)(x + first + (i * kWave + lane) * VEC));
+    for (int i = 0; i < G; i++) w[i] = __builtin_nontemporal_load((const u32x4_any*)(x + first + (i * kWave + lane) * VEC));
 #pragma unroll
     for (int i = 0; i < E; i++) {
       const uint32_t c = w[i / VEC][i % VEC * 4 / VEC];

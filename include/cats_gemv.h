@@ -299,7 +299,8 @@ int cats_kv8_attention_step(const void* h, const void* x, const void* norm_weigh
  * float.  finished (groups, beams) bytes, optional: a beam that has finished goes on only as (b, eos) with its score.  Totals that are not finite
  * count as -infinity (so beams with a score of -infinity take no part).  Outputs (groups, keep): scores, parents (b), tokens (v), and whether a
  * beam has finished (its parent had, or v is eos; eos < 0: none).  Beams are ordered by their logits within a row and by totals in 64 bits between
- * rows.  keep <= beams * V; both up to CATS_MAX_BEAMS.  scratch: 16-byte aligned, at least cats_beam_scratch_bytes(), nothing in it needs to be set. */
+ * rows, with a sum of 32-bit exponentials (the logarithm is within 2^-21) that goes by the logits alone, wherever a row starts: rows that
+ * are the same tie.  keep <= beams * V; both up to CATS_MAX_BEAMS.  scratch: 16-byte aligned, at least cats_beam_scratch_bytes(), nothing in it needs to be set. */
 size_t cats_beam_scratch_bytes(int groups, int beams, int V, int keep);
 int cats_beam_select(const void* logits, int64_t row_stride, const float* scores, const uint8_t* finished, int64_t eos, float* scores_out,
                      int64_t* parents_out, int64_t* tokens_out, uint8_t* finished_out, int groups, int beams, int V, int keep, int dtype,

@@ -275,3 +275,21 @@ def test_offsets_beyond_32_bits():
     flash_gemv.cats_cache_reorder([c], [1], torch.tensor([[1, 0]], device="cuda"), torch.tensor([entries - 3], device="cuda"))
     assert torch.equal(c[:, :, -2000:-3].cpu(), last.flip(0)[:, :, :-3]) and torch.equal(c[:, :, -3:].cpu(), last[:, :, -3:])
     assert int(c[:, :, :-2000].max()) == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("G,n,V", [(1, 2, 50257), (3, 8, 50257), (2, 4, 1001), (1, 16, 100003), (40, 8, 8193), (2, 2, 7)])
+def test_rows_that_are_the_same_tie(G, n, V, dtype):
+    """The same logits and scores in every beam, in rows that start at every offset within 16 bytes: their totals are the same to the bit, so each word's beams
+    come in order."""
+    g = torch.Generator().manual_seed(V + n)
+    x = (torch.randn(G, 1, V, generator=g) * 3).to(dtype).expand(G, n, V).contiguous()
+    s = torch.full((G, n), -1.25)
+    _check(x, s)
+    import flash_gemv
+
+    for pitch in (V + 1, V + 3, V + 8):
+        far = torch.zeros(G * n * pitch + 5, dtype=dtype, device="cuda")[5:].as_strided((G, n, V), (n * pitch, pitch, 1))
+        far.copy_(x)
+        for a, b in zip(flash_gemv.cats_beam_select(far, s.cuda()), flash_gemv.cats_beam_select(x.cuda(), s.cuda())):
+            assert torch.equal(a, b)
