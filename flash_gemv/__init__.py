@@ -156,14 +156,14 @@ def cats_kv8_append(k, v, start, count, k8, v8, k_scale, v_scale, k_tail, v_tail
 
     k, v (B, T, kv_heads, D) half or bfloat16, any strides; start, count int64 on the GPU, one for all rows or one each (count None: all T): row b's
     first ``count`` tokens go to positions ``start ..``, where what it holds already ends.  A smaller start takes tokens back, as far as the start of the block of 64 that holds the
-    last one, or to the start of any block."""
+    last one, or to the start of any block.  No gradient: tensors that record one are refused."""
     torch.ops.flash_gemv.cats_kv8_append(k, v, start, count, k8, v8, k_scale, v_scale, k_tail, v_tail)
 
 
 def cats_kv8_attention(q, start, count, k8, v8, k_scale, v_scale, k_tail, v_tail, scale, window=0):
     """Causal attention of the tokens that cats_kv8_append has stored: q (B, T, heads, D), heads a multiple of the cache's, over the positions up to
     each token's own, at most ``window`` of them (0: all); ``scale`` lies in 2^-64 .. 2^64.
-    Returns (B, T, heads, D); rows behind ``count`` are zeros.  Serving only: no gradient."""
+    Returns (B, T, heads, D); rows behind ``count`` are zeros.  Serving only: no gradient, and a q that records one is refused."""
     return torch.ops.flash_gemv.cats_kv8_attention(q, start, count, k8, v8, k_scale, v_scale, k_tail, v_tail, scale, window)
 
 
@@ -171,7 +171,7 @@ def cats_beam_select(logits, scores, finished=None, eos=-1, keep=0):
     """The best ``keep`` (0: as many as there are beams) of ``scores + log_softmax(logits)`` over the beams and words of each group, on the GPU.
 
     logits (groups, beams, V), scores (groups, beams) float, finished (groups, beams) bool: a beam that has finished goes on only as eos with its
-    score.  Returns scores, parents, tokens, finished, each (groups, keep), best first, ties to the lowest beam and word."""
+    score.  Returns scores, parents, tokens, finished, each (groups, keep), best first, ties to the lowest beam and word; the scores have no gradient."""
     return torch.ops.flash_gemv.cats_beam_select(logits, scores, finished, eos, keep)
 
 
@@ -179,7 +179,7 @@ def cats_cache_reorder(caches, slots, parents, lengths=None):
     """Move caches to the beams that go on, in place: row g * beams + j of each becomes what row g * beams + parents[g, j] was.
 
     caches: contiguous tensors (groups * beams, heads, entries, ...); slots: tokens an entry of each holds (0: all entries are live); lengths: int64,
-    tokens of all rows or of each.  Entries behind a length stay as they are."""
+    tokens of all rows or of each.  Entries behind a length stay as they are.  The caches may not overlap."""
     torch.ops.flash_gemv.cats_cache_reorder(caches, slots, parents, lengths)
 
 

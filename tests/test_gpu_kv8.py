@@ -490,3 +490,21 @@ def test_offsets_beyond_32_bits():
         assert ref.within(out, *ref.attention(small, q, [behind + at], None, 128 ** -0.5, 150))
     assert torch.equal(c.k8[0, :, start // 64:start // 64 + 10].cpu().float(), small["k8"][0, :, 3:13].float())
     assert torch.equal(c.v8[0, :, start // 64:start // 64 + 10].cpu().float(), small["v8"][0, :, 3:13].float())
+
+
+def test_gradients_are_refused():
+    """What records a gradient would be cut off from it; under no_grad, and detached, the same tensors are taken."""
+    from cats_amd.kv8 import Kv8Cache
+
+    c = Kv8Cache(1, 1, 64, 64, F16)
+    x, at = torch.randn(1, 2, 1, 64, dtype=F16, device="cuda"), _words([0])
+    w = x.clone().requires_grad_()
+    for call in (lambda: c.append(w, x, at), lambda: c.append(x, w, at), lambda: c.attend(w, at), lambda: c.attend(w * 2, at)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+    assert not c.k_tail.any() and not c.v_tail.any()
+    c.append(w.detach(), x, at)
+    with torch.no_grad():
+        c.append(w, w, at)
+        out = c.attend(w, at)
+    assert torch.equal(out, c.attend(x, at)) and not out.requires_grad
