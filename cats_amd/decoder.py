@@ -35,7 +35,10 @@ class DecoderConfig:
     rms_eps: float = 1e-5
     rope_theta: float = 10000.0
     max_len: int = 512
-    kv_cache: str = "dtype"  # "e4m3": a cache in 8 bits (cats_amd.kv8), for 16-bit models on the GPU
+    # "e4m3": a cache in 8 bits (cats_amd.kv8), for 16-bit models on the GPU.  Keys and values of complete blocks of 64 tokens are rounded to four bits, and a
+    # step's queries and attention weights to the model's type, where the step over a cache in that type keeps them in 32 bits.  Positions of a call follow
+    # one another, and tokens are taken back only as far as such a cache allows.
+    kv_cache: str = "dtype"
 
     @property
     def head_dim(self):
@@ -207,7 +210,8 @@ class LlamaDecoder(nn.Module):
             layer.self_attn.reset_cache(batch, self.dtype, dev)
 
     def forward(self, tokens, positions):
-        """tokens (B, q) int64; positions (q,) int64 -> logits (B, q, vocab).  Causal over cache slots <= position."""
+        """tokens (B, q) int64; positions (q,) int64 -> logits (B, q, vocab).  Causal over cache slots <= position.  A cache in 8 bits takes positions that
+        follow one another (others store nothing and give NaN) and start where what it holds ends, or as far back as cats_amd.kv8 says."""
         cfg = self.cfg
         h = self.embed_tokens(tokens)
         if self._takes_step(h, positions):
@@ -218,6 +222,12 @@ class LlamaDecoder(nn.Module):
             slots = torch.arange(cfg.max_len, device=tokens.device)
             mask = torch.zeros(positions.numel(), cfg.max_len, dtype=self.dtype, device=tokens.device)
             mask.masked_fill_(slots[None, :] > positions[:, None], float("-inf"))
+        elif positions.shape != tokens.shape[1:]:
+            raise ValueError(f"one position for each of {tokens.shape[1]} tokens, got {tuple(positions.shape)}")
+        elif positions.numel() > 1:
+            # the layers read the first position only: without a row of them it is none, found on the device as positions outside the cache are
+            row = positions == positions[:1] + torch.arange(positions.numel(), device=positions.device)
+            positions = torch.where(row.all(), positions, -1)
         normed = None
         for i, layer in enumerate(self.layers):
             next_norm = self.layers[i + 1].input_layernorm if i + 1 < len(self.layers) else self.norm

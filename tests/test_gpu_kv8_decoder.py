@@ -130,6 +130,23 @@ def test_greedy_with_a_cache_in_8_bits_replays_its_graph():
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
+@pytest.mark.parametrize("positions", [[40, 41, 43], [40, 40, 41], [42, 41, 40], [41, 40, 42], [2, 3, 40]])
+def test_positions_that_are_no_row_give_nan(positions):
+    """A cache in 8 bits stores a call's tokens one behind the other: any other positions leave it as it is, and no logits come of them."""
+    m = _model(F16, "e4m3", 70)
+    toks = torch.randint(0, 120, (2, 43), generator=torch.Generator().manual_seed(6)).cuda()
+    with torch.no_grad():
+        m.reset_cache(2)
+        m(toks[:, :40], torch.arange(40, device="cuda"))
+        kept = [t.clone() for l in m.layers for t in l.self_attn.caches()[0]]
+        assert m(toks[:, 40:], torch.tensor(positions, device="cuda")).isnan().all()
+        for a, l in zip(kept, (t for l in m.layers for t in l.self_attn.caches()[0])):
+            assert torch.equal(a.view(torch.uint8), l.view(torch.uint8))
+        with pytest.raises(ValueError, match="one position"):
+            m(toks[:, 40:], torch.tensor([40], device="cuda"))
+        assert m(toks[:, 40:], torch.arange(40, 43, device="cuda")).isfinite().all()
+
+
 @pytest.mark.parametrize("kv_cache", ["dtype", "e4m3"])
 def test_one_token_has_no_step_to_capture(kv_cache):
     """The only token comes from the prompt: a step made for the capture alone would store its token behind the output."""
