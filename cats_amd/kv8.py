@@ -12,6 +12,17 @@ kept as it was given.  So a token is rounded once, and a cache holds the same wh
 A row ends where the last call left it.  Tokens are taken back by a smaller start, as far as the start of the block that holds the last one, or
 to the start of any block: tokens of an earlier block are there as e4m3 only, and the rest of that block has to be given again.
 
+Drafted tokens may pass the end of a block before they are checked.  Who wants to go on from inside that block keeps the tails (64 tokens a row) over the
+draft, and after it puts them back and stores the accepted tokens again:
+
+    kept = cache.k_tail.clone(), cache.v_tail.clone()
+    cache.append(k, v, start)              # five drafted tokens from 62, say: a block is completed, and the tails begin the next one
+    out = cache.attend(q, start)           # one is accepted
+    cache.k_tail.copy_(kept[0]), cache.v_tail.copy_(kept[1])
+    cache.append(k, v, start, accepted)    # int64 on the GPU, one for all rows or one each; the row ends at start + accepted
+
+Nothing tells a cache from which block its tails are: a start further back than that makes a wrong block of what they hold.
+
 For fp16 and bf16 on the GPU, heads of 32, 64, 128 or 256 elements, without gradients.
 """
 from __future__ import annotations

@@ -260,7 +260,8 @@ int cats_attention_step(const void* h, const void* x, const void* norm_weight, f
 /* Stores the new tokens: quantises the blocks that they complete and leaves the last block in the tails.  What a row holds already has to end at
  * start (a block's tokens before start are taken from the tails).  So the cache is the same whatever pieces the tokens come in.  Tokens may be taken
  * back by a smaller start, as far as the start of the block that holds the last one, or to the start of any block; what an earlier block held in
- * the type is gone.  A row whose tokens do not lie within its blocks is left as it is. */
+ * the type is gone.  To take back drafted tokens that passed a block's end, copy the tails before they are stored, put the copies back, and store the
+ * accepted ones again.  Nothing tells a cache from which block its tails are: a start further back makes a wrong block of what they hold.  A row whose tokens do not lie within its blocks is left as it is. */
 int cats_kv8_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, const int64_t* start, int start_step,
                     const int64_t* count, int count_step, void* k8, void* v8, float* k_scale, float* v_scale, void* k_tail, void* v_tail, int B,
                     int T, int kv_heads, int D, int blocks, int dtype, void* stream);

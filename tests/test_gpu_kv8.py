@@ -508,3 +508,55 @@ def test_gradients_are_refused():
         c.append(w, w, at)
         out = c.attend(w, at)
     assert torch.equal(out, c.attend(x, at)) and not out.requires_grad
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("accepted", [[0, 0, 0], [1, 2, 5], [4, 3, 1]])
+def test_drafts_past_the_end_of_a_block_are_taken_back(accepted, dtype):
+    """Rows at 62, 60 and 127 tokens, five drafted ones, fewer kept: with the tails put back and the accepted tokens stored again a cache is what it
+    would be without the draft, and goes on over the block's end to the same bytes."""
+    from cats_amd.kv8 import Kv8Cache
+
+    g = torch.Generator().manual_seed(sum(accepted))
+    at = [62, 60, 127]
+    k, v, draft_k, draft_v, more_k, more_v, q = (_tokens(g, 3, n, h, 64, dtype).cuda() for n, h in ((127, 2), (127, 2), (5, 2), (5, 2), (70, 2), (70, 2), (70, 4)))
+    caches = [Kv8Cache(3, 2, 256, 64, dtype) for _ in range(2)]
+    start, end = _words(at), _words([a + n for a, n in zip(at, accepted)])
+    for c in caches:
+        c.append(k, v, _words([0]), start)
+    drafted, plain = caches
+    kept = drafted.k_tail.clone(), drafted.v_tail.clone()
+    drafted.append(draft_k, draft_v, start)
+    assert drafted.attend(q[:, :5], start).isfinite().all()
+    drafted.k_tail.copy_(kept[0]), drafted.v_tail.copy_(kept[1])
+    for c in caches:
+        c.append(draft_k, draft_v, start, _words(accepted))
+    one = more_k[:, :1], more_v[:, :1]
+    for c in caches:
+        c.append(*one, end)
+    assert torch.equal(drafted.attend(q[:, :1], end), plain.attend(q[:, :1], end))
+    for c in caches:
+        c.append(more_k[:, 1:], more_v[:, 1:], end + 1)
+    assert torch.equal(drafted.attend(q[:, 1:], end + 1), plain.attend(q[:, 1:], end + 1))
+    for b, e in enumerate((end + 70).tolist()):
+        full = (e - 1) // 64
+        for f in ("k8", "v8", "k_scale", "v_scale"):
+            assert ref.same(getattr(drafted, f)[b, :, :full], getattr(plain, f)[b, :, :full]), f
+        assert ref.same(drafted.k_tail[b, :, : e - full * 64], plain.k_tail[b, :, : e - full * 64])
+        assert ref.same(drafted.v_tail[b, ..., : e - full * 64], plain.v_tail[b, ..., : e - full * 64])
+
+
+def test_elements_in_any_order():
+    """Strides that no vector reads: every second element, elements in front of heads, a transposed batch; the same as of a copy."""
+    g = torch.Generator().manual_seed(16)
+    wide = _tokens(g, 3, 70, 2, 128, F16).cuda()
+    turned = _tokens(g, 3, 70, 64, 2, F16).cuda().transpose(2, 3)
+    batch = _tokens(g, 70, 3, 2, 64, F16).cuda().transpose(0, 1)
+    for x in (wide[..., ::2], wide[..., 1::2], turned, batch, batch[:, ::7], wide.flip(-1)[..., 64:]):
+        T = x.shape[1]
+        want = ref.append(ref.new_cache(3, 2, 2, 64, F16), x.cpu(), x.cpu(), [0] * 3, None)
+        c = ref.new_cache(3, 2, 2, 64, F16, device="cuda")
+        _append(c, x, x, [0])
+        for f in ref.FIELDS:
+            assert ref.same(c[f], want[f]), f
+        assert torch.equal(_attention(c, x, [0]), _attention(c, x.contiguous(), [0])) and x.shape == (3, T, 2, 64)
