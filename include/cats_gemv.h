@@ -269,7 +269,8 @@ int cats_kv8_append(const void* k, const int64_t* k_strides, const void* v, cons
 /* out[b, i, h] = softmax(scale * q[b, i, h] . K^T) . V over the keys at positions p - window + 1 .. p (window 0: 0 .. p), p = start + i, of cached
  * head h / (heads / kv_heads), for new tokens that cats_kv8_append has stored.  Rows i >= count are zeros; a row whose tokens do not lie within
  * its blocks is NaN.  A query that sees a key or an element of a value that is not finite is NaN (in that element).  out (B, T, heads, D) in
- * dtype, 16-byte aligned.  scale lies in 2^-64 .. 2^64.  scratch: 16-byte aligned, at least cats_kv8_attention_scratch_bytes() on the device of the call
+ * dtype, 16-byte aligned.  scale lies in 2^-64 .. 2^64, and scores have to be within 32-bit floats.  Weights are rounded to dtype
+ * (their sum is not).  scratch: 16-byte aligned, at least cats_kv8_attention_scratch_bytes() on the device of the call
  * (which may be 0), nothing in it needs to be set.  The reference's attention is that of the models it patches
  * (experiments/models/sparse_mistral/sparse_silu.py:756-832), over a cache in the model's type. */
 size_t cats_kv8_attention_scratch_bytes(int B, int T, int heads, int kv_heads, int D, int blocks, int window);

@@ -167,3 +167,33 @@ def test_outside_the_cache_and_from_call_to_call_and_in_a_graph():
             assert torch.equal(captured, first)
             assert torch.equal(_attention(cache, q, [2910, 1910]), first)
     side.synchronize()
+
+
+@pytest.mark.parametrize("blocks,lengths", [(20, [1200, 80]), (600, [5000, 900])])
+def test_replayed_on_other_tokens(blocks, lengths):
+    """A captured call of the kernel for many tokens without splits and with them, replayed on other queries, starts and counts, with other work between."""
+    import flash_gemv
+
+    g = torch.Generator().manual_seed(17)
+    heads, kv = (32, 4) if blocks == 20 else (2, 1)
+    _many(2, 63, heads, kv, 64, blocks, splits=1 if blocks == 20 else 2)
+    cache = ref.to(_filled(g, 2, kv, blocks, 64, F16, lengths), "cuda")
+    q, start, count = torch.zeros(2, 63, heads, 64, dtype=F16, device="cuda"), _words([0, 0]), _words([63, 63])
+    call = lambda: flash_gemv.cats_kv8_attention(q, start, count, *_args(cache), 0.125)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = call()
+    torch.cuda.current_stream().wait_stream(side)
+    for n in ([63, 63], [63, 1], [0, 40], [5, 63]):
+        q.copy_(torch.randn(2, 63, heads, 64, generator=g).half())
+        start.copy_(torch.tensor([a - b for a, b in zip(lengths, n)]))
+        count.copy_(torch.tensor(n))
+        out.fill_(7.0)
+        graph.replay()
+        got = out.clone()
+        (q.float() ** 2).sum()
+        assert torch.equal(got, call())
+        for b in range(2):
+            assert not got[b, n[b]:].any() and got[b, : n[b]].isfinite().all()
