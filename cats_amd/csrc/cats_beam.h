@@ -16,7 +16,7 @@ constexpr int kBeamMax = 16;  // beams of a group, before and after
 // more than 64 are each wave's best taken one by one and joined.  beam_join_kernel: a workgroup per group, a wave per beam joins its row's pieces in the same way, and
 // the beams' candidates are ranked by their totals in 64 bits: the order has to be that of the sums, which differ in their last bits only.
 // A row with a NaN or +infinity has no finite total at all, so neither has to be found among the best.
-// 16 groups of 16 beams, 100003 words in 32 bits: 19.6 us, 5.2 TB/s where a read stream reaches 7.1, and 9.3 for the join, whose sixteen waves share a CU.
+// 16 groups of 16 beams, 100003 words in 32 bits: 19.6 us, 5.2 TB/s where a read stream reaches 7.1, and 9.2 for the join, whose sixteen waves share a CU.
 // 32 elements a lane with six waves a SIMD; a bound a wave instead of a workgroup 30.3 us, 64 elements 21 to 26.  4 beams of 32000 words: 4.4 and 4.9 us.
 
 struct BeamArgs {

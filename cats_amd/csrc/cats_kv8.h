@@ -51,12 +51,12 @@ __device__ __forceinline__ bool kv_span(const KvSpan& s, int b, int T, int& star
 }
 
 // What differs between the two types.  HEAD: attention's weights are held as 2^HEAD times themselves: in fp16 the normal numbers reach down to 2^-29
-// of the largest weight, in bf16 2^32 values of the largest size add up within 32 bits.  SLACK: by how many powers of two weights may pass 2^HEAD's part before
-// kv8_attn_prompt_kernel scales its sums again; they start that much lower (8 against 0: a prompt of 2048 tokens 58.8 / 61.3 us, heads of 256 behind 3300 tokens
-// 70.9 / 73.7).
-// VMAX: e4m3 values become operands of the type as what they stand for, so sums have one unit, blocks and the tail alike, and weights are those of the softmax.
-// The conversion multiplies by a power of two; what is stored of an fp16 value is one of 16 bits again, but for 256 times a scale of 2^8, and every bf16 scale
-// reaches the products up to 2^73 a value.  What a scale has beyond VMAX goes into the weights of its block (kv_over).
+// of the largest weight (2^-21 with SLACK), in bf16 2^32 values of the largest size add up within 32 bits.  SLACK: by how many powers of two weights may pass
+// 2^HEAD's part before kv8_attn_prompt_kernel scales its sums again; they start that much lower (8 against 0: a prompt of 2048 tokens 58.8 / 61.3 us, heads of
+// 256 behind 3300 tokens 70.9 / 73.7).
+// VMAX: e4m3 values become operands as what they stand for, so sums have one unit, blocks and the tail alike, and weights are those of the softmax.  The
+// conversion multiplies by a power of two.  In fp16 that is exact: values are multiples of 2^-24, so are those that e4m3 keeps four bits of, and the
+// scale is 2^-32 or more; only 256 times a scale of 2^8 is too large.  In bf16 it is exact up to 2^73.  What a scale has beyond VMAX goes into the weights of its block (kv_over).
 template <class DT> struct Kv;
 template <> struct Kv<F16> {
   static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
@@ -389,7 +389,7 @@ __device__ __forceinline__ float kv_scaled(float s, float sc) {  // rounded, wha
 // 2^(HEAD + w - max w), O sums them times the values, and both are divided at the end.
 // The tail is four times sixteen tokens, for a wave each: tile `wave` of the four, and one product over sixteen tokens.
 // Bound by the cache's bytes where it is long: one row of 131072 tokens, 8 heads of 128 for 32, 43 us, 6.2 TB/s where a read stream reaches 7.1, and 4.6
-// for the join.  16 rows of 2048 to 4096 tokens take 22.8 us where the bytes take 14.5: four tiles a wave do not hide the way of the first and what
+// for the join.  16 rows of 2048 to 4096 tokens take 23.0 us where the bytes take 14.5: four tiles a wave do not hide the way of the first and what
 // the end costs.  100 tokens are the launch and three trips to memory one behind the other (positions, keys and values, the output), 6 us.
 // MASK: queries that see different keys, or a window.  One token without a window sees all of every tile but the tail.
 // SEAL: the tokens are in the tails and nowhere else yet.  One workgroup a pair more quantises the block that they complete; nobody reads that block
@@ -680,10 +680,10 @@ __global__ __launch_bounds__(256, kv_step_waves(D)) void kv8_attn_step_kernel(Kv
 //   O^T   operand of step (u, v): tokens 32 u + 16 h + 8 v .. + 7, again those whose weights the lane has
 // Rows of LDS are 16-byte pieces, exchanged within a row so that any 16 lanes in order find the 64 banks once each.
 // Workgroups with the most keys start first.
-// Bound by what a SIMD issues: a tile is 32 products a wave (1024 cycles of the matrix cores with heads of 128) and some 300 other instructions, of which 128
+// Bound by what a SIMD issues: a tile is 32 products a wave (1024 cycles of the matrix cores with heads of 128) and some 310 other instructions, of which 128
 // turn e4m3 into operands and 32 are exponentials, and the two overlap only in part (a loop of each, alone 1189 and 1169 cycles, on one SIMD 1570); a third
-// wave a SIMD, which heads of 64 have room for, is worth 2 to 6 %.  A prompt of 2048 tokens, 32 heads of 128, takes 49 us, 700 TFLOP/s of what is
-// seen; two pieces of 512 behind 7680 tokens 117 us, 890 (a large product 1125 to 1180).
+// wave a SIMD, which heads of 64 have room for, is worth 2 to 6 %.  A prompt of 2048 tokens, 32 heads of 128, takes 50 us, 690 TFLOP/s of what is
+// seen; two pieces of 512 behind 7680 tokens 118 us, 880 (a large product 1125 to 1180); other cards 51 and 123.
 // 128 rows a workgroup need the registers of one wave a SIMD and were slower.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <class DT> struct Mma32;
