@@ -69,8 +69,11 @@ def build_kernels(jobs: int = 7, timing: bool = False) -> Path:
         (CSRC / "cats_inst_kv8.hip", obj / "cats_inst_kv8_f16.o", ["-DCATS_DT=F16"]),
         (CSRC / "cats_inst_kv8.hip", obj / "cats_inst_kv8_bf16.o", ["-DCATS_DT=BF16"]),
         (CSRC / "cats_inst_kv8.hip", obj / "cats_inst_kv8_f32.o", ["-DCATS_DT=F32"]),
+        (CSRC / "cats_inst_paged.hip", obj / "cats_inst_paged_f16.o", ["-DCATS_DT=F16"]),
+        (CSRC / "cats_inst_paged.hip", obj / "cats_inst_paged_bf16.o", ["-DCATS_DT=BF16"]),
         (CSRC / "cats_api.hip", obj / "cats_api.o", []),
         (CSRC / "cats_api_cache.hip", obj / "cats_api_cache.o", []),
+        (CSRC / "cats_api_paged.hip", obj / "cats_api_paged.o", []),
     ]
     cmds = [[HIPCC, *HIP_FLAGS, *extra, *defs, "-c", str(src), "-o", str(o)] for src, o, defs in units]
     with ThreadPoolExecutor(max_workers=jobs) as pool:

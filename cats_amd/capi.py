@@ -26,7 +26,7 @@ SYMBOLS = (
     "cats_probe_read", "cats_mlp_norm_residual_norm", "cats_linear", "cats_attention_step", "cats_mlp_gate_cols", "cats_silu_mask_mul",
     "cats_prompt_scratch_bytes", "cats_prompt_mlp", "cats_prompt_plan", "cats_kv8_append", "cats_kv8_attention_scratch_bytes",
     "cats_kv8_attention", "cats_kv8_attention_step_scratch_bytes", "cats_kv8_attention_step", "cats_beam_scratch_bytes", "cats_beam_select", "cats_cache_reorder",
-    "cats_kv8_attention_plan",
+    "cats_kv8_attention_plan", "cats_paged_append", "cats_paged_attention_scratch_bytes", "cats_paged_attention", "cats_prompt_attention",
 )
 
 
@@ -91,6 +91,11 @@ def lib() -> ctypes.CDLL:
             L.cats_beam_scratch_bytes.argtypes = [i32] * 4; L.cats_beam_scratch_bytes.restype = sz
             L.cats_beam_select.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, sz, vp]; L.cats_beam_select.restype = i32
             L.cats_cache_reorder.argtypes = [vp, i32, vp, vp, i32, i32, i32, vp]; L.cats_cache_reorder.restype = i32
+        if hasattr(L, "cats_paged_append"):
+            L.cats_paged_append.argtypes = [*[vp] * 10, i32, i32, i32, vp, vp, vp, vp, i64, *[i32] * 9, vp]; L.cats_paged_append.restype = i32
+            L.cats_paged_attention_scratch_bytes.argtypes = [i32] * 9; L.cats_paged_attention_scratch_bytes.restype = sz
+            L.cats_paged_attention.argtypes = [*[vp] * 7, i64, f32, i32, i32, vp, i32, vp, *[i32] * 9, vp, sz, vp]; L.cats_paged_attention.restype = i32
+            L.cats_prompt_attention.argtypes = [*[vp] * 8, f32, i32, vp, *[i32] * 7, vp]; L.cats_prompt_attention.restype = i32
         L.cats_set_tuning.argtypes = [i32, i32, i32, i32]; L.cats_set_tuning.restype = i32
         _lib = L
     return _lib

@@ -1,0 +1,43 @@
+// The cache of pages and packed attention for one dtype.  Compiled twice (-DCATS_DT=F16 / BF16).
+#include "cats_launch_paged.h"
+
+#ifndef CATS_DT
+#error "compile with -DCATS_DT=F16|BF16"
+#endif
+
+namespace cats {
+namespace {
+
+template <class F>
+hipError_t for_head_dim(int D, F f) {
+  switch (D) {
+    case 32: return f(std::integral_constant<int, 32>());
+    case 64: return f(std::integral_constant<int, 64>());
+    case 128: return f(std::integral_constant<int, 128>());
+    case 256: return f(std::integral_constant<int, 256>());
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+template <>
+hipError_t launch_paged_append<CATS_DT>(int D, bool wide, const PagedAppendArgs& a, hipStream_t stream) {
+  return for_head_dim(D, [&](auto d) {
+    constexpr int HD = decltype(d)::value;
+    const int units = (a.heads + 2 * a.pool.heads) * (HD / 16), blocks = (units + 511) / 512, threads = ((units + blocks - 1) / blocks + 63) / 64 * 64;
+    const dim3 grid((a.seq.N + a.per - 1) / a.per, blocks);
+    return launch_kernel(wide ? paged_append_kernel<CATS_DT, HD, true> : paged_append_kernel<CATS_DT, HD, false>, grid, dim3(threads), 0, stream, a);
+  });
+}
+
+template <>
+hipError_t launch_packed_attn<CATS_DT>(int D, bool paged, const PackedAttnArgs& a, hipStream_t stream) {
+  return for_head_dim(D, [&](auto d) {
+    constexpr int HD = decltype(d)::value;
+    const dim3 grid((a.seq.N + 3) / 4, a.kv_heads * a.group);
+    return launch_kernel(paged ? packed_attn_simple_kernel<CATS_DT, HD, true> : packed_attn_simple_kernel<CATS_DT, HD, false>, grid, dim3(256), 0, stream, a);
+  });
+}
+
+}  // namespace cats

@@ -784,6 +784,170 @@ void cats_cache_reorder_op(const at::TensorList caches, const at::IntArrayRef sl
                "cats_cache_reorder");
 }
 
+// ---- a cache of pages, and packed sequences -----------------------------------------------------------------
+
+// q, k or v (N, heads, D) of packed tokens with elements of a head side by side and every head on a 16-byte boundary; anything else is copied.
+at::Tensor packed_of(const at::Tensor& t) {
+  bool fits = t.stride(2) == 1 && ((uintptr_t)t.data_ptr() & 15u) == 0;
+  for (int i = 0; i < 2; i++) fits = fits && (t.size(i) == 1 || (t.stride(i) >= 0 && t.stride(i) % 8 == 0));
+  fits = fits && (t.size(0) == 1 || t.stride(0) <= 1 << 23);
+  return fits ? t : t.contiguous();
+}
+struct PackedStrides {
+  int64_t s[2];
+  explicit PackedStrides(const at::Tensor& t) {
+    for (int i = 0; i < 2; i++) s[i] = t.size(i) == 1 ? 0 : t.stride(i);
+  }
+};
+
+void check_packed(const at::Tensor& t, const at::Tensor& like, const char* name, const char* op) {
+  TORCH_CHECK(t.is_cuda(), "flash_gemv.", op, ": ", name, " must be on the GPU");
+  TORCH_CHECK(t.dim() == 3, "flash_gemv.", op, ": ", name, " must be (N, heads, D), got ", t.sizes());
+  TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, "flash_gemv.", op, ": half or bfloat16, got ", t.scalar_type());
+  TORCH_CHECK(t.scalar_type() == like.scalar_type() && t.device() == like.device() && t.size(2) == like.size(2), "flash_gemv.", op, ": ", name,
+              " must be of one type, device and head size with the others");
+  TORCH_CHECK(t.size(2) == 32 || t.size(2) == 64 || t.size(2) == 128 || t.size(2) == 256, "flash_gemv.", op, ": heads of 32, 64, 128 or 256 elements, got ", t.size(2));
+  TORCH_CHECK(t.size(0) <= CATS_PAGED_MAX_TOKENS && t.size(1) <= 65535, "flash_gemv.", op, ": too large: ", name, " ", t.sizes());
+  check_no_grad(t, op);
+}
+
+// Device words: (n) of int64.
+const int64_t* check_words(const at::Tensor& t, const at::Tensor& like, int64_t n, const char* name, const char* op) {
+  check_dev(t, name);
+  TORCH_CHECK(t.scalar_type() == at::kLong && t.dim() == 1 && t.numel() == n && t.device() == like.device(), "flash_gemv.", op, ": ", name, " must be (", n,
+              ") of int64 on the device of the tokens, got ", t.sizes(), " of ", t.scalar_type());
+  return t.data_ptr<int64_t>();
+}
+int64_t sequences_of(const at::Tensor& offsets, const char* op) {
+  TORCH_CHECK(offsets.dim() == 1 && offsets.numel() >= 2 && offsets.numel() <= 1 << 20, "flash_gemv.", op, ": offsets must be (sequences + 1), got ", offsets.sizes());
+  return offsets.numel() - 1;
+}
+
+struct Pages {
+  int64_t kv_heads, page, pages, width, stride;
+};
+Pages check_pages(const at::Tensor& like, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table, int64_t B, const char* op) {
+  TORCH_CHECK(k_pages.dim() == 4, "flash_gemv.", op, ": k_pages must be (pages, kv_heads, page, D), got ", k_pages.sizes());
+  for (const at::Tensor* t : {&k_pages, &v_pages}) {
+    check_dev(*t, "the pages");
+    TORCH_CHECK(t->sizes() == k_pages.sizes() && t->scalar_type() == like.scalar_type() && t->device() == like.device() && t->size(3) == like.size(2), "flash_gemv.",
+                op, ": k_pages and v_pages must be alike, (pages, kv_heads, page, D) in the type and on the device of the tokens");
+  }
+  TORCH_CHECK(table.is_cuda() && table.device() == like.device() && table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == B &&
+                  table.size(1) >= 1 && (table.size(1) == 1 || table.stride(1) == 1) && (B == 1 || table.stride(0) >= 0),
+              "flash_gemv.", op, ": table must be (", B, ", entries) of int32 on the device of the tokens, a row's entries side by side");
+  const Pages p = {k_pages.size(1), k_pages.size(2), k_pages.size(0), table.size(1), B == 1 ? 0 : table.stride(0)};
+  TORCH_CHECK(p.page >= 16 && p.page <= 1024 && (p.page & (p.page - 1)) == 0, "flash_gemv.", op, ": pages of 16 to 1024 tokens, a power of two, got ", p.page);
+  TORCH_CHECK(p.pages >= 1 && p.kv_heads >= 1 && p.kv_heads <= 65535 && p.pages <= INT_MAX / p.kv_heads && p.width <= (1 << 30) / p.page, "flash_gemv.", op,
+              ": too large, or no pages: ", k_pages.sizes(), ", ", p.width, " entries");
+  return p;
+}
+
+at::Tensor cats_paged_append_op(const c10::optional<at::Tensor>& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, const at::Tensor& start,
+                                const c10::optional<at::Tensor>& cos_table, const c10::optional<at::Tensor>& sin_table, at::Tensor& k_pages,
+                                at::Tensor& v_pages, const at::Tensor& table) {
+  const char* op = "cats_paged_append";
+  check_packed(k, k, "k", op);
+  check_packed(v, k, "v", op);
+  TORCH_CHECK(v.sizes() == k.sizes(), "flash_gemv.cats_paged_append: k and v must be alike, got ", k.sizes(), " and ", v.sizes());
+  const bool with_q = q.has_value() && q->defined();
+  if (with_q) {
+    check_packed(*q, k, "q", op);
+    TORCH_CHECK(q->size(0) == k.size(0), "flash_gemv.cats_paged_append: q must have as many tokens as k, got ", q->size(0), " and ", k.size(0));
+  }
+  const int64_t B = sequences_of(offsets, op);
+  const int64_t* op_ = check_words(offsets, k, B + 1, "offsets", op);
+  const int64_t* sp = check_words(start, k, B, "start", op);
+  const Pages p = check_pages(k, k_pages, v_pages, table, B, op);
+  TORCH_CHECK(k.size(1) == p.kv_heads, "flash_gemv.cats_paged_append: ", k.size(1), " heads of keys for pages of ", p.kv_heads);
+  int64_t rot = 0, positions = 0;
+  const bool turn = cos_table.has_value() && cos_table->defined();
+  TORCH_CHECK(turn == (sin_table.has_value() && sin_table->defined()), "flash_gemv.cats_paged_append: both rotary tables or none");
+  if (turn) {
+    for (const at::Tensor* t : {&*cos_table, &*sin_table}) {
+      check_dev(*t, "a rotary table");
+      TORCH_CHECK(t->dim() == 2 && t->sizes() == cos_table->sizes() && t->scalar_type() == cos_table->scalar_type() && t->device() == k.device() &&
+                      (t->scalar_type() == at::kFloat || t->scalar_type() == k.scalar_type()),
+                  "flash_gemv.cats_paged_append: the rotary tables must be alike, (positions, elements) in float or the type of the tokens, on their device");
+    }
+    positions = cos_table->size(0), rot = cos_table->size(1);
+    TORCH_CHECK(positions >= 1 && positions <= INT_MAX && rot >= 16 && rot <= k.size(2) && rot % 16 == 0,
+                "flash_gemv.cats_paged_append: a multiple of 16 elements of a head may be rotated, got ", cos_table->sizes());
+  }
+  const c10::DeviceGuard guard(k.device());
+  at::Tensor out = with_q ? at::empty(q->sizes(), q->options()) : at::empty({0}, k.options());
+  if (k.size(0) == 0) return out;
+  const int64_t heads = with_q ? q->size(1) : 0;
+  at::Tensor qq;
+  if (heads) qq = packed_of(*q);
+  const at::Tensor kk = packed_of(k), vv = packed_of(v);
+  const PackedStrides qs(heads ? qq : kk);
+  check_status(cats_paged_append(heads ? qq.data_ptr() : nullptr, qs.s, kk.data_ptr(), PackedStrides(kk).s, vv.data_ptr(), PackedStrides(vv).s, op_, sp,
+                                 turn ? cos_table->data_ptr() : nullptr, turn ? sin_table->data_ptr() : nullptr, (int)rot, (int)positions,
+                                 turn ? dtype_code(*cos_table) : CATS_F32, heads ? out.data_ptr() : nullptr, k_pages.data_ptr(), v_pages.data_ptr(),
+                                 table.data_ptr<int32_t>(), p.stride, (int)k.size(0), (int)B, (int)heads, (int)p.kv_heads, (int)k.size(2), (int)p.page,
+                                 (int)p.pages, (int)p.width, dtype_code(k), current_stream(k)),
+               op);
+  return out;
+}
+
+at::Tensor cats_paged_attention_op(const at::Tensor& q, const at::Tensor& offsets, const at::Tensor& start, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                                   const at::Tensor& table, const double scale, const int64_t window, const int64_t group,
+                                   const c10::optional<at::Tensor>& shared) {
+  const char* op = "cats_paged_attention";
+  check_packed(q, q, "q", op);
+  const int64_t B = sequences_of(offsets, op), N = q.size(0), heads = q.size(1);
+  const int64_t* op_ = check_words(offsets, q, B + 1, "offsets", op);
+  const int64_t* sp = check_words(start, q, B, "start", op);
+  const Pages p = check_pages(q, k_pages, v_pages, table, B, op);
+  TORCH_CHECK(heads % p.kv_heads == 0, "flash_gemv.cats_paged_attention: ", heads, " query heads over ", p.kv_heads, " cached heads");
+  TORCH_CHECK(window >= 0 && window <= INT_MAX, "flash_gemv.cats_paged_attention: window must be 0 (all keys) or a number of keys");
+  TORCH_CHECK(group >= 1 && B % group == 0, "flash_gemv.cats_paged_attention: ", B, " sequences in groups of ", group);
+  const bool share = shared.has_value() && shared->defined();
+  TORCH_CHECK(!share || shared->numel() == 1 || shared->numel() == B / group, "flash_gemv.cats_paged_attention: shared must be one int64 or one for each of the ",
+              B / group, " groups");
+  const int64_t* hp = share ? check_words(*shared, q, shared->numel(), "shared", op) : nullptr;
+  const c10::DeviceGuard guard(q.device());
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  if (q.numel() == 0) return out;
+  const at::Tensor qq = packed_of(q);
+  const int members = share ? (int)group : 1;
+  const size_t bytes = cats_paged_attention_scratch_bytes((int)N, (int)B, (int)heads, (int)p.kv_heads, (int)q.size(2), (int)p.page, (int)p.width, (int)window, members);
+  at::Tensor scratch;
+  if (bytes) scratch = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  check_status(cats_paged_attention(qq.data_ptr(), PackedStrides(qq).s, op_, sp, k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr<int32_t>(), p.stride,
+                                    (float)scale, (int)window, members, hp, share && shared->numel() > 1 ? 1 : 0, out.data_ptr(), (int)N, (int)B, (int)heads,
+                                    (int)p.kv_heads, (int)q.size(2), (int)p.page, (int)p.pages, (int)p.width, dtype_code(q), bytes ? scratch.data_ptr() : nullptr,
+                                    bytes, current_stream(q)),
+               op);
+  return out;
+}
+
+at::Tensor cats_prompt_attention_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, const double scale,
+                                    const int64_t window, const c10::optional<at::Tensor>& k_offsets) {
+  const char* op = "cats_prompt_attention";
+  check_packed(q, q, "q", op);
+  check_packed(k, q, "k", op);
+  check_packed(v, q, "v", op);
+  const int64_t B = sequences_of(offsets, op), N = q.size(0), M = k.size(0), heads = q.size(1), kv = k.size(1);
+  TORCH_CHECK(v.sizes() == k.sizes(), "flash_gemv.cats_prompt_attention: k and v must be alike, got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK(kv >= 1 && heads % kv == 0, "flash_gemv.cats_prompt_attention: ", heads, " query heads over ", kv, " heads of keys");
+  TORCH_CHECK(window >= 0 && window <= INT_MAX, "flash_gemv.cats_prompt_attention: window must be 0 (all keys) or a number of keys");
+  const int64_t* op_ = check_words(offsets, q, B + 1, "offsets", op);
+  const bool own = k_offsets.has_value() && k_offsets->defined();
+  const int64_t* kp = own ? check_words(*k_offsets, q, B + 1, "k_offsets", op) : nullptr;
+  TORCH_CHECK(own || M == N, "flash_gemv.cats_prompt_attention: ", M, " keys for ", N, " queries need k_offsets");
+  const c10::DeviceGuard guard(q.device());
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  if (q.numel() == 0) return out;
+  if (M == 0) return out.zero_();
+  const at::Tensor qq = packed_of(q), kk = packed_of(k), vv = packed_of(v);
+  check_status(cats_prompt_attention(qq.data_ptr(), PackedStrides(qq).s, kk.data_ptr(), PackedStrides(kk).s, vv.data_ptr(), PackedStrides(vv).s, op_, kp, (float)scale,
+                                     (int)window, out.data_ptr(), (int)N, (int)M, (int)B, (int)heads, (int)kv, (int)q.size(2), dtype_code(q), current_stream(q)),
+               op);
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(flash_gemv, m) {
@@ -826,4 +990,9 @@ TORCH_LIBRARY(flash_gemv, m) {
         "Tensor position) -> Tensor", cats_kv8_attention_step_op);
   m.def("cats_beam_select", cats_beam_select_op);
   m.def("cats_cache_reorder(Tensor(a!)[] caches, int[] slots, Tensor parents, Tensor? lengths) -> ()", cats_cache_reorder_op);
+  // a cache of pages, packed sequences
+  m.def("cats_paged_append(Tensor? q, Tensor k, Tensor v, Tensor offsets, Tensor start, Tensor? cos_table, Tensor? sin_table, Tensor(a!) k_pages, "
+        "Tensor(b!) v_pages, Tensor table) -> Tensor", cats_paged_append_op);
+  m.def("cats_paged_attention", cats_paged_attention_op);
+  m.def("cats_prompt_attention", cats_prompt_attention_op);
 }

@@ -183,6 +183,36 @@ def cats_cache_reorder(caches, slots, parents, lengths=None):
     torch.ops.flash_gemv.cats_cache_reorder(caches, slots, parents, lengths)
 
 
+def cats_paged_append(q, k, v, offsets, start, cos_table, sin_table, k_pages, v_pages, table):
+    """Rotate new tokens' queries and keys at their positions and store keys and values in pages (``cats_amd.paged.PagedCache`` holds a pool of them).
+
+    Tokens are packed: q (N, heads, D) or None, k, v (N, kv_heads, D) half or bfloat16, any strides; sequence s has the tokens ``offsets[s]`` to
+    ``offsets[s + 1] - 1``, at the positions ``start[s]`` onwards (int64 on the GPU, (B + 1) and (B)).  cos_table, sin_table (positions, R) in float or in the type of
+    the tokens: the first R elements of a head are rotated (rotate-half); None: none.  k_pages, v_pages (pages, kv_heads, page, D), page a power of
+    two from 16 to 1024; table (B, entries) int32: position p of sequence s lies in page ``table[s, p // page]``.
+    Returns the queries, rotated (None for None).  A token that has no page or no row of the tables is not stored, and its query is NaN.  No two tokens of a
+    call may have one place.  No gradient: tensors that record one are refused."""
+    out = torch.ops.flash_gemv.cats_paged_append(q, k, v, offsets, start, cos_table, sin_table, k_pages, v_pages, table)
+    return out if q is not None else None
+
+
+def cats_paged_attention(q, offsets, start, k_pages, v_pages, table, scale, window=0, group=1, shared=None):
+    """Causal attention of packed tokens that cats_paged_append has stored: q (N, heads, D), heads a multiple of the pages', over the positions up to each
+    token's own, at most ``window`` of them (0: all); ``scale`` lies in 2^-64 .. 2^64.
+
+    shared (int64 on the GPU, one or one a group): each ``group`` sequences in order have the same first ``shared`` tokens, which are read once for all of
+    them, through the first one's row of the table.  Returns (N, heads, D); tokens that no sequence has are zeros, and one that sees a page that is none is
+    NaN.  Serving only: no gradient, and a q that records one is refused."""
+    return torch.ops.flash_gemv.cats_paged_attention(q, offsets, start, k_pages, v_pages, table, scale, window, group, shared)
+
+
+def cats_prompt_attention(q, k, v, offsets, scale, window=0, k_offsets=None):
+    """Causal attention over whole prompts, packed: q (N, heads, D), k, v (M, kv_heads, D), any strides; sequence s has the queries ``offsets[s]`` to
+    ``offsets[s + 1] - 1`` and the keys of the same places, or those of ``k_offsets``, of which its queries are the last.  A query sees the keys up to its own,
+    at most ``window`` of them (0: all); one that sees none is zeros.  Returns (N, heads, D).  Serving only: no gradient, and tensors that record one are refused."""
+    return torch.ops.flash_gemv.cats_prompt_attention(q, k, v, offsets, scale, window, k_offsets)
+
+
 __all__ = [
     "fuse_gemv_cmp",
     "fuse_gemv_flag",
@@ -214,4 +244,7 @@ __all__ = [
     "cats_kv8_attention",
     "cats_beam_select",
     "cats_cache_reorder",
+    "cats_paged_append",
+    "cats_paged_attention",
+    "cats_prompt_attention",
 ]

@@ -293,6 +293,46 @@ int cats_kv8_attention_step(const void* h, const void* x, const void* norm_weigh
                             const void* sin_table, const int64_t* position, void* out, int B, int H, int heads, int blocks, int max_len, int dtype,
                             void* scratch, size_t scratch_bytes, void* stream);
 
+/* ---- a cache of pages, and packed sequences (fp16 / bf16 models) ----
+ * A pool of pages, k_pages and v_pages (pages, kv_heads, page, D) in dtype; page: tokens of a page, a power of two from 16 to 1024.  Token p of sequence s
+ * lies in page table[s * table_stride + p / page], place p % page, of the pool.  The table has `width` entries a sequence that are read, and only those of pages
+ * that a call needs: the others may be anything.
+ * Tokens of a call are packed: sequence s of B has the tokens offsets[s] .. offsets[s + 1] - 1 (none, one or many) of the N tokens of q, k, v and out, at the positions
+ * start[s] onwards.  offsets (B + 1) ascend within 0 .. N; tokens before the first and behind the last belong to nobody.  offsets, start, table and shared
+ * are read on the device, so a captured call follows them.  D is 32, 64, 128 or 256.  Strides of q, k and v: of a token and of a head, in elements,
+ * multiples of 8; the elements of a head side by side, 16-byte aligned.  All calls may be captured; nothing is kept between calls. */
+#define CATS_PAGED_MAX_TOKENS (1 << 24)
+
+/* Stores new tokens, rotated on the way:  x' = x cos[p] + (-x[R/2 .. R-1], x[0 .. R/2-1]) sin[p]  over the first R = rot elements of the heads of q and k, p the
+ * token's position, in 32 bits and rounded once; the others, and v, as they are.  cos, sin (positions, rot) in float or in dtype (table_dtype), rot a multiple of 16
+ * up to D; rot 0: no rotation, cos and sin are not read.  q, q_out (N, heads, D, contiguous) NULL with heads 0: keys and values only.  A token whose position
+ * lies outside the rotary tables or the table's entries, or whose entry is no page, is not stored, and its q_out is NaN; q_out of tokens that are nobody's is zeros.  No two tokens of a call may
+ * have one place.  q_out may be q where q is contiguous. */
+int cats_paged_append(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                      const int64_t* offsets, const int64_t* start, const void* cos_table, const void* sin_table, int rot, int positions,
+                      int table_dtype, void* q_out, void* k_pages, void* v_pages, const int32_t* table, int64_t table_stride, int N, int B, int heads,
+                      int kv_heads, int D, int page, int pages, int width, int dtype, void* stream);
+
+/* out[t, h] = softmax(scale * q[t, h] . K^T) . V over the keys at positions p - window + 1 .. p (window 0: 0 .. p), p = start[s] + t - offsets[s], of
+ * cached head h / (heads / kv_heads) of the token's sequence s; the new tokens have been stored.  group > 1 (B is a multiple of it): each `group` sequences in order have the same
+ * first shared[s / group] (shared_step 1) or shared[0] (shared_step 0) tokens, which are read for all of them through the first one's table (up to start[s] of them for sequence s).
+ * A sequence whose tokens do not lie within its table's entries is NaN, and so is a query that sees a token whose entry is no page; rows that are nobody's are zeros.  A query that
+ * sees a NaN in a key, or a value that is not finite, is not finite (in that element); a score of -infinity weighs nothing.  out (N, heads, D), 16-byte aligned.  scale lies in 2^-64 .. 2^64, and scores have to be within 32-bit floats.
+ * Weights are rounded to dtype (their sum is not).  scratch: 16-byte aligned, at least cats_paged_attention_scratch_bytes() on the device of the call (which may be 0), nothing
+ * in it needs to be set. */
+size_t cats_paged_attention_scratch_bytes(int N, int B, int heads, int kv_heads, int D, int page, int width, int window, int group);
+int cats_paged_attention(const void* q, const int64_t* q_strides, const int64_t* offsets, const int64_t* start, const void* k_pages, const void* v_pages,
+                         const int32_t* table, int64_t table_stride, float scale, int window, int group, const int64_t* shared, int shared_step,
+                         void* out, int N, int B, int heads, int kv_heads, int D, int page, int pages, int width, int dtype, void* scratch,
+                         size_t scratch_bytes, void* stream);
+
+/* The same over keys and values of the call itself, k and v (M, kv_heads, D): sequence s has the keys k_offsets[s] .. k_offsets[s + 1] - 1, and its queries are its
+ * last tokens, so that query i of n sees the keys up to i + keys - n.  k_offsets NULL: offsets (M is N), the whole prompt.  A query that sees no key is zeros.
+ * M is at least 1. */
+int cats_prompt_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                          const int64_t* offsets, const int64_t* k_offsets, float scale, int window, void* out, int N, int M, int B, int heads,
+                          int kv_heads, int D, int dtype, void* stream);
+
 /* ---- beam search ---- */
 #define CATS_MAX_BEAMS 16
 
