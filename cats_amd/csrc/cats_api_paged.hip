@@ -9,8 +9,8 @@ namespace cats {
 
 template <> hipError_t launch_paged_append<F16>(int, bool, const PagedAppendArgs&, hipStream_t);
 template <> hipError_t launch_paged_append<BF16>(int, bool, const PagedAppendArgs&, hipStream_t);
-template <> hipError_t launch_packed_attn<F16>(int, bool, const PackedAttnArgs&, hipStream_t);
-template <> hipError_t launch_packed_attn<BF16>(int, bool, const PackedAttnArgs&, hipStream_t);
+template <> hipError_t launch_packed_attn<F16>(int, bool, PackedAttnArgs, hipStream_t);
+template <> hipError_t launch_packed_attn<BF16>(int, bool, PackedAttnArgs, hipStream_t);
 
 namespace {
 
@@ -49,6 +49,12 @@ int fill_pool(Pool& pool, const void* k_pages, const void* v_pages, const int32_
   pool = {(uint16_t*)k_pages, (uint16_t*)v_pages, table, table_stride, kv_heads, __builtin_ctz((unsigned)page), pages, width};
   return CATS_OK;
 }
+
+// A window that no sequence exceeds is none.
+int window_of(int window) { return window >= 1 << 30 ? 0 : window; }
+
+// Workgroups of a launch, whose threads have to be fewer than 2^32.
+bool grid_ok(int N, int B, int heads, int kv_heads) { return (long long)N * heads / 16 + (B + 2ll) * kv_heads < 1 << 24; }
 
 bool scale_ok(float scale) { return scale >= 0x1p-64f && scale <= 0x1p64f; }
 
@@ -108,7 +114,7 @@ int cats_paged_attention(const void* q, const int64_t* q_strides, const int64_t*
                          size_t scratch_bytes, void* stream) {
   if (int st = check_packed(N, B, heads, kv_heads, D, dtype)) return st;
   if (int st = check_pool(page, pages, width, kv_heads)) return st;
-  if (heads < kv_heads || heads % kv_heads != 0 || window < 0 || !scale_ok(scale)) return CATS_ERR_SHAPE;
+  if (heads < kv_heads || heads % kv_heads != 0 || window < 0 || !scale_ok(scale) || !grid_ok(N, B, heads, kv_heads)) return CATS_ERR_SHAPE;
   if (group < 1 || B % group != 0 || (shared_step != 0 && shared_step != 1)) return CATS_ERR_SHAPE;
   if (int st = check_strides(q, q_strides)) return st;
   if (int st = check_words(offsets)) return st;
@@ -130,7 +136,7 @@ int cats_paged_attention(const void* q, const int64_t* q_strides, const int64_t*
   a.scale = 1.44269504088896341f * scale;
   a.kv_heads = kv_heads;
   a.group = heads / kv_heads;
-  a.window = window;
+  a.window = window_of(window);
   const hipError_t e = dtype == CATS_F16 ? launch_packed_attn<F16>(D, true, a, (hipStream_t)stream) : launch_packed_attn<BF16>(D, true, a, (hipStream_t)stream);
   return e == hipSuccess ? CATS_OK : CATS_ERR_LAUNCH;
 }
@@ -140,7 +146,7 @@ int cats_prompt_attention(const void* q, const int64_t* q_strides, const void* k
                           int kv_heads, int D, int dtype, void* stream) {
   if (int st = check_packed(N, B, heads, kv_heads, D, dtype)) return st;
   if (M < 1 || M > CATS_PAGED_MAX_TOKENS || (!k_offsets && M != N)) return CATS_ERR_SHAPE;
-  if (heads < kv_heads || heads % kv_heads != 0 || window < 0 || !scale_ok(scale)) return CATS_ERR_SHAPE;
+  if (heads < kv_heads || heads % kv_heads != 0 || window < 0 || !scale_ok(scale) || !grid_ok(N, B, heads, kv_heads)) return CATS_ERR_SHAPE;
   if (int st = check_strides(q, q_strides)) return st;
   if (int st = check_strides(k, k_strides)) return st;
   if (int st = check_strides(v, v_strides)) return st;
@@ -160,7 +166,7 @@ int cats_prompt_attention(const void* q, const int64_t* q_strides, const void* k
   a.scale = 1.44269504088896341f * scale;
   a.kv_heads = kv_heads;
   a.group = heads / kv_heads;
-  a.window = window;
+  a.window = window_of(window);
   const hipError_t e = dtype == CATS_F16 ? launch_packed_attn<F16>(D, false, a, (hipStream_t)stream) : launch_packed_attn<BF16>(D, false, a, (hipStream_t)stream);
   return e == hipSuccess ? CATS_OK : CATS_ERR_LAUNCH;
 }

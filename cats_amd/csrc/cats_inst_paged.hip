@@ -32,11 +32,12 @@ hipError_t launch_paged_append<CATS_DT>(int D, bool wide, const PagedAppendArgs&
 }
 
 template <>
-hipError_t launch_packed_attn<CATS_DT>(int D, bool paged, const PackedAttnArgs& a, hipStream_t stream) {
+hipError_t launch_packed_attn<CATS_DT>(int D, bool paged, PackedAttnArgs a, hipStream_t stream) {
   return for_head_dim(D, [&](auto d) {
     constexpr int HD = decltype(d)::value;
-    const dim3 grid((a.seq.N + 3) / 4, a.kv_heads * a.group);
-    return launch_kernel(paged ? packed_attn_simple_kernel<CATS_DT, HD, true> : packed_attn_simple_kernel<CATS_DT, HD, false>, grid, dim3(256), 0, stream, a);
+    a.slots = packed_slots(a.seq.N, a.seq.B + 2, a.group, kTileRows);
+    return launch_kernel(paged ? packed_attn_tiles_kernel<CATS_DT, HD, true> : packed_attn_tiles_kernel<CATS_DT, HD, false>, dim3(a.slots * a.kv_heads), dim3(256), 0,
+                         stream, a);
   });
 }
 

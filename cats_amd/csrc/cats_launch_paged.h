@@ -2,13 +2,13 @@
 // per dtype).
 #pragma once
 #include "cats_launch.h"
-#include "cats_paged.h"
+#include "cats_packed.h"
 
 namespace cats {
 
 template <class DT>
 hipError_t launch_paged_append(int D, bool wide, const PagedAppendArgs& a, hipStream_t stream);
 template <class DT>
-hipError_t launch_packed_attn(int D, bool paged, const PackedAttnArgs& a, hipStream_t stream);
+hipError_t launch_packed_attn(int D, bool paged, PackedAttnArgs a, hipStream_t stream);
 
 }  // namespace cats

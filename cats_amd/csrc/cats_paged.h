@@ -149,90 +149,4 @@ __global__ __launch_bounds__(512) void paged_append_kernel(PagedAppendArgs p) {
   }
 }
 
-// ---- attention ---------------------------------------------------------------------------------------------------------------------
-
-struct PackedAttnArgs {
-  const uint16_t* q;  // (N, heads, D) in elements: strides of a token and a head
-  long long q_tok, q_head;
-  uint16_t* out;      // (N, heads, D)
-  Packed seq;
-  // pages
-  const int64_t* start;
-  Pool pool;
-  const int64_t* shared;
-  int shared_step, members;  // sequences of a group
-  // or keys and values of the call
-  const uint16_t* k;  // (M, kv_heads, D)
-  const uint16_t* v;
-  long long k_tok, k_head, v_tok, v_head;
-  Packed keys;
-  float scale;        // log2(e) * the softmax's scale
-  int kv_heads, group;  // group: query heads of a cached head
-  int window;         // keys that a query sees, at most; 0: all
-};
-
-// A wave a token and head, a lane a key.
-template <class DT, int D, bool PAGED>
-__global__ __launch_bounds__(256) void packed_attn_simple_kernel(PackedAttnArgs p) {
-  const int lane = threadIdx.x % kWave, t = blockIdx.x * 4 + threadIdx.x / kWave, head = blockIdx.y, c = head / p.group;
-  if (t >= p.seq.N) return;
-  const int s = packed_row(p.seq, t);
-  uint16_t* out = p.out + ((long long)t * p.kv_heads * p.group + head) * D;
-  auto fill = [&](float x) {
-    for (int d = lane; d < D; d += kWave) out[d] = DT::fromf(x);
-  };
-  if (s < 0) return fill(0.f);
-  const int first_token = packed_at(p.seq, s), n = packed_at(p.seq, s + 1) - first_token;
-  long long pos, key0 = 0, lim = 0;
-  if constexpr (PAGED) {
-    const long long start = p.start[s];
-    if (start < 0 || start > ((long long)p.pool.width << p.pool.page_log) - n) return fill(NAN);
-    pos = start + t - first_token;
-    if (p.shared) lim = max(0ll, min(start, (long long)p.shared[s / p.members * p.shared_step]));
-  } else {
-    key0 = packed_at(p.keys, s);
-    pos = packed_at(p.keys, s + 1) - key0 - n + t - first_token;
-  }
-  if (pos < 0) return fill(0.f);
-  const long long first = p.window ? max(0ll, pos - p.window + 1) : 0;
-  const uint16_t* q = p.q + t * p.q_tok + head * p.q_head;
-  float top = -FLT_MAX, sum = 0.f, o[(D + 63) / 64] = {};
-  bool bad = false;
-  for (long long j0 = first; j0 <= pos; j0 += kWave) {
-    const long long j = min(j0 + lane, pos);
-    const uint16_t *k, *v;
-    if constexpr (PAGED) {
-      const long long owner = j < lim ? s / p.members * p.members : s;
-      int page = p.pool.table[owner * p.pool.table_stride + (j >> p.pool.page_log)];
-      if (page < 0 || page >= p.pool.pages) bad = true, page = 0;
-      const long long at = ((((long long)page * p.pool.heads + c) << p.pool.page_log) + (j & ((1 << p.pool.page_log) - 1))) * D;
-      k = p.pool.k + at, v = p.pool.v + at;
-    } else {
-      k = p.k + (key0 + j) * p.k_tok + c * p.k_head, v = p.v + (key0 + j) * p.v_tok + c * p.v_head;
-    }
-    float x = 0.f;
-    for (int d = 0; d < D; d += 8) x = DT::dot(*(const u32x4*)(q + d), *(const u32x4*)(k + d), x);
-    x = j0 + lane <= pos ? x * p.scale : -INFINITY;
-    float most = x;
-    for (int i = 1; i < kWave; i <<= 1) most = fmaxf(most, __shfl_xor(most, i, kWave));
-    const float now = fmaxf(top, most), keep = __builtin_amdgcn_exp2f(top - now), w = __builtin_amdgcn_exp2f(x - now);
-    sum = sum * keep + wave_sum(w);
-    top = now;
-#pragma unroll
-    for (int i = 0; i < (D + 63) / 64; i++) o[i] *= keep;
-    const int live = (int)min(64ll, pos - j0 + 1);
-    for (int i = 0; i < live; i++) {
-      const float wi = __shfl(w, i, kWave);
-      const uint16_t* vi = (const uint16_t*)__shfl((unsigned long long)v, i, kWave);
-#pragma unroll
-      for (int e = 0; e < (D + 63) / 64; e++)
-        if (64 * e + lane < D) o[e] = fmaf(wi, DT::tof(vi[64 * e + lane]), o[e]);
-    }
-  }
-  if (__any(bad)) return fill(NAN);
-#pragma unroll
-  for (int e = 0; e < (D + 63) / 64; e++)
-    if (64 * e + lane < D) out[64 * e + lane] = DT::fromf(o[e] / sum);
-}
-
 }  // namespace cats
