@@ -9,8 +9,8 @@ namespace cats {
 
 template <> hipError_t launch_paged_append<F16>(int, bool, const PagedAppendArgs&, hipStream_t);
 template <> hipError_t launch_paged_append<BF16>(int, bool, const PagedAppendArgs&, hipStream_t);
-template <> hipError_t launch_packed_attn<F16>(int, bool, PackedAttnArgs, hipStream_t);
-template <> hipError_t launch_packed_attn<BF16>(int, bool, PackedAttnArgs, hipStream_t);
+template <> hipError_t launch_packed_attn<F16>(int, const PackedPlan*, PackedAttnArgs, hipStream_t);
+template <> hipError_t launch_packed_attn<BF16>(int, const PackedPlan*, PackedAttnArgs, hipStream_t);
 
 namespace {
 
@@ -55,6 +55,28 @@ int window_of(int window) { return window >= 1 << 30 ? 0 : window; }
 
 // Workgroups of a launch, whose threads have to be fewer than 2^32.
 bool grid_ok(int N, int B, int heads, int kv_heads) { return (long long)N * heads / 16 + (B + 2ll) * kv_heads < 1 << 24; }
+
+PackedPlan paged_plan(int N, int B, int heads, int kv_heads, int page, int width, int window, int members) {
+  const int cus = current_device_cus(), group = heads / kv_heads;
+  const long long room = (long long)width * page, keys = window ? (room < window + 64ll ? room : window + 64ll) : room;
+  const long long rows = ((long long)N * group + B - 1) / B;  // of a sequence, on average
+  const long long many = (long long)kv_heads * (((long long)N * group + kTileRows - 1) / kTileRows);
+  PackedPlan plan = {rows <= 16 || many < cus, 1, members > 1 ? 1 : 0};
+  if (!plan.step) return {false, 1, 0};
+  auto splits = [&](long long sets, long long set_rows) {
+    const long long groups = kv_heads * sets * ((set_rows + kStepBlock - 1) / kStepBlock), want = (2ll * cus + groups - 1) / groups;
+    const long long units = keys / (set_rows <= 16 ? 128 : 64);
+    return (int)(keys <= 1024 ? 1 : want < units ? want : units);
+  };
+  plan.splits = splits(B, rows);
+  if (members > 1) plan.group_splits = splits(B / members, rows * members);
+  return plan;
+}
+// What the splits leave, for the join.
+size_t paged_bytes(const PackedPlan& plan, int N, int heads, int D) {
+  const int n = plan.splits + plan.group_splits;
+  return n == 1 ? 0 : (size_t)N * heads * n * (D + 2) * sizeof(float);
+}
 
 bool scale_ok(float scale) { return scale >= 0x1p-64f && scale <= 0x1p64f; }
 
@@ -106,7 +128,12 @@ int cats_paged_append(const void* q, const int64_t* q_strides, const void* k, co
   return e == hipSuccess ? CATS_OK : CATS_ERR_LAUNCH;
 }
 
-size_t cats_paged_attention_scratch_bytes(int N, int B, int heads, int kv_heads, int D, int page, int width, int window, int group) { return 0; }
+size_t cats_paged_attention_scratch_bytes(int N, int B, int heads, int kv_heads, int D, int page, int width, int window, int group) {
+  if (check_packed(N, B, heads, kv_heads, D, CATS_F16) || check_pool(page, 1, width, kv_heads) || heads < kv_heads || heads % kv_heads != 0 || window < 0 || group < 1 ||
+      B % group != 0)
+    return 0;
+  return paged_bytes(paged_plan(N, B, heads, kv_heads, page, width, window_of(window), group), N, heads, D);
+}
 
 int cats_paged_attention(const void* q, const int64_t* q_strides, const int64_t* offsets, const int64_t* start, const void* k_pages, const void* v_pages,
                          const int32_t* table, int64_t table_stride, float scale, int window, int group, const int64_t* shared, int shared_step,
@@ -137,7 +164,11 @@ int cats_paged_attention(const void* q, const int64_t* q_strides, const int64_t*
   a.kv_heads = kv_heads;
   a.group = heads / kv_heads;
   a.window = window_of(window);
-  const hipError_t e = dtype == CATS_F16 ? launch_packed_attn<F16>(D, true, a, (hipStream_t)stream) : launch_packed_attn<BF16>(D, true, a, (hipStream_t)stream);
+  const PackedPlan plan = paged_plan(N, B, heads, kv_heads, page, width, a.window, group);
+  const size_t bytes = paged_bytes(plan, N, heads, D);
+  if (bytes && (!scratch || !aligned(scratch, 16) || scratch_bytes < bytes)) return CATS_ERR_WORKSPACE;
+  a.part = (float*)scratch;
+  const hipError_t e = dtype == CATS_F16 ? launch_packed_attn<F16>(D, &plan, a, (hipStream_t)stream) : launch_packed_attn<BF16>(D, &plan, a, (hipStream_t)stream);
   return e == hipSuccess ? CATS_OK : CATS_ERR_LAUNCH;
 }
 
@@ -167,7 +198,7 @@ int cats_prompt_attention(const void* q, const int64_t* q_strides, const void* k
   a.kv_heads = kv_heads;
   a.group = heads / kv_heads;
   a.window = window_of(window);
-  const hipError_t e = dtype == CATS_F16 ? launch_packed_attn<F16>(D, false, a, (hipStream_t)stream) : launch_packed_attn<BF16>(D, false, a, (hipStream_t)stream);
+  const hipError_t e = dtype == CATS_F16 ? launch_packed_attn<F16>(D, nullptr, a, (hipStream_t)stream) : launch_packed_attn<BF16>(D, nullptr, a, (hipStream_t)stream);
   return e == hipSuccess ? CATS_OK : CATS_ERR_LAUNCH;
 }
 

@@ -32,12 +32,21 @@ hipError_t launch_paged_append<CATS_DT>(int D, bool wide, const PagedAppendArgs&
 }
 
 template <>
-hipError_t launch_packed_attn<CATS_DT>(int D, bool paged, PackedAttnArgs a, hipStream_t stream) {
+hipError_t launch_packed_attn<CATS_DT>(int D, const PackedPlan* plan, PackedAttnArgs a, hipStream_t stream) {
   return for_head_dim(D, [&](auto d) {
     constexpr int HD = decltype(d)::value;
-    a.slots = packed_slots(a.seq.N, a.seq.B + 2, a.group, kTileRows);
-    return launch_kernel(paged ? packed_attn_tiles_kernel<CATS_DT, HD, true> : packed_attn_tiles_kernel<CATS_DT, HD, false>, dim3(a.slots * a.kv_heads), dim3(256), 0,
-                         stream, a);
+    if (!plan || !plan->step) {
+      a.slots = packed_slots(a.seq.N, a.seq.B + 2, a.group, kTileRows);
+      return launch_kernel(plan ? packed_attn_tiles_kernel<CATS_DT, HD, true> : packed_attn_tiles_kernel<CATS_DT, HD, false>, dim3(a.slots * a.kv_heads), dim3(256), 0,
+                           stream, a);
+    }
+    a.splits = plan->splits;
+    a.group_splits = plan->group_splits;
+    a.slots = packed_slots(a.seq.N, a.seq.B + 2, a.group, kStepBlock);
+    a.group_slots = a.group_splits ? packed_slots(a.seq.N, a.seq.B / a.members + 2, a.group, kStepBlock) : 0;
+    hipError_t e = launch_kernel(packed_attn_step_kernel<CATS_DT, HD>, dim3((a.slots * a.splits + a.group_slots * a.group_splits) * a.kv_heads), dim3(256), 0, stream, a);
+    if (e != hipSuccess || a.splits + a.group_splits == 1) return e;
+    return launch_kernel(packed_join_kernel<CATS_DT, HD>, dim3((unsigned)(((long long)a.seq.N * a.kv_heads * a.group + 3) / 4)), dim3(256), 0, stream, a);
   });
 }
 

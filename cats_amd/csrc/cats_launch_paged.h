@@ -8,7 +8,14 @@ namespace cats {
 
 template <class DT>
 hipError_t launch_paged_append(int D, bool wide, const PagedAppendArgs& a, hipStream_t stream);
+
+// Which kernel attention over pages takes, and into how many parts it splits keys.
+struct PackedPlan {
+  bool step;                 // packed_attn_step_kernel
+  int splits, group_splits;  // of a sequence's own keys; of those that its group shares (0: none are)
+};
+// plan NULL: keys and values of the call.  launch_packed_attn fills in what the plan decides.
 template <class DT>
-hipError_t launch_packed_attn(int D, bool paged, PackedAttnArgs a, hipStream_t stream);
+hipError_t launch_packed_attn(int D, const PackedPlan* plan, PackedAttnArgs a, hipStream_t stream);
 
 }  // namespace cats

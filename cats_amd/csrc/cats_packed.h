@@ -22,7 +22,11 @@ struct PackedAttnArgs {
   float scale;        // log2(e) * the softmax's scale
   int kv_heads, group;  // group: query heads of a cached head
   int window;         // keys that a query sees, at most; 0: all
-  int slots;
+  int slots;          // of a launch of many tokens, of the sequences' own keys
+  // few tokens: keys are split, and what the splits give is in `part`: [split][token, head][D] sums and, behind them, [split][token, head][2] largest
+  // exponent and sum of weights
+  float* part;
+  int splits, group_slots, group_splits;  // of the sequences' own keys; of what their groups share
 };
 
 // Row r of a (sequence, cached head) pair is head r % group of token r / group, and a workgroup has up to ROWS of them.  Which ones it finds by its slot: set i has the
@@ -86,6 +90,25 @@ __device__ __forceinline__ void packed_fill(const PackedAttnArgs& p, int tok0, i
   }
 }
 
+// Where tokens of pages come from, sixteen at a time, which no page ends within.  Those outside lo .. hi, which nobody sees, are the nearest ones once more: their
+// entries may be anything, and so may the places behind a sequence's last token.
+struct PageRun {
+  long long place;  // token of the pool's head 0
+  int last;         // of the sixteen, the last that may be read
+  bool none;        // no page
+};
+struct PageRows {
+  const int32_t* table;
+  const int32_t* common;  // of the first `alike` pages
+  int alike, lo, hi;
+};
+__device__ __forceinline__ PageRun page_run(const Pool& pool, const PageRows& rows, int t) {
+  const int from = min(max(t, rows.lo & ~15), rows.hi & ~15), page = from >> pool.page_log;
+  const int id = load_uniform((page < rows.alike ? rows.common : rows.table) + page);
+  const bool in = (unsigned)id < (unsigned)pool.pages;
+  return {((long long)(in ? id : 0) * pool.heads << pool.page_log) + (from & ((1 << pool.page_log) - 1)), min(rows.hi - from, 15), !in};
+}
+
 // Four tokens of sixteen elements in LDS turned round: lane i of each sixteen gives the place of elements 4 (i % 4) .. + 3 of token i / 4, and gets the four tokens of
 // element i.
 __device__ __forceinline__ u32x2 read_turned(const char* at) {
@@ -124,17 +147,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
   if (r0 >= rows) return;
   const bool live = s >= 0 && s < B;
   int pos0 = 0;  // position of the sequence's first query
-  const int32_t *table = nullptr, *common = nullptr;  // entries of pages, and of the first `alike` of them, which a group shares
-  int alike = 0;
+  PageRows pages = {};
   const uint16_t *k_base, *v_base;
   bool ok = true;
   if constexpr (PAGED) {
     ok = at.word >= 0 && at.word <= ((long long)p.pool.width << p.pool.page_log) - n;
     pos0 = ok ? (int)at.word : 0;
-    table = common = p.pool.table + s * p.pool.table_stride;
+    pages.table = pages.common = p.pool.table + s * p.pool.table_stride;
     if (p.shared && live) {
-      alike = shared_pages(p, s, pos0);
-      common = p.pool.table + s / p.members * p.members * p.pool.table_stride;
+      pages.alike = shared_pages(p, s, pos0);
+      pages.common = p.pool.table + s / p.members * p.members * p.pool.table_stride;
     }
     k_base = p.pool.k + ((long long)c << p.pool.page_log) * D;
     v_base = p.pool.v + ((long long)c << p.pool.page_log) * D;
@@ -147,7 +169,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
   const int end = pos0 + n;  // keys
   const int pos_lo = pos0 + r0 / p.group, pos_hi = pos0 + (min(r0 + ROWS, rows) - 1) / p.group;
   if (!live || !ok || pos_hi < 0) return packed_fill<D>(p, tok0, c, r0, ROWS, rows, live && !ok ? DT::fromf(NAN) * 0x10001u : 0u);
-  const int tile_lo = p.window ? max(0, pos_lo - p.window + 1) / kTileKeys : 0, tile_hi = pos_hi / kTileKeys;
+  pages.lo = p.window ? max(0, pos_lo - p.window + 1) : 0;
+  pages.hi = pos_hi;
+  const int tile_lo = pages.lo / kTileKeys, tile_hi = pos_hi / kTileKeys;
 
   const int mine = r0 + 32 * wave + m, row = min(mine, rows - 1), tok = row / p.group, pos = pos0 + tok;
   const int first = p.window ? pos - p.window : -1;  // the query sees first + 1 .. pos
@@ -175,35 +199,37 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
     auto load = [&](const char* from, unsigned lane_at, u32x4* to) {
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (size_t)lane_at), (__attribute__((address_space(3))) void*)to, 16, 0, 0);
     };
-    auto loads = [&](const char* kf, const char* vf) {
-#pragma unroll
-      for (int j = 0; j < LOADS; j++) {
-        load(kf + (size_t)j * STEP * k_row, t_lane * k_row + (kp ^ (16u * tile_swap_k<D>(STEP * j))), kt + j * kWave);
-        load(vf + (size_t)j * STEP * v_row, t_lane * v_row + (vp ^ (16u * tile_swap_v<D>(STEP * j))), vt + j * kWave);
-      }
-    };
     const int t0 = tile * kTileKeys + 16 * wave;
+    int last;
+    const uint16_t *kf, *vf;
     if constexpr (PAGED) {
-      const int most = (end - 1) >> p.pool.page_log;
-      int mine = 0;
+      PageRun mine = {};
       none1 = 0;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const int page = min((tile * kTileKeys + 16 * i) >> p.pool.page_log, most), id = load_uniform((page < alike ? common : table) + page);
-        const bool in = (unsigned)id < (unsigned)p.pool.pages;
-        none1 |= in ? 0u : 1u << i;
-        if (i == wave) mine = in ? id : 0;
+        const PageRun run = page_run(p.pool, pages, tile * kTileKeys + 16 * i);
+        none1 |= run.none ? 1u << i : 0u;
+        if (i == wave) mine = run;
       }
-      const long long place = ((((long long)mine * p.pool.heads) << p.pool.page_log) + (t0 & ((1 << p.pool.page_log) - 1))) * D;
-      loads((const char*)(k_base + place), (const char*)(v_base + place));
-    } else if (t0 + 16 <= end) {
-      loads((const char*)(k_base + t0 * p.k_tok), (const char*)(v_base + t0 * p.v_tok));
+      last = mine.last;
+      kf = k_base + mine.place * D, vf = v_base + mine.place * D;
+    } else {
+      const int from = min(t0, end - 1);
+      last = end - 1 - from;
+      kf = k_base + from * p.k_tok, vf = v_base + from * p.v_tok;
+    }
+    if (last >= 15) {
+#pragma unroll
+      for (int j = 0; j < LOADS; j++) {
+        load((const char*)kf + (size_t)j * STEP * k_row, t_lane * k_row + (kp ^ (16u * tile_swap_k<D>(STEP * j))), kt + j * kWave);
+        load((const char*)vf + (size_t)j * STEP * v_row, t_lane * v_row + (vp ^ (16u * tile_swap_v<D>(STEP * j))), vt + j * kWave);
+      }
     } else {  // tokens behind the last one are that one again
 #pragma unroll
       for (int j = 0; j < LOADS; j++) {
-        const long long t = min(t0 + (int)t_lane + STEP * j, end - 1);
-        load((const char*)(k_base + t * p.k_tok), kp ^ (16u * tile_swap_k<D>(STEP * j)), kt + j * kWave);
-        load((const char*)(v_base + t * p.v_tok), vp ^ (16u * tile_swap_v<D>(STEP * j)), vt + j * kWave);
+        const unsigned t = min((int)t_lane + STEP * j, last);
+        load((const char*)kf, t * k_row + (kp ^ (16u * tile_swap_k<D>(STEP * j))), kt + j * kWave);
+        load((const char*)vf, t * v_row + (vp ^ (16u * tile_swap_v<D>(STEP * j))), vt + j * kWave);
       }
     }
   };
@@ -377,11 +403,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
     sweep(std::true_type(), CLEAN);
   }
   sum += __shfl_xor(sum, 32, kWave);
-  const float f = pos < 0 ? 0.f : 1.f / sum;
+  const float f = sum == 0.f ? 0.f : 1.f / sum;  // no key, or none that weighs anything
   store([&](uint16_t* out, int w, int a) {
     float x[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) x[e] = pos < 0 ? 0.f : o[w][4 * a + e] * f;
+    for (int e = 0; e < 4; e++) x[e] = o[w][4 * a + e] * f;
     *(u32x2*)out = u32x2{DT::pack(x[0], x[1]), DT::pack(x[2], x[3])};
   });
   if (again) {
@@ -392,6 +418,443 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
         if (o[w][4 * a + e] > 0.f) out[e] = DT::fromf(NAN);
     });
   }
+}
+
+// Few tokens: up to 64 rows of queries a workgroup, its keys split over workgroups.  Two kinds of workgroups in one launch: those of the keys that a group of sequences shares,
+// whose rows are the tokens of all of them, and those of a sequence's own keys.  Sixteen rows are an operand of v_mfma_f32_16x16x32:
+//   S^T = K . Q^T   tile i, row 4 g + e of the result: token 16 i + 4 g + e, in lanes of group g = lane / 16; columns are queries
+//   O^T += V^T . P  operand of 32 tokens: tokens 4 g .. + 3 and 16 + 4 g .. + 3, those whose weights the lane has; V comes turned round out of LDS
+// Where there are up to sixteen rows each wave has 32 keys of its own at a time, in LDS of its own, and waits for nobody; what the waves give is joined in LDS at the end.
+// Where there are more, a wave has sixteen rows, and all of them read tiles of 64 keys that they bring together.
+constexpr int kStepKeys = 32, kStepBlock = 64;
+template <int D> __device__ __forceinline__ constexpr int step_swap_v(int t) {
+  return D >= 128 ? (t & 7) * 2 : D == 64 ? (t >> 1 & 3) * 2 : (t >> 2 & 1) * 2;
+}
+constexpr int packed_step_waves(int D) { return D == 256 ? 1 : 2; }
+template <class DT, int D>
+__global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_kernel(PackedAttnArgs p) {
+  constexpr int C = D / 32, NU = D / 16, PK = D / 8, STEP = kWave / PK, W = 4, kVecs = kStepKeys * PK;
+  typedef Kv<DT> F;
+  __shared__ u32x4 s_kv[W][2][kVecs];  // a wave's [keys, values]; or [buffer][half] of the workgroup's keys and, behind them, values: see kt, vt
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
+  const int c = blockIdx.x % p.kv_heads, B = p.seq.B, N = p.seq.N;
+  int rest = blockIdx.x / p.kv_heads;
+  const bool common = rest < p.group_slots * p.group_splits;
+  if (!common) rest -= p.group_slots * p.group_splits;
+  const int splits = common ? p.group_splits : p.splits, slot = rest / splits, split = rest - slot * splits;
+  const int members = common ? p.members : 1, sets = B / members + 2;
+  const PackedRows at = packed_rows<kStepBlock>(sets, slot, p.group, [&](int i) { return i == 0 ? 0 : i == sets ? N : packed_at(p.seq, (i - 1) * members); },
+                                                [&](int i) -> long long { return p.start[min(max(i - 1, 0) * members, B - 1)]; });
+  const int rows = at.n * p.group, r0 = at.r0, tok0 = at.tok0, here = min(kStepBlock, rows - r0);
+  if (here <= 0) return;
+  const bool live = at.set >= 1 && at.set < sets - 1;
+  const int s0 = live ? (at.set - 1) * members : 0;
+  const bool joined = p.splits + p.group_splits > 1;  // what this workgroup gives goes to `part`
+  const long long all = (long long)N * p.kv_heads * p.group;  // rows of a split
+  const long long part0 = (long long)((common ? 0 : p.group_splits) + split) * all;
+  float* part_ml = p.part + (long long)(p.splits + p.group_splits) * all * D;
+  auto out_row = [&](int r) {  // of (token, head)
+    const int t = r / p.group;
+    return (long long)(tok0 + t) * p.kv_heads * p.group + c * p.group + (r - t * p.group);
+  };
+  auto nothing = [&](float sum) {  // rows that see none of the keys, or (NaN) are no sequence's
+    if (!joined) return packed_fill<D>(p, tok0, c, r0, here, rows, sum == 0.f ? 0u : DT::fromf(NAN) * 0x10001u);
+    if (tid < here) {
+      float* ml = part_ml + 2 * (part0 + out_row(r0 + tid));
+      ml[0] = -FLT_MAX;
+      ml[1] = sum;
+    }
+  };
+  if (!live) return nothing(0.f);
+
+  // the keys of row r of this workgroup: lo .. hi, and its position
+  struct Keys {
+    int lo, hi;
+  };
+  auto page_tokens = [&](int n) { return n << p.pool.page_log; };
+  const long long room = page_tokens(p.pool.width);
+  bool ok = true;
+  int alike = 0, start0 = 0;
+  if (!common) {
+    ok = at.word >= 0 && at.word <= room - at.n;
+    start0 = ok ? (int)at.word : 0;
+    if (p.shared) alike = shared_pages(p, s0, start0);
+  }
+  if (!ok) return nothing(NAN);
+  auto keys_of = [&](int r) -> Keys {
+    const int t = tok0 + r / p.group;
+    if (!common) {
+      const int pos = start0 + t - tok0;
+      return {max(page_tokens(alike), p.window ? pos - p.window + 1 : 0), pos};
+    }
+    // the sequence among the group's: a token each, or looked for
+    int b = s0 + min(t - tok0, members - 1);
+    if (!__all(packed_at(p.seq, b) <= t && t < packed_at(p.seq, b + 1))) {
+      int e = s0 + members;
+      b = s0;
+      for (int n = members; n > 1; n = (n + 1) / 2) {
+        const int mid = (b + e) / 2;
+        const bool in = mid > b && packed_at(p.seq, mid) <= t;
+        b = in ? mid : b;
+        e = in ? e : max(mid, b + 1);
+      }
+    }
+    const long long start = p.start[b];
+    const int first = packed_at(p.seq, b), n = packed_at(p.seq, b + 1) - first;
+    if (!(start >= 0 && start <= room - n)) return {0, -1};
+    const int pos = (int)start + t - first;
+    const long long shared = p.shared[s0 / members * p.shared_step];
+    const int pages = (int)max(0ll, min(shared, start)) >> p.pool.page_log;
+    return {p.window ? max(0, pos - p.window + 1) : 0, page_tokens(pages) - 1};
+  };
+  auto least = [](int v) {
+#pragma unroll
+    for (int i = 1; i < kWave; i <<= 1) v = min(v, __shfl_xor(v, i, kWave));
+    return __builtin_amdgcn_readfirstlane(v);
+  };
+  auto most = [&](int v) { return -least(-v); };
+  // of all rows here, a lane each
+  Keys k = keys_of(r0 + min(lane, here - 1));
+  const bool some = k.lo <= k.hi;
+  PageRows pages;
+  pages.lo = least(some ? k.lo : INT_MAX);
+  pages.hi = most(some ? k.hi : -1);
+  if (pages.hi < 0) return nothing(0.f);
+  pages.table = pages.common = p.pool.table + s0 * p.pool.table_stride;
+  pages.alike = 0;
+  if (alike) {
+    pages.alike = alike;
+    pages.common = p.pool.table + s0 / p.members * p.members * p.pool.table_stride;
+  }
+
+  // each wave its keys and all rows, or its rows and all keys
+  const bool apart = here <= 16;
+  const int wave_rows = apart ? 0 : 16 * wave, keys = apart ? kStepKeys : 2 * kStepKeys;
+  const int row = r0 + min(wave_rows + m, here - 1);
+  const int src = min(wave_rows + m, here - 1);
+  k.lo = __shfl(k.lo, src, kWave), k.hi = __shfl(k.hi, src, kWave);
+  const int all_lo = most(k.lo), all_hi = least(k.hi);  // what all of the wave's rows see
+  const bool idle = wave_rows >= here;                  // a wave without rows, that only brings
+  u32x4 qf[C];
+  {
+    const int t = row / p.group;
+    const uint16_t* q = p.q + (tok0 + t) * p.q_tok + (c * p.group + row - t * p.group) * p.q_head;
+#pragma unroll
+    for (int i = 0; i < C; i++) qf[i] = *(const u32x4*)(q + 32 * i + 8 * g);
+  }
+  const int tile_lo = pages.lo / keys, tile_hi = pages.hi / keys;
+  const int unit = apart ? W : 1, active = min(splits, (tile_hi - tile_lo + unit) / unit);
+  if (split >= active) return nothing(0.f);
+
+  const unsigned t_lane = lane / PK;
+  unsigned k_piece = ((lane % PK) ^ tile_swap_k<D>(t_lane)) * 16, v_piece = ((lane % PK) ^ step_swap_v<D>(t_lane)) * 16;
+  unsigned k_at = (m * PK + (g ^ tile_swap_k<D>(m))) * 16;
+  unsigned v_at = ((4 * g + (m >> 2)) * PK + ((m >> 1 & 1) ^ step_swap_v<D>(4 * (g & 1) + (m >> 2)))) * 16 + 8 * (m & 1);
+  asm volatile("" : "+v"(k_at), "+v"(v_at));
+  const uint16_t* k_base = p.pool.k + page_tokens(c) * (long long)D;
+  const uint16_t* v_base = p.pool.v + page_tokens(c) * (long long)D;
+  // sixteen tokens of a run into LDS at k, v
+  auto bring16 = [&](const PageRun& run, u32x4* kt, u32x4* vt) {
+    const char *kf = (const char*)(k_base + run.place * D), *vf = (const char*)(v_base + run.place * D);
+    unsigned kp = k_piece, vp = v_piece;
+    asm volatile("" : "+v"(kp), "+v"(vp));  // not a register for every load over the loop
+#pragma unroll
+    for (int j = 0; j < PK / 4; j++) {
+      const unsigned t = run.last >= 15 ? t_lane + STEP * j : min((int)t_lane + STEP * j, run.last);
+      auto load = [&](const char* from, unsigned lane_at, u32x4* to) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (size_t)lane_at), (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+      };
+      load(kf, t * (2 * D) + (kp ^ (16u * tile_swap_k<D>(STEP * j))), kt + j * kWave);
+      load(vf, t * (2 * D) + (vp ^ (16u * step_swap_v<D>(STEP * j))), vt + j * kWave);
+    }
+  };
+  unsigned none = 0;  // bit i: tokens 16 i .. + 15 of the tile have no page
+
+  float top = -FLT_MAX, sum = 0.f;
+  bool far = false;
+  f32x4 o[NU];
+  auto weigh = [&](f32x4 (&s)[2]) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[i][e]);
+    mx = max_mod16(mx);
+    const float now = fmaxf(top, kv_scaled(mx, p.scale));
+    if (__any(now > top)) {
+      const float keep = __builtin_amdgcn_exp2f(top - now);
+      sum *= keep;
+#pragma unroll
+      for (int u = 0; u < NU; u++) o[u] *= keep;
+      top = now;
+      far = __any(kv_far(top));
+    }
+    float off = F::HEAD - top;
+    if (far) {
+      const float ref = fmaxf(mx, -FLT_MAX);
+      off = fminf(kv_scaled(mx, p.scale) - top, 0.f) + F::HEAD;
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[i][e] -= ref;
+    }
+    float add = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], p.scale, off));
+        add += s[i][e];
+      }
+    sum += add;
+  };
+  enum { PLAIN, CLEAN, COUNT };  // as above
+  // 32 keys from key0 on; `behind` once they are in registers
+  auto take = [&](auto AGAIN, int mode, int key0, unsigned none, const u32x4* kt, const u32x4* vt, auto behind) {
+    u32x4 kk[2][C], vv[NU];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int j = 0; j < C; j++) kk[i][j] = *(const u32x4*)((const char*)kt + (k_at ^ 64u * j) + 16 * i * PK * 16);
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+      const u32x2 lo = read_turned((const char*)vt + (v_at ^ 32u * u)), hi = read_turned((const char*)vt + (v_at ^ 32u * u) + 16 * PK * 16);
+      vv[u] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
+    behind();
+    f32x4 s[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < C; j++) s[i] = Mma<DT>::run(kk[i][j], qf[j], s[i]);
+    }
+    if (none) {
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        if (none >> i & 1) s[i] = f32x4{NAN, NAN, NAN, NAN};
+    }
+    auto seen = [&](int i, int e) {
+      const int key = key0 + 16 * i + 4 * g + e;
+      return key >= k.lo && key <= k.hi;
+    };
+    if (key0 < all_lo || key0 + kStepKeys - 1 > all_hi) {
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[i][e] = seen(i, e) ? s[i][e] : -INFINITY;
+    }
+    if (!AGAIN || mode == CLEAN) weigh(s);
+    if constexpr (AGAIN) {
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[i][e] = mode == COUNT ? (seen(i, e) ? 1.f : 0.f) : s[i][e];
+#pragma unroll
+      for (int u = 0; u < NU; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint32_t bad = kv_nan16<DT>(vv[u][e]);
+          vv[u][e] = mode == COUNT ? bad * F::kOne : vv[u][e] & ~(bad * 0xffffu);
+        }
+    }
+    const u32x4 pf = u32x4{DT::pack(s[0][0], s[0][1]), DT::pack(s[0][2], s[0][3]), DT::pack(s[1][0], s[1][1]), DT::pack(s[1][2], s[1][3])};
+#pragma unroll
+    for (int u = 0; u < NU; u++) o[u] = Mma<DT>::run(vv[u], pf, o[u]);
+  };
+  auto here_now = [] {  // what was brought
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    asm volatile("" ::: "memory");
+  };
+  auto sweep = [&](auto AGAIN, int mode) {
+#pragma unroll
+    for (int u = 0; u < NU; u++) o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (apart) {
+      u32x4 *kt = s_kv[wave][0], *vt = s_kv[wave][1];
+      const int step = active * W;
+      int tile = tile_lo + split * W + wave;
+      PageRun run[2];
+      auto ask = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) run[i] = page_run(p.pool, pages, min(tile, tile_hi) * kStepKeys + 16 * i);
+      };
+      auto bring = [&] {
+#pragma unroll
+        for (int i = 0; i < 2; i++) bring16(run[i], kt + 16 * i * PK, vt + 16 * i * PK);
+      };
+      ask(tile);
+      if (tile <= tile_hi) bring();
+      for (; tile <= tile_hi; tile += step) {
+        none = run[0].none | run[1].none << 1;
+        ask(tile + step);
+        here_now();
+        take(AGAIN, mode, tile * kStepKeys, none, kt, vt, [&] {
+          __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): read
+          __builtin_amdgcn_sched_barrier(0);
+          if (tile + step <= tile_hi) bring();
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      }
+    } else {
+      // [buffer][keys, values] of 64 tokens
+      auto kt = [&](int buf) { return s_kv[2 * buf][0]; };
+      auto vt = [&](int buf) { return s_kv[2 * buf + 1][0]; };
+      unsigned none1 = 0;
+      auto bring = [&](int tile, int buf) {
+        PageRun mine = {};
+        none1 = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const PageRun run = page_run(p.pool, pages, tile * 2 * kStepKeys + 16 * i);
+          none1 |= run.none ? 1u << i : 0u;
+          if (i == wave) mine = run;
+        }
+        bring16(mine, kt(buf) + 16 * wave * PK, vt(buf) + 16 * wave * PK);
+      };
+      int tile = tile_lo + split, buf = 0;
+      bring(min(tile, tile_hi), 0);
+      here_now();
+      none = none1;
+      lds_barrier();
+      for (; tile <= tile_hi; tile += active, buf ^= 1) {
+        const bool more = tile + active <= tile_hi;
+        if (idle) {
+          if (more) bring(tile + active, buf ^ 1);
+        } else {
+          take(AGAIN, mode, tile * 2 * kStepKeys, none & 3, kt(buf), vt(buf), [] {});
+          take(AGAIN, mode, tile * 2 * kStepKeys + kStepKeys, none >> 2, kt(buf) + kStepKeys * PK, vt(buf) + kStepKeys * PK, [&] {
+            __builtin_amdgcn_s_waitcnt(0xc07f);
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) bring(tile + active, buf ^ 1);
+            __builtin_amdgcn_sched_barrier(0);
+          });
+        }
+        here_now();
+        none = none1;
+        lds_barrier();
+      }
+    }
+  };
+  sweep(std::false_type(), PLAIN);
+  float odd = 0.f;
+#pragma unroll
+  for (int u = 0; u < NU; u++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) odd = fmaf(o[u][e], 0.f, odd);
+  const bool again = __syncthreads_or(odd != 0.f);
+  if (again) {
+    top = -FLT_MAX, sum = 0.f, far = false;
+    sweep(std::true_type(), CLEAN);
+    __syncthreads();
+  }
+  sum += __shfl_xor(sum, 16, kWave);
+  sum += __shfl_xor(sum, 32, kWave);
+
+  // the waves' results, and where the tiles have to be gone over again, what is to be put there instead
+  __shared__ float s_top[W][16], s_sum[W][16];
+  float* s_o = (float*)s_kv;  // [wave or 0][16][D + 4]
+  constexpr int PITCH = D + 4;
+  auto write_row = [&](int r, int d, f32x4 x, float mx, float den) {  // r: of the workgroup's
+    const long long to = out_row(r0 + r);
+    if (!joined) {
+      const float f = den == 0.f ? 0.f : 1.f / den;
+      *(u32x2*)(p.out + to * D + d) = u32x2{DT::pack(x[0] * f, x[1] * f), DT::pack(x[2] * f, x[3] * f)};
+    } else {
+      *(f32x4*)(p.part + (part0 + to) * D + d) = x;
+      if (d == 0) {
+        float* ml = part_ml + 2 * (part0 + to);
+        ml[0] = mx;
+        ml[1] = den;
+      }
+    }
+  };
+  auto spoil_row = [&](int r, int d, f32x4 x) {  // not finite where x counts something
+    const long long to = out_row(r0 + r);
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (x[e] > 0.f) {
+        if (!joined) p.out[to * D + d + e] = DT::fromf(NAN);
+        else p.part[(part0 + to) * D + d + e] = NAN;
+      }
+  };
+  auto finish = [&](bool count) {
+    if (!apart) {
+      if (wave_rows + m >= here) return;
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
+        if (count) spoil_row(wave_rows + m, 16 * u + 4 * g, o[u]);
+        else write_row(wave_rows + m, 16 * u + 4 * g, o[u], top, sum);
+      }
+      return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < NU; u++) *(f32x4*)(s_o + (wave * 16 + m) * PITCH + 16 * u + 4 * g) = o[u];
+    if (!count && g == 0) {
+      s_top[wave][m] = top;
+      s_sum[wave][m] = sum;
+    }
+    __syncthreads();
+    for (int i = tid; i < here * (D / 4); i += 256) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float mx = s_top[0][r];
+#pragma unroll
+      for (int w = 1; w < W; w++) mx = fmaxf(mx, s_top[w][r]);
+      f32x4 num = f32x4{0.f, 0.f, 0.f, 0.f};
+      float den = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; w++) {
+        const float f = count ? 1.f : __builtin_amdgcn_exp2f(s_top[w][r] - mx);
+        const f32x4 x = *(const f32x4*)(s_o + (w * 16 + r) * PITCH + d);
+#pragma unroll
+        for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e]);
+        den = fmaf(f, s_sum[w][r], den);
+      }
+      if (count) spoil_row(r, d, num);
+      else write_row(r, d, num, mx, den);
+    }
+  };
+  finish(false);
+  if (again) {
+    __syncthreads();
+    sweep(std::true_type(), COUNT);
+    finish(true);
+  }
+}
+
+// The splits' results, in a fixed order: a wave a row, whose groups of D / 4 lanes take every so manieth split.
+template <class DT, int D>
+__global__ __launch_bounds__(256) void packed_join_kernel(PackedAttnArgs p) {
+  constexpr int L = D / 4, G = kWave / L;
+  const int lane = threadIdx.x & (kWave - 1), grp = lane / L, d = lane % L * 4, n = p.splits + p.group_splits;
+  const long long all = (long long)p.seq.N * p.kv_heads * p.group, r = (long long)blockIdx.x * 4 + threadIdx.x / kWave;
+  if (r >= all) return;
+  const float* ml = p.part + n * all * D + 2 * r;
+  const float* part = p.part + r * D + d;
+  float top = -FLT_MAX, den = 0.f;
+  f32x4 num = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = grp; s < n; s += G) {
+    const float mx = ml[2 * s * all], sm = ml[2 * s * all + 1];
+    if (sm == 0.f) continue;  // nothing has been written
+    const f32x4 x = *(const f32x4*)(part + s * all * D);
+    const float now = fmaxf(top, mx), keep = __builtin_amdgcn_exp2f(top - now), f = __builtin_amdgcn_exp2f(mx - now);
+#pragma unroll
+    for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e] * keep);
+    den = fmaf(f, sm, den * keep);
+    top = now;
+  }
+#pragma unroll
+  for (int i = L; i < kWave; i <<= 1) {
+    const float mx = __shfl_xor(top, i, kWave), now = fmaxf(top, mx), keep = __builtin_amdgcn_exp2f(top - now), f = __builtin_amdgcn_exp2f(mx - now);
+#pragma unroll
+    for (int e = 0; e < 4; e++) num[e] = fmaf(f, __shfl_xor(num[e], i, kWave), num[e] * keep);
+    den = fmaf(f, __shfl_xor(den, i, kWave), den * keep);
+    top = now;
+  }
+  if (grp != 0) return;
+  const float f = den == 0.f ? 0.f : 1.f / den;
+  *(u32x2*)(p.out + r * D + d) = u32x2{DT::pack(num[0] * f, num[1] * f), DT::pack(num[2] * f, num[3] * f)};
 }
 
 }  // namespace cats
