@@ -61,7 +61,7 @@ PackedPlan paged_plan(int N, int B, int heads, int kv_heads, int page, int width
   const long long room = (long long)width * page, keys = window ? (room < window + 64ll ? room : window + 64ll) : room;
   const long long rows = ((long long)N * group + B - 1) / B;  // of a sequence, on average
   const long long many = (long long)kv_heads * (((long long)N * group + kTileRows - 1) / kTileRows);
-  PackedPlan plan = {rows <= 16 || many < cus, 1, members > 1 ? 1 : 0};
+  PackedPlan plan = {rows <= 16 || many < cus / 2, 1, members > 1 ? 1 : 0};
   if (!plan.step) return {false, 1, 0};
   auto splits = [&](long long sets, long long set_rows) {
     const long long groups = kv_heads * sets * ((set_rows + kStepBlock - 1) / kStepBlock), want = (2ll * cus + groups - 1) / groups;

@@ -22,6 +22,7 @@ struct PackedAttnArgs {
   float scale;        // log2(e) * the softmax's scale
   int kv_heads, group;  // group: query heads of a cached head
   int window;         // keys that a query sees, at most; 0: all
+  int turn;           // workgroups from here on come the other way round
   int slots;          // of a launch of many tokens, of the sequences' own keys
   // few tokens: keys are split, and what the splits give is in `part`: [split][token, head][D] sums and, behind them, [split][token, head][2] largest
   // exponent and sum of weights
@@ -57,11 +58,11 @@ __device__ __forceinline__ PackedRows packed_rows(int sets, int slot, int group,
   const uint64_t below = __ballot(lane < n && base(i, tok) <= slot);
   const int last = below ? 63 - __builtin_clzll(below) : 0;
   PackedRows r;
-  r.set = lo + last;
+  r.set = __builtin_amdgcn_readfirstlane(lo + last);  // (the compiler does not see that these are the same in all lanes)
   r.tok0 = __builtin_amdgcn_readlane(tok, last);
-  r.n = max(0, __builtin_amdgcn_readlane(tok, last + 1) - r.tok0);
+  r.n = __builtin_amdgcn_readfirstlane(max(0, __builtin_amdgcn_readlane(tok, last + 1) - r.tok0));
   const long long first = slot - base(r.set, r.tok0);
-  r.r0 = first < 0 || first > INT_MAX / ROWS ? INT_MAX : (int)first * ROWS;
+  r.r0 = __builtin_amdgcn_readfirstlane(first < 0 || first > INT_MAX / ROWS ? INT_MAX : (int)first * ROWS);
   r.word = (long long)((unsigned)__builtin_amdgcn_readlane((int)w, last) | (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(w >> 32), last) << 32);
   return r;
 }
@@ -93,9 +94,7 @@ __device__ __forceinline__ void packed_fill(const PackedAttnArgs& p, int tok0, i
 // Where tokens of pages come from, sixteen at a time, which no page ends within.  Those outside lo .. hi, which nobody sees, are the nearest ones once more: their
 // entries may be anything, and so may the places behind a sequence's last token.
 struct PageRun {
-  long long place;  // token of the pool's head 0
-  int last;         // of the sixteen, the last that may be read
-  bool none;        // no page
+  int from, id;  // first token that is read, and its entry
 };
 struct PageRows {
   const int32_t* table;
@@ -104,9 +103,11 @@ struct PageRows {
 };
 __device__ __forceinline__ PageRun page_run(const Pool& pool, const PageRows& rows, int t) {
   const int from = min(max(t, rows.lo & ~15), rows.hi & ~15), page = from >> pool.page_log;
-  const int id = load_uniform((page < rows.alike ? rows.common : rows.table) + page);
-  const bool in = (unsigned)id < (unsigned)pool.pages;
-  return {((long long)(in ? id : 0) * pool.heads << pool.page_log) + (from & ((1 << pool.page_log) - 1)), min(rows.hi - from, 15), !in};
+  return {from, load_uniform((page < rows.alike ? rows.common : rows.table) + page)};
+}
+__device__ __forceinline__ bool page_none(const Pool& pool, const PageRun& run) { return (unsigned)run.id >= (unsigned)pool.pages; }
+__device__ __forceinline__ long long page_place(const Pool& pool, const PageRun& run) {  // token of the pool's head 0
+  return ((long long)(page_none(pool, run) ? 0 : run.id) * pool.heads << pool.page_log) + (run.from & ((1 << pool.page_log) - 1));
 }
 
 // Four tokens of sixteen elements in LDS turned round: lane i of each sixteen gives the place of elements 4 (i % 4) .. + 3 of token i / 4, and gets the four tokens of
@@ -122,6 +123,20 @@ __device__ __forceinline__ u32x2 read_turned(const char* at) {
 //   O^T += V^T . P  operand of step v (16 tokens): tokens 16 v + 4 h + (0 .. 3) and 8 behind them, those whose weights the lane has; V comes turned round out of LDS
 // Rows of LDS are 16-byte pieces, exchanged within a row so that lanes that read together find different banks.
 constexpr int kTileKeys = 64, kTileRows = 128;
+template <class DT> struct Limit { static constexpr float SUM = 0x1p15f; };  // 2^HEAD
+template <> struct Limit<BF16> { static constexpr float SUM = 0x1p-32f; };
+
+// A pointer that is the same in all lanes, as one that the compiler knows to be.
+__device__ __forceinline__ const char* uniform(const void* p) {
+  const uint64_t a = (uint64_t)p;
+  return (const char*)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)a));
+}
+// 1 KiB from memory straight into LDS, sixteen bytes a lane, in the lanes' order from `to` on.  As an instruction of its own and not the builtin: behind that one every
+// read of LDS would wait for memory, whatever it reads.  It has no result in a register; who reads what it brings waits for vmcnt(0) first.
+__device__ __forceinline__ void load_lds(const void* from, unsigned lane_at, const void* to) {
+  const unsigned lds = (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)to;
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0" ::"s"(from), "v"(lane_at), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
+}
 template <int D> __device__ __forceinline__ constexpr int tile_swap_k(int t) {
   return D >= 128 ? t & 15 : D == 64 ? t >> 1 & 7 : t >> 2 & 3;
 }
@@ -135,7 +150,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
   typedef Kv<DT> F;
   __shared__ u32x4 s_kv[2][2][kVecs];  // [buffer][keys, values]
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 31, h = lane >> 5;
-  const int c = blockIdx.x % p.kv_heads, slot = p.slots - 1 - blockIdx.x / p.kv_heads;
+  int turn = blockIdx.x;
+  if (turn >= p.turn) turn = gridDim.x - 1 - (turn - p.turn);
+  const int c = turn % p.kv_heads, slot = p.slots - 1 - turn / p.kv_heads;
   const int B = p.seq.B;
   const PackedRows at = packed_rows<ROWS>(B + 2, slot, p.group, [&](int i) { return i == 0 ? 0 : i > B + 1 ? p.seq.N : packed_at(p.seq, i - 1); },
                                           [&](int i) -> long long {
@@ -143,9 +160,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
                                             if constexpr (PAGED) return p.start[s];
                                             return (long long)packed_at(p.keys, s) << 32 | packed_at(p.keys, s + 1);
                                           });
-  const int s = at.set - 1, n = at.n, rows = n * p.group, r0 = at.r0, tok0 = at.tok0;
+  const int seq = at.set - 1, n = at.n, rows = n * p.group, r0 = at.r0, tok0 = at.tok0;
   if (r0 >= rows) return;
-  const bool live = s >= 0 && s < B;
+  const bool live = seq >= 0 && seq < B;
   int pos0 = 0;  // position of the sequence's first query
   PageRows pages = {};
   const uint16_t *k_base, *v_base;
@@ -153,10 +170,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
   if constexpr (PAGED) {
     ok = at.word >= 0 && at.word <= ((long long)p.pool.width << p.pool.page_log) - n;
     pos0 = ok ? (int)at.word : 0;
-    pages.table = pages.common = p.pool.table + s * p.pool.table_stride;
+    pages.table = pages.common = p.pool.table + seq * p.pool.table_stride;
     if (p.shared && live) {
-      pages.alike = shared_pages(p, s, pos0);
-      pages.common = p.pool.table + s / p.members * p.members * p.pool.table_stride;
+      pages.alike = shared_pages(p, seq, pos0);
+      pages.common = p.pool.table + seq / p.members * p.members * p.pool.table_stride;
     }
     k_base = p.pool.k + ((long long)c << p.pool.page_log) * D;
     v_base = p.pool.v + ((long long)c << p.pool.page_log) * D;
@@ -191,135 +208,119 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
   unsigned v_at = ((4 * h + (m >> 2 & 3)) * PK + ((2 * (m >> 4) + (m >> 1 & 1)) ^ tile_swap_v<D>(m >> 2 & 3))) * 16 + 8 * (m & 1);
   asm volatile("" : "+v"(k_at), "+v"(v_at));
   const unsigned k_row = PAGED ? D * 2 : (unsigned)p.k_tok * 2, v_row = PAGED ? D * 2 : (unsigned)p.v_tok * 2;  // bytes
-  unsigned none = 0, none1 = 0;  // bit i: tokens 16 i .. + 15 of the tile, and of the next one, have no page
-  auto bring = [&](int tile, int buf) {
-    u32x4 *kt = s_kv[buf][0] + 16 * wave * PK, *vt = s_kv[buf][1] + 16 * wave * PK;
-    unsigned kp = k_piece, vp = v_piece;
-    asm volatile("" : "+v"(kp), "+v"(vp));  // not a register for every load over the loop
-    auto load = [&](const char* from, unsigned lane_at, u32x4* to) {
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (size_t)lane_at), (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-    };
-    const int t0 = tile * kTileKeys + 16 * wave;
-    int last;
-    const uint16_t *kf, *vf;
+  // Where the wave's sixteen tokens of a tile come from.  Entries of pages are asked for a tile ahead of that.
+  struct Place {
+    long long at;   // element of the keys and (PAGED) of the values, of the head
+    int last;       // of the sixteen, the last that may be read: tokens behind it are that one again
+    unsigned none;  // bit i: tokens 16 i .. + 15 of the tile have no page
+  };
+  PageRun runs[4] = {};
+  auto ask = [&](int tile) {
     if constexpr (PAGED) {
-      PageRun mine = {};
-      none1 = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) runs[i] = page_run(p.pool, pages, tile * kTileKeys + 16 * i);
+    }
+  };
+  auto place_of = [&](int tile) -> Place {  // PAGED: of the tile that was asked for
+    if constexpr (PAGED) {
+      PageRun mine = runs[0];
+      unsigned none = 0;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const PageRun run = page_run(p.pool, pages, tile * kTileKeys + 16 * i);
-        none1 |= run.none ? 1u << i : 0u;
-        if (i == wave) mine = run;
+        none |= page_none(p.pool, runs[i]) ? 1u << i : 0u;
+        if (i == wave) mine = runs[i];
       }
-      last = mine.last;
-      kf = k_base + mine.place * D, vf = v_base + mine.place * D;
+      return {page_place(p.pool, mine) * D, pages.hi - mine.from, none};
     } else {
-      const int from = min(t0, end - 1);
-      last = end - 1 - from;
-      kf = k_base + from * p.k_tok, vf = v_base + from * p.v_tok;
+      const int from = min(tile * kTileKeys + 16 * wave, end - 1);
+      return {from, end - 1 - from, 0u};
     }
+  };
+  auto bring = [&](const Place& pl, bool values, u32x4* to) {
+    unsigned piece = values ? v_piece : k_piece;
+    asm volatile("" : "+v"(piece));  // not a register for every load over the loop
+    const unsigned step = values ? v_row : k_row;
+    const char* from = uniform((values ? v_base : k_base) + (PAGED ? pl.at : pl.at * (values ? p.v_tok : p.k_tok)));
+    const int last = __builtin_amdgcn_readfirstlane(pl.last);
+    to += 16 * wave * PK;
+    auto swap = [&](int j) { return 16u * (values ? tile_swap_v<D>(STEP * j) : tile_swap_k<D>(STEP * j)); };
     if (last >= 15) {
 #pragma unroll
-      for (int j = 0; j < LOADS; j++) {
-        load((const char*)kf + (size_t)j * STEP * k_row, t_lane * k_row + (kp ^ (16u * tile_swap_k<D>(STEP * j))), kt + j * kWave);
-        load((const char*)vf + (size_t)j * STEP * v_row, t_lane * v_row + (vp ^ (16u * tile_swap_v<D>(STEP * j))), vt + j * kWave);
-      }
-    } else {  // tokens behind the last one are that one again
+      for (int j = 0; j < LOADS; j++) load_lds(from + (size_t)j * STEP * step, t_lane * step + (piece ^ swap(j)), to + j * kWave);
+    } else {
 #pragma unroll
-      for (int j = 0; j < LOADS; j++) {
-        const unsigned t = min((int)t_lane + STEP * j, last);
-        load((const char*)kf, t * k_row + (kp ^ (16u * tile_swap_k<D>(STEP * j))), kt + j * kWave);
-        load((const char*)vf, t * v_row + (vp ^ (16u * tile_swap_v<D>(STEP * j))), vt + j * kWave);
-      }
+      for (int j = 0; j < LOADS; j++) load_lds(from, min((int)t_lane + STEP * j, last) * step + (piece ^ swap(j)), to + j * kWave);
     }
   };
 
   float top = -FLT_MAX, sum = 0.f;
   bool far = false;  // whether some query's scores are
-  f32x16 o[NW];
-  auto zeros = [] {
-    f32x16 z;
+  f32x16 s[2], o[NW];
+  u32x4 pf[4];
+  // Weights of a tile from its scores, as operands: 2^(HEAD - SLACK) times what they are relative to `top`, which was the largest score when it was last looked at.
+  // It is looked at again where a lane's weights add up to more than 2^HEAD.
+  auto weights = [&](float off, u32x4 (&pf)[4]) {
+    float add = 0.f;
 #pragma unroll
-    for (int e = 0; e < 16; e++) z[e] = 0.f;
-    return z;
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float a = __builtin_amdgcn_exp2f(fmaf(s[i / 2][8 * (i % 2) + 2 * e], p.scale, off)), b = __builtin_amdgcn_exp2f(fmaf(s[i / 2][8 * (i % 2) + 2 * e + 1], p.scale, off));
+        add += a;
+        add += b;
+        pf[i][e] = DT::pack(a, b);
+      }
+    return add;
   };
-  // weights of a tile from its scores, as operands
-  auto weigh = [&](f32x16 (&s)[2], u32x4 (&pf)[4]) {
-    float mx = s[0][0];
+  auto settle = [&](float add) {  // of the weights that are in pf now; what o holds is of tiles before
+    if (__any(add > (far ? -1.f : Limit<DT>::SUM))) {
+      float mx = s[0][0];
 #pragma unroll
-    for (int u = 0; u < 2; u++)
+      for (int u = 0; u < 2; u++)
 #pragma unroll
-      for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[u][e]);
-    mx = max_mod32(mx);
-    const float now = fmaxf(top, kv_scaled(mx, p.scale));
-    if (__any(now > top + F::SLACK)) {
-      const float keep = __builtin_amdgcn_exp2f(top - now);
+        for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[u][e]);
+      mx = max_mod32(mx);
+      const float at = kv_scaled(mx, p.scale), now = fmaxf(top, at), keep = __builtin_amdgcn_exp2f(top - now);
       sum *= keep;
 #pragma unroll
       for (int w = 0; w < NW; w++) o[w] *= keep;
       top = now;
       far = __any(kv_far(top));
-    }
-    float off = F::HEAD - F::SLACK - top;
-    if (far) {
-      const float ref = fmaxf(mx, -FLT_MAX);
-      off = fminf(kv_scaled(mx, p.scale) - top, F::SLACK) + F::HEAD - F::SLACK;
+      float off = F::HEAD - F::SLACK - top;
+      if (far) {
+        const float ref = fmaxf(mx, -FLT_MAX);
+        off = fminf(at - top, F::SLACK) + F::HEAD - F::SLACK;
 #pragma unroll
-      for (int u = 0; u < 2; u++)
+        for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) s[u][e] -= ref;
-    }
-    float add = 0.f;
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-#pragma unroll
-      for (int e = 0; e < 16; e++) {
-        s[u][e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], p.scale, off));
-        add += s[u][e];
+          for (int e = 0; e < 16; e++) s[u][e] -= ref;
       }
-#pragma unroll
-      for (int v = 0; v < 2; v++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) pf[2 * u + v][e] = DT::pack(s[u][8 * v + 2 * e], s[u][8 * v + 2 * e + 1]);
+      add = weights(off, pf);
     }
     sum += add;
   };
-  // whether the query sees a key: all of the tile's, in turn
-  auto each_seen = [&](int tile, auto f) {
-    const int most = pos - tile * kTileKeys - 4 * h, least = max(most, -kTileKeys) - (p.window ? p.window : INT_MAX / 2);
+  // tiles that a window cuts, tiles that all of the workgroup's queries see, tiles that hold some of their own keys
+  const int cut = p.window && pos_hi >= p.window ? (pos_hi - p.window) / kTileKeys : -1, own = (pos_lo + 1) / kTileKeys;  // last and first of them
+  // scores of a tile that comes next; its keys are read four operands ahead
+  auto score = [&](const u32x4* keys) {
+    u32x4 x[4];
+    auto key = [&](int i) { return *(const u32x4*)((const char*)keys + (k_at ^ 32u * (i / 2)) + 32 * (i % 2) * PK * 16); };
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = key(i);
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const int t = 32 * u + 8 * (e / 4) + e % 4;
-        f(u, e, t <= most && t > least);
-      }
-  };
-  // A masked weight is 0, but 0 times a NaN is not.  So where a sum is not finite at the end, the tiles are gone over again: once with numbers of V that are not
-  // finite set to 0, and once to count, for each element, those that a query sees.
-  enum { PLAIN, CLEAN, COUNT };
-  // one tile; PART: some query of the wave does not see all of it
-  auto take = [&](auto PART, auto AGAIN, int mode, int tile, int buf, auto behind) {
-    f32x16 s[2] = {zeros(), zeros()};
-    const char *kt = (const char*)s_kv[buf][0], *vt = (const char*)s_kv[buf][1];
+      for (int e = 0; e < 16; e++) s[u][e] = 0.f;
 #pragma unroll
-    for (int i = 0; i < C; i++)
-#pragma unroll
-      for (int u = 0; u < 2; u++) s[u] = Mma32<DT>::run(*(const u32x4*)(kt + (k_at ^ 32u * i) + 32 * u * PK * 16), qf[i], s[u]);
-    // All values are asked for before the next tile, which a read of LDS behind its loads would wait for.  (Heads of 256 elements do not have the registers.)
-    constexpr bool ASK = D <= 128;
-    auto values = [&](int w, int v) {
-      const u32x2 lo = read_turned(vt + (v_at ^ 64u * w) + 16 * v * PK * 16), hi = read_turned(vt + (v_at ^ 64u * w) + (16 * v + 8) * PK * 16);
-      return u32x4{lo[0], lo[1], hi[0], hi[1]};
-    };
-    u32x4 x[ASK ? 4 * NW : 1];
-    if constexpr (ASK) {
-#pragma unroll
-      for (int i = 0; i < 4 * NW; i++) x[i] = values(i % NW, i / NW);
+    for (int i = 0; i < 2 * C; i++) {
       __builtin_amdgcn_sched_barrier(0);
-      behind();
-      __builtin_amdgcn_sched_barrier(0);
+      s[i % 2] = Mma32<DT>::run(x[i % 4], qf[i / 2], s[i % 2]);
+      if (i + 4 < 2 * C) x[i % 4] = key(i + 4);
     }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // what replaces scores of keys that the query does not see, those behind it and those that a window hides, and of places that are no page's
+  auto mask = [&](int tile, unsigned none, float hidden) {
     if (PAGED && none) {
 #pragma unroll
       for (int u = 0; u < 2; u++)
@@ -327,60 +328,157 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
         for (int e = 0; e < 16; e++)
           if (none >> (2 * u + e / 8) & 1) s[u][e] = NAN;
     }
-    if constexpr (PART) each_seen(tile, [&](int u, int e, bool seen) { s[u][e] = seen ? s[u][e] : -INFINITY; });
-    u32x4 pf[4];
-    if (!AGAIN || mode == CLEAN) {
-      weigh(s, pf);
+    const int most = pos - tile * kTileKeys - 4 * h;
+    if (tile >= own) {
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[u][e] = 32 * u + 8 * (e / 4) + e % 4 <= most ? s[u][e] : hidden;
     }
-    if constexpr (AGAIN) {
-      if (mode == COUNT) {
-        each_seen(tile, [&](int u, int e, bool seen) { s[u][e] = seen ? 1.f : 0.f; });
+    if (tile <= cut) {
+      const int least = max(most, -kTileKeys) - p.window;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[u][e] = 32 * u + 8 * (e / 4) + e % 4 > least ? s[u][e] : hidden;
+    }
+  };
+  auto operand = [&](const u32x4* values, int w, int v) {
+    const char* at = (const char*)values + (v_at ^ 64u * w) + 16 * v * PK * 16;
+    const u32x2 lo = read_turned(at), hi = read_turned(at + 8 * PK * 16);
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  auto products = [&](const u32x4* values) {
+#pragma unroll
+    for (int i = 0; i < 4 * NW; i++) o[i % NW] = Mma32<DT>::run(operand(values, i % NW, i / NW), pf[i / NW], o[i % NW]);
+  };
+  auto clear = [&] {
+#pragma unroll
+    for (int w = 0; w < NW; w++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) o[w][e] = 0.f;
+  };
+  auto arrive = [&] {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): in LDS
+    lds_barrier();
+  };
+  // Tile by tile: the weights of one while the products of the values of the one before run, then the next one's scores, which take the scores' place.  Meanwhile
+  // its values come, and the keys of the one behind the next.
+  clear();
+  Place at0, at1, at2 = {};  // of the tile whose weights are next, and of the two behind it
+  int tile = tile_lo;
+  ask(tile);
+  at0 = place_of(tile);
+  bring(at0, false, s_kv[0][0]);
+  ask(tile + 1);
+  at1 = place_of(tile + 1);
+  bring(at1, false, s_kv[1][0]);
+  ask(tile + 2);
+  arrive();
+  score(s_kv[0][0]);
+  lds_barrier();  // all have read what is overwritten now
+  int buf = 0;    // of the tile
+  auto step = [&](auto PART, auto FIRST) {
+    at2 = place_of(tile + 2);
+    bring(at0, true, s_kv[buf][1]);
+    if (tile + 2 <= tile_hi) bring(at2, false, s_kv[buf][0]);
+    ask(tile + 3);
+    if (PART || at0.none) mask(tile, at0.none, -INFINITY);
+    const float off = F::HEAD - F::SLACK - top;
+    float add = 0.f;
+    u32x4 next[4];
+    if constexpr (FIRST) {
+      add = weights(off, next);
+    } else {
+      // A sixteenth of the products and of the weights in turn, the instructions of one beside the other's: its operands read two ahead, the argument of
+      // an exponential one ahead, its sum one behind.
+      constexpr int N = 4 * NW;
+      const u32x4* values = s_kv[buf ^ 1][1];
+      u32x4 x[3];
+      f32x2v arg[2], w[2];
+      auto argument = [&](int j) { arg[j & 1] = f32x2v{fmaf(s[j / 8][2 * j % 16], p.scale, off), fmaf(s[j / 8][2 * j % 16 + 1], p.scale, off)}; };
+      auto finish = [&](int j) {
+        add += w[j & 1][0];
+        add += w[j & 1][1];
+        next[j / 4][j % 4] = DT::pack(w[j & 1][0], w[j & 1][1]);
+      };
+      x[0] = operand(values, 0, 0);
+      x[1] = operand(values, 1 % NW, 1 / NW);
+      argument(0);
+#pragma unroll
+      for (int i = 0, j = 0; i < (N > 16 ? N : 16); i++) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (i * N % 16 == 0 || N > 16) {
+          const int k = N > 16 ? i : i * N / 16;
+          o[k % NW] = Mma32<DT>::run(x[k % 3], pf[k / NW], o[k % NW]);
+          if (k + 2 < N) x[(k + 2) % 3] = operand(values, (k + 2) % NW, (k + 2) / NW);
+        }
+        if (N <= 16 || i * 16 % N == 0) {
+          w[j & 1] = f32x2v{__builtin_amdgcn_exp2f(arg[j & 1][0]), __builtin_amdgcn_exp2f(arg[j & 1][1])};
+          if (j + 1 < 16) argument(j + 1);
+          if (j > 0) finish(j - 1);
+          j++;
+        }
+      }
+      finish(15);
+#pragma unroll
+      for (int i = 0; i < 4; i++) asm volatile("" : "+v"(next[i]));  // here, and not where it is known that they are wanted
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) pf[i] = next[i];
+    settle(add);
+    if (tile < tile_hi) score(s_kv[buf ^ 1][0]);
+    arrive();
+    at0 = at1, at1 = at2;
+    buf ^= 1;
+    tile++;
+  };
+  const std::true_type yes;
+  const std::false_type no;
+  step(yes, yes);
+  while (tile <= min(cut, tile_hi)) step(yes, no);
+  while (tile <= min(own - 1, tile_hi)) step(no, no);
+  while (tile <= tile_hi) step(yes, no);
+  products(s_kv[buf ^ 1][1]);
+
+  // A masked weight is 0, but 0 times a NaN is not.  So where a sum is not finite now, the tiles are gone over again: once with numbers of V that are not finite set
+  // to 0, and once to count, for each element, those that a query sees.
+  auto again = [&](bool count) {
+    clear();
+    for (int tile = tile_lo; tile <= tile_hi; tile++) {
+      ask(tile);
+      const Place at = place_of(tile);
+      lds_barrier();
+      bring(at, false, s_kv[0][0]);
+      bring(at, true, s_kv[0][1]);
+      arrive();
+      score(s_kv[0][0]);
+      mask(tile, at.none, -INFINITY);
+      if (count) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) s[u][e] = 1.f;
+        mask(tile, 0, 0.f);
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
           for (int e = 0; e < 4; e++) pf[i][e] = DT::pack(s[i / 2][8 * (i % 2) + 2 * e], s[i / 2][8 * (i % 2) + 2 * e + 1]);
+      } else {
+        settle(weights(F::HEAD - F::SLACK - top, pf));
       }
-    }
 #pragma unroll
-    for (int i = 0; i < 4 * NW; i++) {
-      u32x4 y = ASK ? x[ASK ? i : 0] : values(i % NW, i / NW);
-      if constexpr (AGAIN) {
+      for (int i = 0; i < 4 * NW; i++) {
+        u32x4 y = operand(s_kv[0][1], i % NW, i / NW);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const uint32_t bad = kv_nan16<DT>(y[e]);
-          y[e] = mode == COUNT ? bad * F::kOne : y[e] & ~(bad * 0xffffu);
+          y[e] = count ? bad * F::kOne : y[e] & ~(bad * 0xffffu);
         }
+        o[i % NW] = Mma32<DT>::run(y, pf[i / NW], o[i % NW]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      o[i % NW] = Mma32<DT>::run(y, pf[i / NW], o[i % NW]);
-    }
-    if constexpr (!ASK) behind();
-  };
-
-  // tiles that a window cuts, tiles that all of the workgroup's queries see, tiles that hold some of their own keys
-  const int cut = p.window && pos_hi >= p.window ? (pos_hi - p.window) / kTileKeys : -1, own = (pos_lo + 1) / kTileKeys;  // last and first of them
-  auto sweep = [&](auto AGAIN, int mode) {
-#pragma unroll
-    for (int w = 0; w < NW; w++) o[w] = zeros();
-    int tile = tile_lo, buf = 0;
-    bring(tile, 0);
-    auto arrive = [&] {
-      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): in LDS
-      none = none1;
-      lds_barrier();
-    };
-    arrive();
-    auto run = [&](auto PART, int to) {
-      for (; tile <= to; tile++, buf ^= 1) {
-        take(PART, AGAIN, mode, tile, buf, [&] { bring(min(tile + 1, tile_hi), buf ^ 1); });
-        arrive();
-      }
-    };
-    if constexpr (AGAIN) {
-      run(std::true_type(), tile_hi);
-    } else {
-      run(std::true_type(), min(cut, tile_hi));
-      run(std::false_type(), min(own - 1, tile_hi));
-      run(std::true_type(), tile_hi);
     }
   };
   auto store = [&](auto value) {
@@ -391,16 +489,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
 #pragma unroll
       for (int a = 0; a < 4; a++) value(out + 32 * w + 8 * a + 4 * h, w, a);
   };
-  sweep(std::false_type(), PLAIN);
   float odd = 0.f;
 #pragma unroll
   for (int w = 0; w < NW; w++)
 #pragma unroll
     for (int e = 0; e < 16; e++) odd = fmaf(o[w][e], 0.f, odd);
-  const bool again = __syncthreads_or(odd != 0.f);  // NaN is
-  if (again) {
+  const bool bad = __syncthreads_or(odd != 0.f);  // NaN is
+  if (bad) {
     top = -FLT_MAX, sum = 0.f, far = false;
-    sweep(std::true_type(), CLEAN);
+    again(false);
   }
   sum += __shfl_xor(sum, 32, kWave);
   const float f = sum == 0.f ? 0.f : 1.f / sum;  // no key, or none that weighs anything
@@ -410,8 +507,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
     for (int e = 0; e < 4; e++) x[e] = o[w][4 * a + e] * f;
     *(u32x2*)out = u32x2{DT::pack(x[0], x[1]), DT::pack(x[2], x[3])};
   });
-  if (again) {
-    sweep(std::true_type(), COUNT);
+  if (bad) {
+    again(true);
     store([&](uint16_t* out, int w, int a) {
 #pragma unroll
       for (int e = 0; e < 4; e++)
@@ -555,12 +652,14 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
   const uint16_t* v_base = p.pool.v + page_tokens(c) * (long long)D;
   // sixteen tokens of a run into LDS at k, v
   auto bring16 = [&](const PageRun& run, u32x4* kt, u32x4* vt) {
-    const char *kf = (const char*)(k_base + run.place * D), *vf = (const char*)(v_base + run.place * D);
+    const long long place = page_place(p.pool, run);
+    const int last = pages.hi - run.from;  // of the sixteen, the last that may be read
+    const char *kf = uniform(k_base + place * D), *vf = uniform(v_base + place * D);
     unsigned kp = k_piece, vp = v_piece;
     asm volatile("" : "+v"(kp), "+v"(vp));  // not a register for every load over the loop
 #pragma unroll
     for (int j = 0; j < PK / 4; j++) {
-      const unsigned t = run.last >= 15 ? t_lane + STEP * j : min((int)t_lane + STEP * j, run.last);
+      const unsigned t = min((int)t_lane + STEP * j, last);
       auto load = [&](const char* from, unsigned lane_at, u32x4* to) {
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (size_t)lane_at), (__attribute__((address_space(3))) void*)to, 16, 0, 0);
       };
@@ -608,7 +707,7 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
       }
     sum += add;
   };
-  enum { PLAIN, CLEAN, COUNT };  // as above
+  enum { PLAIN, CLEAN, COUNT };  // gone over again as above
   // 32 keys from key0 on; `behind` once they are in registers
   auto take = [&](auto AGAIN, int mode, int key0, unsigned none, const u32x4* kt, const u32x4* vt, auto behind) {
     u32x4 kk[2][C], vv[NU];
@@ -685,7 +784,7 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
       ask(tile);
       if (tile <= tile_hi) bring();
       for (; tile <= tile_hi; tile += step) {
-        none = run[0].none | run[1].none << 1;
+        none = page_none(p.pool, run[0]) | page_none(p.pool, run[1]) << 1;
         ask(tile + step);
         here_now();
         take(AGAIN, mode, tile * kStepKeys, none, kt, vt, [&] {
@@ -700,32 +799,42 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
       auto kt = [&](int buf) { return s_kv[2 * buf][0]; };
       auto vt = [&](int buf) { return s_kv[2 * buf + 1][0]; };
       unsigned none1 = 0;
-      auto bring = [&](int tile, int buf) {
-        PageRun mine = {};
+      PageRun runs[4];
+      auto ask = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) runs[i] = page_run(p.pool, pages, tile * 2 * kStepKeys + 16 * i);
+      };
+      auto bring = [&](int buf) {
+        PageRun mine = runs[0];
         none1 = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const PageRun run = page_run(p.pool, pages, tile * 2 * kStepKeys + 16 * i);
-          none1 |= run.none ? 1u << i : 0u;
-          if (i == wave) mine = run;
+          none1 |= page_none(p.pool, runs[i]) ? 1u << i : 0u;
+          if (i == wave) mine = runs[i];
         }
         bring16(mine, kt(buf) + 16 * wave * PK, vt(buf) + 16 * wave * PK);
       };
       int tile = tile_lo + split, buf = 0;
-      bring(min(tile, tile_hi), 0);
+      ask(tile);
+      bring(0);
+      ask(tile + active);
       here_now();
       none = none1;
       lds_barrier();
       for (; tile <= tile_hi; tile += active, buf ^= 1) {
         const bool more = tile + active <= tile_hi;
+        auto next = [&] {
+          if (more) bring(buf ^ 1);
+          ask(tile + 2 * active);
+        };
         if (idle) {
-          if (more) bring(tile + active, buf ^ 1);
+          next();
         } else {
           take(AGAIN, mode, tile * 2 * kStepKeys, none & 3, kt(buf), vt(buf), [] {});
           take(AGAIN, mode, tile * 2 * kStepKeys + kStepKeys, none >> 2, kt(buf) + kStepKeys * PK, vt(buf) + kStepKeys * PK, [&] {
             __builtin_amdgcn_s_waitcnt(0xc07f);
             __builtin_amdgcn_sched_barrier(0);
-            if (more) bring(tile + active, buf ^ 1);
+            next();
             __builtin_amdgcn_sched_barrier(0);
           });
         }
