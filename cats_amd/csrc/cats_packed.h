@@ -131,11 +131,20 @@ __device__ __forceinline__ const char* uniform(const void* p) {
   const uint64_t a = (uint64_t)p;
   return (const char*)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)a));
 }
-// 1 KiB from memory straight into LDS, sixteen bytes a lane, in the lanes' order from `to` on.  As an instruction of its own and not the builtin: behind that one every
-// read of LDS would wait for memory, whatever it reads.  It has no result in a register; who reads what it brings waits for vmcnt(0) first.
-__device__ __forceinline__ void load_lds(const void* from, unsigned lane_at, const void* to) {
-  const unsigned lds = (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)to;
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0" ::"s"(from), "v"(lane_at), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
+// N KiB from memory straight into LDS, N up to 4: sixteen bytes a lane and load, load j of lane l from  from + at[j]  to  to + 1024 j + 16 l.  As instructions of their own and not
+// the builtin: behind that one every read of LDS would wait for memory, whatever it reads.  They have no result in a register; who reads what they bring waits for
+// vmcnt(0) first.  An offset in the instruction counts on both sides, so one setting of M0 does for four: at[j] has 4096 - 1024 j more than it says, `from` 4096 less.
+template <int N>
+__device__ __forceinline__ void load_lds(const char* from, const unsigned (&at)[N], const void* to) {
+  const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)to);
+  const char* base = from - 4096;
+  if constexpr (N == 4)
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024\n\t"
+                 "global_load_lds_dwordx4 %4, %0 offset:2048\n\tglobal_load_lds_dwordx4 %5, %0 offset:3072" ::"s"(base), "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]) : "memory");
+  else if constexpr (N == 2)
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024" ::"s"(base), "s"(lds), "v"(at[0]), "v"(at[1]) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0" ::"s"(base), "s"(lds), "v"(at[0]) : "memory");
 }
 template <int D> __device__ __forceinline__ constexpr int tile_swap_k(int t) {
   return D >= 128 ? t & 15 : D == 64 ? t >> 1 & 7 : t >> 2 & 3;
@@ -191,8 +200,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
   const int tile_lo = pages.lo / kTileKeys, tile_hi = pos_hi / kTileKeys;
 
   const int mine = r0 + 32 * wave + m, row = min(mine, rows - 1), tok = row / p.group, pos = pos0 + tok;
-  const int first = p.window ? pos - p.window : -1;  // the query sees first + 1 .. pos
-  const int hi_pos = pos0 + min(r0 + 32 * wave + 31, rows - 1) / p.group, lo_pos = pos0 + min(r0 + 32 * wave, rows - 1) / p.group;
   u32x4 qf[C];
   {
     const uint16_t* q = p.q + (tok0 + tok) * p.q_tok + (c * p.group + row - tok * p.group) * p.q_head;
@@ -236,49 +243,55 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
       return {from, end - 1 - from, 0u};
     }
   };
+  constexpr int AT = LOADS < 4 ? LOADS : 4, PARTS = LOADS / AT;  // loads of one instruction sequence, and how many of those
+  // where the lanes read, in bytes from the first of the sixteen tokens on, for load_lds; last: the last token that is read
+  auto lanes = [&](bool values, int last, unsigned (&to)[PARTS][AT]) {
+    const unsigned piece = values ? v_piece : k_piece, step = values ? v_row : k_row;
+#pragma unroll
+    for (int j = 0; j < LOADS; j++)
+      to[j / AT][j % AT] = min((int)t_lane + STEP * j, last) * step + (piece ^ (16u * (values ? tile_swap_v<D>(STEP * j) : tile_swap_k<D>(STEP * j)))) + 4096 - 1024 * (j % AT);
+  };
+  unsigned k_lanes[PARTS][AT], v_lanes[PARTS][AT];
+  lanes(false, 15, k_lanes);
+  lanes(true, 15, v_lanes);
+#pragma unroll
+  for (int j = 0; j < LOADS; j++) asm volatile("" : "+v"(k_lanes[j / AT][j % AT]), "+v"(v_lanes[j / AT][j % AT]));
   auto bring = [&](const Place& pl, bool values, u32x4* to) {
-    unsigned piece = values ? v_piece : k_piece;
-    asm volatile("" : "+v"(piece));  // not a register for every load over the loop
-    const unsigned step = values ? v_row : k_row;
     const char* from = uniform((values ? v_base : k_base) + (PAGED ? pl.at : pl.at * (values ? p.v_tok : p.k_tok)));
     const int last = __builtin_amdgcn_readfirstlane(pl.last);
     to += 16 * wave * PK;
-    auto swap = [&](int j) { return 16u * (values ? tile_swap_v<D>(STEP * j) : tile_swap_k<D>(STEP * j)); };
     if (last >= 15) {
 #pragma unroll
-      for (int j = 0; j < LOADS; j++) load_lds(from + (size_t)j * STEP * step, t_lane * step + (piece ^ swap(j)), to + j * kWave);
+      for (int i = 0; i < PARTS; i++) load_lds<AT>(from, values ? v_lanes[i] : k_lanes[i], to + i * AT * kWave);
     } else {
+      unsigned some[PARTS][AT];
+      lanes(values, last, some);
 #pragma unroll
-      for (int j = 0; j < LOADS; j++) load_lds(from, min((int)t_lane + STEP * j, last) * step + (piece ^ swap(j)), to + j * kWave);
+      for (int i = 0; i < PARTS; i++) load_lds<AT>(from, some[i], to + i * AT * kWave);
     }
   };
 
   float top = -FLT_MAX, sum = 0.f;
   bool far = false;  // whether some query's scores are
-  f32x16 s[2], o[NW];
-  u32x4 pf[4];
-  // Weights of a tile from its scores, as operands: 2^(HEAD - SLACK) times what they are relative to `top`, which was the largest score when it was last looked at.
-  // It is looked at again where a lane's weights add up to more than 2^HEAD.
-  auto weights = [&](float off, u32x4 (&pf)[4]) {
+  f32x16 o[NW];
+  // Weights of half a tile from its scores, as operands: 2^(HEAD - SLACK) times what they are relative to `top`, which was the largest score when it was last looked
+  // at.  It is looked at again where a lane's weights add up to more than 2^HEAD.
+  auto weights = [&](const f32x16& s, float off, u32x4 (&pf)[2]) {
     float add = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float a = __builtin_amdgcn_exp2f(fmaf(s[i / 2][8 * (i % 2) + 2 * e], p.scale, off)), b = __builtin_amdgcn_exp2f(fmaf(s[i / 2][8 * (i % 2) + 2 * e + 1], p.scale, off));
-        add += a;
-        add += b;
-        pf[i][e] = DT::pack(a, b);
-      }
+    for (int j = 0; j < 8; j++) {
+      const float a = __builtin_amdgcn_exp2f(fmaf(s[2 * j], p.scale, off)), b = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], p.scale, off));
+      add += a;
+      add += b;
+      pf[j / 4][j % 4] = DT::pack(a, b);
+    }
     return add;
   };
-  auto settle = [&](float add) {  // of the weights that are in pf now; what o holds is of tiles before
+  auto settle = [&](f32x16& s, u32x4 (&pf)[2], float add) {  // of the weights that are in pf now; what o holds is of keys before
     if (__any(add > (far ? -1.f : Limit<DT>::SUM))) {
-      float mx = s[0][0];
+      float mx = s[0];
 #pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[u][e]);
+      for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[e]);
       mx = max_mod32(mx);
       const float at = kv_scaled(mx, p.scale), now = fmaxf(top, at), keep = __builtin_amdgcn_exp2f(top - now);
       sum *= keep;
@@ -291,66 +304,38 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
         const float ref = fmaxf(mx, -FLT_MAX);
         off = fminf(at - top, F::SLACK) + F::HEAD - F::SLACK;
 #pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) s[u][e] -= ref;
+        for (int e = 0; e < 16; e++) s[e] -= ref;
       }
-      add = weights(off, pf);
+      add = weights(s, off, pf);
     }
     sum += add;
   };
   // tiles that a window cuts, tiles that all of the workgroup's queries see, tiles that hold some of their own keys
   const int cut = p.window && pos_hi >= p.window ? (pos_hi - p.window) / kTileKeys : -1, own = (pos_lo + 1) / kTileKeys;  // last and first of them
-  // scores of a tile that comes next; its keys are read four operands ahead
-  auto score = [&](const u32x4* keys) {
-    u32x4 x[4];
-    auto key = [&](int i) { return *(const u32x4*)((const char*)keys + (k_at ^ 32u * (i / 2)) + 32 * (i % 2) * PK * 16); };
-#pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = key(i);
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) s[u][e] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2 * C; i++) {
-      __builtin_amdgcn_sched_barrier(0);
-      s[i % 2] = Mma32<DT>::run(x[i % 4], qf[i / 2], s[i % 2]);
-      if (i + 4 < 2 * C) x[i % 4] = key(i + 4);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  // what replaces scores of keys that the query does not see, those behind it and those that a window hides, and of places that are no page's
-  auto mask = [&](int tile, unsigned none, float hidden) {
+  // half u of a tile: what replaces scores of keys that the query does not see, those behind it and those that a window hides, and of places that are no page's
+  auto mask = [&](f32x16& s, int tile, int u, unsigned none, float hidden) {
     if (PAGED && none) {
 #pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int e = 0; e < 16; e++)
-          if (none >> (2 * u + e / 8) & 1) s[u][e] = NAN;
+      for (int e = 0; e < 16; e++)
+        if (none >> (2 * u + e / 8) & 1) s[e] = NAN;
     }
-    const int most = pos - tile * kTileKeys - 4 * h;
+    const int most = pos - tile * kTileKeys - 32 * u - 4 * h;
     if (tile >= own) {
 #pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) s[u][e] = 32 * u + 8 * (e / 4) + e % 4 <= most ? s[u][e] : hidden;
+      for (int e = 0; e < 16; e++) s[e] = 8 * (e / 4) + e % 4 <= most ? s[e] : hidden;
     }
     if (tile <= cut) {
       const int least = max(most, -kTileKeys) - p.window;
 #pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) s[u][e] = 32 * u + 8 * (e / 4) + e % 4 > least ? s[u][e] : hidden;
+      for (int e = 0; e < 16; e++) s[e] = 8 * (e / 4) + e % 4 > least ? s[e] : hidden;
     }
   };
-  auto operand = [&](const u32x4* values, int w, int v) {
-    const char* at = (const char*)values + (v_at ^ 64u * w) + 16 * v * PK * 16;
+  // operands of half a tile, in the order of the products
+  auto key = [&](const u32x4* keys, int i) { return *(const u32x4*)((const char*)keys + (k_at ^ 32u * i)); };
+  auto value = [&](const u32x4* values, int i) {
+    const char* at = (const char*)values + (v_at ^ 64u * (i % NW)) + 16 * (i / NW) * PK * 16;
     const u32x2 lo = read_turned(at), hi = read_turned(at + 8 * PK * 16);
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
-  };
-  auto products = [&](const u32x4* values) {
-#pragma unroll
-    for (int i = 0; i < 4 * NW; i++) o[i % NW] = Mma32<DT>::run(operand(values, i % NW, i / NW), pf[i / NW], o[i % NW]);
   };
   auto clear = [&] {
 #pragma unroll
@@ -358,89 +343,108 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
 #pragma unroll
       for (int e = 0; e < 16; e++) o[w][e] = 0.f;
   };
+  auto zeros = [] {
+    f32x16 z;
+#pragma unroll
+    for (int e = 0; e < 16; e++) z[e] = 0.f;
+    return z;
+  };
   auto arrive = [&] {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): in LDS
     lds_barrier();
   };
-  // Tile by tile: the weights of one while the products of the values of the one before run, then the next one's scores, which take the scores' place.  Meanwhile
-  // its values come, and the keys of the one behind the next.
+  // The weights of half a tile from its scores `now`, beside the products of the half before, whose weights are `before`, and the scores of the half behind: of each an
+  // eighth in turn, operands read two ahead, the argument of an exponential one.  Matrix cores and the rest of a SIMD then work at once.
+  auto turn_of = [&](auto VALUES, auto KEYS, f32x16& now, f32x16& behind, const u32x4 (&before)[2], u32x4 (&pf)[2], const u32x4* values, const u32x4* keys) {
+    constexpr int N = 2 * NW, STEPS = N > 8 ? N : 8;
+    const float off = F::HEAD - F::SLACK - top;
+    u32x4 x[3], y[3];
+    f32x2v arg[2], w[2];
+    float add = 0.f;
+    auto argument = [&](int j) { arg[j & 1] = f32x2v{fmaf(now[2 * j], p.scale, off), fmaf(now[2 * j + 1], p.scale, off)}; };
+    auto finish = [&](int j) {
+      add += w[j & 1][0];
+      add += w[j & 1][1];
+      pf[j / 4][j % 4] = DT::pack(w[j & 1][0], w[j & 1][1]);
+    };
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      if constexpr (KEYS) y[i] = key(keys, i);
+      if constexpr (VALUES) x[i] = value(values, i);
+    }
+    if constexpr (KEYS) behind = zeros();
+    argument(0);
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i * N % STEPS == 0) {
+        const int k = i * N / STEPS;
+        if constexpr (KEYS) {
+          behind = Mma32<DT>::run(y[k % 3], qf[k], behind);
+          if (k + 2 < N) y[(k + 2) % 3] = key(keys, k + 2);
+        }
+        if constexpr (VALUES) {
+          o[k % NW] = Mma32<DT>::run(x[k % 3], before[k / NW], o[k % NW]);
+          if (k + 2 < N) x[(k + 2) % 3] = value(values, k + 2);
+        }
+      }
+      if (i * 8 % STEPS == 0) {
+        const int j = i * 8 / STEPS;
+        w[j & 1] = f32x2v{__builtin_amdgcn_exp2f(arg[j & 1][0]), __builtin_amdgcn_exp2f(arg[j & 1][1])};
+        if (j + 1 < 8) argument(j + 1);
+        if (j > 0) finish(j - 1);
+      }
+    }
+    finish(7);
+#pragma unroll
+    for (int i = 0; i < 2; i++) asm volatile("" : "+v"(pf[i]));  // here, and not where it is known that they are wanted
+    __builtin_amdgcn_sched_barrier(0);
+    settle(now, pf, add);
+  };
+  const std::true_type yes;
+  const std::false_type no;
+
+  // Halves in turn, 0 and 1 of a tile.  Between them, when all waves have read the one half, the keys of the tile behind the next come, and the values of the next.
   clear();
-  Place at0, at1, at2 = {};  // of the tile whose weights are next, and of the two behind it
-  int tile = tile_lo;
+  f32x16 s0, s1;
+  u32x4 p0[2], p1[2];
+  Place at0, at1, at2;  // of the tile, and of the two behind it
+  int tile = tile_lo, buf = 0;
+  constexpr int HALF = 32 * PK;
   ask(tile);
   at0 = place_of(tile);
   bring(at0, false, s_kv[0][0]);
+  bring(at0, true, s_kv[0][1]);
   ask(tile + 1);
   at1 = place_of(tile + 1);
   bring(at1, false, s_kv[1][0]);
   ask(tile + 2);
   arrive();
-  score(s_kv[0][0]);
-  lds_barrier();  // all have read what is overwritten now
-  int buf = 0;    // of the tile
-  auto step = [&](auto PART, auto FIRST) {
+  s0 = zeros();
+#pragma unroll
+  for (int i = 0; i < C; i++) s0 = Mma32<DT>::run(key(s_kv[0][0], i), qf[i], s0);
+  auto masked = [&](f32x16& s, int tile, int u, unsigned none) {
+    if (tile >= own || tile <= cut || none) mask(s, tile, u, none, -INFINITY);
+  };
+  masked(s0, tile, 0, at0.none);
+  turn_of(no, yes, s0, s1, p1, p0, nullptr, s_kv[0][0] + HALF);
+  for (; tile < tile_hi; tile++, buf ^= 1) {
     at2 = place_of(tile + 2);
-    bring(at0, true, s_kv[buf][1]);
+    arrive();
+    bring(at1, true, s_kv[buf ^ 1][1]);
     if (tile + 2 <= tile_hi) bring(at2, false, s_kv[buf][0]);
     ask(tile + 3);
-    if (PART || at0.none) mask(tile, at0.none, -INFINITY);
-    const float off = F::HEAD - F::SLACK - top;
-    float add = 0.f;
-    u32x4 next[4];
-    if constexpr (FIRST) {
-      add = weights(off, next);
-    } else {
-      // A sixteenth of the products and of the weights in turn, the instructions of one beside the other's: its operands read two ahead, the argument of
-      // an exponential one ahead, its sum one behind.
-      constexpr int N = 4 * NW;
-      const u32x4* values = s_kv[buf ^ 1][1];
-      u32x4 x[3];
-      f32x2v arg[2], w[2];
-      auto argument = [&](int j) { arg[j & 1] = f32x2v{fmaf(s[j / 8][2 * j % 16], p.scale, off), fmaf(s[j / 8][2 * j % 16 + 1], p.scale, off)}; };
-      auto finish = [&](int j) {
-        add += w[j & 1][0];
-        add += w[j & 1][1];
-        next[j / 4][j % 4] = DT::pack(w[j & 1][0], w[j & 1][1]);
-      };
-      x[0] = operand(values, 0, 0);
-      x[1] = operand(values, 1 % NW, 1 / NW);
-      argument(0);
-#pragma unroll
-      for (int i = 0, j = 0; i < (N > 16 ? N : 16); i++) {
-        __builtin_amdgcn_sched_barrier(0);
-        if (i * N % 16 == 0 || N > 16) {
-          const int k = N > 16 ? i : i * N / 16;
-          o[k % NW] = Mma32<DT>::run(x[k % 3], pf[k / NW], o[k % NW]);
-          if (k + 2 < N) x[(k + 2) % 3] = operand(values, (k + 2) % NW, (k + 2) / NW);
-        }
-        if (N <= 16 || i * 16 % N == 0) {
-          w[j & 1] = f32x2v{__builtin_amdgcn_exp2f(arg[j & 1][0]), __builtin_amdgcn_exp2f(arg[j & 1][1])};
-          if (j + 1 < 16) argument(j + 1);
-          if (j > 0) finish(j - 1);
-          j++;
-        }
-      }
-      finish(15);
-#pragma unroll
-      for (int i = 0; i < 4; i++) asm volatile("" : "+v"(next[i]));  // here, and not where it is known that they are wanted
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) pf[i] = next[i];
-    settle(add);
-    if (tile < tile_hi) score(s_kv[buf ^ 1][0]);
-    arrive();
+    masked(s1, tile, 1, at0.none);
+    turn_of(yes, yes, s1, s0, p0, p1, s_kv[buf][1], s_kv[buf ^ 1][0]);
+    masked(s0, tile + 1, 0, at1.none);
+    turn_of(yes, yes, s0, s1, p1, p0, s_kv[buf][1] + HALF, s_kv[buf ^ 1][0] + HALF);
     at0 = at1, at1 = at2;
-    buf ^= 1;
-    tile++;
-  };
-  const std::true_type yes;
-  const std::false_type no;
-  step(yes, yes);
-  while (tile <= min(cut, tile_hi)) step(yes, no);
-  while (tile <= min(own - 1, tile_hi)) step(no, no);
-  while (tile <= tile_hi) step(yes, no);
-  products(s_kv[buf ^ 1][1]);
+  }
+  arrive();
+  masked(s1, tile, 1, at0.none);
+  turn_of(yes, no, s1, s0, p0, p1, s_kv[buf][1], nullptr);
+#pragma unroll
+  for (int i = 0; i < 2 * NW; i++) o[i % NW] = Mma32<DT>::run(value(s_kv[buf][1] + HALF, i), p1[i / NW], o[i % NW]);
 
   // A masked weight is 0, but 0 times a NaN is not.  So where a sum is not finite now, the tiles are gone over again: once with numbers of V that are not finite set
   // to 0, and once to count, for each element, those that a query sees.
@@ -453,41 +457,41 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
       bring(at, false, s_kv[0][0]);
       bring(at, true, s_kv[0][1]);
       arrive();
-      score(s_kv[0][0]);
-      mask(tile, at.none, -INFINITY);
-      if (count) {
+      for (int u = 0; u < 2; u++) {
+        s0 = zeros();
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int i = 0; i < C; i++) s0 = Mma32<DT>::run(key(s_kv[0][0] + u * HALF, i), qf[i], s0);
+        mask(s0, tile, u, at.none, -INFINITY);
+        if (count) {
 #pragma unroll
-          for (int e = 0; e < 16; e++) s[u][e] = 1.f;
-        mask(tile, 0, 0.f);
+          for (int e = 0; e < 16; e++) s0[e] = 1.f;
+          mask(s0, tile, u, 0, 0.f);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) pf[i][e] = DT::pack(s[i / 2][8 * (i % 2) + 2 * e], s[i / 2][8 * (i % 2) + 2 * e + 1]);
-      } else {
-        settle(weights(F::HEAD - F::SLACK - top, pf));
-      }
-#pragma unroll
-      for (int i = 0; i < 4 * NW; i++) {
-        u32x4 y = operand(s_kv[0][1], i % NW, i / NW);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const uint32_t bad = kv_nan16<DT>(y[e]);
-          y[e] = count ? bad * F::kOne : y[e] & ~(bad * 0xffffu);
+          for (int j = 0; j < 8; j++) p0[j / 4][j % 4] = DT::pack(s0[2 * j], s0[2 * j + 1]);
+        } else {
+          settle(s0, p0, weights(s0, F::HEAD - F::SLACK - top, p0));
         }
-        o[i % NW] = Mma32<DT>::run(y, pf[i / NW], o[i % NW]);
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 2 * NW; i++) {
+          u32x4 y = value(s_kv[0][1] + u * HALF, i);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const uint32_t bad = kv_nan16<DT>(y[e]);
+            y[e] = count ? bad * F::kOne : y[e] & ~(bad * 0xffffu);
+          }
+          o[i % NW] = Mma32<DT>::run(y, p0[i / NW], o[i % NW]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
   };
-  auto store = [&](auto value) {
+  auto store = [&](auto write) {
     if (mine >= rows) return;
     uint16_t* out = packed_out(p, tok0, c, mine, D);
 #pragma unroll
     for (int w = 0; w < NW; w++)
 #pragma unroll
-      for (int a = 0; a < 4; a++) value(out + 32 * w + 8 * a + 4 * h, w, a);
+      for (int a = 0; a < 4; a++) write(out + 32 * w + 8 * a + 4 * h, w, a);
   };
   float odd = 0.f;
 #pragma unroll
