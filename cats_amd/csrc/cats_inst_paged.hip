@@ -38,7 +38,7 @@ hipError_t launch_packed_attn<CATS_DT>(int D, const PackedPlan* plan, PackedAttn
     if (!plan || !plan->step) {
       a.slots = packed_slots(a.seq.N, a.seq.B + 2, a.group, kTileRows);
       const int all = a.seq.N * a.group / kTileRows * a.kv_heads, cus = current_device_cus();
-      a.turn = all <= 2 * cus && all > cus ? cus + 2 * a.kv_heads : INT_MAX;
+      a.turn = all <= 2 * cus && all > cus ? cus : INT_MAX;
       return launch_kernel(plan ? packed_attn_tiles_kernel<CATS_DT, HD, true> : packed_attn_tiles_kernel<CATS_DT, HD, false>, dim3(a.slots * a.kv_heads), dim3(256), 0,
                            stream, a);
     }

@@ -159,9 +159,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
   typedef Kv<DT> F;
   __shared__ u32x4 s_kv[2][2][kVecs];  // [buffer][keys, values]
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 31, h = lane >> 5;
+  // The last slots first, which have the most keys of a sequence; two that hold nothing if the tokens are all somebody's behind the others.  Where a CU has two workgroups
+  // at once, the second ones come the other way round, so that those with the most keys are beside those with the fewest.
+  const int all = (p.slots - 2) * p.kv_heads;
   int turn = blockIdx.x;
-  if (turn >= p.turn) turn = gridDim.x - 1 - (turn - p.turn);
-  const int c = turn % p.kv_heads, slot = p.slots - 1 - turn / p.kv_heads;
+  if (turn < all && turn >= p.turn) turn = all - 1 - (turn - p.turn);
+  const int c = turn % p.kv_heads, slot = turn < all ? p.slots - 3 - turn / p.kv_heads : 2 * p.slots - 3 - turn / p.kv_heads;
   const int B = p.seq.B;
   const PackedRows at = packed_rows<ROWS>(B + 2, slot, p.group, [&](int i) { return i == 0 ? 0 : i > B + 1 ? p.seq.N : packed_at(p.seq, i - 1); },
                                           [&](int i) -> long long {
