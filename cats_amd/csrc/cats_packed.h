@@ -131,20 +131,11 @@ __device__ __forceinline__ const char* uniform(const void* p) {
   const uint64_t a = (uint64_t)p;
   return (const char*)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)a));
 }
-// N KiB from memory straight into LDS, N up to 4: sixteen bytes a lane and load, load j of lane l from  from + at[j]  to  to + 1024 j + 16 l.  As instructions of their own and not
-// the builtin: behind that one every read of LDS would wait for memory, whatever it reads.  They have no result in a register; who reads what they bring waits for
-// vmcnt(0) first.  An offset in the instruction counts on both sides, so one setting of M0 does for four: at[j] has 4096 - 1024 j more than it says, `from` 4096 less.
-template <int N>
-__device__ __forceinline__ void load_lds(const char* from, const unsigned (&at)[N], const void* to) {
+// 1 KiB from memory straight into LDS, sixteen bytes a lane, in the lanes' order from `to` on.  As an instruction of its own and not the builtin: behind that one every read of LDS
+// would wait for memory, whatever it reads.  It has no result in a register; who reads what it brings waits for vmcnt(0) first.
+__device__ __forceinline__ void load_lds(const char* from, unsigned lane_at, const void* to) {
   const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)to);
-  const char* base = from - 4096;
-  if constexpr (N == 4)
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024\n\t"
-                 "global_load_lds_dwordx4 %4, %0 offset:2048\n\tglobal_load_lds_dwordx4 %5, %0 offset:3072" ::"s"(base), "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]) : "memory");
-  else if constexpr (N == 2)
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024" ::"s"(base), "s"(lds), "v"(at[0]), "v"(at[1]) : "memory");
-  else
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0" ::"s"(base), "s"(lds), "v"(at[0]) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0" ::"s"(from), "s"(lds), "v"(lane_at) : "memory");
 }
 template <int D> __device__ __forceinline__ constexpr int tile_swap_k(int t) {
   return D >= 128 ? t & 15 : D == 64 ? t >> 1 & 7 : t >> 2 & 3;
@@ -246,32 +237,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
       return {from, end - 1 - from, 0u};
     }
   };
-  constexpr int AT = LOADS < 4 ? LOADS : 4, PARTS = LOADS / AT;  // loads of one instruction sequence, and how many of those
-  // where the lanes read, in bytes from the first of the sixteen tokens on, for load_lds; last: the last token that is read
-  auto lanes = [&](bool values, int last, unsigned (&to)[PARTS][AT]) {
+  // where the lanes read, in bytes from the first of the sixteen tokens on; last: the last token that is read
+  auto lanes = [&](bool values, int last, unsigned (&to)[LOADS]) {
     const unsigned piece = values ? v_piece : k_piece, step = values ? v_row : k_row;
 #pragma unroll
-    for (int j = 0; j < LOADS; j++)
-      to[j / AT][j % AT] = min((int)t_lane + STEP * j, last) * step + (piece ^ (16u * (values ? tile_swap_v<D>(STEP * j) : tile_swap_k<D>(STEP * j)))) + 4096 - 1024 * (j % AT);
+    for (int j = 0; j < LOADS; j++) to[j] = min((int)t_lane + STEP * j, last) * step + (piece ^ (16u * (values ? tile_swap_v<D>(STEP * j) : tile_swap_k<D>(STEP * j))));
   };
-  unsigned k_lanes[PARTS][AT], v_lanes[PARTS][AT];
-  lanes(false, 15, k_lanes);
-  lanes(true, 15, v_lanes);
+  unsigned k_lanes[LOADS], v_lanes[LOADS];
+  auto all_lanes = [&] {
+    lanes(false, 15, k_lanes);
+    lanes(true, 15, v_lanes);
 #pragma unroll
-  for (int j = 0; j < LOADS; j++) asm volatile("" : "+v"(k_lanes[j / AT][j % AT]), "+v"(v_lanes[j / AT][j % AT]));
-  auto bring = [&](const Place& pl, bool values, u32x4* to) {
-    const char* from = uniform((values ? v_base : k_base) + (PAGED ? pl.at : pl.at * (values ? p.v_tok : p.k_tok)));
+    for (int j = 0; j < LOADS; j++) asm volatile("" : "+v"(k_lanes[j]), "+v"(v_lanes[j]));
+  };
+  all_lanes();
+  // Where a tile's keys or values are; behind one whose tokens end, none is read whose tokens do not.
+  auto aim = [&](const Place& pl, bool values) {
     const int last = __builtin_amdgcn_readfirstlane(pl.last);
-    to += 16 * wave * PK;
-    if (last >= 15) {
+    if (__builtin_expect(last < 15, 0)) lanes(values, last, values ? v_lanes : k_lanes);
+    return uniform((values ? v_base : k_base) + (PAGED ? pl.at : pl.at * (values ? p.v_tok : p.k_tok)));
+  };
+  auto bring = [&](const Place& pl, bool values, u32x4* to) {
+    const char* from = aim(pl, values);
 #pragma unroll
-      for (int i = 0; i < PARTS; i++) load_lds<AT>(from, values ? v_lanes[i] : k_lanes[i], to + i * AT * kWave);
-    } else {
-      unsigned some[PARTS][AT];
-      lanes(values, last, some);
-#pragma unroll
-      for (int i = 0; i < PARTS; i++) load_lds<AT>(from, some[i], to + i * AT * kWave);
-    }
+    for (int j = 0; j < LOADS; j++) load_lds(from, values ? v_lanes[j] : k_lanes[j], to + 16 * wave * PK + j * kWave);
   };
 
   float top = -FLT_MAX, sum = 0.f;
@@ -291,7 +280,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
     return add;
   };
   auto settle = [&](f32x16& s, u32x4 (&pf)[2], float add) {  // of the weights that are in pf now; what o holds is of keys before
-    if (__any(add > (far ? -1.f : Limit<DT>::SUM))) {
+    if (__builtin_expect(__any(add > (far ? -1.f : Limit<DT>::SUM)), 0)) {
       float mx = s[0];
 #pragma unroll
       for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[e]);
@@ -317,7 +306,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
   const int cut = p.window && pos_hi >= p.window ? (pos_hi - p.window) / kTileKeys : -1, own = (pos_lo + 1) / kTileKeys;  // last and first of them
   // half u of a tile: what replaces scores of keys that the query does not see, those behind it and those that a window hides, and of places that are no page's
   auto mask = [&](f32x16& s, int tile, int u, unsigned none, float hidden) {
-    if (PAGED && none) {
+    if (PAGED && __builtin_expect(none != 0, 0)) {
 #pragma unroll
       for (int e = 0; e < 16; e++)
         if (none >> (2 * u + e / 8) & 1) s[e] = NAN;
@@ -357,8 +346,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
     lds_barrier();
   };
   // The weights of half a tile from its scores `now`, beside the products of the half before, whose weights are `before`, and the scores of the half behind: of each an
-  // eighth in turn, operands read two ahead, the argument of an exponential one.  Matrix cores and the rest of a SIMD then work at once.
-  auto turn_of = [&](auto VALUES, auto KEYS, f32x16& now, f32x16& behind, const u32x4 (&before)[2], u32x4 (&pf)[2], const u32x4* values, const u32x4* keys) {
+  // eighth in turn, operands read two ahead, the argument of an exponential one.  Matrix cores and the rest of a SIMD then work at once.  load(i): the i-th of 2 LOADS
+  // loads into LDS, which take their time to be issued.
+  auto turn_of = [&](auto VALUES, auto KEYS, f32x16& now, f32x16& behind, const u32x4 (&before)[2], u32x4 (&pf)[2], const u32x4* values, const u32x4* keys, auto load) {
     constexpr int N = 2 * NW, STEPS = N > 8 ? N : 8;
     const float off = F::HEAD - F::SLACK - top;
     u32x4 x[3], y[3];
@@ -391,6 +381,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
           if (k + 2 < N) x[(k + 2) % 3] = value(values, k + 2);
         }
       }
+      if (i * 2 * LOADS % STEPS == 0) load(i * 2 * LOADS / STEPS);
       if (i * 8 % STEPS == 0) {
         const int j = i * 8 / STEPS;
         w[j & 1] = f32x2v{__builtin_amdgcn_exp2f(arg[j & 1][0]), __builtin_amdgcn_exp2f(arg[j & 1][1])};
@@ -427,25 +418,28 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
 #pragma unroll
   for (int i = 0; i < C; i++) s0 = Mma32<DT>::run(key(s_kv[0][0], i), qf[i], s0);
   auto masked = [&](f32x16& s, int tile, int u, unsigned none) {
-    if (tile >= own || tile <= cut || none) mask(s, tile, u, none, -INFINITY);
+    if (__builtin_expect(tile >= own || tile <= cut || none, 0)) mask(s, tile, u, none, -INFINITY);
   };
   masked(s0, tile, 0, at0.none);
-  turn_of(no, yes, s0, s1, p1, p0, nullptr, s_kv[0][0] + HALF);
+  const auto nothing = [](int) {};
+  turn_of(no, yes, s0, s1, p1, p0, nullptr, s_kv[0][0] + HALF, nothing);
   for (; tile < tile_hi; tile++, buf ^= 1) {
     at2 = place_of(tile + 2);
     arrive();
-    bring(at1, true, s_kv[buf ^ 1][1]);
-    if (tile + 2 <= tile_hi) bring(at2, false, s_kv[buf][0]);
+    const char *v_from = aim(at1, true), *k_from = aim(at2, false);
     ask(tile + 3);
     masked(s1, tile, 1, at0.none);
-    turn_of(yes, yes, s1, s0, p0, p1, s_kv[buf][1], s_kv[buf ^ 1][0]);
+    turn_of(yes, yes, s1, s0, p0, p1, s_kv[buf][1], s_kv[buf ^ 1][0], [&](int i) {
+      if (i < LOADS) load_lds(v_from, v_lanes[i], s_kv[buf ^ 1][1] + 16 * wave * PK + i * kWave);
+      else load_lds(k_from, k_lanes[i - LOADS], s_kv[buf][0] + 16 * wave * PK + (i - LOADS) * kWave);
+    });
     masked(s0, tile + 1, 0, at1.none);
-    turn_of(yes, yes, s0, s1, p1, p0, s_kv[buf][1] + HALF, s_kv[buf ^ 1][0] + HALF);
+    turn_of(yes, yes, s0, s1, p1, p0, s_kv[buf][1] + HALF, s_kv[buf ^ 1][0] + HALF, nothing);
     at0 = at1, at1 = at2;
   }
   arrive();
   masked(s1, tile, 1, at0.none);
-  turn_of(yes, no, s1, s0, p0, p1, s_kv[buf][1], nullptr);
+  turn_of(yes, no, s1, s0, p0, p1, s_kv[buf][1], nullptr, nothing);
 #pragma unroll
   for (int i = 0; i < 2 * NW; i++) o[i % NW] = Mma32<DT>::run(value(s_kv[buf][1] + HALF, i), p1[i / NW], o[i % NW]);
 
@@ -457,6 +451,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
       ask(tile);
       const Place at = place_of(tile);
       lds_barrier();
+      if (tile == tile_lo) all_lanes();
       bring(at, false, s_kv[0][0]);
       bring(at, true, s_kv[0][1]);
       arrive();
