@@ -35,6 +35,9 @@ template <>
 hipError_t launch_packed_attn<CATS_DT>(int D, const PackedPlan* plan, PackedAttnArgs a, hipStream_t stream) {
   return for_head_dim(D, [&](auto d) {
     constexpr int HD = decltype(d)::value;
+    a.by_group = divisor(a.group);
+    a.by_heads = divisor(a.kv_heads);
+    a.by_members = divisor(a.members > 0 ? a.members : 1);
     if (!plan || !plan->step) {
       a.slots = packed_slots(a.seq.N, a.seq.B + 2, a.group, kTileRows);
       const int all = a.seq.N * a.group / kTileRows * a.kv_heads, cus = current_device_cus();
@@ -46,6 +49,8 @@ hipError_t launch_packed_attn<CATS_DT>(int D, const PackedPlan* plan, PackedAttn
     a.group_splits = plan->group_splits;
     a.slots = packed_slots(a.seq.N, a.seq.B + 2, a.group, kStepBlock);
     a.group_slots = a.group_splits ? packed_slots(a.seq.N, a.seq.B / a.members + 2, a.group, kStepBlock) : 0;
+    a.by_splits = divisor(a.splits);
+    a.by_group_splits = divisor(a.group_splits > 0 ? a.group_splits : 1);
     hipError_t e = launch_kernel(packed_attn_step_kernel<CATS_DT, HD>, dim3((a.slots * a.splits + a.group_slots * a.group_splits) * a.kv_heads), dim3(256), 0, stream, a);
     if (e != hipSuccess || a.splits + a.group_splits == 1) return e;
     return launch_kernel(packed_join_kernel<CATS_DT, HD>, dim3((unsigned)(((long long)a.seq.N * a.kv_heads * a.group + 3) / 4)), dim3(256), 0, stream, a);

@@ -4,6 +4,18 @@
 
 namespace cats {
 
+// n / d for n below 2^31, by a product: 2^(31 + shift) / d rounded up has 32 bits, and is near enough for 31 of n.
+struct Divisor {
+  unsigned mul;
+  int shift;
+  __device__ __forceinline__ int operator()(int n) const { return (int)(__umulhi((unsigned)n << 1, mul) >> shift); }
+};
+inline Divisor divisor(int d) {
+  int shift = 0;
+  while ((1ll << shift) < d) shift++;
+  return {(unsigned)(((1ull << (31 + shift)) + d - 1) / d), shift};
+}
+
 struct PackedAttnArgs {
   const uint16_t* q;  // (N, heads, D) in elements: strides of a token and a head
   long long q_tok, q_head;
@@ -28,6 +40,7 @@ struct PackedAttnArgs {
   // exponent and sum of weights
   float* part;
   int splits, group_slots, group_splits;  // of the sequences' own keys; of what their groups share
+  Divisor by_group, by_heads, by_members, by_splits, by_group_splits;  // group, kv_heads ..
 };
 
 // Row r of a (sequence, cached head) pair is head r % group of token r / group, and a workgroup has up to ROWS of them.  Which ones it finds by its slot: set i has the
@@ -74,12 +87,12 @@ __device__ __forceinline__ T load_uniform(const T* p) {  // through the scalar c
 
 // Pages that sequence s, whose first new token is at `start`, reads through the first one of its group: those that lie wholly within what is shared.
 __device__ __forceinline__ int shared_pages(const PackedAttnArgs& p, int s, int start) {
-  const long long n = load_uniform(p.shared + s / p.members * p.shared_step);
+  const long long n = load_uniform(p.shared + p.by_members(s) * p.shared_step);
   return (int)(n < 0 ? 0 : n > start ? start : n) >> p.pool.page_log;
 }
 
 __device__ __forceinline__ uint16_t* packed_out(const PackedAttnArgs& p, int tok0, int c, int r, int D) {
-  const int t = r / p.group;
+  const int t = p.by_group(r);
   return p.out + ((long long)(tok0 + t) * p.kv_heads * p.group + c * p.group + (r - t * p.group)) * D;
 }
 // Rows r0 .. r0 + count - 1 of `rows` all alike.
@@ -150,12 +163,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
   typedef Kv<DT> F;
   __shared__ u32x4 s_kv[2][2][kVecs];  // [buffer][keys, values]
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 31, h = lane >> 5;
-  // The last slots first, which have the most keys of a sequence; two that hold nothing if the tokens are all somebody's behind the others.  Where a CU has two workgroups
+  // The last slots first, which have the most keys of a sequence; three that hold nothing if the tokens are all somebody's behind the others.  Where a CU has two workgroups
   // at once, the second ones come the other way round, so that those with the most keys are beside those with the fewest.
-  const int all = (p.slots - 2) * p.kv_heads;
+  const int all = (p.slots - 3) * p.kv_heads;
   int turn = blockIdx.x;
   if (turn < all && turn >= p.turn) turn = all - 1 - (turn - p.turn);
-  const int c = turn % p.kv_heads, slot = turn < all ? p.slots - 3 - turn / p.kv_heads : 2 * p.slots - 3 - turn / p.kv_heads;
+  const int order = p.by_heads(turn), c = turn - order * p.kv_heads, slot = turn < all ? p.slots - 3 - order : order == p.slots - 3 ? 0 : order;
   const int B = p.seq.B;
   const PackedRows at = packed_rows<ROWS>(B + 2, slot, p.group, [&](int i) { return i == 0 ? 0 : i > B + 1 ? p.seq.N : packed_at(p.seq, i - 1); },
                                           [&](int i) -> long long {
@@ -176,7 +189,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
     pages.table = pages.common = p.pool.table + seq * p.pool.table_stride;
     if (p.shared && live) {
       pages.alike = shared_pages(p, seq, pos0);
-      pages.common = p.pool.table + seq / p.members * p.members * p.pool.table_stride;
+      pages.common = p.pool.table + p.by_members(seq) * p.members * p.pool.table_stride;
     }
     k_base = p.pool.k + ((long long)c << p.pool.page_log) * D;
     v_base = p.pool.v + ((long long)c << p.pool.page_log) * D;
@@ -187,13 +200,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
     v_base = p.v + key0 * p.v_tok + c * p.v_head;
   }
   const int end = pos0 + n;  // keys
-  const int pos_lo = pos0 + r0 / p.group, pos_hi = pos0 + (min(r0 + ROWS, rows) - 1) / p.group;
+  const int pos_lo = pos0 + p.by_group(r0), pos_hi = pos0 + p.by_group(min(r0 + ROWS, rows) - 1);
   if (!live || !ok || pos_hi < 0) return packed_fill<D>(p, tok0, c, r0, ROWS, rows, live && !ok ? DT::fromf(NAN) * 0x10001u : 0u);
   pages.lo = p.window ? max(0, pos_lo - p.window + 1) : 0;
   pages.hi = pos_hi;
   const int tile_lo = pages.lo / kTileKeys, tile_hi = pos_hi / kTileKeys;
 
-  const int mine = r0 + 32 * wave + m, row = min(mine, rows - 1), tok = row / p.group, pos = pos0 + tok;
+  const int mine = r0 + 32 * wave + m, row = min(mine, rows - 1), tok = p.by_group(row), pos = pos0 + tok;
   u32x4 qf[C];
   {
     const uint16_t* q = p.q + (tok0 + tok) * p.q_tok + (c * p.group + row - tok * p.group) * p.q_head;
@@ -536,12 +549,12 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
   typedef Kv<DT> F;
   __shared__ u32x4 s_kv[W][2][kVecs];  // a wave's [keys, values]; or [buffer][half] of the workgroup's keys and, behind them, values: see kt, vt
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
-  const int c = blockIdx.x % p.kv_heads, B = p.seq.B, N = p.seq.N;
-  int rest = blockIdx.x / p.kv_heads;
+  int rest = p.by_heads(blockIdx.x);
+  const int c = blockIdx.x - rest * p.kv_heads, B = p.seq.B, N = p.seq.N;
   const bool common = rest < p.group_slots * p.group_splits;
   if (!common) rest -= p.group_slots * p.group_splits;
-  const int splits = common ? p.group_splits : p.splits, slot = rest / splits, split = rest - slot * splits;
-  const int members = common ? p.members : 1, sets = B / members + 2;
+  const int splits = common ? p.group_splits : p.splits, slot = common ? p.by_group_splits(rest) : p.by_splits(rest), split = rest - slot * splits;
+  const int members = common ? p.members : 1, sets = (common ? p.by_members(B) : B) + 2;
   const PackedRows at = packed_rows<kStepBlock>(sets, slot, p.group, [&](int i) { return i == 0 ? 0 : i == sets ? N : packed_at(p.seq, (i - 1) * members); },
                                                 [&](int i) -> long long { return p.start[min(max(i - 1, 0) * members, B - 1)]; });
   const int rows = at.n * p.group, r0 = at.r0, tok0 = at.tok0, here = min(kStepBlock, rows - r0);
@@ -553,7 +566,7 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
   const long long part0 = (long long)((common ? 0 : p.group_splits) + split) * all;
   float* part_ml = p.part + (long long)(p.splits + p.group_splits) * all * D;
   auto out_row = [&](int r) {  // of (token, head)
-    const int t = r / p.group;
+    const int t = p.by_group(r);
     return (long long)(tok0 + t) * p.kv_heads * p.group + c * p.group + (r - t * p.group);
   };
   auto nothing = [&](float sum) {  // rows that see none of the keys, or (NaN) are no sequence's
@@ -581,7 +594,7 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
   }
   if (!ok) return nothing(NAN);
   auto keys_of = [&](int r) -> Keys {
-    const int t = tok0 + r / p.group;
+    const int t = tok0 + p.by_group(r);
     if (!common) {
       const int pos = start0 + t - tok0;
       return {max(page_tokens(alike), p.window ? pos - p.window + 1 : 0), pos};
@@ -602,7 +615,7 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
     const int first = packed_at(p.seq, b), n = packed_at(p.seq, b + 1) - first;
     if (!(start >= 0 && start <= room - n)) return {0, -1};
     const int pos = (int)start + t - first;
-    const long long shared = p.shared[s0 / members * p.shared_step];
+    const long long shared = p.shared[(at.set - 1) * p.shared_step];
     const int pages = (int)max(0ll, min(shared, start)) >> p.pool.page_log;
     return {p.window ? max(0, pos - p.window + 1) : 0, page_tokens(pages) - 1};
   };
@@ -623,7 +636,7 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
   pages.alike = 0;
   if (alike) {
     pages.alike = alike;
-    pages.common = p.pool.table + s0 / p.members * p.members * p.pool.table_stride;
+    pages.common = p.pool.table + p.by_members(s0) * p.members * p.pool.table_stride;
   }
 
   // each wave its keys and all rows, or its rows and all keys
@@ -636,7 +649,7 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
   const bool idle = wave_rows >= here;                  // a wave without rows, that only brings
   u32x4 qf[C];
   {
-    const int t = row / p.group;
+    const int t = p.by_group(row);
     const uint16_t* q = p.q + (tok0 + t) * p.q_tok + (c * p.group + row - t * p.group) * p.q_head;
 #pragma unroll
     for (int i = 0; i < C; i++) qf[i] = *(const u32x4*)(q + 32 * i + 8 * g);
