@@ -53,7 +53,9 @@ hipError_t launch_packed_attn<CATS_DT>(int D, const PackedPlan* plan, PackedAttn
     a.by_group_splits = divisor(a.group_splits > 0 ? a.group_splits : 1);
     hipError_t e = launch_kernel(packed_attn_step_kernel<CATS_DT, HD>, dim3((a.slots * a.splits + a.group_slots * a.group_splits) * a.kv_heads), dim3(256), 0, stream, a);
     if (e != hipSuccess || a.splits + a.group_splits == 1) return e;
-    return launch_kernel(packed_join_kernel<CATS_DT, HD>, dim3((unsigned)(((long long)a.seq.N * a.kv_heads * a.group + 3) / 4)), dim3(256), 0, stream, a);
+    const long long rows = (long long)a.seq.N * a.kv_heads * a.group;
+    if (a.splits + a.group_splits > 8) return launch_kernel(packed_join_kernel<CATS_DT, HD, true>, dim3((unsigned)rows), dim3(256), 0, stream, a);
+    return launch_kernel(packed_join_kernel<CATS_DT, HD, false>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
   });
 }
 

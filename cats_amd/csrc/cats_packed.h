@@ -536,18 +536,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
 // whose rows are the tokens of all of them, and those of a sequence's own keys.  Sixteen rows are an operand of v_mfma_f32_16x16x32:
 //   S^T = K . Q^T   tile i, row 4 g + e of the result: token 16 i + 4 g + e, in lanes of group g = lane / 16; columns are queries
 //   O^T += V^T . P  operand of 32 tokens: tokens 4 g .. + 3 and 16 + 4 g .. + 3, those whose weights the lane has; V comes turned round out of LDS
-// Where there are up to sixteen rows each wave has 32 keys of its own at a time, in LDS of its own, and waits for nobody; what the waves give is joined in LDS at the end.
-// Where there are more, a wave has sixteen rows, and all of them read tiles of 64 keys that they bring together.
+// Where there are up to sixteen rows each wave has 32 keys of its own at a time and waits for nobody: keys come as operands, values into LDS of the wave's own. What the
+// waves give is joined in LDS at the end.  Where there are more, a wave has sixteen rows, and all of them read tiles of 32 keys that they bring into LDS together.
 constexpr int kStepKeys = 32, kStepBlock = 64;
 template <int D> __device__ __forceinline__ constexpr int step_swap_v(int t) {
   return D >= 128 ? (t & 7) * 2 : D == 64 ? (t >> 1 & 3) * 2 : (t >> 2 & 1) * 2;
 }
-constexpr int packed_step_waves(int D) { return D == 256 ? 1 : 2; }
+constexpr int packed_step_waves(int D) { return D == 256 ? 2 : D == 128 ? 3 : 4; }
 template <class DT, int D>
 __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_kernel(PackedAttnArgs p) {
   constexpr int C = D / 32, NU = D / 16, PK = D / 8, STEP = kWave / PK, W = 4, kVecs = kStepKeys * PK;
   typedef Kv<DT> F;
-  __shared__ u32x4 s_kv[W][2][kVecs];  // a wave's [keys, values]; or [buffer][half] of the workgroup's keys and, behind them, values: see kt, vt
+  constexpr int PITCH = D + 4;
+  __shared__ union {
+    u32x4 own[W][kVecs];        // a wave's values
+    u32x4 common[2][2][kVecs];  // [buffer][keys, values]
+    float joined[W][16][PITCH];
+  } lds;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
   int rest = p.by_heads(blockIdx.x);
   const int c = blockIdx.x - rest * p.kv_heads, B = p.seq.B, N = p.seq.N;
@@ -620,17 +625,37 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
     return {p.window ? max(0, pos - p.window + 1) : 0, page_tokens(pages) - 1};
   };
   auto least = [](int v) {
-#pragma unroll
-    for (int i = 1; i < kWave; i <<= 1) v = min(v, __shfl_xor(v, i, kWave));
-    return __builtin_amdgcn_readfirstlane(v);
+    auto step = [&](auto ctrl) { v = min(v, __builtin_amdgcn_update_dpp(v, v, decltype(ctrl)::value, 0xf, 0xf, false)); };
+    step(std::integral_constant<int, 0xB1>());   // as in wave_sum
+    step(std::integral_constant<int, 0x4E>());
+    step(std::integral_constant<int, 0x141>());
+    step(std::integral_constant<int, 0x140>());
+    return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)), min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
   };
   auto most = [&](int v) { return -least(-v); };
-  // of all rows here, a lane each
-  Keys k = keys_of(r0 + min(lane, here - 1));
-  const bool some = k.lo <= k.hi;
+  // each wave its keys and all rows, or its rows and all keys
+  const bool apart = here <= 16;
+  const int wave_rows = apart ? 0 : 16 * wave;
+  const int src = min(wave_rows + m, here - 1), row = r0 + src;
   PageRows pages;
-  pages.lo = least(some ? k.lo : INT_MAX);
-  pages.hi = most(some ? k.hi : -1);
+  Keys k;
+  int all_lo, all_hi;  // what all of the wave's rows see
+  if (common) {
+    k = keys_of(r0 + min(lane, here - 1));  // of all rows here, a lane each
+    const bool some = k.lo <= k.hi;
+    pages.lo = least(some ? k.lo : INT_MAX);
+    pages.hi = most(some ? k.hi : -1);
+    k.lo = __shfl(k.lo, src, kWave), k.hi = __shfl(k.hi, src, kWave);
+    all_lo = most(k.lo), all_hi = least(k.hi);
+  } else {  // both ends ascend with the row
+    auto ends = [&](int r) {
+      const Keys e = keys_of(r0 + min(r, here - 1));
+      return Keys{__builtin_amdgcn_readfirstlane(e.lo), __builtin_amdgcn_readfirstlane(e.hi)};
+    };
+    k = keys_of(row);
+    pages.lo = ends(0).lo, pages.hi = ends(here - 1).hi;
+    all_lo = ends(wave_rows + 15).lo, all_hi = ends(wave_rows).hi;
+  }
   if (pages.hi < 0) return nothing(0.f);
   pages.table = pages.common = p.pool.table + s0 * p.pool.table_stride;
   pages.alike = 0;
@@ -639,14 +664,7 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
     pages.common = p.pool.table + p.by_members(s0) * p.members * p.pool.table_stride;
   }
 
-  // each wave its keys and all rows, or its rows and all keys
-  const bool apart = here <= 16;
-  const int wave_rows = apart ? 0 : 16 * wave, keys = apart ? kStepKeys : 2 * kStepKeys;
-  const int row = r0 + min(wave_rows + m, here - 1);
-  const int src = min(wave_rows + m, here - 1);
-  k.lo = __shfl(k.lo, src, kWave), k.hi = __shfl(k.hi, src, kWave);
-  const int all_lo = most(k.lo), all_hi = least(k.hi);  // what all of the wave's rows see
-  const bool idle = wave_rows >= here;                  // a wave without rows, that only brings
+  const bool idle = wave_rows >= here;  // a wave without rows, that only brings
   u32x4 qf[C];
   {
     const int t = p.by_group(row);
@@ -654,35 +672,23 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
 #pragma unroll
     for (int i = 0; i < C; i++) qf[i] = *(const u32x4*)(q + 32 * i + 8 * g);
   }
-  const int tile_lo = pages.lo / keys, tile_hi = pages.hi / keys;
-  const int unit = apart ? W : 1, active = min(splits, (tile_hi - tile_lo + unit) / unit);
+  const int tile_lo = pages.lo / kStepKeys, tile_hi = pages.hi / kStepKeys;
+  const int unit = apart ? W : 2, active = min(splits, (tile_hi - tile_lo + unit) / unit);
   if (split >= active) return nothing(0.f);
 
   const unsigned t_lane = lane / PK;
-  unsigned k_piece = ((lane % PK) ^ tile_swap_k<D>(t_lane)) * 16, v_piece = ((lane % PK) ^ step_swap_v<D>(t_lane)) * 16;
   unsigned k_at = (m * PK + (g ^ tile_swap_k<D>(m))) * 16;
   unsigned v_at = ((4 * g + (m >> 2)) * PK + ((m >> 1 & 1) ^ step_swap_v<D>(4 * (g & 1) + (m >> 2)))) * 16 + 8 * (m & 1);
   asm volatile("" : "+v"(k_at), "+v"(v_at));
   const uint16_t* k_base = p.pool.k + page_tokens(c) * (long long)D;
   const uint16_t* v_base = p.pool.v + page_tokens(c) * (long long)D;
-  // sixteen tokens of a run into LDS at k, v
-  auto bring16 = [&](const PageRun& run, u32x4* kt, u32x4* vt) {
-    const long long place = page_place(p.pool, run);
-    const int last = pages.hi - run.from;  // of the sixteen, the last that may be read
-    const char *kf = uniform(k_base + place * D), *vf = uniform(v_base + place * D);
-    unsigned kp = k_piece, vp = v_piece;
-    asm volatile("" : "+v"(kp), "+v"(vp));  // not a register for every load over the loop
-#pragma unroll
-    for (int j = 0; j < PK / 4; j++) {
-      const unsigned t = min((int)t_lane + STEP * j, last);
-      auto load = [&](const char* from, unsigned lane_at, u32x4* to) {
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (size_t)lane_at), (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-      };
-      load(kf, t * (2 * D) + (kp ^ (16u * tile_swap_k<D>(STEP * j))), kt + j * kWave);
-      load(vf, t * (2 * D) + (vp ^ (16u * step_swap_v<D>(STEP * j))), vt + j * kWave);
-    }
+  // Sixteen tokens into LDS; lane l of load j writes piece 64 j + l of them and reads what belongs there.
+  const bool brings_k = !apart && wave < 2;
+  auto lane_at = [&](int j, int last) {
+    const unsigned t = t_lane + STEP * j, piece = (lane % PK) ^ (brings_k ? tile_swap_k<D>(t) : step_swap_v<D>(t));
+    return min((int)t, last) * (2 * D) + piece * 16;
   };
-  unsigned none = 0;  // bit i: tokens 16 i .. + 15 of the tile have no page
+  constexpr int LOADS = PK / 4;
 
   float top = -FLT_MAX, sum = 0.f;
   bool far = false;
@@ -723,27 +729,20 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
     sum += add;
   };
   enum { PLAIN, CLEAN, COUNT };  // gone over again as above
-  // 32 keys from key0 on; `behind` once they are in registers
-  auto take = [&](auto AGAIN, int mode, int key0, unsigned none, const u32x4* kt, const u32x4* vt, auto behind) {
-    u32x4 kk[2][C], vv[NU];
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int j = 0; j < C; j++) kk[i][j] = *(const u32x4*)((const char*)kt + (k_at ^ 64u * j) + 16 * i * PK * 16);
-#pragma unroll
-    for (int u = 0; u < NU; u++) {
-      const u32x2 lo = read_turned((const char*)vt + (v_at ^ 32u * u)), hi = read_turned((const char*)vt + (v_at ^ 32u * u) + 16 * PK * 16);
-      vv[u] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-    }
-    behind();
+  // a tile's scores, its keys and values in LDS or (the keys) in registers
+  auto take = [&](auto AGAIN, int mode, int tile, unsigned none, const u32x4* vt, auto key, auto behind) {
+    const int key0 = tile * kStepKeys;
     f32x4 s[2];
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < C; j++) s[i] = Mma<DT>::run(kk[i][j], qf[j], s[i]);
+      for (int j = 0; j < C; j++) s[i] = Mma<DT>::run(key(i, j), qf[j], s[i]);
     }
-    if (none) {
+    __builtin_amdgcn_sched_barrier(0);
+    behind();
+    __builtin_amdgcn_sched_barrier(0);
+    if (__builtin_expect(none != 0, 0)) {
 #pragma unroll
       for (int i = 0; i < 2; i++)
         if (none >> i & 1) s[i] = f32x4{NAN, NAN, NAN, NAN};
@@ -764,99 +763,102 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
       for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++) s[i][e] = mode == COUNT ? (seen(i, e) ? 1.f : 0.f) : s[i][e];
-#pragma unroll
-      for (int u = 0; u < NU; u++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const uint32_t bad = kv_nan16<DT>(vv[u][e]);
-          vv[u][e] = mode == COUNT ? bad * F::kOne : vv[u][e] & ~(bad * 0xffffu);
-        }
     }
     const u32x4 pf = u32x4{DT::pack(s[0][0], s[0][1]), DT::pack(s[0][2], s[0][3]), DT::pack(s[1][0], s[1][1]), DT::pack(s[1][2], s[1][3])};
+    constexpr int AHEAD = NU < 4 ? NU : 4;  // operands are read four ahead
+    u32x4 x[AHEAD];
+    auto value = [&](int u) {
+      const u32x2 lo = read_turned((const char*)vt + (v_at ^ 32u * u)), hi = read_turned((const char*)vt + (v_at ^ 32u * u) + 16 * PK * 16);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
 #pragma unroll
-    for (int u = 0; u < NU; u++) o[u] = Mma<DT>::run(vv[u], pf, o[u]);
+    for (int u = 0; u < AHEAD; u++) x[u] = value(u);
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4 v = x[u % AHEAD];
+      if (u + AHEAD < NU) x[u % AHEAD] = value(u + AHEAD);
+      if constexpr (AGAIN) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint32_t bad = kv_nan16<DT>(v[e]);
+          v[e] = mode == COUNT ? bad * F::kOne : v[e] & ~(bad * 0xffffu);
+        }
+      }
+      o[u] = Mma<DT>::run(v, pf, o[u]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   };
-  auto here_now = [] {  // what was brought
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    asm volatile("" ::: "memory");
-  };
+  auto none_of = [&](const PageRun (&runs)[2]) { return (unsigned)page_none(p.pool, runs[0]) | (unsigned)page_none(p.pool, runs[1]) << 1; };
   auto sweep = [&](auto AGAIN, int mode) {
 #pragma unroll
     for (int u = 0; u < NU; u++) o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    PageRun runs[2];
+    auto ask = [&](int tile) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) runs[i] = page_run(p.pool, pages, min(tile, tile_hi) * kStepKeys + 16 * i);
+    };
     if (apart) {
-      u32x4 *kt = s_kv[wave][0], *vt = s_kv[wave][1];
       const int step = active * W;
       int tile = tile_lo + split * W + wave;
-      PageRun run[2];
-      auto ask = [&](int tile) {
+      u32x4 kk[2][C];
+      u32x4* vt = lds.own[wave];
+      auto fetch_k = [&] {
 #pragma unroll
-        for (int i = 0; i < 2; i++) run[i] = page_run(p.pool, pages, min(tile, tile_hi) * kStepKeys + 16 * i);
+        for (int i = 0; i < 2; i++) {
+          const char* from = uniform(k_base + page_place(p.pool, runs[i]) * D);
+#pragma unroll
+          for (int j = 0; j < C; j++) kk[i][j] = load_stream((const u32x4*)(from + (size_t)((unsigned)(m * 2 * D + 16 * g) + 64u * j)));
+        }
       };
-      auto bring = [&] {
+      auto bring_v = [&](const PageRun (&runs)[2]) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) bring16(run[i], kt + 16 * i * PK, vt + 16 * i * PK);
+        for (int i = 0; i < 2; i++) {
+          const char* from = uniform(v_base + page_place(p.pool, runs[i]) * D);
+#pragma unroll
+          for (int j = 0; j < LOADS; j++)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (size_t)lane_at(j, pages.hi - runs[i].from)),
+                                             (__attribute__((address_space(3))) void*)(vt + 16 * i * PK + j * kWave), 16, 0, 2);
+        }
       };
       ask(tile);
-      if (tile <= tile_hi) bring();
-      for (; tile <= tile_hi; tile += step) {
-        none = page_none(p.pool, run[0]) | page_none(p.pool, run[1]) << 1;
+      if (tile <= tile_hi) {
+        fetch_k();
+        bring_v(runs);
+      }
+      while (tile <= tile_hi) {
+        const unsigned none = none_of(runs);
+        const bool more = tile + step <= tile_hi;
         ask(tile + step);
-        here_now();
-        take(AGAIN, mode, tile * kStepKeys, none, kt, vt, [&] {
-          __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): read
-          __builtin_amdgcn_sched_barrier(0);
-          if (tile + step <= tile_hi) bring();
-          __builtin_amdgcn_sched_barrier(0);
+        take(AGAIN, mode, tile, none, vt, [&](int i, int j) { return kk[i][j]; }, [&] {
+          if (more) fetch_k();
         });
+        tile += step;
+        if (more) bring_v(runs);
       }
     } else {
-      // [buffer][keys, values] of 64 tokens
-      auto kt = [&](int buf) { return s_kv[2 * buf][0]; };
-      auto vt = [&](int buf) { return s_kv[2 * buf + 1][0]; };
-      unsigned none1 = 0;
-      PageRun runs[4];
-      auto ask = [&](int tile) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) runs[i] = page_run(p.pool, pages, tile * 2 * kStepKeys + 16 * i);
-      };
-      auto bring = [&](int buf) {
-        PageRun mine = runs[0];
-        none1 = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          none1 |= page_none(p.pool, runs[i]) ? 1u << i : 0u;
-          if (i == wave) mine = runs[i];
-        }
-        bring16(mine, kt(buf) + 16 * wave * PK, vt(buf) + 16 * wave * PK);
-      };
       int tile = tile_lo + split, buf = 0;
+      auto bring = [&](int buf) {
+        const PageRun run = {wave & 1 ? runs[1].from : runs[0].from, wave & 1 ? runs[1].id : runs[0].id};
+        const char* from = uniform((brings_k ? k_base : v_base) + page_place(p.pool, run) * D);
+#pragma unroll
+        for (int j = 0; j < LOADS; j++) load_lds(from, lane_at(j, pages.hi - run.from), lds.common[buf][!brings_k] + 16 * (wave & 1) * PK + j * kWave);
+      };
       ask(tile);
       bring(0);
+      unsigned none = none_of(runs);
       ask(tile + active);
-      here_now();
-      none = none1;
-      lds_barrier();
       for (; tile <= tile_hi; tile += active, buf ^= 1) {
-        const bool more = tile + active <= tile_hi;
-        auto next = [&] {
-          if (more) bring(buf ^ 1);
-          ask(tile + 2 * active);
-        };
-        if (idle) {
-          next();
-        } else {
-          take(AGAIN, mode, tile * 2 * kStepKeys, none & 3, kt(buf), vt(buf), [] {});
-          take(AGAIN, mode, tile * 2 * kStepKeys + kStepKeys, none >> 2, kt(buf) + kStepKeys * PK, vt(buf) + kStepKeys * PK, [&] {
-            __builtin_amdgcn_s_waitcnt(0xc07f);
-            __builtin_amdgcn_sched_barrier(0);
-            next();
-            __builtin_amdgcn_sched_barrier(0);
-          });
-        }
-        here_now();
-        none = none1;
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): what was brought is in LDS, and all have read what is overwritten
         lds_barrier();
+        if (tile + active <= tile_hi) bring(buf ^ 1);
+        const unsigned now = none;
+        none = none_of(runs);
+        ask(tile + 2 * active);
+        if (!idle)
+          take(AGAIN, mode, tile, now, lds.common[buf][1], [&](int i, int j) { return *(const u32x4*)((const char*)lds.common[buf][0] + (k_at ^ 64u * j) + 16 * i * PK * 16); }, [] {});
       }
+      lds_barrier();
     }
   };
   sweep(std::false_type(), PLAIN);
@@ -876,8 +878,6 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
 
   // the waves' results, and where the tiles have to be gone over again, what is to be put there instead
   __shared__ float s_top[W][16], s_sum[W][16];
-  float* s_o = (float*)s_kv;  // [wave or 0][16][D + 4]
-  constexpr int PITCH = D + 4;
   auto write_row = [&](int r, int d, f32x4 x, float mx, float den) {  // r: of the workgroup's
     const long long to = out_row(r0 + r);
     if (!joined) {
@@ -913,7 +913,7 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
     }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < NU; u++) *(f32x4*)(s_o + (wave * 16 + m) * PITCH + 16 * u + 4 * g) = o[u];
+    for (int u = 0; u < NU; u++) *(f32x4*)&lds.joined[wave][m][16 * u + 4 * g] = o[u];
     if (!count && g == 0) {
       s_top[wave][m] = top;
       s_sum[wave][m] = sum;
@@ -929,7 +929,7 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
 #pragma unroll
       for (int w = 0; w < W; w++) {
         const float f = count ? 1.f : __builtin_amdgcn_exp2f(s_top[w][r] - mx);
-        const f32x4 x = *(const f32x4*)(s_o + (w * 16 + r) * PITCH + d);
+        const f32x4 x = *(const f32x4*)&lds.joined[w][r][d];
 #pragma unroll
         for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e]);
         den = fmaf(f, s_sum[w][r], den);
@@ -946,12 +946,12 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
   }
 }
 
-// The splits' results, in a fixed order: a wave a row, whose groups of D / 4 lanes take every so manieth split.
-template <class DT, int D>
+// The splits' results, in a fixed order.  ALONE: a workgroup a row, else a wave a row; groups of D / 4 lanes take every so manieth split.
+template <class DT, int D, bool ALONE>
 __global__ __launch_bounds__(256) void packed_join_kernel(PackedAttnArgs p) {
-  constexpr int L = D / 4, G = kWave / L;
-  const int lane = threadIdx.x & (kWave - 1), grp = lane / L, d = lane % L * 4, n = p.splits + p.group_splits;
-  const long long all = (long long)p.seq.N * p.kv_heads * p.group, r = (long long)blockIdx.x * 4 + threadIdx.x / kWave;
+  constexpr int L = D / 4, G = (ALONE ? 256 : kWave) / L;
+  const int tid = ALONE ? threadIdx.x : threadIdx.x & (kWave - 1), grp = tid / L, d = tid % L * 4, n = p.splits + p.group_splits;
+  const long long all = (long long)p.seq.N * p.kv_heads * p.group, r = ALONE ? blockIdx.x : (long long)blockIdx.x * 4 + threadIdx.x / kWave;
   if (r >= all) return;
   const float* ml = p.part + n * all * D + 2 * r;
   const float* part = p.part + r * D + d;
@@ -960,8 +960,8 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedAttnArgs p) {
 #pragma unroll 4
   for (int s = grp; s < n; s += G) {
     const float mx = ml[2 * s * all], sm = ml[2 * s * all + 1];
-    if (sm == 0.f) continue;  // nothing has been written
-    const f32x4 x = *(const f32x4*)(part + s * all * D);
+    f32x4 x = *(const f32x4*)(part + s * all * D);
+    if (sm == 0.f) x = f32x4{0.f, 0.f, 0.f, 0.f};  // nothing has been written
     const float now = fmaxf(top, mx), keep = __builtin_amdgcn_exp2f(top - now), f = __builtin_amdgcn_exp2f(mx - now);
 #pragma unroll
     for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e] * keep);
@@ -976,7 +976,36 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedAttnArgs p) {
     den = fmaf(f, __shfl_xor(den, i, kWave), den * keep);
     top = now;
   }
-  if (grp != 0) return;
+  if constexpr (ALONE) {
+    constexpr int W = 4;
+    __shared__ __align__(16) float s_o[W][D];
+    __shared__ float s_top[W], s_sum[W];
+    const int wave = threadIdx.x / kWave;
+    if ((threadIdx.x & (kWave - 1)) < L) {
+      *(f32x4*)&s_o[wave][d] = num;
+      if (d == 0) {
+        s_top[wave] = top;
+        s_sum[wave] = den;
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x >= L) return;
+    float most = s_top[0];
+#pragma unroll
+    for (int i = 1; i < W; i++) most = fmaxf(most, s_top[i]);
+    num = f32x4{0.f, 0.f, 0.f, 0.f};
+    den = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+      const float f = __builtin_amdgcn_exp2f(s_top[i] - most);
+      const f32x4 x = *(const f32x4*)&s_o[i][d];
+#pragma unroll
+      for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e]);
+      den = fmaf(f, s_sum[i], den);
+    }
+  } else if (grp != 0) {
+    return;
+  }
   const float f = den == 0.f ? 0.f : 1.f / den;
   *(u32x2*)(p.out + r * D + d) = u32x2{DT::pack(num[0] * f, num[1] * f), DT::pack(num[2] * f, num[3] * f)};
 }
