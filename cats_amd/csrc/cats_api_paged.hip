@@ -60,16 +60,19 @@ PackedPlan paged_plan(int N, int B, int heads, int kv_heads, int page, int width
   const int cus = current_device_cus(), group = heads / kv_heads;
   const long long room = (long long)width * page, keys = window ? (room < window + 64ll ? room : window + 64ll) : room;
   const long long rows = ((long long)N * group + B - 1) / B;  // of a sequence, on average
-  const long long many = (long long)kv_heads * (((long long)N * group + kTileRows - 1) / kTileRows);
-  PackedPlan plan = {rows <= 16 || many < cus / 2, 1, members > 1 ? 1 : 0};
-  if (!plan.step) return {false, 1, 0};
-  auto splits = [&](long long sets, long long set_rows) {
-    const long long groups = kv_heads * sets * ((set_rows + kStepBlock - 1) / kStepBlock), want = (2ll * cus + groups - 1) / groups;
-    const long long units = keys / (set_rows <= 16 ? 128 : 64);
+  auto splits = [&](bool tiles, long long sets, long long set_rows) {
+    const int most = tiles ? kTileRows : kStepRows;
+    const long long groups = kv_heads * sets * ((set_rows + most - 1) / most), want = ((tiles ? 1ll : 2ll) * cus + groups - 1) / groups;
+    const long long units = keys / (tiles ? kSplitTiles * kTileKeys : 128);
     return (int)(keys <= 1024 ? 1 : want < units ? want : units);
   };
-  plan.splits = splits(B, rows);
-  if (members > 1) plan.group_splits = splits(B / members, rows * members);
+  PackedPlan plan = {};
+  plan.tiles = rows > 32;
+  plan.splits = splits(plan.tiles, B, rows);
+  if (members > 1 && !plan.tiles) {
+    plan.group_tiles = rows * members > 32;
+    plan.group_splits = splits(plan.group_tiles, B / members, rows * members);
+  }
   return plan;
 }
 // What the splits leave, for the join.

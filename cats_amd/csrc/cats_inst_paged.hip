@@ -38,20 +38,24 @@ hipError_t launch_packed_attn<CATS_DT>(int D, const PackedPlan* plan, PackedAttn
     a.by_group = divisor(a.group);
     a.by_heads = divisor(a.kv_heads);
     a.by_members = divisor(a.members > 0 ? a.members : 1);
-    if (!plan || !plan->step) {
-      a.slots = packed_slots(a.seq.N, a.seq.B + 2, a.group, kTileRows);
-      const int all = a.seq.N * a.group / kTileRows * a.kv_heads, cus = current_device_cus();
-      a.turn = all <= 2 * cus && all > cus ? cus : INT_MAX;
-      return launch_kernel(plan ? packed_attn_tiles_kernel<CATS_DT, HD, true> : packed_attn_tiles_kernel<CATS_DT, HD, false>, dim3(a.slots * a.kv_heads), dim3(256), 0,
+    const int N = a.seq.N, B = a.seq.B;
+    if (!plan || (plan->tiles && plan->splits + plan->group_splits == 1)) {
+      a.slots = packed_slots(N, B + 2, a.group, kTileRows);
+      a.cus = current_device_cus();
+      return launch_kernel(plan ? packed_attn_tiles_kernel<CATS_DT, HD, PAGES> : packed_attn_tiles_kernel<CATS_DT, HD, PROMPT>, dim3(a.slots * a.kv_heads), dim3(256), 0,
                            stream, a);
     }
     a.splits = plan->splits;
     a.group_splits = plan->group_splits;
-    a.slots = packed_slots(a.seq.N, a.seq.B + 2, a.group, kStepBlock);
-    a.group_slots = a.group_splits ? packed_slots(a.seq.N, a.seq.B / a.members + 2, a.group, kStepBlock) : 0;
     a.by_splits = divisor(a.splits);
     a.by_group_splits = divisor(a.group_splits > 0 ? a.group_splits : 1);
-    hipError_t e = launch_kernel(packed_attn_step_kernel<CATS_DT, HD>, dim3((a.slots * a.splits + a.group_slots * a.group_splits) * a.kv_heads), dim3(256), 0, stream, a);
+    const int rows_of[2] = {kStepRows, kTileRows};
+    a.group_blocks = a.group_splits ? a.group_splits * packed_slots(N, B / a.members + 2, a.group, rows_of[plan->group_tiles]) : 0;
+    const dim3 grid((a.group_blocks + a.splits * packed_slots(N, B + 2, a.group, rows_of[plan->tiles])) * a.kv_heads);
+    const hipError_t e = launch_kernel(plan->tiles         ? packed_attn_tiles_kernel<CATS_DT, HD, SPLIT>
+                                       : plan->group_tiles ? packed_attn_both_kernel<CATS_DT, HD>
+                                                           : packed_attn_step_kernel<CATS_DT, HD>,
+                                       grid, dim3(256), 0, stream, a);
     if (e != hipSuccess || a.splits + a.group_splits == 1) return e;
     const long long rows = (long long)a.seq.N * a.kv_heads * a.group;
     if (a.splits + a.group_splits > 8) return launch_kernel(packed_join_kernel<CATS_DT, HD, true>, dim3((unsigned)rows), dim3(256), 0, stream, a);

@@ -11,8 +11,8 @@ hipError_t launch_paged_append(int D, bool wide, const PagedAppendArgs& a, hipSt
 
 // Which kernel attention over pages takes, and into how many parts it splits keys.
 struct PackedPlan {
-  bool step;                 // packed_attn_step_kernel
-  int splits, group_splits;  // of a sequence's own keys; of those that its group shares (0: none are)
+  bool tiles, group_tiles;   // packed_attn_tiles_kernel, and not packed_attn_step_kernel, for a sequence's own keys, and for those that its group shares
+  int splits, group_splits;  // 0: none are shared
 };
 // plan NULL: keys and values of the call.  launch_packed_attn fills in what the plan decides.
 template <class DT>

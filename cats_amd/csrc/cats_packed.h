@@ -34,47 +34,109 @@ struct PackedAttnArgs {
   float scale;        // log2(e) * the softmax's scale
   int kv_heads, group;  // group: query heads of a cached head
   int window;         // keys that a query sees, at most; 0: all
-  int turn;           // workgroups from here on come the other way round
-  int slots;          // of a launch of many tokens, of the sequences' own keys
-  // few tokens: keys are split, and what the splits give is in `part`: [split][token, head][D] sums and, behind them, [split][token, head][2] largest
-  // exponent and sum of weights
+  int cus;
+  int slots;          // of the launch
+  // Keys that are split: what the splits give is in `part`: [split][token, head][D] sums and, behind them, [split][token, head][2] largest exponent and sum of
+  // weights.  The first group_splits are of the keys that a group of sequences shares, the others of a sequence's own.
   float* part;
-  int splits, group_slots, group_splits;  // of the sequences' own keys; of what their groups share
+  int splits, group_splits;
+  int group_blocks;  // of the launch, without kv_heads: those of shared keys, which come first
   Divisor by_group, by_heads, by_members, by_splits, by_group_splits;  // group, kv_heads ..
 };
 
-// Row r of a (sequence, cached head) pair is head r % group of token r / group, and a workgroup has up to ROWS of them.  Which ones it finds by its slot: set i has the
-// slots from  first token of it * group / ROWS + i  on, which is room enough for any lengths.  Set 0 are the tokens before the first sequence, set i sequence i - 1,
-// and the last one the tokens behind the last; a call has packed_slots() of them.
+// Row r of a (sequence, cached head) pair is head r % group of token r / group, and a workgroup has up to ROWS of them.  Which ones it finds by its slot: set 0 are the
+// tokens before the first sequence, set i sequence i - 1, and the last one the tokens behind the last.  Up to 255 of them, their slots come one
+// behind the other and those that nobody needs behind them all; else set i has those from  first token of it * group / ROWS + i  on.  packed_slots() are enough
+// for any lengths.  (With gaps everywhere the workgroups that have work are spread unevenly over the CUs: a step of 32 sequences took 88 us for 72.)
 inline int packed_slots(int N, int sets, int group, int rows) { return (int)((long long)N * group / rows) + sets; }
+constexpr int kPackedScan = 4;  // sets that a lane has, at most
 struct PackedRows {
   int set, tok0, n, r0;  // n: tokens of the set; r0: the workgroup's first row of it
   long long word;        // what the caller asked for of the set
 };
-// start_of(i): first token of set i (i = sets: N); word(i): something of set i that is worth a trip to memory beside it.
-template <int ROWS, class S, class W>
-__device__ __forceinline__ PackedRows packed_rows(int sets, int slot, int group, S start_of, W word) {
+__device__ __forceinline__ int sum_up_to(int v) {  // of the lanes up to this one
+  auto step = [&](auto ctrl, auto rows) { v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false); };
+  step(std::integral_constant<int, 0x111>(), std::integral_constant<int, 0xf>());  // row_shr
+  step(std::integral_constant<int, 0x112>(), std::integral_constant<int, 0xf>());
+  step(std::integral_constant<int, 0x114>(), std::integral_constant<int, 0xf>());
+  step(std::integral_constant<int, 0x118>(), std::integral_constant<int, 0xf>());
+  step(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());  // row_bcast:15
+  step(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());  // row_bcast:31
+  return v;
+}
+// slot_of(n): the workgroup's slot, of n that may have work.  start_of(i): first token of set i (i = sets: N); word(i): something of set i that is worth a trip to memory
+// beside it.
+template <int ROWS, class O, class S, class W>
+__device__ __forceinline__ PackedRows packed_rows(int sets, int slots, int group, O slot_of, S start_of, W word) {
   const int lane = threadIdx.x & (kWave - 1);
-  int lo = 0, n = sets;
-  auto base = [&](int i, int tok) { return (long long)tok * group / ROWS + i; };
-  while (n >= kWave) {
-    const int step = (n + kWave - 1) / kWave;
-    const bool in = lane * step < n;
-    const int i = lo + (in ? lane * step : 0);
-    const uint64_t below = __ballot(in && base(i, start_of(i)) <= slot);
-    const int last = below ? 63 - __builtin_clzll(below) : 0;
-    lo += last * step;
-    n = min(step, n - last * step);
-  }
-  const int i = lo + min(lane, n), tok = start_of(i);  // one more than the candidates: where the last of them ends
-  const long long w = word(min(i, sets - 1));
-  const uint64_t below = __ballot(lane < n && base(i, tok) <= slot);
-  const int last = below ? 63 - __builtin_clzll(below) : 0;
   PackedRows r;
-  r.set = __builtin_amdgcn_readfirstlane(lo + last);  // (the compiler does not see that these are the same in all lanes)
-  r.tok0 = __builtin_amdgcn_readlane(tok, last);
-  r.n = __builtin_amdgcn_readfirstlane(max(0, __builtin_amdgcn_readlane(tok, last + 1) - r.tok0));
-  const long long first = slot - base(r.set, r.tok0);
+  long long w, first;
+  int last;
+  auto scan = [&](auto chunks) {
+    constexpr int C = decltype(chunks)::value;
+    int tok[C], n[C], upto[C], all = 0;
+    long long words[C];
+#pragma unroll
+    for (int i = 0; i < C; i++) {
+      tok[i] = n[i] = words[i] = 0;
+      if (i == 0 || i * kWave < sets) {
+        const int set = i * kWave + lane;
+        tok[i] = start_of(min(set, sets));
+        n[i] = max(0, start_of(min(set + 1, sets)) - tok[i]);
+        words[i] = word(min(set, sets - 1));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < C; i++) {
+      upto[i] = all;
+      if (i == 0 || i * kWave < sets) {
+        upto[i] += sum_up_to((n[i] * group + ROWS - 1) / ROWS);
+        all = __builtin_amdgcn_readlane(upto[i], kWave - 1);
+      }
+    }
+    const int slot = slot_of(all);
+    int at = 0, toks = 0, ns = 0, before = 0;  // of the chunk that it is in, which the last one is that begins at or before it
+    w = 0, last = 0;
+#pragma unroll
+    for (int i = C - 1; i >= 0; i--) {
+      const uint64_t above = __ballot(upto[i] > slot);
+      if (above) {
+        last = __builtin_ctzll(above), at = i, toks = tok[i], ns = n[i], w = words[i];
+        before = __builtin_amdgcn_readlane(upto[i], last) - (__builtin_amdgcn_readlane(n[i], last) * group + ROWS - 1) / ROWS;
+      }
+    }
+    r.set = at * kWave + last;
+    r.tok0 = __builtin_amdgcn_readlane(toks, last);
+    r.n = __builtin_amdgcn_readlane(ns, last);
+    first = slot < all ? slot - before : INT_MAX;
+  };
+  if (sets < kWave) {
+    scan(std::integral_constant<int, 1>());
+  } else if (sets < kPackedScan * kWave) {
+    scan(std::integral_constant<int, kPackedScan>());
+  } else {
+    const int slot = slot_of(slots);
+    int lo = 0, n = sets;
+    auto base = [&](int i, int tok) { return (long long)tok * group / ROWS + i; };
+    while (n >= kWave) {
+      const int step = (n + kWave - 1) / kWave;
+      const bool in = lane * step < n;
+      const int i = lo + (in ? lane * step : 0);
+      const uint64_t below = __ballot(in && base(i, start_of(i)) <= slot);
+      const int at = below ? 63 - __builtin_clzll(below) : 0;
+      lo += at * step;
+      n = min(step, n - at * step);
+    }
+    const int i = lo + min(lane, n), tok = start_of(i);  // one more than the candidates: where the last of them ends
+    w = word(min(i, sets - 1));
+    const uint64_t below = __ballot(lane < n && base(i, tok) <= slot);
+    last = below ? 63 - __builtin_clzll(below) : 0;
+    r.set = lo + last;
+    r.tok0 = __builtin_amdgcn_readlane(tok, last);
+    r.n = max(0, __builtin_amdgcn_readlane(tok, last + 1) - r.tok0);
+    first = slot - base(r.set, r.tok0);
+  }
+  for (int* i : {&r.set, &r.tok0, &r.n, &last}) *i = __builtin_amdgcn_readfirstlane(*i);  // (the compiler does not see that these are the same in all lanes)
   r.r0 = __builtin_amdgcn_readfirstlane(first < 0 || first > INT_MAX / ROWS ? INT_MAX : (int)first * ROWS);
   r.word = (long long)((unsigned)__builtin_amdgcn_readlane((int)w, last) | (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(w >> 32), last) << 32);
   return r;
@@ -104,6 +166,114 @@ __device__ __forceinline__ void packed_fill(const PackedAttnArgs& p, int tok0, i
   }
 }
 
+// A workgroup's share of attention whose keys are split: up to ROWS rows of a sequence over a part of its own keys, or of a group of sequences over a part of those that
+// they share.
+struct PackedPart {
+  int set, tok0, n, r0, rows, here;  // tokens of the set; the first row, all of the set and those here
+  bool common, live, ok;
+  int split, splits;
+  int s0, alike, start0;  // first sequence; of own keys: pages that come before them, which its group shares, and the first position
+  long long at;           // in units of rows, where its results go in `part`
+};
+__device__ __forceinline__ long long packed_all_rows(const PackedAttnArgs& p) { return (long long)p.seq.N * p.kv_heads * p.group; }
+template <int ROWS>
+__device__ __forceinline__ PackedPart packed_part(const PackedAttnArgs& p, int block) {
+  PackedPart s;
+  const int B = p.seq.B, N = p.seq.N;
+  s.common = block < p.group_blocks;
+  if (!s.common) block -= p.group_blocks;
+  s.splits = s.common ? p.group_splits : p.splits;
+  const int slot = s.common ? p.by_group_splits(block) : p.by_splits(block), members = s.common ? p.members : 1, sets = (s.common ? p.by_members(B) : B) + 2;
+  s.split = block - slot * s.splits;
+  const PackedRows at = packed_rows<ROWS>(sets, INT_MAX, p.group, [&](int) { return slot; }, [&](int i) { return i == 0 ? 0 : i == sets ? N : packed_at(p.seq, (i - 1) * members); },
+                                          [&](int i) -> long long { return p.start[min(max(i - 1, 0) * members, B - 1)]; });
+  s.set = at.set, s.tok0 = at.tok0, s.n = at.n, s.r0 = at.r0;
+  s.rows = at.n * p.group, s.here = min(ROWS, s.rows - at.r0);
+  s.live = at.set >= 1 && at.set < sets - 1;
+  s.s0 = s.live ? (at.set - 1) * members : 0;
+  s.at = ((s.common ? 0 : p.group_splits) + s.split) * packed_all_rows(p);
+  s.ok = true;
+  s.alike = s.start0 = 0;
+  if (!s.common && s.live) {
+    s.ok = at.word >= 0 && at.word <= ((long long)p.pool.width << p.pool.page_log) - at.n;
+    s.start0 = s.ok ? (int)at.word : 0;
+    if (p.shared) s.alike = shared_pages(p, s.s0, s.start0);
+  }
+  return s;
+}
+__device__ __forceinline__ long long packed_row_at(const PackedAttnArgs& p, const PackedPart& s, int c, int r) {  // of (token, head)
+  const int t = p.by_group(r);
+  return (long long)(s.tok0 + t) * p.kv_heads * p.group + c * p.group + (r - t * p.group);
+}
+__device__ __forceinline__ float* packed_part_ml(const PackedAttnArgs& p, int D) { return p.part + (p.splits + p.group_splits) * packed_all_rows(p) * D; }
+// Rows that see none of these keys, or (sum NaN) are of a sequence whose tokens do not lie in its pages.
+template <class DT, int D>
+__device__ __forceinline__ void packed_nothing(const PackedAttnArgs& p, const PackedPart& s, int c, float sum) {
+  if (p.splits + p.group_splits == 1) return packed_fill<D>(p, s.tok0, c, s.r0, s.here, s.rows, sum == 0.f ? 0u : DT::fromf(NAN) * 0x10001u);
+  if ((int)threadIdx.x < s.here) {
+    float* ml = packed_part_ml(p, D) + 2 * (s.at + packed_row_at(p, s, c, s.r0 + threadIdx.x));
+    ml[0] = -FLT_MAX;
+    ml[1] = sum;
+  }
+}
+// Keys lo .. hi that row r sees of these.
+struct PackedKeys {
+  int lo, hi;
+};
+__device__ __forceinline__ PackedKeys packed_keys(const PackedAttnArgs& p, const PackedPart& s, int r) {
+  const int t = s.tok0 + p.by_group(r);
+  if (!s.common) {
+    const int pos = s.start0 + t - s.tok0;
+    return {max(p.group_splits ? s.alike << p.pool.page_log : 0, p.window ? pos - p.window + 1 : 0), pos};
+  }
+  // the sequence among the group's: a token each, or looked for
+  int b = s.s0 + min(t - s.tok0, p.members - 1);
+  if (!__all(packed_at(p.seq, b) <= t && t < packed_at(p.seq, b + 1))) {
+    int e = s.s0 + p.members;
+    b = s.s0;
+    for (int n = p.members; n > 1; n = (n + 1) / 2) {
+      const int mid = (b + e) / 2;
+      const bool in = mid > b && packed_at(p.seq, mid) <= t;
+      b = in ? mid : b;
+      e = in ? e : max(mid, b + 1);
+    }
+  }
+  const long long start = p.start[b], room = (long long)p.pool.width << p.pool.page_log;
+  const int first = packed_at(p.seq, b), n = packed_at(p.seq, b + 1) - first;
+  if (!(start >= 0 && start <= room - n)) return {0, -1};
+  const long long shared = p.shared[(s.set - 1) * p.shared_step];
+  const int pos = (int)start + t - first, pages = (int)max(0ll, min(shared, start)) >> p.pool.page_log;
+  return {p.window ? max(0, pos - p.window + 1) : 0, (pages << p.pool.page_log) - 1};
+}
+// Of all rows r0 .. r0 + ROWS - 1 that are here: the first key that any sees and the last one, and those that all see.
+struct PackedBounds {
+  int lo, hi, all_lo, all_hi;
+};
+__device__ __forceinline__ int least_of(int v) {
+  auto step = [&](auto ctrl) { v = min(v, __builtin_amdgcn_update_dpp(v, v, decltype(ctrl)::value, 0xf, 0xf, false)); };
+  step(std::integral_constant<int, 0xB1>());  // as in wave_sum
+  step(std::integral_constant<int, 0x4E>());
+  step(std::integral_constant<int, 0x141>());
+  step(std::integral_constant<int, 0x140>());
+  return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)), min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+template <int ROWS>
+__device__ __forceinline__ PackedBounds packed_bounds(const PackedAttnArgs& p, const PackedPart& s) {
+  if (!s.common) {  // both ends ascend with the row
+    const PackedKeys a = packed_keys(p, s, s.r0), z = packed_keys(p, s, s.r0 + s.here - 1);
+    return {__builtin_amdgcn_readfirstlane(a.lo), __builtin_amdgcn_readfirstlane(z.hi), __builtin_amdgcn_readfirstlane(z.lo), __builtin_amdgcn_readfirstlane(a.hi)};
+  }
+  int lo = INT_MAX, hi = -1, all_lo = 0, all_hi = INT_MAX;
+  const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int i = 0; i < ROWS; i += kWave) {
+    const PackedKeys k = packed_keys(p, s, s.r0 + min(lane + i, s.here - 1));
+    if (k.lo <= k.hi) lo = min(lo, k.lo), hi = max(hi, k.hi);
+    all_lo = max(all_lo, k.lo), all_hi = min(all_hi, k.hi);
+  }
+  return {least_of(lo), -least_of(-hi), -least_of(-all_lo), least_of(all_hi)};
+}
+
 // Where tokens of pages come from, sixteen at a time, which no page ends within.  Those outside lo .. hi, which nobody sees, are the nearest ones once more: their
 // entries may be anything, and so may the places behind a sequence's last token.
 struct PageRun {
@@ -114,6 +284,10 @@ struct PageRows {
   const int32_t* common;  // of the first `alike` pages
   int alike, lo, hi;
 };
+__device__ __forceinline__ PageRows page_rows(const PackedAttnArgs& p, int s, int alike, int lo, int hi) {  // of sequence s
+  const int32_t* table = p.pool.table + s * p.pool.table_stride;
+  return {table, alike ? p.pool.table + p.by_members(s) * p.members * p.pool.table_stride : table, alike, lo, hi};
+}
 __device__ __forceinline__ PageRun page_run(const Pool& pool, const PageRows& rows, int t) {
   const int from = min(max(t, rows.lo & ~15), rows.hi & ~15), page = from >> pool.page_log;
   return {from, load_uniform((page < rows.alike ? rows.common : rows.table) + page)};
@@ -156,57 +330,93 @@ template <int D> __device__ __forceinline__ constexpr int tile_swap_k(int t) {
 template <int D> __device__ __forceinline__ constexpr int tile_swap_v(int t) {
   return D >= 128 ? (t & 3) * 4 : D == 64 ? (t >> 1 & 1) * 4 : 0;
 }
-template <class DT, int D, bool PAGED>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kernel(PackedAttnArgs p) {
-  constexpr int ROWS = kTileRows, C = D / 16, NW = D / 32, PK = D / 8, kVecs = kTileKeys * PK;
+// PROMPT: keys and values of the call.  PAGES: of pages.  SPLIT: of pages, a part of them (see PackedPart).
+enum PackedMode { PROMPT, PAGES, SPLIT };
+constexpr int kSplitTiles = 4;  // of a part, at least
+constexpr int packed_tiles_waves(int D) { return D == 256 ? 1 : 2; }
+template <int D> struct TilesLds {
+  u32x4 kv[2][2][kTileKeys * D / 8];  // [buffer][keys, values]
+};
+template <class DT, int D, PackedMode MODE>
+__device__ __forceinline__ void packed_attn_tiles(const PackedAttnArgs& p, TilesLds<D>& lds) {
+  constexpr bool PAGED = MODE != PROMPT;
+  constexpr int ROWS = kTileRows, C = D / 16, NW = D / 32, PK = D / 8;
   constexpr int LOADS = PK / 4, STEP = kWave / PK;  // a wave's loads of a tile of keys (16 tokens), and tokens a load
   typedef Kv<DT> F;
-  __shared__ u32x4 s_kv[2][2][kVecs];  // [buffer][keys, values]
+  auto& s_kv = lds.kv;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 31, h = lane >> 5;
-  // The last slots first, which have the most keys of a sequence; three that hold nothing if the tokens are all somebody's behind the others.  Where a CU has two workgroups
-  // at once, the second ones come the other way round, so that those with the most keys are beside those with the fewest.
-  const int all = (p.slots - 3) * p.kv_heads;
-  int turn = blockIdx.x;
-  if (turn < all && turn >= p.turn) turn = all - 1 - (turn - p.turn);
-  const int order = p.by_heads(turn), c = turn - order * p.kv_heads, slot = turn < all ? p.slots - 3 - order : order == p.slots - 3 ? 0 : order;
-  const int B = p.seq.B;
-  const PackedRows at = packed_rows<ROWS>(B + 2, slot, p.group, [&](int i) { return i == 0 ? 0 : i > B + 1 ? p.seq.N : packed_at(p.seq, i - 1); },
-                                          [&](int i) -> long long {
-                                            const int s = min(max(i - 1, 0), B - 1);
-                                            if constexpr (PAGED) return p.start[s];
-                                            return (long long)packed_at(p.keys, s) << 32 | packed_at(p.keys, s + 1);
-                                          });
-  const int seq = at.set - 1, n = at.n, rows = n * p.group, r0 = at.r0, tok0 = at.tok0;
-  if (r0 >= rows) return;
-  const bool live = seq >= 0 && seq < B;
-  int pos0 = 0;  // position of the sequence's first query
+  int c, rows, r0, tok0, tile_lo, tile_hi, all_lo, all_hi;  // the keys all_lo .. all_hi are seen by all queries
   PageRows pages = {};
+  PackedKeys seen;                                          // by the lane's query
   const uint16_t *k_base, *v_base;
-  bool ok = true;
-  if constexpr (PAGED) {
-    ok = at.word >= 0 && at.word <= ((long long)p.pool.width << p.pool.page_log) - n;
-    pos0 = ok ? (int)at.word : 0;
-    pages.table = pages.common = p.pool.table + seq * p.pool.table_stride;
-    if (p.shared && live) {
-      pages.alike = shared_pages(p, seq, pos0);
-      pages.common = p.pool.table + p.by_members(seq) * p.members * p.pool.table_stride;
+  PackedPart part;
+  if constexpr (MODE == SPLIT) {
+    const int block = p.by_heads(blockIdx.x);
+    c = blockIdx.x - block * p.kv_heads;
+    part = packed_part<ROWS>(p, block);
+    rows = part.rows, r0 = part.r0, tok0 = part.tok0;
+    if (part.here <= 0) return;
+    if (!part.live || !part.ok) return packed_nothing<DT, D>(p, part, c, part.live ? NAN : 0.f);
+    const PackedBounds ends = packed_bounds<ROWS>(p, part);
+    const int first = ends.lo / kTileKeys, count = ends.hi / kTileKeys - first + 1, per = max(kSplitTiles, (part.common ? p.by_group_splits : p.by_splits)(count + part.splits - 1));
+    tile_lo = first + part.split * per;
+    tile_hi = min(tile_lo + per, first + count) - 1;
+    if (ends.hi < 0 || tile_lo > tile_hi) return packed_nothing<DT, D>(p, part, c, 0.f);
+    pages = page_rows(p, part.s0, part.alike, ends.lo, ends.hi);
+    all_lo = ends.all_lo, all_hi = ends.all_hi;
+  } else {
+    // The last slots first, which have the most keys of a sequence.  Where a CU has two workgroups at once, the second ones come the other way round, so that those
+    // with the most keys are beside those with the fewest.
+    const int B = p.seq.B;
+    const PackedRows at = packed_rows<ROWS>(
+        B + 2, p.slots, p.group,
+        [&](int slots) {
+          const int all = slots * p.kv_heads, at = blockIdx.x, turn = at >= p.cus && at < all && all <= 2 * p.cus ? all - 1 - (at - p.cus) : at, order = p.by_heads(turn);
+          c = turn - order * p.kv_heads;
+          return order < slots ? slots - 1 - order : order;
+        },
+        [&](int i) { return i == 0 ? 0 : i > B + 1 ? p.seq.N : packed_at(p.seq, i - 1); },
+        [&](int i) -> long long {
+          const int s = min(max(i - 1, 0), B - 1);
+          if constexpr (PAGED) return p.start[s];
+          return (long long)packed_at(p.keys, s) << 32 | packed_at(p.keys, s + 1);
+        });
+    const int seq = at.set - 1, n = at.n;
+    rows = n * p.group, r0 = at.r0, tok0 = at.tok0;
+    if (r0 >= rows) return;
+    const bool live = seq >= 0 && seq < B;
+    int pos0;  // position of the sequence's first query
+    bool ok = true;
+    if constexpr (PAGED) {
+      ok = at.word >= 0 && at.word <= ((long long)p.pool.width << p.pool.page_log) - n;
+      pos0 = ok ? (int)at.word : 0;
+    } else {
+      const int key0 = (int)(at.word >> 32), key1 = (int)at.word;
+      pos0 = key1 - key0 - n;
+      k_base = p.k + key0 * p.k_tok + c * p.k_head;
+      v_base = p.v + key0 * p.v_tok + c * p.v_head;
     }
+    const int pos_lo = pos0 + p.by_group(r0), pos_hi = pos0 + p.by_group(min(r0 + ROWS, rows) - 1);
+    if (!live || !ok || pos_hi < 0) return packed_fill<D>(p, tok0, c, r0, ROWS, rows, live && !ok ? DT::fromf(NAN) * 0x10001u : 0u);
+    const int lo = p.window ? max(0, pos_lo - p.window + 1) : 0;
+    if constexpr (PAGED) pages = page_rows(p, seq, p.shared ? shared_pages(p, seq, pos0) : 0, lo, pos_hi);
+    tile_lo = lo / kTileKeys, tile_hi = pos_hi / kTileKeys;
+    all_lo = p.window ? pos_hi - p.window + 1 : 0, all_hi = pos_lo;
+    seen.hi = pos0;
+  }
+  if constexpr (PAGED) {
     k_base = p.pool.k + ((long long)c << p.pool.page_log) * D;
     v_base = p.pool.v + ((long long)c << p.pool.page_log) * D;
-  } else {
-    const int key0 = (int)(at.word >> 32), key1 = (int)at.word;
-    pos0 = key1 - key0 - n;
-    k_base = p.k + key0 * p.k_tok + c * p.k_head;
-    v_base = p.v + key0 * p.v_tok + c * p.v_head;
   }
-  const int end = pos0 + n;  // keys
-  const int pos_lo = pos0 + p.by_group(r0), pos_hi = pos0 + p.by_group(min(r0 + ROWS, rows) - 1);
-  if (!live || !ok || pos_hi < 0) return packed_fill<D>(p, tok0, c, r0, ROWS, rows, live && !ok ? DT::fromf(NAN) * 0x10001u : 0u);
-  pages.lo = p.window ? max(0, pos_lo - p.window + 1) : 0;
-  pages.hi = pos_hi;
-  const int tile_lo = pages.lo / kTileKeys, tile_hi = pos_hi / kTileKeys;
-
-  const int mine = r0 + 32 * wave + m, row = min(mine, rows - 1), tok = p.by_group(row), pos = pos0 + tok;
+  for (int* w : {&tile_lo, &tile_hi, &all_lo, &all_hi, &pages.lo, &pages.hi, &pages.alike}) *w = __builtin_amdgcn_readfirstlane(*w);
+  const int mine = r0 + 32 * wave + m, row = min(mine, rows - 1), tok = p.by_group(row);
+  if constexpr (MODE == SPLIT) {
+    seen = packed_keys(p, part, row);
+  } else {
+    seen.hi += tok;
+    seen.lo = p.window ? seen.hi - p.window + 1 : 0;
+  }
+  const int end = MODE == PROMPT ? all_hi - p.by_group(r0) + p.by_group(rows) : 0;  // keys of the call
   u32x4 qf[C];
   {
     const uint16_t* q = p.q + (tok0 + tok) * p.q_tok + (c * p.group + row - tok * p.group) * p.q_head;
@@ -216,8 +426,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
 
   // A wave brings sixteen tokens of a tile.  Lane l of load j writes piece 64 j + l of them and reads what belongs there; what is exchanged goes by bits of the
   // token, so load j differs from load 0 by constants, and reads of LDS differ by constants too.
-  const unsigned t_lane = lane / PK;
-  unsigned k_piece = ((lane % PK) ^ tile_swap_k<D>(t_lane)) * 16, v_piece = ((lane % PK) ^ tile_swap_v<D>(t_lane)) * 16;
   unsigned k_at = (m * PK + (h ^ tile_swap_k<D>(m))) * 16;
   unsigned v_at = ((4 * h + (m >> 2 & 3)) * PK + ((2 * (m >> 4) + (m >> 1 & 1)) ^ tile_swap_v<D>(m >> 2 & 3))) * 16 + 8 * (m & 1);
   asm volatile("" : "+v"(k_at), "+v"(v_at));
@@ -252,9 +460,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
   };
   // where the lanes read, in bytes from the first of the sixteen tokens on; last: the last token that is read
   auto lanes = [&](bool values, int last, unsigned (&to)[LOADS]) {
-    const unsigned piece = values ? v_piece : k_piece, step = values ? v_row : k_row;
+    int l = lane;
+    asm volatile("" : "+v"(l));  // nothing that follows from it has a register over the loop
+    const int t = l / PK, piece = (l % PK) ^ (values ? tile_swap_v<D>(t) : tile_swap_k<D>(t));
 #pragma unroll
-    for (int j = 0; j < LOADS; j++) to[j] = min((int)t_lane + STEP * j, last) * step + (piece ^ (16u * (values ? tile_swap_v<D>(STEP * j) : tile_swap_k<D>(STEP * j))));
+    for (int j = 0; j < LOADS; j++)
+      to[j] = min(t + STEP * j, last) * (values ? v_row : k_row) + 16u * (piece ^ (values ? tile_swap_v<D>(STEP * j) : tile_swap_k<D>(STEP * j)));
   };
   unsigned k_lanes[LOADS], v_lanes[LOADS];
   auto all_lanes = [&] {
@@ -293,7 +504,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
     return add;
   };
   auto settle = [&](f32x16& s, u32x4 (&pf)[2], float add) {  // of the weights that are in pf now; what o holds is of keys before
-    if (__builtin_expect(__any(add > (far ? -1.f : Limit<DT>::SUM)), 0)) {
+    // (the same in all lanes: where the compiler doubts that, it keeps o twice)
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(__any(add > (far ? -1.f : Limit<DT>::SUM)) ? 1 : 0), 0)) {
       float mx = s[0];
 #pragma unroll
       for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[e]);
@@ -316,7 +528,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
     sum += add;
   };
   // tiles that a window cuts, tiles that all of the workgroup's queries see, tiles that hold some of their own keys
-  const int cut = p.window && pos_hi >= p.window ? (pos_hi - p.window) / kTileKeys : -1, own = (pos_lo + 1) / kTileKeys;  // last and first of them
+  const int cut = all_lo > 0 ? (all_lo - 1) / kTileKeys : -1, own = all_hi < 0 ? 0 : (all_hi + 1) / kTileKeys;  // last and first of them
   // half u of a tile: what replaces scores of keys that the query does not see, those behind it and those that a window hides, and of places that are no page's
   auto mask = [&](f32x16& s, int tile, int u, unsigned none, float hidden) {
     if (PAGED && __builtin_expect(none != 0, 0)) {
@@ -324,15 +536,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
       for (int e = 0; e < 16; e++)
         if (none >> (2 * u + e / 8) & 1) s[e] = NAN;
     }
-    const int most = pos - tile * kTileKeys - 32 * u - 4 * h;
+    const int key0 = tile * kTileKeys + 32 * u + 4 * h, most = seen.hi - key0, least = seen.lo - key0;
     if (tile >= own) {
 #pragma unroll
       for (int e = 0; e < 16; e++) s[e] = 8 * (e / 4) + e % 4 <= most ? s[e] : hidden;
     }
     if (tile <= cut) {
-      const int least = max(most, -kTileKeys) - p.window;
 #pragma unroll
-      for (int e = 0; e < 16; e++) s[e] = 8 * (e / 4) + e % 4 > least ? s[e] : hidden;
+      for (int e = 0; e < 16; e++) s[e] = 8 * (e / 4) + e % 4 >= least ? s[e] : hidden;
     }
   };
   // operands of half a tile, in the order of the products
@@ -496,13 +707,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
       }
     }
   };
-  auto store = [&](auto write) {
+  auto store = [&](auto write) {  // four elements in order
     if (mine >= rows) return;
-    uint16_t* out = packed_out(p, tok0, c, mine, D);
+    long long to;
+    if constexpr (MODE == SPLIT) to = (part.at + packed_row_at(p, part, c, mine)) * D;
+    else to = packed_out(p, tok0, c, mine, D) - p.out;
 #pragma unroll
     for (int w = 0; w < NW; w++)
 #pragma unroll
-      for (int a = 0; a < 4; a++) write(out + 32 * w + 8 * a + 4 * h, w, a);
+      for (int a = 0; a < 4; a++) write(to + 32 * w + 8 * a + 4 * h, w, a);
   };
   float odd = 0.f;
 #pragma unroll
@@ -515,156 +728,68 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void packed_attn_tiles_kerne
     again(false);
   }
   sum += __shfl_xor(sum, 32, kWave);
-  const float f = sum == 0.f ? 0.f : 1.f / sum;  // no key, or none that weighs anything
-  store([&](uint16_t* out, int w, int a) {
-    float x[4];
+  if constexpr (MODE == SPLIT) {
+    store([&](long long to, int w, int a) { *(f32x4*)(p.part + to) = f32x4{o[w][4 * a], o[w][4 * a + 1], o[w][4 * a + 2], o[w][4 * a + 3]}; });
+    if (h == 0 && mine < rows) {
+      float* ml = packed_part_ml(p, D) + 2 * (part.at + packed_row_at(p, part, c, mine));
+      ml[0] = top + F::SLACK;  // what weights of 2^HEAD are relative to
+      ml[1] = sum;
+    }
+  } else {
+    const float f = sum == 0.f ? 0.f : 1.f / sum;  // no key, or none that weighs anything
+    store([&](long long to, int w, int a) {
+      float x[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) x[e] = o[w][4 * a + e] * f;
-    *(u32x2*)out = u32x2{DT::pack(x[0], x[1]), DT::pack(x[2], x[3])};
-  });
+      for (int e = 0; e < 4; e++) x[e] = o[w][4 * a + e] * f;
+      *(u32x2*)(p.out + to) = u32x2{DT::pack(x[0], x[1]), DT::pack(x[2], x[3])};
+    });
+  }
   if (bad) {
     again(true);
-    store([&](uint16_t* out, int w, int a) {
+    store([&](long long to, int w, int a) {
 #pragma unroll
       for (int e = 0; e < 4; e++)
-        if (o[w][4 * a + e] > 0.f) out[e] = DT::fromf(NAN);
+        if (o[w][4 * a + e] > 0.f) {
+          if constexpr (MODE == SPLIT) p.part[to + e] = NAN;
+          else p.out[to + e] = DT::fromf(NAN);
+        }
     });
   }
 }
 
-// Few tokens: up to 64 rows of queries a workgroup, its keys split over workgroups.  Two kinds of workgroups in one launch: those of the keys that a group of sequences shares,
-// whose rows are the tokens of all of them, and those of a sequence's own keys.  Sixteen rows are an operand of v_mfma_f32_16x16x32:
+// Few tokens: up to sixteen rows of queries a workgroup, which are an operand of v_mfma_f32_16x16x32, and keys split over workgroups.  In one launch those of the keys that a group
+// of sequences shares, whose rows are the tokens of all of them, and those of a sequence's own keys.
 //   S^T = K . Q^T   tile i, row 4 g + e of the result: token 16 i + 4 g + e, in lanes of group g = lane / 16; columns are queries
 //   O^T += V^T . P  operand of 32 tokens: tokens 4 g .. + 3 and 16 + 4 g .. + 3, those whose weights the lane has; V comes turned round out of LDS
-// Where there are up to sixteen rows each wave has 32 keys of its own at a time and waits for nobody: keys come as operands, values into LDS of the wave's own. What the
-// waves give is joined in LDS at the end.  Where there are more, a wave has sixteen rows, and all of them read tiles of 32 keys that they bring into LDS together.
-constexpr int kStepKeys = 32, kStepBlock = 64;
+// Each wave has 32 keys of its own at a time and waits for nobody: keys come as operands, values into LDS of the wave's own.  What the waves give is joined in LDS at the end.
+constexpr int kStepKeys = 32, kStepRows = 16;
 template <int D> __device__ __forceinline__ constexpr int step_swap_v(int t) {
   return D >= 128 ? (t & 7) * 2 : D == 64 ? (t >> 1 & 3) * 2 : (t >> 2 & 1) * 2;
 }
 constexpr int packed_step_waves(int D) { return D == 256 ? 2 : D == 128 ? 3 : 4; }
+template <int D> struct StepLds {
+  union {
+    u32x4 v[4][kStepKeys * D / 8];  // of each wave
+    float joined[4][kStepRows][D + 4];
+  };
+  float top[4][kStepRows], sum[4][kStepRows];
+};
 template <class DT, int D>
-__global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_kernel(PackedAttnArgs p) {
-  constexpr int C = D / 32, NU = D / 16, PK = D / 8, STEP = kWave / PK, W = 4, kVecs = kStepKeys * PK;
+__device__ __forceinline__ void packed_attn_step(const PackedAttnArgs& p, StepLds<D>& lds) {
+  constexpr int C = D / 32, NU = D / 16, PK = D / 8, STEP = kWave / PK, W = 4, LOADS = PK / 4;
   typedef Kv<DT> F;
-  constexpr int PITCH = D + 4;
-  __shared__ union {
-    u32x4 own[W][kVecs];        // a wave's values
-    u32x4 common[2][2][kVecs];  // [buffer][keys, values]
-    float joined[W][16][PITCH];
-  } lds;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
-  int rest = p.by_heads(blockIdx.x);
-  const int c = blockIdx.x - rest * p.kv_heads, B = p.seq.B, N = p.seq.N;
-  const bool common = rest < p.group_slots * p.group_splits;
-  if (!common) rest -= p.group_slots * p.group_splits;
-  const int splits = common ? p.group_splits : p.splits, slot = common ? p.by_group_splits(rest) : p.by_splits(rest), split = rest - slot * splits;
-  const int members = common ? p.members : 1, sets = (common ? p.by_members(B) : B) + 2;
-  const PackedRows at = packed_rows<kStepBlock>(sets, slot, p.group, [&](int i) { return i == 0 ? 0 : i == sets ? N : packed_at(p.seq, (i - 1) * members); },
-                                                [&](int i) -> long long { return p.start[min(max(i - 1, 0) * members, B - 1)]; });
-  const int rows = at.n * p.group, r0 = at.r0, tok0 = at.tok0, here = min(kStepBlock, rows - r0);
+  const int block = p.by_heads(blockIdx.x), c = blockIdx.x - block * p.kv_heads;
+  const PackedPart part = packed_part<kStepRows>(p, block);
+  const int r0 = part.r0, here = part.here, tok0 = part.tok0;
   if (here <= 0) return;
-  const bool live = at.set >= 1 && at.set < sets - 1;
-  const int s0 = live ? (at.set - 1) * members : 0;
-  const bool joined = p.splits + p.group_splits > 1;  // what this workgroup gives goes to `part`
-  const long long all = (long long)N * p.kv_heads * p.group;  // rows of a split
-  const long long part0 = (long long)((common ? 0 : p.group_splits) + split) * all;
-  float* part_ml = p.part + (long long)(p.splits + p.group_splits) * all * D;
-  auto out_row = [&](int r) {  // of (token, head)
-    const int t = p.by_group(r);
-    return (long long)(tok0 + t) * p.kv_heads * p.group + c * p.group + (r - t * p.group);
-  };
-  auto nothing = [&](float sum) {  // rows that see none of the keys, or (NaN) are no sequence's
-    if (!joined) return packed_fill<D>(p, tok0, c, r0, here, rows, sum == 0.f ? 0u : DT::fromf(NAN) * 0x10001u);
-    if (tid < here) {
-      float* ml = part_ml + 2 * (part0 + out_row(r0 + tid));
-      ml[0] = -FLT_MAX;
-      ml[1] = sum;
-    }
-  };
-  if (!live) return nothing(0.f);
-
-  // the keys of row r of this workgroup: lo .. hi, and its position
-  struct Keys {
-    int lo, hi;
-  };
-  auto page_tokens = [&](int n) { return n << p.pool.page_log; };
-  const long long room = page_tokens(p.pool.width);
-  bool ok = true;
-  int alike = 0, start0 = 0;
-  if (!common) {
-    ok = at.word >= 0 && at.word <= room - at.n;
-    start0 = ok ? (int)at.word : 0;
-    if (p.shared) alike = shared_pages(p, s0, start0);
-  }
-  if (!ok) return nothing(NAN);
-  auto keys_of = [&](int r) -> Keys {
-    const int t = tok0 + p.by_group(r);
-    if (!common) {
-      const int pos = start0 + t - tok0;
-      return {max(page_tokens(alike), p.window ? pos - p.window + 1 : 0), pos};
-    }
-    // the sequence among the group's: a token each, or looked for
-    int b = s0 + min(t - tok0, members - 1);
-    if (!__all(packed_at(p.seq, b) <= t && t < packed_at(p.seq, b + 1))) {
-      int e = s0 + members;
-      b = s0;
-      for (int n = members; n > 1; n = (n + 1) / 2) {
-        const int mid = (b + e) / 2;
-        const bool in = mid > b && packed_at(p.seq, mid) <= t;
-        b = in ? mid : b;
-        e = in ? e : max(mid, b + 1);
-      }
-    }
-    const long long start = p.start[b];
-    const int first = packed_at(p.seq, b), n = packed_at(p.seq, b + 1) - first;
-    if (!(start >= 0 && start <= room - n)) return {0, -1};
-    const int pos = (int)start + t - first;
-    const long long shared = p.shared[(at.set - 1) * p.shared_step];
-    const int pages = (int)max(0ll, min(shared, start)) >> p.pool.page_log;
-    return {p.window ? max(0, pos - p.window + 1) : 0, page_tokens(pages) - 1};
-  };
-  auto least = [](int v) {
-    auto step = [&](auto ctrl) { v = min(v, __builtin_amdgcn_update_dpp(v, v, decltype(ctrl)::value, 0xf, 0xf, false)); };
-    step(std::integral_constant<int, 0xB1>());   // as in wave_sum
-    step(std::integral_constant<int, 0x4E>());
-    step(std::integral_constant<int, 0x141>());
-    step(std::integral_constant<int, 0x140>());
-    return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)), min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
-  };
-  auto most = [&](int v) { return -least(-v); };
-  // each wave its keys and all rows, or its rows and all keys
-  const bool apart = here <= 16;
-  const int wave_rows = apart ? 0 : 16 * wave;
-  const int src = min(wave_rows + m, here - 1), row = r0 + src;
-  PageRows pages;
-  Keys k;
-  int all_lo, all_hi;  // what all of the wave's rows see
-  if (common) {
-    k = keys_of(r0 + min(lane, here - 1));  // of all rows here, a lane each
-    const bool some = k.lo <= k.hi;
-    pages.lo = least(some ? k.lo : INT_MAX);
-    pages.hi = most(some ? k.hi : -1);
-    k.lo = __shfl(k.lo, src, kWave), k.hi = __shfl(k.hi, src, kWave);
-    all_lo = most(k.lo), all_hi = least(k.hi);
-  } else {  // both ends ascend with the row
-    auto ends = [&](int r) {
-      const Keys e = keys_of(r0 + min(r, here - 1));
-      return Keys{__builtin_amdgcn_readfirstlane(e.lo), __builtin_amdgcn_readfirstlane(e.hi)};
-    };
-    k = keys_of(row);
-    pages.lo = ends(0).lo, pages.hi = ends(here - 1).hi;
-    all_lo = ends(wave_rows + 15).lo, all_hi = ends(wave_rows).hi;
-  }
-  if (pages.hi < 0) return nothing(0.f);
-  pages.table = pages.common = p.pool.table + s0 * p.pool.table_stride;
-  pages.alike = 0;
-  if (alike) {
-    pages.alike = alike;
-    pages.common = p.pool.table + p.by_members(s0) * p.members * p.pool.table_stride;
-  }
-
-  const bool idle = wave_rows >= here;  // a wave without rows, that only brings
+  if (!part.live || !part.ok) return packed_nothing<DT, D>(p, part, c, part.live ? NAN : 0.f);
+  const PackedBounds ends = packed_bounds<kStepRows>(p, part);
+  const int tile_lo = ends.lo / kStepKeys, tile_hi = ends.hi / kStepKeys, active = min(part.splits, (tile_hi - tile_lo + W) / W), split = part.split;
+  if (ends.hi < 0 || split >= active) return packed_nothing<DT, D>(p, part, c, 0.f);
+  const PageRows pages = page_rows(p, part.s0, part.alike, ends.lo, ends.hi);
+  const int row = r0 + min(m, here - 1);
+  const PackedKeys k = packed_keys(p, part, row);
   u32x4 qf[C];
   {
     const int t = p.by_group(row);
@@ -672,23 +797,16 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
 #pragma unroll
     for (int i = 0; i < C; i++) qf[i] = *(const u32x4*)(q + 32 * i + 8 * g);
   }
-  const int tile_lo = pages.lo / kStepKeys, tile_hi = pages.hi / kStepKeys;
-  const int unit = apart ? W : 2, active = min(splits, (tile_hi - tile_lo + unit) / unit);
-  if (split >= active) return nothing(0.f);
-
   const unsigned t_lane = lane / PK;
-  unsigned k_at = (m * PK + (g ^ tile_swap_k<D>(m))) * 16;
   unsigned v_at = ((4 * g + (m >> 2)) * PK + ((m >> 1 & 1) ^ step_swap_v<D>(4 * (g & 1) + (m >> 2)))) * 16 + 8 * (m & 1);
-  asm volatile("" : "+v"(k_at), "+v"(v_at));
-  const uint16_t* k_base = p.pool.k + page_tokens(c) * (long long)D;
-  const uint16_t* v_base = p.pool.v + page_tokens(c) * (long long)D;
+  asm volatile("" : "+v"(v_at));
+  const uint16_t* k_base = p.pool.k + ((long long)c << p.pool.page_log) * D;
+  const uint16_t* v_base = p.pool.v + ((long long)c << p.pool.page_log) * D;
   // Sixteen tokens into LDS; lane l of load j writes piece 64 j + l of them and reads what belongs there.
-  const bool brings_k = !apart && wave < 2;
   auto lane_at = [&](int j, int last) {
-    const unsigned t = t_lane + STEP * j, piece = (lane % PK) ^ (brings_k ? tile_swap_k<D>(t) : step_swap_v<D>(t));
+    const unsigned t = t_lane + STEP * j, piece = (lane % PK) ^ step_swap_v<D>(t);
     return min((int)t, last) * (2 * D) + piece * 16;
   };
-  constexpr int LOADS = PK / 4;
 
   float top = -FLT_MAX, sum = 0.f;
   bool far = false;
@@ -729,15 +847,15 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
     sum += add;
   };
   enum { PLAIN, CLEAN, COUNT };  // gone over again as above
-  // a tile's scores, its keys and values in LDS or (the keys) in registers
-  auto take = [&](auto AGAIN, int mode, int tile, unsigned none, const u32x4* vt, auto key, auto behind) {
+  // a tile; `behind` once its keys have been used
+  auto take = [&](auto AGAIN, int mode, int tile, unsigned none, const u32x4* vt, u32x4 (&kk)[2][C], auto behind) {
     const int key0 = tile * kStepKeys;
     f32x4 s[2];
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < C; j++) s[i] = Mma<DT>::run(key(i, j), qf[j], s[i]);
+      for (int j = 0; j < C; j++) s[i] = Mma<DT>::run(kk[i][j], qf[j], s[i]);
     }
     __builtin_amdgcn_sched_barrier(0);
     behind();
@@ -751,7 +869,7 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
       const int key = key0 + 16 * i + 4 * g + e;
       return key >= k.lo && key <= k.hi;
     };
-    if (key0 < all_lo || key0 + kStepKeys - 1 > all_hi) {
+    if (key0 < ends.all_lo || key0 + kStepKeys - 1 > ends.all_hi) {
 #pragma unroll
       for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -789,7 +907,6 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto none_of = [&](const PageRun (&runs)[2]) { return (unsigned)page_none(p.pool, runs[0]) | (unsigned)page_none(p.pool, runs[1]) << 1; };
   auto sweep = [&](auto AGAIN, int mode) {
 #pragma unroll
     for (int u = 0; u < NU; u++) o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -798,67 +915,42 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
 #pragma unroll
       for (int i = 0; i < 2; i++) runs[i] = page_run(p.pool, pages, min(tile, tile_hi) * kStepKeys + 16 * i);
     };
-    if (apart) {
-      const int step = active * W;
-      int tile = tile_lo + split * W + wave;
-      u32x4 kk[2][C];
-      u32x4* vt = lds.own[wave];
-      auto fetch_k = [&] {
+    const int step = active * W;
+    int tile = tile_lo + split * W + wave;
+    u32x4 kk[2][C];
+    u32x4* vt = lds.v[wave];
+    auto fetch_k = [&] {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const char* from = uniform(k_base + page_place(p.pool, runs[i]) * D);
+      for (int i = 0; i < 2; i++) {
+        const char* from = uniform(k_base + page_place(p.pool, runs[i]) * D);
 #pragma unroll
-          for (int j = 0; j < C; j++) kk[i][j] = load_stream((const u32x4*)(from + (size_t)((unsigned)(m * 2 * D + 16 * g) + 64u * j)));
-        }
-      };
-      auto bring_v = [&](const PageRun (&runs)[2]) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const char* from = uniform(v_base + page_place(p.pool, runs[i]) * D);
-#pragma unroll
-          for (int j = 0; j < LOADS; j++)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (size_t)lane_at(j, pages.hi - runs[i].from)),
-                                             (__attribute__((address_space(3))) void*)(vt + 16 * i * PK + j * kWave), 16, 0, 2);
-        }
-      };
-      ask(tile);
-      if (tile <= tile_hi) {
-        fetch_k();
-        bring_v(runs);
+        for (int j = 0; j < C; j++) kk[i][j] = load_stream((const u32x4*)(from + (size_t)((unsigned)(m * 2 * D + 16 * g) + 64u * j)));
       }
-      while (tile <= tile_hi) {
-        const unsigned none = none_of(runs);
-        const bool more = tile + step <= tile_hi;
-        ask(tile + step);
-        take(AGAIN, mode, tile, none, vt, [&](int i, int j) { return kk[i][j]; }, [&] {
-          if (more) fetch_k();
-        });
-        tile += step;
-        if (more) bring_v(runs);
-      }
-    } else {
-      int tile = tile_lo + split, buf = 0;
-      auto bring = [&](int buf) {
-        const PageRun run = {wave & 1 ? runs[1].from : runs[0].from, wave & 1 ? runs[1].id : runs[0].id};
-        const char* from = uniform((brings_k ? k_base : v_base) + page_place(p.pool, run) * D);
+    };
+    auto bring_v = [&] {
 #pragma unroll
-        for (int j = 0; j < LOADS; j++) load_lds(from, lane_at(j, pages.hi - run.from), lds.common[buf][!brings_k] + 16 * (wave & 1) * PK + j * kWave);
-      };
-      ask(tile);
-      bring(0);
-      unsigned none = none_of(runs);
-      ask(tile + active);
-      for (; tile <= tile_hi; tile += active, buf ^= 1) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): what was brought is in LDS, and all have read what is overwritten
-        lds_barrier();
-        if (tile + active <= tile_hi) bring(buf ^ 1);
-        const unsigned now = none;
-        none = none_of(runs);
-        ask(tile + 2 * active);
-        if (!idle)
-          take(AGAIN, mode, tile, now, lds.common[buf][1], [&](int i, int j) { return *(const u32x4*)((const char*)lds.common[buf][0] + (k_at ^ 64u * j) + 16 * i * PK * 16); }, [] {});
+      for (int i = 0; i < 2; i++) {
+        const char* from = uniform(v_base + page_place(p.pool, runs[i]) * D);
+#pragma unroll
+        for (int j = 0; j < LOADS; j++)
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (size_t)lane_at(j, pages.hi - runs[i].from)),
+                                           (__attribute__((address_space(3))) void*)(vt + 16 * i * PK + j * kWave), 16, 0, 2);
       }
-      lds_barrier();
+    };
+    ask(tile);
+    if (tile <= tile_hi) {
+      fetch_k();
+      bring_v();
+    }
+    while (tile <= tile_hi) {
+      const unsigned none = (unsigned)page_none(p.pool, runs[0]) | (unsigned)page_none(p.pool, runs[1]) << 1;
+      const bool more = tile + step <= tile_hi;
+      ask(tile + step);
+      take(AGAIN, mode, tile, none, vt, kk, [&] {
+        if (more) fetch_k();
+      });
+      tile += step;
+      if (more) bring_v();
     }
   };
   sweep(std::false_type(), PLAIN);
@@ -876,74 +968,80 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
   sum += __shfl_xor(sum, 16, kWave);
   sum += __shfl_xor(sum, 32, kWave);
 
-  // the waves' results, and where the tiles have to be gone over again, what is to be put there instead
-  __shared__ float s_top[W][16], s_sum[W][16];
-  auto write_row = [&](int r, int d, f32x4 x, float mx, float den) {  // r: of the workgroup's
-    const long long to = out_row(r0 + r);
-    if (!joined) {
-      const float f = den == 0.f ? 0.f : 1.f / den;
-      *(u32x2*)(p.out + to * D + d) = u32x2{DT::pack(x[0] * f, x[1] * f), DT::pack(x[2] * f, x[3] * f)};
-    } else {
-      *(f32x4*)(p.part + (part0 + to) * D + d) = x;
-      if (d == 0) {
-        float* ml = part_ml + 2 * (part0 + to);
-        ml[0] = mx;
-        ml[1] = den;
-      }
-    }
-  };
-  auto spoil_row = [&](int r, int d, f32x4 x) {  // not finite where x counts something
-    const long long to = out_row(r0 + r);
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (x[e] > 0.f) {
-        if (!joined) p.out[to * D + d + e] = DT::fromf(NAN);
-        else p.part[(part0 + to) * D + d + e] = NAN;
-      }
-  };
-  auto finish = [&](bool count) {
-    if (!apart) {
-      if (wave_rows + m >= here) return;
-#pragma unroll
-      for (int u = 0; u < NU; u++) {
-        if (count) spoil_row(wave_rows + m, 16 * u + 4 * g, o[u]);
-        else write_row(wave_rows + m, 16 * u + 4 * g, o[u], top, sum);
-      }
-      return;
-    }
+  // the waves' results, and where the tiles have been gone over again, what is to be put there instead
+  auto join = [&](bool count) {
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < NU; u++) *(f32x4*)&lds.joined[wave][m][16 * u + 4 * g] = o[u];
     if (!count && g == 0) {
-      s_top[wave][m] = top;
-      s_sum[wave][m] = sum;
+      lds.top[wave][m] = top;
+      lds.sum[wave][m] = sum;
     }
     __syncthreads();
     for (int i = tid; i < here * (D / 4); i += 256) {
       const int r = i / (D / 4), d = i % (D / 4) * 4;
-      float mx = s_top[0][r];
+      float mx = lds.top[0][r];
 #pragma unroll
-      for (int w = 1; w < W; w++) mx = fmaxf(mx, s_top[w][r]);
+      for (int w = 1; w < W; w++) mx = fmaxf(mx, lds.top[w][r]);
       f32x4 num = f32x4{0.f, 0.f, 0.f, 0.f};
       float den = 0.f;
 #pragma unroll
       for (int w = 0; w < W; w++) {
-        const float f = count ? 1.f : __builtin_amdgcn_exp2f(s_top[w][r] - mx);
+        const float f = count ? 1.f : __builtin_amdgcn_exp2f(lds.top[w][r] - mx);
         const f32x4 x = *(const f32x4*)&lds.joined[w][r][d];
 #pragma unroll
         for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e]);
-        den = fmaf(f, s_sum[w][r], den);
+        den = fmaf(f, lds.sum[w][r], den);
       }
-      if (count) spoil_row(r, d, num);
-      else write_row(r, d, num, mx, den);
+      const long long to = packed_row_at(p, part, c, r0 + r);
+      const bool whole = p.splits + p.group_splits == 1;
+      if (count) {  // not finite where something has been counted
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (num[e] > 0.f) {
+            if (whole) p.out[to * D + d + e] = DT::fromf(NAN);
+            else p.part[(part.at + to) * D + d + e] = NAN;
+          }
+      } else if (whole) {
+        const float f = den == 0.f ? 0.f : 1.f / den;
+        *(u32x2*)(p.out + to * D + d) = u32x2{DT::pack(num[0] * f, num[1] * f), DT::pack(num[2] * f, num[3] * f)};
+      } else {
+        *(f32x4*)(p.part + (part.at + to) * D + d) = num;
+        if (d == 0) {
+          float* ml = packed_part_ml(p, D) + 2 * (part.at + to);
+          ml[0] = mx;
+          ml[1] = den;
+        }
+      }
     }
   };
-  finish(false);
+  join(false);
   if (again) {
     __syncthreads();
     sweep(std::true_type(), COUNT);
-    finish(true);
+    join(true);
   }
+}
+
+template <class DT, int D, PackedMode MODE>
+__global__ __launch_bounds__(256, packed_tiles_waves(D)) void packed_attn_tiles_kernel(PackedAttnArgs p) {
+  __shared__ TilesLds<D> lds;
+  packed_attn_tiles<DT, D, MODE>(p, lds);
+}
+template <class DT, int D>
+__global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_kernel(PackedAttnArgs p) {
+  __shared__ StepLds<D> lds;
+  packed_attn_step<DT, D>(p, lds);
+}
+// Many rows behind keys that they share, and few with keys of their own: the first wait for the matrix cores, the others for memory, so they run side by side.
+template <class DT, int D>
+__global__ __launch_bounds__(256, packed_tiles_waves(D)) void packed_attn_both_kernel(PackedAttnArgs p) {
+  __shared__ union {
+    TilesLds<D> tiles;
+    StepLds<D> step;
+  } lds;
+  if (p.by_heads(blockIdx.x) < p.group_blocks) packed_attn_tiles<DT, D, SPLIT>(p, lds.tiles);
+  else packed_attn_step<DT, D>(p, lds.step);
 }
 
 // The splits' results, in a fixed order.  ALONE: a workgroup a row, else a wave a row; groups of D / 4 lanes take every so manieth split.
