@@ -2,6 +2,8 @@
 // No allocation, no synchronisation, everything on the caller's stream.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "cats_gemv.h"
 #include "cats_launch_paged.h"
 
@@ -56,21 +58,27 @@ int window_of(int window) { return window >= 1 << 30 ? 0 : window; }
 // Workgroups of a launch, whose threads have to be fewer than 2^32.
 bool grid_ok(int N, int B, int heads, int kv_heads) { return (long long)N * heads / 16 + (B + 2ll) * kv_heads < 1 << 24; }
 
+// The rule goes by what the host knows: how many tokens there are, and how long a sequence can be at most.
+//   tiles   More than one workgroup's 16 rows a sequence (8 x 5 tokens x 4 heads behind 4000: 39 us with the kernel of few tokens, 34 with that of many; 8 x 8 tokens
+//           39 and 34), or a group (8 groups of 8 sequences behind 2048: 34 us and 30).
+//   splits  As many as bring workgroups to two a CU, whose loads cover for each other (1 row behind 131072 with two 87 us, 6.2 TB/s), and to one where
+//           the matrix cores bound (piece of 512 behind 7680 with two 131 us, with one 117), or where keys are shared: a sequence's own ones are few then (4 x 8 beams
+//           on 2000 with two 39 us, with one 37; 4 rows behind 8192 21 and 16).  No part is of fewer than 128 or 256 keys, and 1024 are not split: the join, and the
+//           writing and reading of parts, would cost what they give (1 row behind 1000 takes 9 us whole).
 PackedPlan paged_plan(int N, int B, int heads, int kv_heads, int page, int width, int window, int members) {
   const int cus = current_device_cus(), group = heads / kv_heads;
-  const long long room = (long long)width * page, keys = window ? (room < window + 64ll ? room : window + 64ll) : room;
+  const long long room = (long long)width * page, keys = window ? std::min(room, window + 64ll) : room;
   const long long rows = ((long long)N * group + B - 1) / B;  // of a sequence, on average
   auto splits = [&](bool tiles, long long sets, long long set_rows) {
     const int most = tiles ? kTileRows : kStepRows;
-    const long long groups = kv_heads * sets * ((set_rows + most - 1) / most), want = ((tiles ? 1ll : 2ll) * cus + groups - 1) / groups;
-    const long long units = keys / (tiles ? kSplitTiles * kTileKeys : 128);
-    return (int)(keys <= 1024 ? 1 : want < units ? want : units);
+    const long long groups = kv_heads * sets * ((set_rows + most - 1) / most), want = ((tiles || members > 1 ? 1ll : 2ll) * cus + groups - 1) / groups;
+    return keys <= 1024 ? 1 : (int)std::min(want, keys / (tiles ? kSplitTiles * kTileKeys : 128));
   };
   PackedPlan plan = {};
-  plan.tiles = rows > 32;
+  plan.tiles = rows > kStepRows;
   plan.splits = splits(plan.tiles, B, rows);
   if (members > 1 && !plan.tiles) {
-    plan.group_tiles = rows * members > 32;
+    plan.group_tiles = rows * members > kStepRows;
     plan.group_splits = splits(plan.group_tiles, B / members, rows * members);
   }
   return plan;
