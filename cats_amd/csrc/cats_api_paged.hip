@@ -55,8 +55,10 @@ int fill_pool(Pool& pool, const void* k_pages, const void* v_pages, const int32_
 // A window that no sequence exceeds is none.
 int window_of(int window) { return window >= 1 << 30 ? 0 : window; }
 
-// Workgroups of a launch, whose threads have to be fewer than 2^32.
-bool grid_ok(int N, int B, int heads, int kv_heads) { return (long long)N * heads / 16 + (B + 2ll) * kv_heads < 1 << 24; }
+// Workgroups of a launch, whose threads have to be fewer than 2^32.  Those of a join are four rows each, and where there are many rows there is one only for groups.
+bool grid_ok(int N, int B, int heads, int kv_heads, int members = 1) {
+  return (long long)N * heads / 16 + (B + 2ll) * kv_heads < 1 << (members > 1 ? 21 : 24);
+}
 
 // The rule goes by what the host knows: how many tokens there are, and how long a sequence can be at most.
 //   tiles   More than one workgroup's 16 rows a sequence (8 x 5 tokens x 4 heads behind 4000: 39 us with the kernel of few tokens, 34 with that of many; 8 x 8 tokens
@@ -152,7 +154,7 @@ int cats_paged_attention(const void* q, const int64_t* q_strides, const int64_t*
                          size_t scratch_bytes, void* stream) {
   if (int st = check_packed(N, B, heads, kv_heads, D, dtype)) return st;
   if (int st = check_pool(page, pages, width, kv_heads)) return st;
-  if (heads < kv_heads || heads % kv_heads != 0 || window < 0 || !scale_ok(scale) || !grid_ok(N, B, heads, kv_heads)) return CATS_ERR_SHAPE;
+  if (heads < kv_heads || heads % kv_heads != 0 || window < 0 || !scale_ok(scale) || !grid_ok(N, B, heads, kv_heads, group)) return CATS_ERR_SHAPE;
   if (group < 1 || B % group != 0 || (shared_step != 0 && shared_step != 1)) return CATS_ERR_SHAPE;
   if (int st = check_strides(q, q_strides)) return st;
   if (int st = check_words(offsets)) return st;
