@@ -304,11 +304,18 @@ __device__ __forceinline__ u32x2 read_turned(const char* at) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
 }
 
-// Many tokens: 128 rows of queries a workgroup, 32 a wave, over tiles of 64 keys that come into LDS straight from memory, the next one while the weights of
-// this one are computed.
+// Many tokens: 128 rows of queries a workgroup, 32 a wave, over tiles of 64 keys that come into LDS straight from memory.
 //   S^T = K . Q^T   v_mfma_f32_32x32x16; tile u, row 8 a + 4 h + i of the result: token 32 u + 8 a + 4 h + i, in lanes of half h = lane / 32; columns are queries
 //   O^T += V^T . P  operand of step v (16 tokens): tokens 16 v + 4 h + (0 .. 3) and 8 behind them, those whose weights the lane has; V comes turned round out of LDS
-// Rows of LDS are 16-byte pieces, exchanged within a row so that lanes that read together find different banks.
+// So weights never leave their lane, and each number of a tile is read once out of LDS for 32 rows.  Rows of LDS are 16-byte pieces, exchanged within a row so that lanes
+// that read together find different banks (no conflicts are counted).
+// Bound by the matrix cores' and the vector units' power and issue: a tile and wave are 32 matrix and 150 other instructions, the weights of half a tile beside the products
+// of the half before and the scores of the half behind.  8192 tokens of 32 heads over 8 in bf16 take 483 to 515 us (card by card), 1.07 to 1.14 PFLOP/s, where a product of
+// 8192^3 reaches 1.25; with weights, scores and products one behind the other it was 536, with these side by side in whole tiles 515.  Two workgroups a CU (256 registers,
+// 64 KiB of LDS): one alone needs 1.0 to 1.3 us a tile and two together 1.95, so what their first loads (4 us) and ends (2 to 3 us) take is hidden where there are
+// enough of them: 2048 tokens of 32 heads, 512 workgroups of 2 to 32 tiles, take 47.5 us where the tiles alone are 33.
+// Tried: a ring of half tiles with a barrier for each (1.3 us a tile); operands read four ahead (no gain); all sequences' longest first (16 prompts to 1500 no gain, and
+// 16 of 512 88 us for 65: more keys at once than a part of the chip's second cache holds).
 constexpr int kTileKeys = 64, kTileRows = 128;
 template <class DT> struct Limit { static constexpr float SUM = 0x1p15f; };  // 2^HEAD
 template <> struct Limit<BF16> { static constexpr float SUM = 0x1p-32f; };
@@ -762,6 +769,8 @@ __device__ __forceinline__ void packed_attn_tiles(const PackedAttnArgs& p, Tiles
 //   S^T = K . Q^T   tile i, row 4 g + e of the result: token 16 i + 4 g + e, in lanes of group g = lane / 16; columns are queries
 //   O^T += V^T . P  operand of 32 tokens: tokens 4 g .. + 3 and 16 + 4 g .. + 3, those whose weights the lane has; V comes turned round out of LDS
 // Each wave has 32 keys of its own at a time and waits for nobody: keys come as operands, values into LDS of the wave's own.  What the waves give is joined in LDS at the end.
+// Bound by memory: 32 rows of 32 heads over 8 behind 4096 tokens, 537 MB, take 86.5 us, 6.2 TB/s; with lengths to 4096 (407 MB) 72.5, 4.6 of them the join's.  Three workgroups a
+// CU for heads of 128, which their registers allow (with keys by way of LDS there were two: 78 us).  More than 16 rows would need the matrix cores' other form: see above.
 constexpr int kStepKeys = 32, kStepRows = 16;
 template <int D> __device__ __forceinline__ constexpr int step_swap_v(int t) {
   return D >= 128 ? (t & 7) * 2 : D == 64 ? (t >> 1 & 3) * 2 : (t >> 2 & 1) * 2;
@@ -1033,7 +1042,8 @@ __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_ke
   __shared__ StepLds<D> lds;
   packed_attn_step<DT, D>(p, lds);
 }
-// Many rows behind keys that they share, and few with keys of their own: the first wait for the matrix cores, the others for memory, so they run side by side.
+// Many rows behind keys that they share, and few with keys of their own: the first wait for the matrix cores, the others for memory, so they run side by side (64 rows
+// behind 16384 tokens they share and 500 each: 45 us, in two launches 58, with the shared ones in parts of 16 rows 54).
 template <class DT, int D>
 __global__ __launch_bounds__(256, packed_tiles_waves(D)) void packed_attn_both_kernel(PackedAttnArgs p) {
   __shared__ union {
@@ -1044,7 +1054,9 @@ __global__ __launch_bounds__(256, packed_tiles_waves(D)) void packed_attn_both_k
   else packed_attn_step<DT, D>(p, lds.step);
 }
 
-// The splits' results, in a fixed order.  ALONE: a workgroup a row, else a wave a row; groups of D / 4 lanes take every so manieth split.
+// The splits' results, in a fixed order: part s counts sum_s = sum of 2^(score - top_s), and num / sum = (sum of 2^(top_s - top) num_s) / (sum of 2^(top_s - top) sum_s).  A launch
+// of its own behind the other, 3 to 4.6 us for two parts of 1024 rows, and 5.4 for 17 of 2048, which would be one wave's loop over them.  ALONE: a workgroup a row, for more than
+// eight parts, else a wave a row; groups of D / 4 lanes take every so manieth.
 template <class DT, int D, bool ALONE>
 __global__ __launch_bounds__(256) void packed_join_kernel(PackedAttnArgs p) {
   constexpr int L = D / 4, G = (ALONE ? 256 : kWave) / L;

@@ -200,8 +200,8 @@ def cats_paged_attention(q, offsets, start, k_pages, v_pages, table, scale, wind
     """Causal attention of packed tokens that cats_paged_append has stored: q (N, heads, D), heads a multiple of the pages', over the positions up to each
     token's own, at most ``window`` of them (0: all); ``scale`` lies in 2^-64 .. 2^64.
 
-    shared (int64 on the GPU, one or one a group): each ``group`` sequences in order have the same first ``shared`` tokens, which are read once for all of
-    them, through the first one's row of the table.  Returns (N, heads, D); tokens that no sequence has are zeros, and one that sees a page that is none is
+    shared (int64 on the GPU, one or one a group): each ``group`` sequences in order have the same first ``shared`` tokens, whose whole pages are read once for
+    all of them, through the first one's row of the table.  Returns (N, heads, D); tokens that no sequence has are zeros, and one that sees a page that is none is
     NaN.  Serving only: no gradient, and a q that records one is refused."""
     return torch.ops.flash_gemv.cats_paged_attention(q, offsets, start, k_pages, v_pages, table, scale, window, group, shared)
 

@@ -314,12 +314,17 @@ int cats_paged_append(const void* q, const int64_t* q_strides, const void* k, co
                       int kv_heads, int D, int page, int pages, int width, int dtype, void* stream);
 
 /* out[t, h] = softmax(scale * q[t, h] . K^T) . V over the keys at positions p - window + 1 .. p (window 0: 0 .. p), p = start[s] + t - offsets[s], of
- * cached head h / (heads / kv_heads) of the token's sequence s; the new tokens have been stored.  group > 1 (B is a multiple of it): each `group` sequences in order have the same
- * first shared[s / group] (shared_step 1) or shared[0] (shared_step 0) tokens, which are read for all of them through the first one's table (up to start[s] of them for sequence s).
- * A sequence whose tokens do not lie within its table's entries is NaN, and so is a query that sees a token whose entry is no page; rows that are nobody's are zeros.  A query that
- * sees a NaN in a key, or a value that is not finite, is not finite (in that element); a score of -infinity weighs nothing.  out (N, heads, D), 16-byte aligned.  scale lies in 2^-64 .. 2^64, and scores have to be within 32-bit floats.
- * Weights are rounded to dtype (their sum is not).  scratch: 16-byte aligned, at least cats_paged_attention_scratch_bytes() on the device of the call (which may be 0), nothing
- * in it needs to be set. */
+ * cached head h / (heads / kv_heads) of the token's sequence s; the new tokens have been stored.  scale lies in 2^-64 .. 2^64, and scores have to be within 32-bit floats.
+ * Weights are rounded to dtype (their sum is not).
+ * group > 1 (B is a multiple of it): each `group` sequences in order have the same first n tokens, n = shared[s / group] (shared_step 1) or shared[0]
+ * (shared_step 0), up to start[s] of them for sequence s.  Whole pages of these are read once for all, through the first one's row of the table, whose
+ * entries have to be there for them; the page in which they end is each one's own.
+ * A sequence whose tokens do not lie within its table's entries is NaN, and so is a query that sees a token whose entry is no page; rows that are nobody's are zeros, and
+ * so is a query whose scores are all -infinity.  A query that sees a NaN in a key, or a value that is not finite, is not finite (in that element); a score of -infinity
+ * weighs nothing.  Keys that a query does not see, and places behind a sequence's last token, may hold anything.
+ * out (N, heads, D), 16-byte aligned.  scratch: 16-byte aligned, at least cats_paged_attention_scratch_bytes() on the device of the call (which may be 0), one for each
+ * call that runs at the same time, nothing in it needs to be set.  N * heads / 16 + (B + 2) * kv_heads is below 2^24,
+ * and below 2^21 where group > 1. */
 size_t cats_paged_attention_scratch_bytes(int N, int B, int heads, int kv_heads, int D, int page, int width, int window, int group);
 int cats_paged_attention(const void* q, const int64_t* q_strides, const int64_t* offsets, const int64_t* start, const void* k_pages, const void* v_pages,
                          const int32_t* table, int64_t table_stride, float scale, int window, int group, const int64_t* shared, int shared_step,
