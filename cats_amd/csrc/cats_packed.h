@@ -744,12 +744,20 @@ __device__ __forceinline__ void packed_attn_tiles(const PackedAttnArgs& p, Tiles
     }
   } else {
     const float f = sum == 0.f ? 0.f : 1.f / sum;  // no key, or none that weighs anything
-    store([&](long long to, int w, int a) {
-      float x[4];
+    const long long to = packed_out(p, tok0, c, min(mine, rows - 1), D) - p.out + 8 * h;
 #pragma unroll
-      for (int e = 0; e < 4; e++) x[e] = o[w][4 * a + e] * f;
-      *(u32x2*)(p.out + to) = u32x2{DT::pack(x[0], x[1]), DT::pack(x[2], x[3])};
-    });
+    for (int w = 0; w < NW; w++)
+#pragma unroll
+      for (int a = 0; a < 4; a += 2) {  // the halves of the wave exchange what they have of eights a and a + 1, and each writes one of them
+        u32x4 x;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const auto r = __builtin_amdgcn_permlane32_swap(DT::pack(o[w][4 * a + 2 * e] * f, o[w][4 * a + 2 * e + 1] * f),
+                                                          DT::pack(o[w][4 * a + 4 + 2 * e] * f, o[w][4 * a + 5 + 2 * e] * f), false, false);
+          x[e] = r[0], x[2 + e] = r[1];
+        }
+        if (mine < rows) *(u32x4*)(p.out + to + 32 * w + 8 * a) = x;
+      }
   }
   if (bad) {
     again(true);
