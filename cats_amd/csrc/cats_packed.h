@@ -313,7 +313,8 @@ __device__ __forceinline__ u32x2 read_turned(const char* at) {
 // of the half before and the scores of the half behind.  8192 tokens of 32 heads over 8 in bf16 take 483 to 515 us (card by card), 1.07 to 1.14 PFLOP/s, where a product of
 // 8192^3 reaches 1.25; with weights, scores and products one behind the other it was 536, with these side by side in whole tiles 515.  Two workgroups a CU (256 registers,
 // 64 KiB of LDS): one alone needs 1.0 to 1.3 us a tile and two together 1.95, so what their first loads (4 us) and ends (2 to 3 us) take is hidden where there are
-// enough of them: 2048 tokens of 32 heads, 512 workgroups of 2 to 32 tiles, take 47.5 us where the tiles alone are 33.
+// enough of them: 2048 tokens of 32 heads, 512 workgroups of 2 to 32 tiles, take 47 to 50 us where the tiles alone are 33.
+// Results leave sixteen bytes a lane, which two lanes put together (eight bytes each: 64 prompts of 128 tokens 52.2 us for 43.7).
 // Tried: a ring of half tiles with a barrier for each (1.3 us a tile); operands read four ahead (no gain); all sequences' longest first (16 prompts to 1500 no gain, and
 // 16 of 512 88 us for 65: more keys at once than a part of the chip's second cache holds).
 constexpr int kTileKeys = 64, kTileRows = 128;
