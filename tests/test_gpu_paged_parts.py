@@ -146,3 +146,25 @@ def test_workgroups_find_their_sequence(B, n):
     ref.fill(pool, rows, g)
     q = torch.randn(ref.offsets_of(rows, 3)[-1] + 40, 2, 32, generator=g).half()
     assert ref.within(_attention(q, rows, 3, pool, 0.2), *ref.paged_attention(q, rows, 3, pool, 0.2))
+
+
+@pytest.mark.parametrize("B,group", [(120, 2), (126, 2), (504, 2), (600, 2), (600, 3), (900, 300)])
+@pytest.mark.parametrize("n", [1, 4])
+def test_workgroups_find_their_group(B, group, n):
+    """Groups of which some have no tokens, some of one workgroup's rows and some of several."""
+    rows = [(40 + b % 5, (b // group % 7 != 3) * (n + (b % 11 == 0) * 5)) for b in range(B)]
+    g = torch.Generator().manual_seed(20)
+    pool = ref.new_pool(rows, 16, 1, 32, BF16, group=group, shared=32)
+    ref.fill(pool, rows, g)
+    q = torch.randn(ref.offsets_of(rows, 2)[-1] + 9, 3, 32, generator=g).bfloat16()
+    assert ref.within(_attention(q, rows, 2, pool, 0.2, 0, group, [32]), *ref.paged_attention(q, rows, 2, pool, 0.2))
+
+
+@pytest.mark.parametrize("heads,kv", [(130, 1), (96, 1), (64, 64)])
+@pytest.mark.parametrize("rows", [[(30, 1), (200, 2)], [(1500, 1)]])
+def test_many_heads(heads, kv, rows):
+    """More rows a token than a workgroup has."""
+    g = torch.Generator().manual_seed(22)
+    pool = _pool(rows, 64, kv, 64, F16, g)
+    q = torch.randn(ref.offsets_of(rows)[-1], heads, 64, generator=g).half()
+    assert ref.within(_attention(q, rows, 0, pool, 0.125), *ref.paged_attention(q, rows, 0, pool, 0.125))

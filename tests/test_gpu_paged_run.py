@@ -128,6 +128,10 @@ def _step_state(B, group, shared, length, dtype=F16, heads=8, kv=2, D=64, page=1
     return s, calls
 
 
+def _same(a, b):
+    return torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
 @pytest.mark.parametrize("B,group,shared,length", [(3, 1, 0, 60), (2, 1, 0, 3000), (4, 4, 200, 200), (24, 24, 1100, 1100)])
 def test_captured_steps(B, group, shared, length):
     """A captured step follows its tensors: new tokens, positions, lengths of prompts and tables.  The result is the eager one's, whatever runs between."""
@@ -143,12 +147,13 @@ def test_captured_steps(B, group, shared, length):
             s[n].normal_()
         s["start"] += 1
         s["at"].copy_(_words([[0, 40, 41, 41, 100], [5, 10, 80, 80, 90], [0, 100, 100, 100, 100], [0, 1, 2, 3, 4], [0, 0, 0, 0, 0]][t]))
-        moved = s["table"].clone()
+        if t == 3 and group == 1:  # sequences change places: an entry may be no page now, and the query that sees it NaN
+            s["table"].copy_(s["table"].roll(1, 0))
+        table = s["table"].clone()
         want = [x.clone() for x in calls()]
         pages = s["kp"].clone(), s["vp"].clone()
         graph.replay()
-        assert all(torch.equal(a, b) for a, b in zip(outs, want)) and torch.equal(s["table"], moved)
-        assert torch.equal(s["kp"].nan_to_num(), pages[0].nan_to_num()) and torch.equal(s["vp"].nan_to_num(), pages[1].nan_to_num())
+        assert all(_same(a, b) for a, b in zip([*outs, s["kp"], s["vp"]], [*want, *pages])) and torch.equal(s["table"], table)
         torch.randn(1000, 1000, device="cuda").sum().item()
 
 
