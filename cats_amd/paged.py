@@ -68,15 +68,20 @@ class PagedCache:
             self._pages[s] += [self._take() for _ in range(n)]
 
     def trim(self, seq, length):
-        """Gives back the pages behind the first `length` tokens, from where the sequence may go on.  The page in which they end becomes its own."""
+        """Gives back the pages behind the first `length` tokens, from where the sequence may go on.  The page in which they end becomes its own: where others have
+        it too, it is copied, and if there is no page for the copy, nor one among those that come free, the sequence stays as it is."""
         pages = self._pages[seq]
         if not 0 <= length <= len(pages) * self.page:
             raise ValueError(f"the first {length} tokens of a sequence with {len(pages)} pages of {self.page}")
         whole, rest = divmod(length, self.page)
-        for p in pages[whole + (rest > 0):]:
+        kept = whole + (rest > 0)
+        copied = rest > 0 and self._users[pages[whole]] > 1
+        if copied and not self._free and all(self._users[p] > 1 for p in pages[kept:]):
+            raise RuntimeError("1 page is needed and 0 are free")
+        for p in pages[kept:]:
             self._give(p)
-        del pages[whole + (rest > 0):]
-        if rest and self._users[pages[whole]] > 1:
+        del pages[kept:]
+        if copied:
             pages[whole] = self._copy(pages[whole], rest)
 
     def fork(self, seq, count, length):

@@ -75,6 +75,43 @@ def test_an_end_within_a_shared_page_is_the_sequence_s_own():
     assert c.pages_of(a)[0] != c.pages_of(b)[0] and c.free == 7  # its second page is free, and it has a copy of the first
 
 
+@pytest.mark.parametrize("more", [0, 1])
+def test_an_end_that_finds_no_page_takes_nothing(more):
+    """Where the page in which the end lies is shared and none is there for the copy, the sequence stays as it was; a page that it gives back itself is one."""
+    c = _cache(2 + more)
+    a = c.open()
+    c.reserve([a], 32)
+    (b,) = c.fork(a, 1, 32)
+    if more:
+        c.reserve([a], 48)  # somebody's
+    c.k.copy_(torch.arange(c.k.numel()).reshape(c.k.shape) % 1000)
+    before = c.pages_of(a), c.pages_of(b), list(c._users), list(c._free), c.k.clone()
+    assert c.free == 0
+    for length in (4, 20):
+        with pytest.raises(RuntimeError, match="1 page is needed and 0 are free"):
+            c.trim(b, length)
+        assert before[:4] == (c.pages_of(a), c.pages_of(b), c._users, c._free) and torch.equal(c.k, before[4])
+    c.trim(b, 16)  # whole pages need none
+    assert c.pages_of(b) == c.pages_of(a)[:1]
+    if more:
+        c.trim(a, 20)
+        assert c.free == 1 and c.pages_of(a) == before[0][:2]  # nobody else has that one now
+        c.trim(a, 4)
+        assert c.pages_of(a)[0] != c.pages_of(b)[0] and c.free == 1 and torch.equal(c.k[:, c.pages_of(a)[0], :, :4], c.k[:, c.pages_of(b)[0], :, :4])
+
+
+def test_an_end_may_lie_in_a_page_that_comes_free():
+    c = _cache(3)
+    a = c.open()
+    c.reserve([a], 16)
+    (b,) = c.fork(a, 1, 16)
+    c.reserve([b], 48)
+    c.k.copy_(torch.arange(c.k.numel()).reshape(c.k.shape) % 1000)
+    assert c.free == 0
+    c.trim(b, 5)
+    assert c.free == 1 and c.pages_of(b) != c.pages_of(a) and torch.equal(c.k[:, c.pages_of(b)[0], :, :5], c.k[:, c.pages_of(a)[0], :, :5])
+
+
 def test_a_table_in_place():
     c = _cache()
     a = c.open()
