@@ -808,7 +808,6 @@ void check_packed(const at::Tensor& t, const at::Tensor& like, const char* name,
               " must be of one type, device and head size with the others");
   TORCH_CHECK(t.size(2) == 32 || t.size(2) == 64 || t.size(2) == 128 || t.size(2) == 256, "flash_gemv.", op, ": heads of 32, 64, 128 or 256 elements, got ", t.size(2));
   TORCH_CHECK(t.size(0) <= CATS_PAGED_MAX_TOKENS && t.size(1) <= 65535, "flash_gemv.", op, ": too large: ", name, " ", t.sizes());
-  check_no_grad(t, op);
 }
 
 // Device words: (n) of int64.
@@ -847,6 +846,9 @@ at::Tensor cats_paged_append_op(const c10::optional<at::Tensor>& q, const at::Te
                                 const c10::optional<at::Tensor>& cos_table, const c10::optional<at::Tensor>& sin_table, at::Tensor& k_pages,
                                 at::Tensor& v_pages, const at::Tensor& table) {
   const char* op = "cats_paged_append";
+  for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&k, &v, &k_pages, &v_pages}) check_no_grad(*t, op);
+  for (const auto* t : {&q, &cos_table, &sin_table})
+    if (t->has_value() && (*t)->defined()) check_no_grad(**t, op);
   check_packed(k, k, "k", op);
   check_packed(v, k, "v", op);
   TORCH_CHECK(v.sizes() == k.sizes(), "flash_gemv.cats_paged_append: k and v must be alike, got ", k.sizes(), " and ", v.sizes());
@@ -895,6 +897,7 @@ at::Tensor cats_paged_attention_op(const at::Tensor& q, const at::Tensor& offset
                                    const at::Tensor& table, const double scale, const int64_t window, const int64_t group,
                                    const c10::optional<at::Tensor>& shared) {
   const char* op = "cats_paged_attention";
+  for (const at::Tensor* t : {&q, &k_pages, &v_pages}) check_no_grad(*t, op);
   check_packed(q, q, "q", op);
   const int64_t B = sequences_of(offsets, op), N = q.size(0), heads = q.size(1);
   const int64_t* op_ = check_words(offsets, q, B + 1, "offsets", op);
@@ -926,6 +929,7 @@ at::Tensor cats_paged_attention_op(const at::Tensor& q, const at::Tensor& offset
 at::Tensor cats_prompt_attention_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, const double scale,
                                     const int64_t window, const c10::optional<at::Tensor>& k_offsets) {
   const char* op = "cats_prompt_attention";
+  for (const at::Tensor* t : {&q, &k, &v}) check_no_grad(*t, op);
   check_packed(q, q, "q", op);
   check_packed(k, q, "k", op);
   check_packed(v, q, "v", op);

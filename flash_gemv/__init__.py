@@ -191,7 +191,7 @@ def cats_paged_append(q, k, v, offsets, start, cos_table, sin_table, k_pages, v_
     the tokens: the first R elements of a head are rotated (rotate-half); None: none.  k_pages, v_pages (pages, kv_heads, page, D), page a power of
     two from 16 to 1024; table (B, entries) int32: position p of sequence s lies in page ``table[s, p // page]``.
     Returns the queries, rotated (None for None).  A token that has no page or no row of the tables is not stored, and its query is NaN.  No two tokens of a
-    call may have one place.  No gradient: tensors that record one are refused."""
+    call may have one place.  No gradient: tokens, pages and tables that record one are refused."""
     out = torch.ops.flash_gemv.cats_paged_append(q, k, v, offsets, start, cos_table, sin_table, k_pages, v_pages, table)
     return out if q is not None else None
 
@@ -202,7 +202,7 @@ def cats_paged_attention(q, offsets, start, k_pages, v_pages, table, scale, wind
 
     shared (int64 on the GPU, one or one a group): each ``group`` sequences in order have the same first ``shared`` tokens, whose whole pages are read once for
     all of them, through the first one's row of the table.  Returns (N, heads, D); tokens that no sequence has are zeros, and one that sees a page that is none is
-    NaN.  Serving only: no gradient, and a q that records one is refused."""
+    NaN.  Serving only: no gradient, and a q or pages that record one are refused."""
     return torch.ops.flash_gemv.cats_paged_attention(q, offsets, start, k_pages, v_pages, table, scale, window, group, shared)
 
 

@@ -103,3 +103,26 @@ def test_tensors_of_the_host_are_refused():
                  lambda: flash_gemv.cats_prompt_attention(x, x, x, w, 0.1)):
         with pytest.raises(RuntimeError, match="GPU"):
             call()
+
+
+def _ops():
+    """Each op of torch on tensors of the host, and those of its tensors that hold numbers."""
+    import flash_gemv
+
+    x, w, pool, turn = (torch.zeros(2, 2, 64).half() for _ in range(3)), torch.tensor([0, 2]), [torch.zeros(2, 2, 16, 64).half() for _ in range(2)], [torch.zeros(4, 64) for _ in range(2)]
+    a, table = dict(zip(("q", "k", "v", "k_pages", "v_pages", "cos", "sin"), (*x, *pool, *turn))), torch.zeros(1, 2, dtype=torch.int32)
+    append = lambda q, k, v, k_pages, v_pages, cos, sin: flash_gemv.cats_paged_append(q, k, v, w, w[:1], cos, sin, k_pages, v_pages, table)
+    attention = lambda q, k_pages, v_pages: flash_gemv.cats_paged_attention(q, w, w[:1], k_pages, v_pages, table, 0.1)
+    prompt = lambda q, k, v: flash_gemv.cats_prompt_attention(q, k, v, w, 0.1)
+    return [(append, a), (attention, {n: a[n] for n in ("q", "k_pages", "v_pages")}), (prompt, {n: a[n] for n in "qkv"})]
+
+
+@pytest.mark.parametrize("op,name", [(0, n) for n in ("q", "k", "v", "k_pages", "v_pages", "cos", "sin")] + [(1, n) for n in ("q", "k_pages", "v_pages")] + [(2, n) for n in "qkv"])
+def test_what_records_a_gradient_is_refused(op, name):
+    """Tokens, pages and rotary tables alike.  Where nothing is recorded they are as any others, and what is wrong with these is that they are not on the GPU."""
+    call, args = _ops()[op]
+    args[name].requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        call(**args)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
+        call(**args)
