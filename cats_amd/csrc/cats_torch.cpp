@@ -7,6 +7,7 @@
 // status becomes a c10::Error (the reference printf()s and exit()s: fuse_gemv_cmp_cuda.cu:2096-2097).
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
@@ -595,9 +596,12 @@ const int64_t* words_of(const at::Tensor& t, const at::Tensor& like, int64_t row
   return t.data_ptr<int64_t>();
 }
 
-// Neither storing nor attending has a gradient, so a tensor that records one is refused rather than cut off from it in silence.
+// Neither storing nor attending has a gradient, so a tensor that records one, or carries a tangent (which no_grad does not end), is refused rather than cut off
+// from it in silence.
 void check_no_grad(const at::Tensor& t, const char* op) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), "flash_gemv.", op, ": no gradient; call it under torch.no_grad() or on detached tensors");
+  TORCH_CHECK(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()), "flash_gemv.", op,
+              ": no gradient, forward differentiation's either; call it on the primal tensors");
 }
 
 struct Kv8 {
@@ -629,9 +633,9 @@ Kv8 check_kv8(const at::Tensor& like, const at::Tensor& k8, const at::Tensor& v8
 
 void cats_kv8_append_op(const at::Tensor& k, const at::Tensor& v, const at::Tensor& start, const c10::optional<at::Tensor>& count, at::Tensor& k8,
                         at::Tensor& v8, at::Tensor& k_scale, at::Tensor& v_scale, at::Tensor& k_tail, at::Tensor& v_tail) {
-  const Kv8 c = check_kv8(k, k8, v8, k_scale, v_scale, k_tail, v_tail, "cats_kv8_append");
   check_no_grad(k, "cats_kv8_append");
   check_no_grad(v, "cats_kv8_append");
+  const Kv8 c = check_kv8(k, k8, v8, k_scale, v_scale, k_tail, v_tail, "cats_kv8_append");
   TORCH_CHECK(k.size(2) == c.heads && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(),
               "flash_gemv.cats_kv8_append: k and v must be alike, (B, T, kv_heads, D)");
   int ss = 0, cs = 0;
@@ -649,8 +653,8 @@ void cats_kv8_append_op(const at::Tensor& k, const at::Tensor& v, const at::Tens
 at::Tensor cats_kv8_attention_op(const at::Tensor& q, const at::Tensor& start, const c10::optional<at::Tensor>& count, const at::Tensor& k8,
                                  const at::Tensor& v8, const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& k_tail,
                                  const at::Tensor& v_tail, const double scale, const int64_t window) {
-  const Kv8 c = check_kv8(q, k8, v8, k_scale, v_scale, k_tail, v_tail, "cats_kv8_attention");
   check_no_grad(q, "cats_kv8_attention");
+  const Kv8 c = check_kv8(q, k8, v8, k_scale, v_scale, k_tail, v_tail, "cats_kv8_attention");
   const int64_t T = q.size(1), heads = q.size(2);
   TORCH_CHECK(c.heads >= 1 && heads % c.heads == 0, "flash_gemv.cats_kv8_attention: ", heads, " query heads over ", c.heads, " cached heads");
   TORCH_CHECK(window >= 0 && window <= INT_MAX, "flash_gemv.cats_kv8_attention: window must be 0 (all keys) or a number of keys");

@@ -126,3 +126,36 @@ def test_what_records_a_gradient_is_refused(op, name):
         call(**args)
     with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
         call(**args)
+
+
+@pytest.mark.parametrize("op,name", [(0, "q"), (0, "k"), (0, "v_pages"), (0, "sin"), (1, "q"), (1, "k_pages"), (2, "q"), (2, "v")])
+def test_tangents_are_refused(op, name):
+    """Of forward differentiation, which no_grad does not end."""
+    from torch.autograd import forward_ad
+
+    call, args = _ops()[op]
+    with forward_ad.dual_level():
+        args[name] = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(**args)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
+            call(**args)
+        with torch.inference_mode(), pytest.raises(RuntimeError, match="GPU"):
+            call(**args)
+    with pytest.raises(RuntimeError, match="GPU"):  # it has none any more
+        call(**args)
+
+
+def test_tangents_of_a_cache_in_8_bits_are_refused():
+    """The ops of the other cache look at their tokens in the same way."""
+    import flash_gemv
+    from torch.autograd import forward_ad
+    from cats_amd.kv8 import Kv8Cache
+
+    c, x, w = Kv8Cache(1, 2, 64, 64, device="cpu"), torch.zeros(1, 1, 2, 64).half(), torch.tensor([0])
+    t = [getattr(c, n) for n in Kv8Cache.FIELDS]
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: flash_gemv.cats_kv8_append(d, x, w, None, *t), lambda: flash_gemv.cats_kv8_append(x, d, w, None, *t), lambda: flash_gemv.cats_kv8_attention(d, w, None, *t, 0.125)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
