@@ -740,7 +740,7 @@ __device__ __forceinline__ void packed_attn_tiles(const PackedAttnArgs& p, Tiles
     store([&](long long to, int w, int a) { *(f32x4*)(p.part + to) = f32x4{o[w][4 * a], o[w][4 * a + 1], o[w][4 * a + 2], o[w][4 * a + 3]}; });
     if (h == 0 && mine < rows) {
       float* ml = packed_part_ml(p, D) + 2 * (part.at + packed_row_at(p, part, c, mine));
-      ml[0] = top + F::SLACK;  // what weights of 2^HEAD are relative to
+      ml[0] = top;  // as it is: at 2^27 and beyond 32 bits hold no top + SLACK.  Weights of 2^(HEAD - SLACK) are relative to it
       ml[1] = sum;
     }
   } else {
@@ -792,10 +792,13 @@ template <int D> struct StepLds {
   };
   float top[4][kStepRows], sum[4][kStepRows];
 };
-template <class DT, int D>
+// BESIDE: parts of packed_attn_tiles are joined with these, whose weights are 2^SLACK times as large: what goes to the join is scaled by 2^-SLACK, which is exact.
+template <class DT, int D, bool BESIDE>
 __device__ __forceinline__ void packed_attn_step(const PackedAttnArgs& p, StepLds<D>& lds) {
   constexpr int C = D / 32, NU = D / 16, PK = D / 8, STEP = kWave / PK, W = 4, LOADS = PK / 4;
   typedef Kv<DT> F;
+  static_assert(F::SLACK == 8.f);
+  constexpr float UNIT = BESIDE ? 0x1p-8f : 1.f;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
   const int block = p.by_heads(blockIdx.x), c = blockIdx.x - block * p.kv_heads;
   const PackedPart part = packed_part<kStepRows>(p, block);
@@ -1005,7 +1008,7 @@ __device__ __forceinline__ void packed_attn_step(const PackedAttnArgs& p, StepLd
       float den = 0.f;
 #pragma unroll
       for (int w = 0; w < W; w++) {
-        const float f = count ? 1.f : __builtin_amdgcn_exp2f(lds.top[w][r] - mx);
+        const float f = count ? 1.f : __builtin_amdgcn_exp2f(lds.top[w][r] - mx) * UNIT;
         const f32x4 x = *(const f32x4*)&lds.joined[w][r][d];
 #pragma unroll
         for (int e = 0; e < 4; e++) num[e] = fmaf(f, x[e], num[e]);
@@ -1049,7 +1052,7 @@ __global__ __launch_bounds__(256, packed_tiles_waves(D)) void packed_attn_tiles_
 template <class DT, int D>
 __global__ __launch_bounds__(256, packed_step_waves(D)) void packed_attn_step_kernel(PackedAttnArgs p) {
   __shared__ StepLds<D> lds;
-  packed_attn_step<DT, D>(p, lds);
+  packed_attn_step<DT, D, false>(p, lds);
 }
 // Many rows behind keys that they share, and few with keys of their own: the first wait for the matrix cores, the others for memory, so they run side by side (64 rows
 // behind 16384 tokens they share and 500 each: 45 us, in two launches 58, with the shared ones in parts of 16 rows 54).
@@ -1060,7 +1063,7 @@ __global__ __launch_bounds__(256, packed_tiles_waves(D)) void packed_attn_both_k
     StepLds<D> step;
   } lds;
   if (p.by_heads(blockIdx.x) < p.group_blocks) packed_attn_tiles<DT, D, SPLIT>(p, lds.tiles);
-  else packed_attn_step<DT, D>(p, lds.step);
+  else packed_attn_step<DT, D, true>(p, lds.step);
 }
 
 // The splits' results, in a fixed order: part s counts sum_s = sum of 2^(score - top_s), and num / sum = (sum of 2^(top_s - top) num_s) / (sum of 2^(top_s - top) sum_s).  A launch
