@@ -330,7 +330,10 @@ __device__ __forceinline__ const char* uniform(const void* p) {
 // would wait for memory, whatever it reads.  It has no result in a register; who reads what it brings waits for vmcnt(0) first.
 __device__ __forceinline__ void load_lds(const char* from, unsigned lane_at, const void* to) {
   const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)to);
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // that nobody keeps m0 for us is what the list is to say
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0" ::"s"(from), "s"(lds), "v"(lane_at) : "memory", "m0");
+#pragma clang diagnostic pop
 }
 template <int D> __device__ __forceinline__ constexpr int tile_swap_k(int t) {
   return D >= 128 ? t & 15 : D == 64 ? t >> 1 & 7 : t >> 2 & 3;
