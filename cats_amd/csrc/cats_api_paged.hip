@@ -65,7 +65,8 @@ bool grid_ok(int N, int B, int heads, int kv_heads, int members = 1) {
 //           39 and 34), or a group (8 groups of 8 sequences behind 2048: 34 us and 30).
 //   splits  As many as bring workgroups to two a CU, whose loads cover for each other (1 row behind 131072 with two 87 us, 6.2 TB/s), and to one where
 //           the matrix cores bound (piece of 512 behind 7680 with two 131 us, with one 117), or where keys are shared: a sequence's own ones are few then (4 x 8 beams
-//           on 2000 with two 39 us, with one 37; 4 rows behind 8192 21 and 16).  No part is of fewer than 128 or 256 keys, and 1024 are not split: the join, and the
+//           on 2000 with two 39 us, with one 37; 4 rows behind 8192 21 and 16).  Sequences of 17 to 64 rows, which memory bounds, go by the same rule and have not
+//           been measured with two.  No part is of fewer than 128 or 256 keys, and 1024 are not split: the join, and the
 //           writing and reading of parts, would cost what they give (1 row behind 1000 takes 9 us whole).
 PackedPlan paged_plan(int N, int B, int heads, int kv_heads, int page, int width, int window, int members) {
   const int cus = current_device_cus(), group = heads / kv_heads;

@@ -315,7 +315,9 @@ int cats_paged_append(const void* q, const int64_t* q_strides, const void* k, co
 
 /* out[t, h] = softmax(scale * q[t, h] . K^T) . V over the keys at positions p - window + 1 .. p (window 0: 0 .. p), p = start[s] + t - offsets[s], of
  * cached head h / (heads / kv_heads) of the token's sequence s; the new tokens have been stored.  scale lies in 2^-64 .. 2^64, and scores have to be within 32-bit floats.
- * Weights are rounded to dtype (their sum is not).
+ * Weights are rounded to dtype (their sum is not): fp16 ones are off by half a step down to 2^-21 of the largest and by 2^-32 of it below that, bf16 ones by half a step
+ * down to 2^-86, below which they may be 0.  Products with values are summed in 32 bits, where bf16 weights begin at 2^-40: values below 2^-100 lose bits, and those
+ * below 2^-109 may count as 0.
  * group > 1 (B is a multiple of it): each `group` sequences in order have the same first n tokens, n = shared[s / group] (shared_step 1) or shared[0]
  * (shared_step 0), up to start[s] of them for sequence s.  Whole pages of these are read once for all, through the first one's row of the table, whose
  * entries have to be there for them; the page in which they end is each one's own.

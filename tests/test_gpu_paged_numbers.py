@@ -105,8 +105,9 @@ def test_large_scores_of_prompts(window, levels, scale, delta, side, dtype, D):
     _check(_prompt(q, k, v, at, scale, window), want, _bound(want, size, dtype, delta))
 
 
-# fp16: single steps of the smallest numbers, and the largest ones.  bf16: the largest, and those down to 2^-80; weights are held as 2^-40 and more times themselves.
-SIZES = [(F16, 64, 2.0 ** -24), (F16, 128, 2.0 ** -17), (F16, 64, 16000.0), (BF16, 128, 2.0 ** -80), (BF16, 64, 2.0 ** -40), (BF16, 64, 2.0 ** 125)]
+# fp16: single steps of the smallest numbers, and the largest ones.  bf16: the largest, and those down to 2^-100: weights begin at 2^-40, so products with these are numbers of
+# 2^-140, which lie 2^-149 apart, and a sum of some hundred of them is off by far less than half a step of bf16.
+SIZES = [(F16, 64, 2.0 ** -24), (F16, 128, 2.0 ** -17), (F16, 64, 16000.0), (BF16, 128, 2.0 ** -80), (BF16, 64, 2.0 ** -100), (BF16, 64, 2.0 ** -40), (BF16, 64, 2.0 ** 125)]
 
 
 def _values(g, shape, size, dtype):
@@ -134,3 +135,26 @@ def test_sizes_of_values_of_prompts(dtype, D, size):
     q, k = (torch.randn(900, h, D, generator=g).to(dtype) for h in (2, 1))
     v = _values(g, (900, 1, D), size, dtype)
     _check(_prompt(q, k, v, at, D ** -0.5), *ref.prompt_attention(q, k, v, at, at, D ** -0.5))
+
+
+@pytest.mark.parametrize("dtype,D", [(F16, 64), (F16, 128), (BF16, 64)])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -13, 2.0 ** -17, 2.0 ** -19])
+@pytest.mark.parametrize("name", CALLS)
+def test_light_weights_count(name, size, dtype, D):
+    """Keys alike whose weights are 1.2 times 2^-13 of the first one's, whose values are zeros: all that is left of the output is theirs.  In fp16 weights have the fewest bits."""
+    g = torch.Generator().manual_seed(55)
+
+    def of(position):
+        k = torch.zeros(len(position), D)
+        k[position == 0, 0] = (13 * math.log(2) - math.log(1.2)) * 8
+        return k.to(dtype)
+
+    rows, group, shared, pool = _cached(name, of, dtype, D, g)
+    pool[1].copy_(((1 + 0.2 * torch.randn(pool[1].shape, generator=g)) * size).to(dtype))
+    for b in range(len(rows)):
+        pool[1][int(pool[2][b, 0]), 0, 0] = 0
+    _copy_shared(pool, rows, group, CALLS[name][3])
+    q = torch.zeros(ref.offsets_of(rows)[-1], 2, D)
+    q[..., 0] = 1
+    q = q.to(dtype)
+    _check(_attention(q, rows, 0, pool, 0.125, 0, group, shared), *ref.paged_attention(q, rows, 0, pool, 0.125))
