@@ -578,7 +578,7 @@ at::Tensor cats_prompt_mlp_op(const at::Tensor& x, const at::Tensor& w_gate, con
 at::Tensor tokens_of(const at::Tensor& t) {
   bool fits = t.stride(3) == 1 && ((uintptr_t)t.data_ptr() & 15u) == 0;
   for (int i = 0; i < 3; i++) fits = fits && (t.size(i) == 1 || (t.stride(i) >= 0 && t.stride(i) % 8 == 0));
-  return fits ? t : t.contiguous();
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);  // contiguous() would give one back that only begins off a boundary
 }
 struct Strides {
   int64_t s[3];
@@ -795,7 +795,7 @@ at::Tensor packed_of(const at::Tensor& t) {
   bool fits = t.stride(2) == 1 && ((uintptr_t)t.data_ptr() & 15u) == 0;
   for (int i = 0; i < 2; i++) fits = fits && (t.size(i) == 1 || (t.stride(i) >= 0 && t.stride(i) % 8 == 0));
   fits = fits && (t.size(0) == 1 || t.stride(0) <= 1 << 23);
-  return fits ? t : t.contiguous();
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);  // contiguous() would give one back that only begins off a boundary
 }
 struct PackedStrides {
   int64_t s[2];
