@@ -87,7 +87,7 @@ class PagedCache:
     def fork(self, seq, count, length):
         """`count` new sequences that begin with the first `length` tokens of this one.  Whole pages are shared, the page in which they end is copied, in all
         layers.  Sequences that stand together in a call and were forked at `length` may be attended as a group with `shared` = length: of that the whole
-        pages count."""
+        pages count, and the first one's are read, so it may not have been cut within them."""
         pages = self._pages[seq]
         if not 0 <= length <= len(pages) * self.page:
             raise ValueError(f"the first {length} tokens of a sequence with {len(pages)} pages of {self.page}")

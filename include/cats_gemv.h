@@ -300,7 +300,7 @@ int cats_kv8_attention_step(const void* h, const void* x, const void* norm_weigh
  * Tokens of a call are packed: sequence s of B has the tokens offsets[s] .. offsets[s + 1] - 1 (none, one or many) of the N tokens of q, k, v and out, at the positions
  * start[s] onwards.  offsets (B + 1) ascend within 0 .. N; tokens before the first and behind the last belong to nobody.  offsets, start, table and shared
  * are read on the device, so a captured call follows them.  D is 32, 64, 128 or 256.  Strides of q, k and v: of a token and of a head, in elements,
- * multiples of 8; the elements of a head side by side, 16-byte aligned.  All calls may be captured; nothing is kept between calls. */
+ * multiples of 8, a token's at most 2^23; the elements of a head side by side, 16-byte aligned.  All calls may be captured; nothing is kept between calls. */
 #define CATS_PAGED_MAX_TOKENS (1 << 24)
 
 /* Stores new tokens, rotated on the way:  x' = x cos[p] + (-x[R/2 .. R-1], x[0 .. R/2-1]) sin[p]  over the first R = rot elements of the heads of q and k, p the
